@@ -259,11 +259,13 @@ def plain_route(s):
 
 
 def plain_act(act, g):
-    """silu with its exponential in 64 bits, or gelu of the input in fp16, rounded to fp16."""
+    """silu with its exponential in 64 bits, or the library's gelu: of the input in fp16, the formula in 32 bits with
+    its tanh in 64, rounded to fp16."""
     if act == "silu":
         return (g.double() / (1.0 + torch.exp(-g.double()).float()).double()).float()
-    h = g.to(torch.float16).double()
-    t = (0.5 * h * (1.0 + torch.tanh(math.sqrt(2.0 / math.pi) * h * (1.0 + 0.044715 * h * h)))).to(torch.float16).float()
+    h = g.to(torch.float16).float()
+    inner = 0.7978845608028654 * h * (1.0 + 0.044715 * h * h)
+    t = (0.5 * h * (1.0 + torch.tanh(inner.double()).float())).to(torch.float16).float()
     return torch.where(g <= -10.0, 0.0, torch.where(g >= 10.0, g, t))
 
 
@@ -348,13 +350,18 @@ def work(case):
 # ------------------------------------------------------------------------------------------------ float64
 
 
+def f32(v):
+    """A float64 value rounded to float32, where a definition rounds it."""
+    return v.float().double()
+
+
 def exact_act(act, g):
     """The activation of values given in float32: the intermediate roundings are part of its definition."""
     if act == "silu":
-        return (g / (1.0 + torch.exp(-g).float().double()).float().double()).float().double()
-    h = g.half().double()
-    t = torch.tanh(0.7978845608028654 * (h + 0.044715 * h ** 3))
-    t = (h * 0.5 * (1.0 + t)).half().double()
+        return f32(g / f32(1.0 + f32(torch.exp(-g))))
+    h, a, b = g.half().double(), *torch.tensor([0.7978845608028654, 0.044715], device=g.device).double()
+    inner = f32(f32(a * h) * f32(1.0 + f32(f32(b * h) * h)))
+    t = f32(f32(0.5 * h) * f32(1.0 + f32(torch.tanh(inner)))).half().double()
     t = torch.where(g >= 10.0, g, t)
     return torch.where(g <= -10.0, torch.zeros_like(t), t)
 
