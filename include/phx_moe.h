@@ -35,6 +35,7 @@ extern "C" {
 
 /* GgmlType codes of the supported tensors (src/Gguf.cs:18-24). */
 #define PHX_F32 0
+#define PHX_F16 1 /* rows of the int8 and routing entry points (GgmlType's number) */
 #define PHX_Q4_0 2
 #define PHX_Q8_0 8
 #define PHX_Q3_K 11 /* 110 B / 256: hmask, 2-bit q, 16 six-bit scales, d (src/CpuRefIQuants.cs:9, 19-43) */
@@ -47,6 +48,7 @@ extern "C" {
 #define PHX_IQ2_XXS 16
 #define PHX_IQ3_S 21
 #define PHX_IQ2_S 22
+#define PHX_BF16 30 /* as PHX_F16 */
 
 /* Layout limits of the reference (src/KernelsMoe.cs:43, checked at src/GemmaCpu.cs:72-73). */
 #define PHX_MAX_EXPERTS 256
@@ -317,6 +319,86 @@ int phx_matmul(phx_moe_ctx* ctx, const phx_weight* w, int T, const int8_t* xq, c
  * sums, the eight float lanes and their fold); on the matrix cores from 8 rows (Q5_K never), else on the
  * vector units straight from xq and xd (same values); asynchronous on the context's stream. */
 int phx_matmul_k(phx_moe_ctx* ctx, const phx_weight* w, int T, const int8_t* xq, const float* xd, float* y);
+
+/* ---------------------------------------------------------------- routing and int8 products
+ * For models whose router is not softmax over one group, and whose weights are int8 with a scale per
+ * output channel.  The reference has neither (its router is src/GemmaCpu.cs:385-407, its int8 weights
+ * Q8_0 blocks): these stand beside phx_moe_ffn's router, phx_quant_q8_0, phx_matmul and the FFN itself.
+ * Like those they take device pointers (memory the GPU can address: a pageable host pointer returns
+ * PHX_ERR_ARG) and are asynchronous on the context's stream (phx_moe_sync waits); inputs are written, and
+ * outputs free to overwrite, before the call.  An output that shares bytes with an input or another output
+ * returns PHX_ERR_ARG. */
+
+/* How a router's scores become a choice of experts. */
+#define PHX_SCORE_SOFTMAX 0
+#define PHX_SCORE_SIGMOID 1
+#define PHX_GROUP_MAX 0  /* a group's score: its largest selection score */
+#define PHX_GROUP_TOP2 1 /* the sum of its two largest (of its one, where it has but one) */
+#define PHX_MAX_GROUPS 64
+typedef struct phx_route_desc {
+    int32_t n_expert;     /* E, 1 .. PHX_MAX_EXPERTS */
+    int32_t n_used;       /* k, 1 .. PHX_MAX_USED */
+    int32_t score;        /* PHX_SCORE_* */
+    int32_t n_group;      /* consecutive groups of E / n_group experts, 1 .. PHX_MAX_GROUPS (1: no groups) */
+    int32_t n_group_used; /* the groups a token may choose from; they hold at least k experts */
+    int32_t group_score;  /* PHX_GROUP_* */
+    int32_t renorm;       /* 1: a token's weights are divided by their sum */
+    int32_t logits_type;  /* PHX_F32, PHX_F16 or PHX_BF16 */
+    float scale;          /* the weights' factor, finite */
+} phx_route_desc;
+
+/* Validation of a routing descriptor, without touching the GPU: PHX_OK, PHX_ERR_ARG, or PHX_ERR_UNSUPPORTED
+ * for sizes past the limits and unknown types. */
+int phx_route_check(const phx_route_desc* desc);
+
+/* Routing of T rows of logits [T][E] (1 <= T <= 2^20):
+ *   s = softmax(logits[t]) or sigmoid(logits[t]);  c = s + bias (bias [E] f32 or NULL)
+ * keeps the n_group_used groups of largest score, then the k experts of largest c in them, best first, ties to
+ * the lower index throughout; ids [T][k], and weights [T][k] = s of the chosen (not c), divided by their
+ * sum with renorm, times scale.  Scores, sums and comparisons in double, the weights rounded once to
+ * float; without a bias c's order is taken from the logits, of which s is an increasing function.
+ * An expert whose logit or bias is -infinity or NaN is not a candidate of that token and has s = 0 (a NaN
+ * or -infinity bias leaves s as it is); +infinity counts as the largest float.  A token with fewer than k
+ * candidates gets id -1 and weight 0 in the last places.  Weights whose sum is 0 are 0 with renorm. */
+int phx_route(phx_moe_ctx* ctx, const phx_route_desc* desc, int T, const void* logits, const float* bias, int32_t* ids,
+              float* weights);
+
+/* Rows to int8 with one float scale per row, the activations of phx_matmul_i8 and phx_experts_i8: row r's n
+ * values v = x, silu(x) * aux, rmsnorm(x) * aux or gelu(x) * aux (mode PHX_QUANT_*, each value rounded to
+ * float as phx_quant_q8_0 forms it; the norm's sum of squares in double), then
+ *   d[r] = max |v| / 127,  qs[r][i] = roundf(v * (1 / d[r]))   (halves away from zero, within +-127)
+ * A row whose d would be under 2^-126 gets d = 0 and zeros; one that holds a NaN or an infinity gets d = NaN
+ * and zeros.  x: rows x n of x_type (PHX_F32, PHX_F16, PHX_BF16), ld values apart (ld >= n); aux as x with
+ * the gated modes (so gate and up may lie side by side in one buffer), float [n] in PHX_QUANT_RMS_NORM, NULL
+ * in PHX_QUANT_PLAIN.  qs [rows][n], d [rows].  n a multiple of 32, at most 65536; ld a multiple of 8; rows <= 2^24;
+ * x and aux 16-byte, qs 8-byte aligned. */
+int phx_quant_i8(phx_moe_ctx* ctx, int mode, int x_type, const void* x, const void* aux, int rows, int n, int64_t ld,
+                 float eps, int8_t* qs, float* d);
+
+/* int8 matrices to the device, laid out once for the products: n_mat matrices (1 for a dense projection,
+ * n_expert for experts, <= 256) of `rows` rows of `cols`, w [n_mat][rows][cols] and a scale per output
+ * channel, scale [n_mat][rows] (host or device memory, read before the call returns).  cols a multiple of
+ * 32, at most 65536; rows <= 2^20.  paired: the rows are gate (first half) and up of a gated FFN, for
+ * phx_experts_i8 (rows a multiple of 64).  phx_weight_free releases the handle. */
+int phx_weight_upload_i8(phx_moe_ctx* ctx, int n_mat, int rows, int cols, int paired, const int8_t* w,
+                         const float* scale, phx_weight** out);
+
+/* y[t][r] = (float)(sum_i xq[t][i] * w[r][i]) * (xd[t] * scale[r]) for T rows as phx_quant_i8 makes them: the sum
+ * exact in int32, one rounding to float, one for the product of the scales, one for the value, and one more to
+ * y_type (PHX_F32, PHX_F16, PHX_BF16).  w: a handle of one matrix, not paired.  1 <= T <= 2^20; xq 16-byte, y
+ * 16-byte aligned. */
+int phx_matmul_i8(phx_moe_ctx* ctx, const phx_weight* w, int T, const int8_t* xq, const float* xd, int y_type, void* y);
+
+/* The gated FFN of int8 experts for T rows and a routing (phx_route's, or any ids):
+ *   g, u = the products of row t with the gate and up rows of expert e = ids[t][j] (phx_matmul_i8's values)
+ *   h = act(g) * u (PHX_QUANT_SILU_MUL or PHX_QUANT_GELU_MUL), made an int8 row as phx_quant_i8 does
+ *   out[t] = sum over j, in order, of weights[t][j] * (the product of that row with down matrix e)
+ * the sum in float, rounded to out_type at the end.  A place whose id is outside [0, n_expert) is skipped; a
+ * row without experts is zero.  An id may come more than once in a row.  gate_up: paired, [n_expert][2 nf][d]; down:
+ * [n_expert][d][nf]; xq [T][d], xd [T], ids and weights [T][k], out [T][d]; 1 <= T <= 2^20, 1 <= k <= PHX_MAX_USED;
+ * xq and out 16-byte aligned. */
+int phx_experts_i8(phx_moe_ctx* ctx, const phx_weight* gate_up, const phx_weight* down, int act, int T, int k,
+                   const int8_t* xq, const float* xd, const int32_t* ids, const float* weights, int out_type, void* out);
 
 #ifdef __cplusplus
 }

@@ -22,6 +22,7 @@ from .moe import (  # noqa: F401
     OutOfDeviceMemoryError,
     LayerDesc,
     PHX,
+    RouteDesc,
     lib_path,
     load_lib,
 )

@@ -2,6 +2,8 @@
 // sanitizer build, which links this file and gguf.cpp alone.
 #include "../../include/phx_moe.h"
 
+#include <math.h>
+
 namespace {
 bool iq_desc_type(int t) { return t == PHX_IQ2_XXS || t == PHX_IQ2_S || t == PHX_IQ3_S; }
 bool quant_type(int t)
@@ -34,5 +36,20 @@ extern "C" int phx_moe_check_desc(const phx_moe_layer_desc* D)
         if (block_elems(D->shared_type) == 256 && D->n_ff_shared % 256 != 0) return PHX_ERR_UNSUPPORTED;
         if (!D->ffn_norm || !D->ffn_gate || !D->ffn_up || !D->ffn_down) return PHX_ERR_ARG;
     }
+    return PHX_OK;
+}
+
+extern "C" int phx_route_check(const phx_route_desc* R)
+{
+    if (!R) return PHX_ERR_ARG;
+    if (R->n_expert <= 0 || R->n_used <= 0 || R->n_group <= 0 || R->n_group_used <= 0) return PHX_ERR_ARG;
+    if (R->n_expert > PHX_MAX_EXPERTS || R->n_used > PHX_MAX_USED || R->n_group > PHX_MAX_GROUPS) return PHX_ERR_UNSUPPORTED;
+    if (R->n_expert % R->n_group != 0 || R->n_group_used > R->n_group) return PHX_ERR_ARG;
+    if (R->n_used > R->n_group_used * (R->n_expert / R->n_group)) return PHX_ERR_ARG;
+    if (R->score != PHX_SCORE_SOFTMAX && R->score != PHX_SCORE_SIGMOID) return PHX_ERR_ARG;
+    if (R->group_score != PHX_GROUP_MAX && R->group_score != PHX_GROUP_TOP2) return PHX_ERR_ARG;
+    if (R->renorm != 0 && R->renorm != 1) return PHX_ERR_ARG;
+    if (R->logits_type != PHX_F32 && R->logits_type != PHX_F16 && R->logits_type != PHX_BF16) return PHX_ERR_UNSUPPORTED;
+    if (!isfinite(R->scale)) return PHX_ERR_ARG;
     return PHX_OK;
 }

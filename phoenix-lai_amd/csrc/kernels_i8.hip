@@ -1,0 +1,347 @@
+// int8 products with a scale per token and per output channel (phx_quant_i8, phx_matmul_i8, phx_experts_i8).
+#include <algorithm>
+
+#include "device_common.h"
+#include "rows_io.h"
+
+namespace phx {
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x16 __attribute__((ext_vector_type(16)));
+
+// ------------------------------------------------------------------------------ rows to int8
+// d = max |v| / 127, q = roundf(v * (1 / d)); a row whose d is under 2^-126 is zeros with d = 0, one that holds a NaN
+// or an infinity zeros with d = NaN.  |v| compared as integers: a NaN or an infinity is then above every number.
+struct RowScale { float d, inv; };
+__device__ __forceinline__ RowScale row_scale(unsigned amax_bits)
+{
+    if (amax_bits >= 0x7F800000u) return {__uint_as_float(0x7FC00000u), 0.0f};
+    const float d = __uint_as_float(amax_bits) / 127.0f;
+    if (!(d >= 1.17549435e-38f)) return {0.0f, 0.0f};
+    return {d, 1.0f / d};
+}
+__device__ __forceinline__ int quant_one(float v, float inv)
+{
+    const float q = fminf(fmaxf(roundf(v * inv), -127.0f), 127.0f);
+    return inv == 0.0f ? 0 : (int)q;
+}
+__device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d)
+{
+    return (uint32_t)(a & 0xFF) | ((uint32_t)(b & 0xFF) << 8) | ((uint32_t)(c & 0xFF) << 16) | ((uint32_t)d << 24);
+}
+__device__ __forceinline__ float silu_ref(float v) { return v / (1.0f + (float)exp(-(double)v)); }
+
+// One workgroup per row, eight consecutive values per thread and step, the row held in registers between its
+// statistics and its integers: one pass over memory.
+template <int NT, int STEPS, int MODE, int DT>
+__global__ __launch_bounds__(NT) void k_quant_i8(int n, int64_t ld, float eps, const void* __restrict__ x,
+                                                 const void* __restrict__ aux, const float* __restrict__ tab,
+                                                 int8_t* __restrict__ qs, float* __restrict__ d)
+{
+    __shared__ double red[NT / 64];
+    __shared__ unsigned redu[NT / 64];
+    const int64_t row = blockIdx.x;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    float v[STEPS][8];
+#pragma unroll
+    for (int s = 0; s < STEPS; s++) {
+        const int i = (s * NT + tid) * 8;
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[s][j] = 0.0f;
+        if (i < n) load_eight<DT>(x, row * ld + i, v[s]);
+    }
+    float scale = 0.0f;
+    if (MODE == PHX_QUANT_RMS_NORM) {
+        double sum = 0.0;
+#pragma unroll
+        for (int s = 0; s < STEPS; s++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) sum += (double)v[s][j] * (double)v[s][j];
+        sum = wave_sum_dpp(sum);
+        if (lane == 0) red[wave] = sum;
+        __syncthreads();
+        sum = 0.0;
+        for (int w = 0; w < NT / 64; w++) sum += red[w];
+        scale = rms_scale_from_mean((float)(sum / (double)n), eps);
+    }
+    unsigned am = 0;
+#pragma unroll
+    for (int s = 0; s < STEPS; s++) {
+        const int i = (s * NT + tid) * 8;
+        if (MODE != PHX_QUANT_PLAIN && i < n) {
+            float a[8];
+            if (MODE == PHX_QUANT_RMS_NORM) load_eight<PHX_F32>(aux, i, a);
+            else load_eight<DT>(aux, row * ld + i, a);
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float u = v[s][j];
+                v[s][j] = MODE == PHX_QUANT_RMS_NORM ? u * scale * a[j] : MODE == PHX_QUANT_SILU_MUL ? silu_ref(u) * a[j]
+                                                                                                   : gelu_ref(u, tab) * a[j];
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; j++) am = max(am, __float_as_uint(v[s][j]) & 0x7FFFFFFFu);
+    }
+    am = wave_max_u32(am);
+    if (lane == 0) redu[wave] = am;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < NT / 64; w++) am = max(am, redu[w]);
+    const RowScale rs = row_scale(am);
+    if (tid == 0) d[row] = rs.d;
+#pragma unroll
+    for (int s = 0; s < STEPS; s++) {
+        const int i = (s * NT + tid) * 8;
+        if (i >= n) continue;
+        int q[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) q[j] = quant_one(v[s][j], rs.inv);
+        *(uint2*)(qs + row * n + i) = make_uint2(pack4(q[0], q[1], q[2], q[3]), pack4(q[4], q[5], q[6], q[7]));
+    }
+}
+
+template <int MODE, int DT>
+static void quant_rows(hipStream_t st, int rows, int n, int64_t ld, float eps, const void* x, const void* aux,
+                       const float* tab, int8_t* qs, float* d)
+{
+    if (n <= 2048) launch(k_quant_i8<256, 1, MODE, DT>, dim3(rows), dim3(256), 0, st, n, ld, eps, x, aux, tab, qs, d);
+    else if (n <= 8192) launch(k_quant_i8<512, 2, MODE, DT>, dim3(rows), dim3(512), 0, st, n, ld, eps, x, aux, tab, qs, d);
+    else launch(k_quant_i8<1024, 8, MODE, DT>, dim3(rows), dim3(1024), 0, st, n, ld, eps, x, aux, tab, qs, d);
+}
+
+template <int DT>
+static void quant_mode(hipStream_t st, int mode, int rows, int n, int64_t ld, float eps, const void* x, const void* aux,
+                       const float* tab, int8_t* qs, float* d)
+{
+    switch (mode) {
+    case PHX_QUANT_SILU_MUL: quant_rows<PHX_QUANT_SILU_MUL, DT>(st, rows, n, ld, eps, x, aux, tab, qs, d); break;
+    case PHX_QUANT_RMS_NORM: quant_rows<PHX_QUANT_RMS_NORM, DT>(st, rows, n, ld, eps, x, aux, tab, qs, d); break;
+    case PHX_QUANT_GELU_MUL: quant_rows<PHX_QUANT_GELU_MUL, DT>(st, rows, n, ld, eps, x, aux, tab, qs, d); break;
+    default: quant_rows<PHX_QUANT_PLAIN, DT>(st, rows, n, ld, eps, x, aux, tab, qs, d);
+    }
+}
+
+void launch_quant_i8(hipStream_t st, int mode, int type, int rows, int n, int64_t ld, float eps, const void* x,
+                     const void* aux, const float* tab, int8_t* qs, float* d)
+{
+    switch (type) {
+    case PHX_F16: quant_mode<PHX_F16>(st, mode, rows, n, ld, eps, x, aux, tab, qs, d); break;
+    case PHX_BF16: quant_mode<PHX_BF16>(st, mode, rows, n, ld, eps, x, aux, tab, qs, d); break;
+    default: quant_mode<PHX_F32>(st, mode, rows, n, ld, eps, x, aux, tab, qs, d);
+    }
+}
+
+// ------------------------------------------------------------------------------ weights
+// I8Mat's layout from matrices as the caller holds them: a thread writes 16 columns of one stored row, zeros past the
+// last row or column.
+__global__ __launch_bounds__(256) void k_i8_pack(I8Mat m, int m0, int64_t n16, const int8_t* __restrict__ w,
+                                                 const float* __restrict__ scale)
+{
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n16) return;
+    const int s32 = (int)(i & 31), kc = (int)((i >> 5) % m.kc);
+    const int64_t g = (i >> 5) / m.kc;  // 32-row group over the matrices from m0
+    const int rg = (int)(g % m.rg), mi = (int)(g / m.rg);
+    const int half = m.rows / 2;
+    int r = rg * 32 + s32;
+    if (m.paired) r = (rg >> 1) * 32 + s32 + (rg & 1) * half;
+    const bool live = r < m.rows && (!m.paired || (rg >> 1) * 32 + s32 < half);
+    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+    if (live && kc * 16 < m.cols) {
+        const int8_t* p = w + ((int64_t)mi * m.rows + r) * m.cols + kc * 16;
+        if (((uintptr_t)w & 15) == 0) v = *(const uint4*)p;
+        else {
+            uint32_t u[4];
+            for (int j = 0; j < 4; j++) u[j] = pack4(p[4 * j], p[4 * j + 1], p[4 * j + 2], p[4 * j + 3]);
+            v = make_uint4(u[0], u[1], u[2], u[3]);
+        }
+    }
+    *(uint4*)(m.w + (int64_t)m0 * m.mat_bytes() + i * 16) = v;
+    if (kc == 0) m.scale[((int64_t)m0 * m.rg + g) * 32 + s32] = live ? scale[(int64_t)mi * m.rows + r] : 0.0f;
+}
+
+void launch_i8_pack(hipStream_t st, const I8Mat& m, int m0, int n_mat, const int8_t* w, const float* scale)
+{
+    const int64_t n16 = (int64_t)n_mat * m.mat_bytes() / 16;
+    launch(k_i8_pack, dim3((unsigned)((n16 + 255) / 256)), dim3(256), 0, st, m, m0, n16, w, scale);
+}
+
+// ------------------------------------------------------------------------------ products
+// The tile of a workgroup: cnt rows of one matrix, the rows list places start .. start + cnt - 1 (or those rows
+// themselves for a dense product).  False past the last tile.
+__device__ __forceinline__ bool i8_tile(const I8Args& g, int tile, Tile* tl)
+{
+    if (!g.tiles) {
+        tl->e = 0;
+        tl->start = tile * g.cap;
+        tl->cnt = min(g.cap, g.nrows - tl->start);
+        return tl->cnt > 0;
+    }
+    if (tile >= *g.ntiles) return false;
+    *tl = g.tiles[tile];
+    return true;
+}
+
+// h = act(gate) * up as phx_quant_i8 forms it
+__device__ __forceinline__ float gated(const I8Args& g, float gate, float up)
+{
+    return (g.act == PHX_QUANT_SILU_MUL ? silu_ref(gate) : gelu_ref(gate, g.tab)) * up;
+}
+
+// v_mfma_i32_32x32x32_i8: lane l holds 16 bytes of A row l % 32 and of B row l % 32, both at k = 16 (l / 32); the
+// result D[i][j] sits in lane j + 32 ((i / 4) % 2), register 4 (i / 8) + i % 4.  Tokens are A, weight rows B, so a
+// register's 32 lanes store 32 consecutive outputs of one token.
+//
+// k_i8_rows: a workgroup of NW waves takes 32 weight rows (PAIRED: 32 channels, 64 rows) and a tile of up to 32 tokens; the
+// waves split the reduction, and their int32 sums meet in LDS (exact in any order).
+template <int NW, bool PAIRED, int DT>
+__global__ __launch_bounds__(64 * NW) void k_i8_rows(I8Args g)
+{
+    constexpr int NB = PAIRED ? 2 : 1;
+    __shared__ int red[NW][NB][16][64];
+    Tile tl;
+    if (!i8_tile(g, blockIdx.y, &tl)) return;  // uniform over the workgroup
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r32 = lane & 31, h = lane >> 5;
+    const int at = tl.start + min(r32, tl.cnt - 1);
+    const int64_t arow = g.perm ? g.perm[at] / g.div : at;
+    const int8_t* xr = g.xq + arow * g.cols;
+    const int8_t* wr = g.w + (int64_t)tl.e * g.mat_bytes + (int64_t)blockIdx.x * NB * g.kc * 512 + lane * 16;
+    i32x16 acc[NB];
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+        for (int v = 0; v < 16; v++) acc[b][v] = 0;
+    const int steps = g.kc / 2, s0 = wave * steps / NW, s1 = (wave + 1) * steps / NW;
+    for (int s = s0; s < s1; s++) {
+        const int k = 32 * s + 16 * h;
+        const i32x4 a = *(const i32x4*)(xr + (k < g.cols ? k : 0));  // the weights past cols are zero
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            const i32x4 w = *(const i32x4*)(wr + (int64_t)b * g.kc * 512 + (int64_t)s * 1024);
+            acc[b] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a, w, acc[b], 0, 0, 0);
+        }
+    }
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+        for (int v = 0; v < 16; v++) red[wave][b][v][lane] = acc[b][v];
+    __syncthreads();
+    for (int o = tid; o < 16 * 64; o += 64 * NW) {
+        const int v = o >> 6, l = o & 63, tok = 8 * (v >> 2) + 4 * (l >> 5) + (v & 3);
+        if (tok >= tl.cnt) continue;
+        int sum[NB];
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            sum[b] = 0;
+#pragma unroll
+            for (int w = 0; w < NW; w++) sum[b] += red[w][b][v][l];
+        }
+        const int64_t a = g.perm ? g.perm[tl.start + tok] : tl.start + tok;
+        const float dx = g.xd[g.perm ? a / g.div : a];
+        const float* sc = g.scale + (int64_t)tl.e * g.mat_scales + blockIdx.x * NB * 32 + (l & 31);
+        const int col = blockIdx.x * 32 + (l & 31);
+        if (col >= g.out_cols) continue;
+        float y = (float)sum[0] * (dx * sc[0]);
+        if (PAIRED) y = gated(g, y, (float)sum[NB - 1] * (dx * sc[32]));
+        store_one<DT>(g.out, a * g.out_cols + col, y);
+    }
+}
+
+void launch_i8_product(hipStream_t st, const I8Mat& m, I8Args g, int max_tiles, int out_type)
+{
+    g.w = m.w;
+    g.scale = m.scale;
+    g.mat_bytes = m.mat_bytes();
+    g.mat_scales = (int64_t)m.rg * 32;
+    g.kc = m.kc;
+    g.cols = m.cols;
+    g.out_cols = m.paired ? m.rows / 2 : m.rows;
+    const dim3 grid(m.paired ? m.rg / 2 : m.rg, max_tiles), blk(256);
+    if (m.paired) launch(k_i8_rows<4, true, PHX_F32>, grid, blk, 0, st, g);
+    else if (out_type == PHX_F16) launch(k_i8_rows<4, false, PHX_F16>, grid, blk, 0, st, g);
+    else if (out_type == PHX_BF16) launch(k_i8_rows<4, false, PHX_BF16>, grid, blk, 0, st, g);
+    else launch(k_i8_rows<4, false, PHX_F32>, grid, blk, 0, st, g);
+}
+
+// ------------------------------------------------------------------------------ experts
+// Each expert's assignments as one run of perm and as tiles of up to cap; ids outside [0, E) are in no run.  The order
+// inside a run is the atomics' and no result depends on it: a place of the list names its own input and output row.
+__global__ __launch_bounds__(1024) void k_i8_lists(int n, int E, int cap, const int* __restrict__ ids, int* __restrict__ perm,
+                                                   Tile* __restrict__ tiles, int* __restrict__ ntiles)
+{
+    __shared__ int count[PHX_MAX_EXPERTS_DEV], start[PHX_MAX_EXPERTS_DEV], first[PHX_MAX_EXPERTS_DEV];
+    const int tid = threadIdx.x;
+    if (tid < PHX_MAX_EXPERTS_DEV) count[tid] = 0;
+    __syncthreads();
+    for (int a = tid; a < n; a += 1024) {
+        const int e = ids[a];
+        if ((unsigned)e < (unsigned)E) atomicAdd(&count[e], 1);
+    }
+    __syncthreads();
+    if (tid < 64) {  // prefix sums over the experts, four to a lane
+        int c[4], t[4], sc = 0, stl = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            c[i] = count[4 * tid + i];
+            t[i] = (c[i] + cap - 1) / cap;
+            sc += c[i];
+            stl += t[i];
+        }
+        int pc = wave_incl_scan_i(sc) - sc, pt = wave_incl_scan_i(stl) - stl;
+        if (tid == 63) *ntiles = pt + stl;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            start[4 * tid + i] = pc;
+            first[4 * tid + i] = pt;
+            pc += c[i];
+            pt += t[i];
+        }
+    }
+    __syncthreads();
+    if (tid < E) {
+        int at = start[tid], left = count[tid];
+        for (int i = first[tid]; left > 0; i++, at += cap, left -= cap) tiles[i] = {tid, at, min(cap, left)};
+    }
+    __syncthreads();
+    for (int a = tid; a < n; a += 1024) {
+        const int e = ids[a];
+        if ((unsigned)e < (unsigned)E) perm[atomicAdd(&start[e], 1)] = a;
+    }
+}
+
+void launch_i8_lists(hipStream_t st, int n, int E, int cap, const int* ids, int* perm, Tile* tiles, int* ntiles)
+{
+    launch(k_i8_lists, dim3(1), dim3(1024), 0, st, n, E, cap, ids, perm, tiles, ntiles);
+}
+
+// out[t] = sum over the places j, in order, of w[t][j] * y[t k + j]; places without an expert are skipped
+template <int DT>
+__global__ __launch_bounds__(256) void k_i8_combine(int d, int k, int E, const float* __restrict__ y, const int* __restrict__ ids,
+                                                    const float* __restrict__ w, void* __restrict__ out)
+{
+    const int64_t t = blockIdx.y;
+    const int c = (blockIdx.x * 256 + threadIdx.x) * 4;
+    if (c >= d) return;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int j = 0; j < k; j++) {
+        if ((unsigned)ids[t * k + j] >= (unsigned)E) continue;  // uniform
+        const float wj = w[t * k + j];
+        const float4 v = *(const float4*)(y + (t * k + j) * d + c);
+        acc.x += v.x * wj;
+        acc.y += v.y * wj;
+        acc.z += v.z * wj;
+        acc.w += v.w * wj;
+    }
+    store_four<DT>(out, t * d + c, acc);
+}
+
+void launch_i8_combine(hipStream_t st, int T, int d, int k, int E, const float* y, const int* ids, const float* w, int out_type,
+                       void* out)
+{
+    const dim3 grid((d + 1023) / 1024, T), blk(256);
+    if (out_type == PHX_F16) launch(k_i8_combine<PHX_F16>, grid, blk, 0, st, d, k, E, y, ids, w, out);
+    else if (out_type == PHX_BF16) launch(k_i8_combine<PHX_BF16>, grid, blk, 0, st, d, k, E, y, ids, w, out);
+    else launch(k_i8_combine<PHX_F32>, grid, blk, 0, st, d, k, E, y, ids, w, out);
+}
+
+}  // namespace phx

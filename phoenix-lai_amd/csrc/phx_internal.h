@@ -277,4 +277,48 @@ void launch_planar_act_k(hipStream_t st, int rows, int n, const int8_t* qs, cons
 void launch_selftest(hipStream_t st, int op, int n, const float* a, const float* b, float* out, const float* gelu_tab);
 void launch_selftest_seq(hipStream_t st, int m, int rows, const float* a, float* out);
 
+
+// ---- routing and int8 products (kernels_route.hip, kernels_i8.hip)
+void launch_route(hipStream_t st, const phx_route_desc& D, int T, const void* logits, const float* bias, int* ids, float* w);
+void launch_quant_i8(hipStream_t st, int mode, int type, int rows, int n, int64_t ld, float eps, const void* x,
+                     const void* aux, const float* tab, int8_t* qs, float* d);
+
+// int8 matrices on the device: groups of 32 stored rows, each [kc][32 rows][16 bytes] with kc = columns / 16 (padded to
+// whole 128-column steps with zeros), so the 16-byte operand of every lane of a 32 x 32 x 32 matrix product is one
+// run of 1 KB.  Stored rows are the matrix's in order, padded with zeros to whole groups; paired, group 2 g holds gate
+// rows 32 g .. + 31 and group 2 g + 1 the up rows of the same channels.  Scales [n_mat][rg][32] in stored order.
+struct I8Mat {
+    int n_mat = 0, rows = 0, cols = 0;
+    bool paired = false;
+    int rg = 0, kc = 0;
+    int8_t* w = nullptr;
+    float* scale = nullptr;
+    __host__ __device__ int64_t mat_bytes() const { return (int64_t)rg * kc * 512; }
+};
+// matrices m0 .. m0 + n_mat - 1 of m from w / scale (device-readable)
+void launch_i8_pack(hipStream_t st, const I8Mat& m, int m0, int n_mat, const int8_t* w, const float* scale);
+
+struct I8Args {
+    // set by the caller: input rows and scales, the tiles and lists of a grouped product (perm's value / div is the input
+    // row, perm's value the output row) or nrows of a dense one in tiles of cap, the output and the activation
+    const int8_t* xq;
+    const float* xd;
+    const Tile* tiles = nullptr;
+    const int* ntiles = nullptr;
+    const int* perm = nullptr;
+    int div = 1, nrows = 0, cap = 32, act = 0;
+    const float* tab = nullptr;
+    void* out;
+    // set by launch_i8_product from the matrix
+    const int8_t* w;
+    const float* scale;
+    int64_t mat_bytes, mat_scales;
+    int kc, cols, out_cols;
+};
+// paired matrices write act(gate) * up as float, the others the product as out_type
+void launch_i8_product(hipStream_t st, const I8Mat& m, I8Args g, int max_tiles, int out_type);
+void launch_i8_lists(hipStream_t st, int n, int E, int cap, const int* ids, int* perm, Tile* tiles, int* ntiles);
+void launch_i8_combine(hipStream_t st, int T, int d, int k, int E, const float* y, const int* ids, const float* w, int out_type,
+                       void* out);
+
 }  // namespace phx

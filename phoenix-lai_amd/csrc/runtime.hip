@@ -10,7 +10,9 @@
 
 #include <algorithm>
 #include <chrono>
+#include <initializer_list>
 #include <mutex>
+#include <new>
 #include <string>
 #include <thread>
 #include <vector>
@@ -431,6 +433,8 @@ struct phx_moe_ctx {
     };
     std::vector<FfnGraph> ffn_graphs;
     uint64_t upload_gen = 0;
+    // workspace of the int8 experts (I8Ws): a table of its own, which no captured graph names
+    std::vector<Buf> ws_i8;
 };
 
 namespace {
@@ -1240,9 +1244,11 @@ int drain_profile(phx_moe_ctx* c)
 }  // namespace
 
 // One dense quantized matrix on the device (GemmaGpu's GW, src/GemmaGpu.cs:344-352), repacked into row
-// groups like the experts, for phx_matmul.
+// groups like the experts, for phx_matmul; or the int8 matrices of phx_weight_upload_i8 (type PHX_I8_WEIGHT, the
+// other fields in i8).
 struct phx_weight {
     QMat q;
+    I8Mat i8;
     int type = 0, rows = 0, cols = 0;
 };
 
@@ -1382,6 +1388,8 @@ void phx_moe_destroy(phx_moe_ctx* c)
     if (c->pin) (void)hipHostFree(c->pin);
     for (auto& L : c->layers) free_layer(L);
     for (auto& b : c->ws)
+        if (b.p) (void)hipFree(b.p);
+    for (auto& b : c->ws_i8)
         if (b.p) (void)hipFree(b.p);
     for (auto& p : c->pending) {
         (void)hipEventDestroy(p.a);
@@ -2069,6 +2077,8 @@ void phx_weight_free(phx_moe_ctx* c, phx_weight* w)
         (void)hipStreamSynchronize(c->stream);
     }
     free_qmat(w->q);
+    if (w->i8.w) (void)hipFree(w->i8.w);
+    if (w->i8.scale) (void)hipFree(w->i8.scale);
     delete w;
 }
 
@@ -2221,3 +2231,253 @@ int phx_matvec(phx_moe_ctx* c, int type, const void* w, int rows, int cols, int 
 }
 
 }  // extern "C"
+
+// ---------------------------------------------------------------------------- routing and int8 products
+
+namespace {
+constexpr int PHX_I8_WEIGHT = 24;  // GgmlType's int8
+constexpr int kMaxRowsI8 = 1 << 20;
+
+// A buffer of a device-pointer call: what it is, its bytes, its alignment, and whether the call writes it.
+struct CallBuf {
+    const char* what;
+    const void* p;
+    int64_t bytes;
+    int align;
+    bool out;
+};
+
+// Present, aligned, addressable by the GPU, and no output in any other buffer's bytes.
+int check_bufs(phx_moe_ctx* c, const char* call, std::initializer_list<CallBuf> bufs)
+{
+    for (const CallBuf& b : bufs) {
+        if (!b.p) return set_err(c, PHX_ERR_ARG, "%s: null %s", call, b.what);
+        if ((uintptr_t)b.p % b.align) return set_err(c, PHX_ERR_ARG, "%s: %s needs %d-byte alignment", call, b.what, b.align);
+        if (!device_accessible(b.p)) return set_err(c, PHX_ERR_ARG, "%s: %s is not device-accessible memory", call, b.what);
+    }
+    for (const CallBuf& o : bufs)
+        for (const CallBuf& b : bufs)
+            if (o.out && &o != &b && (uintptr_t)o.p < (uintptr_t)b.p + b.bytes && (uintptr_t)b.p < (uintptr_t)o.p + o.bytes)
+                return set_err(c, PHX_ERR_ARG, "%s: %s overlaps %s", call, o.what, b.what);
+    return PHX_OK;
+}
+
+int elem_bytes(int type) { return type == PHX_F32 ? 4 : type == PHX_F16 || type == PHX_BF16 ? 2 : 0; }
+
+enum I8Ws { I8_PERM, I8_TILES, I8_NTILES, I8_H, I8_HQ, I8_HD, I8_Y, I8_WS_COUNT };
+
+template <class T>
+int i8_ensure(phx_moe_ctx* c, int id, int64_t n, T** out)
+{
+    if (c->ws_i8.empty()) c->ws_i8.resize(I8_WS_COUNT);
+    Buf& b = c->ws_i8[id];
+    const size_t bytes = std::max<size_t>((size_t)n * sizeof(T), 256);
+    if (b.bytes < bytes) {
+        if (b.p) {
+            HIPCHK(c, hipStreamSynchronize(c->stream));  // an earlier call may still use it
+            HIPCHK(c, hipFree(b.p));
+        }
+        b = Buf{};
+        HIPCHK(c, dev_malloc(c, &b.p, bytes));
+        b.bytes = bytes;
+    }
+    *out = (T*)b.p;
+    return PHX_OK;
+}
+}  // namespace
+
+int phx_route(phx_moe_ctx* c, const phx_route_desc* R, int T, const void* logits, const float* bias, int32_t* ids, float* weights)
+{
+    if (!c) return PHX_ERR_ARG;
+    if (const int rc = phx_route_check(R)) return set_err(c, rc, "route: descriptor refused (phx_route_check)");
+    if (T <= 0 || T > kMaxRowsI8) return set_err(c, PHX_ERR_ARG, "route: T=%d out of range", T);
+    const int eb = elem_bytes(R->logits_type);
+    const int64_t n = (int64_t)T * R->n_used * 4;
+    const CallBuf lo{"logits", logits, (int64_t)T * R->n_expert * eb, eb, false}, id{"ids", ids, n, 4, true},
+        we{"weights", weights, n, 4, true};
+    ENTER(c);
+    const int rc = bias ? check_bufs(c, "route", {lo, id, we, {"bias", bias, R->n_expert * 4ll, 4, false}})
+                        : check_bufs(c, "route", {lo, id, we});
+    if (rc) return rc;
+    launch_route(c->stream, *R, T, logits, bias, ids, weights);
+    HIPCHK(c, launch_status(c));
+    return PHX_OK;
+}
+
+int phx_quant_i8(phx_moe_ctx* c, int mode, int x_type, const void* x, const void* aux, int rows, int n, int64_t ld, float eps,
+                 int8_t* qs, float* d)
+{
+    if (!c) return PHX_ERR_ARG;
+    const int eb = elem_bytes(x_type);
+    if (!eb) return set_err(c, PHX_ERR_UNSUPPORTED, "quant_i8: type %d (PHX_F32, PHX_F16 and PHX_BF16 only)", x_type);
+    if (mode < PHX_QUANT_PLAIN || mode > PHX_QUANT_GELU_MUL) return set_err(c, PHX_ERR_ARG, "quant_i8: mode %d", mode);
+    if (rows <= 0 || rows > kMaxRowsI8 || n <= 0 || n % 32 || n > 65536 || ld < n || ld % 8 || ld > (int64_t)1 << 40)
+        return set_err(c, PHX_ERR_ARG, "quant_i8: %d rows of %d, %lld apart (n a multiple of 32, <= 65536; ld of 8, >= n)", rows,
+                       n, (long long)ld);
+    if (mode == PHX_QUANT_RMS_NORM && !(eps >= 0.0f)) return set_err(c, PHX_ERR_ARG, "quant_i8: eps");
+    const int64_t span = ((rows - 1) * ld + n) * eb;
+    const CallBuf bx{"x", x, span, 16, false}, bq{"qs", qs, (int64_t)rows * n, 8, true}, bd{"d", d, rows * 4ll, 4, true};
+    ENTER(c);
+    const int rc = mode == PHX_QUANT_PLAIN
+                       ? check_bufs(c, "quant_i8", {bx, bq, bd})
+                       : check_bufs(c, "quant_i8", {bx, bq, bd, {"aux", aux, mode == PHX_QUANT_RMS_NORM ? n * 4ll : span, 16, false}});
+    if (rc) return rc;
+    launch_quant_i8(c->stream, mode, x_type, rows, n, ld, eps, x, aux, c->gelu_tab, qs, d);
+    HIPCHK(c, launch_status(c));
+    return PHX_OK;
+}
+
+namespace {
+int upload_i8(phx_moe_ctx* c, I8Mat& m, const int8_t* w, const float* scale)
+{
+    const int64_t src = (int64_t)m.rows * m.cols;
+    const bool dev_w = device_accessible(w), dev_s = device_accessible(scale);
+    HIPCHK(c, dev_malloc(c, (void**)&m.w, (size_t)(m.n_mat * m.mat_bytes())));
+    HIPCHK(c, dev_malloc(c, (void**)&m.scale, (size_t)m.n_mat * m.rg * 32 * 4));
+    // host matrices go through a buffer of one of them
+    struct Staging {
+        void* p = nullptr;
+        ~Staging()
+        {
+            if (p) (void)hipFree(p);
+        }
+    } sw, ss;
+    if (!dev_w) HIPCHK(c, dev_malloc(c, &sw.p, (size_t)src));
+    if (!dev_s) HIPCHK(c, dev_malloc(c, &ss.p, (size_t)m.rows * 4));
+    for (int i = 0; i < m.n_mat; i++) {
+        const int8_t* wi = w + i * src;
+        const float* si = scale + (int64_t)i * m.rows;
+        if (!dev_w) {
+            HIPCHK(c, hipMemcpyAsync(sw.p, wi, (size_t)src, hipMemcpyHostToDevice, c->stream));
+            wi = (const int8_t*)sw.p;
+        }
+        if (!dev_s) {
+            HIPCHK(c, hipMemcpyAsync(ss.p, si, (size_t)m.rows * 4, hipMemcpyHostToDevice, c->stream));
+            si = (const float*)ss.p;
+        }
+        launch_i8_pack(c->stream, m, i, 1, wi, si);
+    }
+    HIPCHK(c, launch_status(c));
+    HIPCHK(c, hipStreamSynchronize(c->stream));
+    return PHX_OK;
+}
+}  // namespace
+
+int phx_weight_upload_i8(phx_moe_ctx* c, int n_mat, int rows, int cols, int paired, const int8_t* w, const float* scale,
+                         phx_weight** out)
+{
+    if (!c || !out) return PHX_ERR_ARG;
+    *out = nullptr;
+    if (n_mat <= 0 || n_mat > PHX_MAX_EXPERTS || rows <= 0 || rows > kMaxRowsI8 || cols <= 0 || cols % 32 || cols > 65536 ||
+        (int64_t)rows * cols > (int64_t)1 << 34 || (paired && rows % 64) || !w || !scale || (uintptr_t)scale % 4)
+        return set_err(c, PHX_ERR_ARG, "weight upload: %d int8 matrices of %d x %d (cols a multiple of 32, <= 65536)", n_mat, rows,
+                       cols);
+    ENTER(c);
+    phx_weight* h = new (std::nothrow) phx_weight();
+    if (!h) return set_err(c, PHX_ERR_OOM, "weight upload: host memory");
+    h->type = PHX_I8_WEIGHT;
+    h->rows = rows;
+    h->cols = cols;
+    I8Mat& m = h->i8;
+    m.n_mat = n_mat;
+    m.rows = rows;
+    m.cols = cols;
+    m.paired = paired != 0;
+    m.rg = (rows + 31) / 32;
+    m.kc = (cols + 127) / 128 * 8;
+    const int rc = upload_i8(c, m, w, scale);
+    if (rc) {
+        phx_weight_free(c, h);
+        return rc;
+    }
+    *out = h;
+    return PHX_OK;
+}
+
+int phx_matmul_i8(phx_moe_ctx* c, const phx_weight* w, int T, const int8_t* xq, const float* xd, int y_type, void* y)
+{
+    if (!c) return PHX_ERR_ARG;
+    if (!w) return set_err(c, PHX_ERR_ARG, "matmul_i8: null weight");
+    if (w->type != PHX_I8_WEIGHT || w->i8.paired || w->i8.n_mat != 1)
+        return set_err(c, PHX_ERR_UNSUPPORTED, "matmul_i8: the weight is not one plain int8 matrix (phx_weight_upload_i8)");
+    const int eb = elem_bytes(y_type);
+    if (!eb) return set_err(c, PHX_ERR_UNSUPPORTED, "matmul_i8: type %d (PHX_F32, PHX_F16 and PHX_BF16 only)", y_type);
+    if (T <= 0 || T > kMaxRowsI8) return set_err(c, PHX_ERR_ARG, "matmul_i8: T=%d out of range", T);
+    ENTER(c);
+    if (const int rc = check_bufs(c, "matmul_i8", {{"xq", xq, (int64_t)T * w->cols, 16, false},
+                                                   {"xd", xd, T * 4ll, 4, false},
+                                                   {"y", y, (int64_t)T * w->rows * eb, 16, true}}))
+        return rc;
+    I8Args g{};
+    g.xq = xq;
+    g.xd = xd;
+    g.nrows = T;
+    g.cap = 32;
+    g.out = y;
+    launch_i8_product(c->stream, w->i8, g, (T + 31) / 32, y_type);
+    HIPCHK(c, launch_status(c));
+    return PHX_OK;
+}
+
+int phx_experts_i8(phx_moe_ctx* c, const phx_weight* gu, const phx_weight* dn, int act, int T, int k, const int8_t* xq,
+                   const float* xd, const int32_t* ids, const float* weights, int out_type, void* out)
+{
+    if (!c) return PHX_ERR_ARG;
+    if (!gu || !dn) return set_err(c, PHX_ERR_ARG, "experts_i8: null weight");
+    if (gu->type != PHX_I8_WEIGHT || !gu->i8.paired || dn->type != PHX_I8_WEIGHT || dn->i8.paired)
+        return set_err(c, PHX_ERR_UNSUPPORTED, "experts_i8: takes a paired int8 gate_up and a plain int8 down");
+    const int E = gu->i8.n_mat, d = gu->cols, nf = gu->rows / 2;
+    if (dn->i8.n_mat != E || dn->rows != d || dn->cols != nf)
+        return set_err(c, PHX_ERR_ARG, "experts_i8: gate_up [%d][%d][%d] and down [%d][%d][%d] do not fit", E, gu->rows, d,
+                       dn->i8.n_mat, dn->rows, dn->cols);
+    const int eb = elem_bytes(out_type);
+    if (!eb) return set_err(c, PHX_ERR_UNSUPPORTED, "experts_i8: type %d (PHX_F32, PHX_F16 and PHX_BF16 only)", out_type);
+    if (act != PHX_QUANT_SILU_MUL && act != PHX_QUANT_GELU_MUL) return set_err(c, PHX_ERR_ARG, "experts_i8: act %d", act);
+    if (T <= 0 || T > kMaxRowsI8 || k <= 0 || k > PHX_MAX_USED)
+        return set_err(c, PHX_ERR_ARG, "experts_i8: T=%d, k=%d out of range", T, k);
+    ENTER(c);
+    if (const int rc = check_bufs(c, "experts_i8", {{"xq", xq, (int64_t)T * d, 16, false},
+                                                    {"xd", xd, T * 4ll, 4, false},
+                                                    {"ids", ids, (int64_t)T * k * 4, 4, false},
+                                                    {"weights", weights, (int64_t)T * k * 4, 4, false},
+                                                    {"out", out, (int64_t)T * d * eb, 16, true}}))
+        return rc;
+    // long batches go through in chunks, so that the workspace stays bounded
+    const int chunk = std::min(T, 65535 / k), A = chunk * k, cap = 32, max_tiles = (A + cap - 1) / cap + std::min(E, A);
+    int *perm, *ntiles;
+    Tile* tiles;
+    float *h, *hd, *y;
+    int8_t* hq;
+    int rc;
+    if ((rc = i8_ensure(c, I8_PERM, A, &perm)) || (rc = i8_ensure(c, I8_TILES, max_tiles, &tiles)) ||
+        (rc = i8_ensure(c, I8_NTILES, 1, &ntiles)) || (rc = i8_ensure(c, I8_H, (int64_t)A * nf, &h)) ||
+        (rc = i8_ensure(c, I8_HQ, (int64_t)A * nf, &hq)) || (rc = i8_ensure(c, I8_HD, A, &hd)) ||
+        (rc = i8_ensure(c, I8_Y, (int64_t)A * d, &y)))
+        return rc;
+    hipStream_t st = c->stream;
+    for (int t0 = 0; t0 < T; t0 += chunk) {
+        const int n = std::min(chunk, T - t0);
+        const int32_t* id = ids + (int64_t)t0 * k;
+        launch_i8_lists(st, n * k, E, cap, id, perm, tiles, ntiles);
+        I8Args g{};
+        g.xq = xq + (int64_t)t0 * d;
+        g.xd = xd + t0;
+        g.tiles = tiles;
+        g.ntiles = ntiles;
+        g.perm = perm;
+        g.div = k;
+        g.act = act;
+        g.tab = c->gelu_tab;
+        g.out = h;
+        launch_i8_product(st, gu->i8, g, max_tiles, PHX_F32);
+        launch_quant_i8(st, PHX_QUANT_PLAIN, PHX_F32, n * k, nf, nf, 0.0f, h, nullptr, nullptr, hq, hd);
+        g.xq = hq;
+        g.xd = hd;
+        g.div = 1;
+        g.out = y;
+        launch_i8_product(st, dn->i8, g, max_tiles, PHX_F32);
+        launch_i8_combine(st, n, d, k, E, y, id, weights + (int64_t)t0 * k, out_type, (char*)out + (int64_t)t0 * d * eb);
+    }
+    HIPCHK(c, launch_status(c));
+    return PHX_OK;
+}

@@ -18,6 +18,7 @@ _HERE = Path(__file__).resolve().parent
 class PHX:
     OK, ERR_ARG, ERR_OOM, ERR_UNSUPPORTED, ERR_DEVICE_LOST, ERR_HIP, ERR_FORMAT = 0, -1, -2, -3, -4, -5, -6
     F32, Q4_0, Q8_0, Q3_K, Q4_K, Q5_K, Q6_K, IQ2_XXS, IQ3_S, IQ2_S = 0, 2, 8, 11, 12, 13, 14, 16, 21, 22
+    F16, BF16 = 1, 30
     WEIGHTS_SOFTMAX, WEIGHTS_CPUREF = 0, 1
     FLAG_DEVICE_PTRS, FLAG_ASYNC, FLAG_RESIDUAL, FLAG_EXACT_ROUTER, FLAG_FAST_MATH = 1, 2, 4, 8, 16
     FLAG_KEEP_INTERMEDIATES = 32
@@ -25,6 +26,8 @@ class PHX:
     MAX_EXPERTS, MAX_USED = 256, 16
     # activation quantizer modes (KernelsQuant.Mode, src/KernelsQuant.cs:13)
     QUANT_PLAIN, QUANT_SILU_MUL, QUANT_RMS_NORM, QUANT_GELU_MUL = 0, 1, 2, 3
+    SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
+    GROUP_MAX, GROUP_TOP2, MAX_GROUPS = 0, 1, 64
 
 
 class MoeError(RuntimeError):
@@ -98,6 +101,26 @@ class LayerDesc(C.Structure):
         return d
 
 
+class RouteDesc(C.Structure):
+    """phx_route_desc (include/phx_moe.h): how a router's scores become a choice of experts."""
+
+    _fields_ = [
+        ("n_expert", C.c_int32), ("n_used", C.c_int32), ("score", C.c_int32), ("n_group", C.c_int32),
+        ("n_group_used", C.c_int32), ("group_score", C.c_int32), ("renorm", C.c_int32), ("logits_type", C.c_int32),
+        ("scale", C.c_float),
+    ]
+
+    def __init__(self, n_expert: int, n_used: int, score: int = PHX.SCORE_SOFTMAX, n_group: int = 1, n_group_used: int = 1,
+                 group_score: int = PHX.GROUP_MAX, renorm: int = 1, logits_type: int = PHX.F32, scale: float = 1.0):
+        super().__init__(n_expert, n_used, score, n_group, n_group_used, group_score, renorm, logits_type, scale)
+
+    def check(self):
+        """phx_route_check, raised as the exception of its code."""
+        rc = load_lib().phx_route_check(C.byref(self))
+        if rc:
+            _raise(rc, f"routing of {self.n_used} of {self.n_expert} experts refused")
+
+
 def lib_path() -> Path:
     """libphxmoe.so in the package directory, or the file PHX_MOE_LIB names (an instrumented build)."""
     return Path(os.environ["PHX_MOE_LIB"]) if os.environ.get("PHX_MOE_LIB") else _HERE / "libphxmoe.so"
@@ -149,6 +172,12 @@ def load_lib():
         "phx_weight_free": (None, [vp, vp]),
         "phx_matmul": (i32, [vp, vp, i32, vp, vp, vp]),
         "phx_matmul_k": (i32, [vp, vp, i32, vp, vp, vp]),
+        "phx_route_check": (i32, [C.POINTER(RouteDesc)]),
+        "phx_route": (i32, [vp, C.POINTER(RouteDesc), i32, vp, vp, vp, vp]),
+        "phx_quant_i8": (i32, [vp, i32, i32, vp, vp, i32, i32, C.c_int64, C.c_float, vp, vp]),
+        "phx_weight_upload_i8": (i32, [vp, i32, i32, i32, i32, vp, vp, C.POINTER(vp)]),
+        "phx_matmul_i8": (i32, [vp, vp, i32, vp, vp, i32, vp]),
+        "phx_experts_i8": (i32, [vp, vp, vp, i32, i32, i32, vp, vp, vp, vp, i32, vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
@@ -504,6 +533,116 @@ class MoeContext:
         finally:
             for b in bufs:
                 b.free()
+
+    # ------------------------------------------------------------------ routing and int8 products
+    def _on_device(self, arrays, outputs, call):
+        """call(pointers of device copies of arrays (None stays None), then of buffers of outputs' (shape, dtype)); the
+        outputs downloaded."""
+        bufs = []
+        try:
+            ptrs = []
+            for a in arrays:
+                if a is not None:
+                    bufs.append(self.alloc(max(a.nbytes, 16)))
+                    bufs[-1].upload(a)
+                ptrs.append(None if a is None else bufs[-1].ptr)
+            outs = [self.alloc(max(int(np.prod(s)) * np.dtype(t).itemsize, 16)) for s, t in outputs]
+            bufs += outs
+            call(*ptrs, *(o.ptr for o in outs))
+            self.sync()
+            return tuple(o.download(s, t) for o, (s, t) in zip(outs, outputs))
+        finally:
+            for b in bufs:
+                b.free()
+
+    def route_device(self, desc: RouteDesc, T: int, logits_ptr: int, bias_ptr, ids_ptr: int, weights_ptr: int):
+        """Enqueue phx_route on device buffers (sync() waits)."""
+        self._check(self.lib.phx_route(self.h, desc, T, logits_ptr, bias_ptr, ids_ptr, weights_ptr))
+
+    def Route(self, desc: RouteDesc, logits: np.ndarray, bias: np.ndarray | None = None):
+        """phx_route on host arrays: logits [T][E] (float32, float16, or uint16 holding bf16 bits, as desc.logits_type
+        says), bias [E]; returns (ids [T][k] int32, -1 where a token has too few candidates, weights [T][k] f32)."""
+        desc.check()
+        dtype = {PHX.F32: np.float32, PHX.F16: np.float16, PHX.BF16: np.uint16}[desc.logits_type]
+        logits = np.ascontiguousarray(logits)
+        if logits.dtype != dtype or logits.ndim != 2 or logits.shape[1] != desc.n_expert:
+            raise ArgumentError(PHX.ERR_ARG, f"logits {logits.shape} {logits.dtype} for {desc.n_expert} experts")
+        if bias is not None and (bias := _f32(bias)).size != desc.n_expert:
+            raise ArgumentError(PHX.ERR_ARG, f"bias of {bias.size} values for {desc.n_expert} experts")
+        T, shape = logits.shape[0], (logits.shape[0], desc.n_used)
+        return self._on_device([logits, bias], [(shape, np.int32), (shape, np.float32)],
+                               lambda *p: self.route_device(desc, T, *p))
+
+    def quant_i8_device(self, mode: int, x_type: int, x_ptr: int, aux_ptr, rows: int, n: int, ld: int, eps: float,
+                        qs_ptr: int, d_ptr: int):
+        """Enqueue phx_quant_i8 on device buffers (sync() waits)."""
+        self._check(self.lib.phx_quant_i8(self.h, mode, x_type, x_ptr, aux_ptr, rows, n, ld, eps, qs_ptr, d_ptr))
+
+    def QuantI8(self, mode: int, x: np.ndarray, aux: np.ndarray | None = None, eps: float = 1e-6):
+        """phx_quant_i8 on host arrays: x [rows][n] float32 or float16 (aux alike, or the norm weight [n] f32); returns
+        (qs int8 [rows][n], d f32 [rows])."""
+        x = np.ascontiguousarray(x) if x.dtype == np.float16 else _f32(x)
+        if x.ndim != 2:
+            raise ArgumentError(PHX.ERR_ARG, f"rows of shape {x.shape}")
+        if aux is not None:
+            aux = _f32(aux) if mode == PHX.QUANT_RMS_NORM else np.ascontiguousarray(aux, dtype=x.dtype)
+            if aux.shape != (x.shape[1:] if mode == PHX.QUANT_RMS_NORM else x.shape):
+                raise ArgumentError(PHX.ERR_ARG, f"aux of shape {aux.shape} for rows of shape {x.shape}")
+        rows, n = x.shape
+        return self._on_device(
+            [x, aux], [((rows, n), np.int8), ((rows,), np.float32)],
+            lambda px, pa, pq, pd: self.quant_i8_device(mode, PHX.F32 if x.dtype == np.float32 else PHX.F16, px, pa, rows, n, n,
+                                                        eps, pq, pd))
+
+    def weight_upload_i8(self, n_mat: int, rows: int, cols: int, w, scale, paired: bool = False) -> int:
+        """phx_weight_upload_i8: n_mat int8 matrices [rows][cols] with scales [n_mat][rows] laid out on the device once
+        (paired: gate rows, then up rows); w and scale numpy arrays or addresses (host or device memory).  Returns the
+        handle for matmul_i8_device / experts_i8_device / weight_free."""
+        if isinstance(w, np.ndarray):
+            w = np.ascontiguousarray(w, dtype=np.int8)
+            if w.size != n_mat * rows * cols:
+                raise ArgumentError(PHX.ERR_ARG, f"{w.size} weights for {n_mat} matrices of {rows} x {cols}")
+        if isinstance(scale, np.ndarray):
+            scale = _f32(scale)
+            if scale.size != n_mat * rows:
+                raise ArgumentError(PHX.ERR_ARG, f"{scale.size} scales for {n_mat} matrices of {rows} rows")
+        h = C.c_void_p()
+        at = [a.ctypes.data if isinstance(a, np.ndarray) else a for a in (w, scale)]
+        self._check(self.lib.phx_weight_upload_i8(self.h, n_mat, rows, cols, 1 if paired else 0, *at, C.byref(h)))
+        return h.value
+
+    def matmul_i8_device(self, handle: int, T: int, xq_ptr: int, xd_ptr: int, y_type: int, y_ptr: int):
+        """Enqueue phx_matmul_i8 on device buffers (sync() waits)."""
+        self._check(self.lib.phx_matmul_i8(self.h, handle, T, xq_ptr, xd_ptr, y_type, y_ptr))
+
+    def MatMulI8(self, handle: int, rows: int, cols: int, xq: np.ndarray, xd: np.ndarray) -> np.ndarray:
+        """phx_matmul_i8 on host arrays: y [T][rows] f32 from T int8 rows and their scales (as QuantI8 returns them)."""
+        xq = np.ascontiguousarray(xq, dtype=np.int8)
+        xd = _f32(xd)
+        if cols <= 0 or xq.size % cols or xd.size * cols != xq.size:
+            raise ArgumentError(PHX.ERR_ARG, f"input of {xq.size} quants and {xd.size} scales for {cols} columns")
+        T = xd.size
+        return self._on_device([xq, xd], [((T, rows), np.float32)],
+                               lambda pq, pd, py: self.matmul_i8_device(handle, T, pq, pd, PHX.F32, py))[0]
+
+    def experts_i8_device(self, gate_up: int, down: int, act: int, T: int, k: int, xq_ptr: int, xd_ptr: int, ids_ptr: int,
+                          weights_ptr: int, out_type: int, out_ptr: int):
+        """Enqueue phx_experts_i8 on device buffers (sync() waits)."""
+        self._check(self.lib.phx_experts_i8(self.h, gate_up, down, act, T, k, xq_ptr, xd_ptr, ids_ptr, weights_ptr, out_type,
+                                            out_ptr))
+
+    def ExpertsI8(self, gate_up: int, down: int, act: int, xq: np.ndarray, xd: np.ndarray, ids: np.ndarray,
+                  weights: np.ndarray) -> np.ndarray:
+        """phx_experts_i8 on host arrays: out [T][d] f32 from int8 rows (as QuantI8 returns them) and a routing (as Route
+        returns it)."""
+        xq = np.ascontiguousarray(xq, dtype=np.int8)
+        ids = np.ascontiguousarray(ids, dtype=np.int32)
+        xd, weights = _f32(xd), _f32(weights)
+        if xq.ndim != 2 or ids.ndim != 2 or xd.shape != xq.shape[:1] or weights.shape != ids.shape or len(ids) != len(xq):
+            raise ArgumentError(PHX.ERR_ARG, f"rows {xq.shape}, scales {xd.shape}, ids {ids.shape}, weights {weights.shape}")
+        return self._on_device([xq, xd, ids, weights], [(xq.shape, np.float32)],
+                               lambda *p: self.experts_i8_device(gate_up, down, act, xq.shape[0], ids.shape[1], *p[:4], PHX.F32,
+                                                                 p[4]))[0]
 
     def stack_run_device(self, x_ptr: int, T: int):
         """Replay the captured stack on a device-resident x (async; sync() waits)."""
