@@ -247,6 +247,150 @@ __global__ __launch_bounds__(64 * NW) void k_i8_rows(I8Args g)
     }
 }
 
+// k_i8_tile: four waves, each 64 stored weight rows (PAIRED: the gate and up rows of 32 channels), by a tile of up to 128
+// tokens.  The weights go straight from memory to each wave's registers (the layout has every operand as one run of
+// 1 KB, and no other wave of the workgroup wants it), one 128-column step ahead; the tokens, which all four waves read, go
+// through an LDS ring by direct loads two steps ahead, row-major runs of 128 bytes with the 16-byte chunks XOR-swizzled by
+// the row (an operand's 8 consecutive lanes hit all 32 banks).
+constexpr int TI_RING = 3;
+
+template <int NT, bool PAIRED, int DT>
+__device__ __forceinline__ void i8_tile_product(const I8Args& g, const Tile& tl, int bx, unsigned char* ring, int* orow, float* dxs)
+{
+    constexpr int STAGE = NT * 32 * 128;
+    const int tid = threadIdx.x, lane = tid & 63, r32 = lane & 31, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int S = g.kc / 8;
+    // this lane's rows of the direct loads: one per load, the last row again past the tile's end
+    const int chunk = ((lane & 7) ^ (lane >> 3)) * 16;
+    const __amdgpu_buffer_rsrc_t rsrc = buf_rsrc(g.xq + (g.perm ? 0 : (int64_t)tl.start * g.cols));
+    uint32_t xr[NT];  // a list's rows lie within 2^32 bytes of xq (phx_experts_i8's chunks), a dense tile's of its first
+#pragma unroll
+    for (int i = 0; i < NT; i++) {
+        const int at = min(8 * (wave * NT + i) + (lane >> 3), tl.cnt - 1);
+        xr[i] = (uint32_t)(g.perm ? g.perm[tl.start + at] / g.div : at) * (uint32_t)g.cols;
+    }
+    if (tid < NT * 32) {
+        const int at = tl.start + min(tid, tl.cnt - 1);
+        const int a = g.perm ? g.perm[at] : at;
+        orow[tid] = a;
+        dxs[tid] = g.xd[g.perm ? a / g.div : a];
+    }
+    auto dma = [&](int s) {
+        const uint32_t off = min(s, S - 1) * 128 + chunk, o = off < (uint32_t)g.cols ? off : 0;  // the weights past cols are 0
+        unsigned char* to = ring + (s % TI_RING) * STAGE + wave * NT * 1024;
+#pragma unroll
+        for (int i = 0; i < NT; i++)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void_t)(to + i * 1024), 16, xr[i] + o, 0, 0, 0);
+    };
+    const int rg0 = (bx * 4 + wave) * 2, rgs = g.rgs;
+    const int8_t* wb[2];
+#pragma unroll
+    for (int b = 0; b < 2; b++)
+        wb[b] = g.w + (int64_t)tl.e * g.mat_bytes + (int64_t)min(rg0 + b, rgs - 1) * g.kc * 512;
+    i32x4 wv[2][2][4];
+    auto weights = [&](int s, auto P) {
+        const int64_t o = (int64_t)min(s, S - 1) * 4096;
+#pragma unroll
+        for (int b = 0; b < 2; b++)
+#pragma unroll
+            for (int kk = 0; kk < 4; kk++) wv[decltype(P)::value][b][kk] = *(const i32x4*)(wb[b] + o + kk * 1024 + lane * 16);
+    };
+    i32x16 acc[NT][2];
+#pragma unroll
+    for (int j = 0; j < NT; j++)
+#pragma unroll
+        for (int b = 0; b < 2; b++)
+#pragma unroll
+            for (int v = 0; v < 16; v++) acc[j][b][v] = 0;
+    const uint32_t lds = (uint32_t)(uintptr_t)(lds_void_t)ring + r32 * 128, swz = (h ^ (r32 & 7)) * 16;
+    auto step = [&](int s, auto P) {
+        constexpr int p = decltype(P)::value;
+        __builtin_amdgcn_s_waitcnt(vm_wait(NT + 8));  // step s's rows have landed (step s + 1's and its weights may not)
+        __builtin_amdgcn_s_barrier();                 // in every wave, and nobody reads slot s + 2 any more
+        __builtin_amdgcn_sched_barrier(0);
+        dma(s + 2);
+        weights(s + 1, ic<1 - p>{});
+        __builtin_amdgcn_sched_barrier(0);
+        const uint32_t at = lds + (s % TI_RING) * STAGE;
+        u32x4 a[2][NT];
+        auto read = [&](auto KK) {
+            constexpr int kk = decltype(KK)::value;
+            const uint32_t ad = at + (swz ^ (kk * 32));
+            static_for<NT>([&](auto J) { a[kk & 1][decltype(J)::value] = ds_r128<decltype(J)::value * 4096>(ad); });
+        };
+        read(ic<0>{});
+        static_for<4>([&](auto KK) {
+            constexpr int kk = decltype(KK)::value;
+            if constexpr (kk < 3) read(ic<kk + 1>{});
+            asm volatile("s_waitcnt lgkmcnt(%0)" ::"i"(kk < 3 ? NT : 0) : "memory");
+#pragma unroll
+            for (int j = 0; j < NT; j++) tie(a[kk & 1][j]);
+#pragma unroll
+            for (int j = 0; j < NT; j++)
+#pragma unroll
+                for (int b = 0; b < 2; b++)
+                    acc[j][b] = __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4, a[kk & 1][j]), wv[p][b][kk],
+                                                                      acc[j][b], 0, 0, 0);
+        });
+    };
+    dma(0);
+    dma(1);
+    weights(0, ic<0>{});
+    for (int s = 0; s + 1 < S; s += 2) {
+        step(s, ic<0>{});
+        step(s + 1, ic<1>{});
+    }
+    if (S & 1) step(S - 1, ic<0>{});
+    const float* sc = g.scale + (int64_t)tl.e * g.mat_scales;
+    float dw[2];
+#pragma unroll
+    for (int b = 0; b < 2; b++) dw[b] = sc[min(rg0 + b, rgs - 1) * 32 + r32];
+    // the scales have landed before the first store (a later wait for them would wait for the stores too), and the direct
+    // loads past the last step before the workgroup's LDS goes
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < NT; j++)
+#pragma unroll
+        for (int v = 0; v < 16; v++) {
+            const int tok = 32 * j + 8 * (v >> 2) + 4 * h + (v & 3);
+            if (tok >= tl.cnt) continue;
+            const float dx = dxs[tok];
+            const int64_t o = (int64_t)orow[tok] * g.out_cols;
+            if (PAIRED) {
+                const int col = (rg0 >> 1) * 32 + r32;
+                if (col < g.out_cols)
+                    store_one<DT>(g.out, o + col, gated(g, (float)acc[j][0][v] * (dx * dw[0]), (float)acc[j][1][v] * (dx * dw[1])));
+            } else {
+#pragma unroll
+                for (int b = 0; b < 2; b++) {
+                    const int col = (rg0 + b) * 32 + r32;
+                    if (col < g.out_cols) store_one<DT>(g.out, o + col, (float)acc[j][b][v] * (dx * dw[b]));
+                }
+            }
+        }
+}
+
+template <bool PAIRED, int DT>
+__global__ __launch_bounds__(256, 2) void k_i8_tile(I8Args g)
+{
+    __shared__ __align__(16) unsigned char ring[TI_RING * 128 * 128];
+    __shared__ int orow[128];
+    __shared__ float dxs[128];
+    // workgroup L runs on XCD L % 8: it takes tile 8 (k / gridDim.x) + L % 8 and row block k % gridDim.x, k = L / 8, so a
+    // tile's row blocks share that XCD's L2 for the tile's rows
+    const int gx = gridDim.x, L = blockIdx.y * gx + blockIdx.x, k = L >> 3;
+    Tile tl;
+    if (!i8_tile(g, 8 * (k / gx) + (L & 7), &tl)) return;  // uniform over the workgroup
+    switch ((tl.cnt + 31) / 32) {
+    case 1: i8_tile_product<1, PAIRED, DT>(g, tl, k % gx, ring, orow, dxs); break;
+    case 2: i8_tile_product<2, PAIRED, DT>(g, tl, k % gx, ring, orow, dxs); break;
+    case 3: i8_tile_product<3, PAIRED, DT>(g, tl, k % gx, ring, orow, dxs); break;
+    default: i8_tile_product<4, PAIRED, DT>(g, tl, k % gx, ring, orow, dxs);
+    }
+}
+
 void launch_i8_product(hipStream_t st, const I8Mat& m, I8Args g, int max_tiles, int out_type)
 {
     g.w = m.w;
@@ -256,7 +400,17 @@ void launch_i8_product(hipStream_t st, const I8Mat& m, I8Args g, int max_tiles, 
     g.kc = m.kc;
     g.cols = m.cols;
     g.out_cols = m.paired ? m.rows / 2 : m.rows;
-    const dim3 grid(m.paired ? m.rg / 2 : m.rg, max_tiles), blk(256);
+    g.rgs = m.rg;
+    const dim3 blk(256);
+    if (g.cap == kI8Tile) {
+        const dim3 grid((m.rg + 7) / 8, (max_tiles + 7) / 8 * 8);
+        if (m.paired) launch(k_i8_tile<true, PHX_F32>, grid, blk, 0, st, g);
+        else if (out_type == PHX_F16) launch(k_i8_tile<false, PHX_F16>, grid, blk, 0, st, g);
+        else if (out_type == PHX_BF16) launch(k_i8_tile<false, PHX_BF16>, grid, blk, 0, st, g);
+        else launch(k_i8_tile<false, PHX_F32>, grid, blk, 0, st, g);
+        return;
+    }
+    const dim3 grid(m.paired ? m.rg / 2 : m.rg, max_tiles);
     if (m.paired) launch(k_i8_rows<4, true, PHX_F32>, grid, blk, 0, st, g);
     else if (out_type == PHX_F16) launch(k_i8_rows<4, false, PHX_F16>, grid, blk, 0, st, g);
     else if (out_type == PHX_BF16) launch(k_i8_rows<4, false, PHX_BF16>, grid, blk, 0, st, g);

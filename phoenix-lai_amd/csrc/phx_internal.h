@@ -306,15 +306,17 @@ struct I8Args {
     const Tile* tiles = nullptr;
     const int* ntiles = nullptr;
     const int* perm = nullptr;
-    int div = 1, nrows = 0, cap = 32, act = 0;
+    int div = 1, nrows = 0, cap = 0, act = 0;
     const float* tab = nullptr;
     void* out;
     // set by launch_i8_product from the matrix
     const int8_t* w;
     const float* scale;
     int64_t mat_bytes, mat_scales;
-    int kc, cols, out_cols;
+    int kc, cols, out_cols, rgs;
 };
+// tile capacities: the tile kernel's and the row kernel's
+constexpr int kI8Tile = 128, kI8Rows = 32;
 // paired matrices write act(gate) * up as float, the others the product as out_type
 void launch_i8_product(hipStream_t st, const I8Mat& m, I8Args g, int max_tiles, int out_type);
 void launch_i8_lists(hipStream_t st, int n, int E, int cap, const int* ids, int* perm, Tile* tiles, int* ntiles);

@@ -40,11 +40,19 @@ __device__ __forceinline__ void load_eight(const void* p, int64_t i, float (&v)[
     }
 }
 
+// A product that is stored as fp16 is rounded to float first: left to itself the compiler may round it once, in one mixed
+// instruction, in one kernel and not in another.
+__device__ __forceinline__ uint32_t f2h_of(float v)
+{
+    asm("" : "+v"(v));
+    return f2h_bits(v);
+}
+
 template <int DT>
 __device__ __forceinline__ void store_one(void* p, int64_t i, float v)
 {
     if (DT == PHX_F32) ((float*)p)[i] = v;
-    else ((uint16_t*)p)[i] = (uint16_t)(DT == PHX_F16 ? f2h_bits(v) : f2bf(v));
+    else ((uint16_t*)p)[i] = (uint16_t)(DT == PHX_F16 ? f2h_of(v) : f2bf(v));
 }
 
 // four consecutive values; p + i aligned to four of them
@@ -53,7 +61,7 @@ __device__ __forceinline__ void store_four(void* p, int64_t i, float4 v)
 {
     if (DT == PHX_F32) *(float4*)((float*)p + i) = v;
     else if (DT == PHX_F16)
-        *(uint2*)((uint16_t*)p + i) = make_uint2(f2h_bits(v.x) | (f2h_bits(v.y) << 16), f2h_bits(v.z) | (f2h_bits(v.w) << 16));
+        *(uint2*)((uint16_t*)p + i) = make_uint2(f2h_of(v.x) | (f2h_of(v.y) << 16), f2h_of(v.z) | (f2h_of(v.w) << 16));
     else *(uint2*)((uint16_t*)p + i) = make_uint2(f2bf(v.x) | (f2bf(v.y) << 16), f2bf(v.z) | (f2bf(v.w) << 16));
 }
 

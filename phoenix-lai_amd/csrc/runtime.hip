@@ -2412,9 +2412,9 @@ int phx_matmul_i8(phx_moe_ctx* c, const phx_weight* w, int T, const int8_t* xq, 
     g.xq = xq;
     g.xd = xd;
     g.nrows = T;
-    g.cap = 32;
+    g.cap = T > kI8Rows ? kI8Tile : kI8Rows;
     g.out = y;
-    launch_i8_product(c->stream, w->i8, g, (T + 31) / 32, y_type);
+    launch_i8_product(c->stream, w->i8, g, (T + g.cap - 1) / g.cap, y_type);
     HIPCHK(c, launch_status(c));
     return PHX_OK;
 }
@@ -2443,7 +2443,7 @@ int phx_experts_i8(phx_moe_ctx* c, const phx_weight* gu, const phx_weight* dn, i
                                                     {"out", out, (int64_t)T * d * eb, 16, true}}))
         return rc;
     // long batches go through in chunks, so that the workspace stays bounded
-    const int chunk = std::min(T, 65535 / k), A = chunk * k, cap = 32, max_tiles = (A + cap - 1) / cap + std::min(E, A);
+    const int chunk = std::min(T, 65535 / k), A = chunk * k, cap = A > 8 * E ? kI8Tile : kI8Rows, max_tiles = (A + cap - 1) / cap + std::min(E, A);
     int *perm, *ntiles;
     Tile* tiles;
     float *h, *hd, *y;
@@ -2465,6 +2465,7 @@ int phx_experts_i8(phx_moe_ctx* c, const phx_weight* gu, const phx_weight* dn, i
         g.tiles = tiles;
         g.ntiles = ntiles;
         g.perm = perm;
+        g.cap = cap;
         g.div = k;
         g.act = act;
         g.tab = c->gelu_tab;
