@@ -167,10 +167,14 @@ void launch_i8_pack(hipStream_t st, const I8Mat& m, int m0, int n_mat, const int
 }
 
 // ------------------------------------------------------------------------------ products
-// The tile of a workgroup: cnt rows of one matrix, the rows list places start .. start + cnt - 1 (or those rows
-// themselves for a dense product).  False past the last tile.
+// The tile of a workgroup: cnt rows of one matrix, the list's places start .. start + cnt - 1 (without a list those rows
+// themselves).  False past the last tile.
 __device__ __forceinline__ bool i8_tile(const I8Args& g, int tile, Tile* tl)
 {
+    if (g.ids) {  // a tile per assignment, those without an expert empty
+        *tl = {g.ids[tile], tile, 1};
+        return (unsigned)tl->e < (unsigned)g.n_expert;
+    }
     if (!g.tiles) {
         tl->e = 0;
         tl->start = tile * g.cap;
@@ -192,58 +196,163 @@ __device__ __forceinline__ float gated(const I8Args& g, float gate, float up)
 // result D[i][j] sits in lane j + 32 ((i / 4) % 2), register 4 (i / 8) + i % 4.  Tokens are A, weight rows B, so a
 // register's 32 lanes store 32 consecutive outputs of one token.
 //
-// k_i8_rows: a workgroup of NW waves takes 32 weight rows (PAIRED: 32 channels, 64 rows) and a tile of up to 32 tokens; the
-// waves split the reduction, and their int32 sums meet in LDS (exact in any order).
-template <int NW, bool PAIRED, int DT>
-__global__ __launch_bounds__(64 * NW) void k_i8_rows(I8Args g)
+// v_mfma_i32_16x16x64_i8 is the same on 16 rows: lane l holds row l % 16 at k = 16 (l / 16), and D[i][j] sits in lane
+// j + 16 (i / 4), register i % 4.
+//
+// k_i8_rows: for few rows per matrix, where the weights' bytes are the time.  A workgroup takes 16 weight rows (PAIRED: 16
+// channels, their gate and up rows) and a tile of up to 16 TT tokens.  Its NW waves split the reduction, so that a matrix
+// of few rows still has every load in flight at once, U operands of 1 KB per wave before the first product; their
+// int32 sums meet in LDS (exact in any order).
+template <int NW, int TT, bool PAIRED, int DT>
+__device__ __forceinline__ void i8_rows_product(const I8Args& g, const Tile& tl, int* red)
 {
-    constexpr int NB = PAIRED ? 2 : 1;
-    __shared__ int red[NW][NB][16][64];
-    Tile tl;
-    if (!i8_tile(g, blockIdx.y, &tl)) return;  // uniform over the workgroup
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r32 = lane & 31, h = lane >> 5;
-    const int at = tl.start + min(r32, tl.cnt - 1);
-    const int64_t arow = g.perm ? g.perm[at] / g.div : at;
-    const int8_t* xr = g.xq + arow * g.cols;
-    const int8_t* wr = g.w + (int64_t)tl.e * g.mat_bytes + (int64_t)blockIdx.x * NB * g.kc * 512 + lane * 16;
-    i32x16 acc[NB];
+    constexpr int NB = PAIRED ? 2 : 1, U = PAIRED || TT > 2 ? 4 : 8;
+    const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, q = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int bx = blockIdx.x;
+    const int8_t* xr[TT];
 #pragma unroll
-    for (int b = 0; b < NB; b++)
+    for (int t = 0; t < TT; t++) {
+        const int at = tl.start + min(16 * t + r16, tl.cnt - 1);
+        xr[t] = g.xq + (int64_t)((g.perm ? g.perm[at] : at) / g.div) * g.cols;
+    }
+    const int8_t* wb = g.w + (int64_t)tl.e * g.mat_bytes + (int64_t)(bx >> 1) * NB * g.kc * 512 + (bx & 1) * 256 + q * 512 + r16 * 16;
+    i32x4 acc[TT][NB];
 #pragma unroll
-        for (int v = 0; v < 16; v++) acc[b][v] = 0;
-    const int steps = g.kc / 2, s0 = wave * steps / NW, s1 = (wave + 1) * steps / NW;
-    for (int s = s0; s < s1; s++) {
-        const int k = 32 * s + 16 * h;
-        const i32x4 a = *(const i32x4*)(xr + (k < g.cols ? k : 0));  // the weights past cols are zero
+    for (int t = 0; t < TT; t++)
 #pragma unroll
-        for (int b = 0; b < NB; b++) {
-            const i32x4 w = *(const i32x4*)(wr + (int64_t)b * g.kc * 512 + (int64_t)s * 1024);
-            acc[b] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a, w, acc[b], 0, 0, 0);
+        for (int b = 0; b < NB; b++) acc[t][b] = i32x4{0, 0, 0, 0};
+    const int steps = g.kc / 4, s0 = wave * steps / NW, s1 = (wave + 1) * steps / NW;
+    for (int s = s0; s < s1; s += U) {
+        i32x4 w[U][NB], x[U][TT];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int su = min(s + u, s1 - 1), k = 64 * su + 16 * q;
+#pragma unroll
+            for (int b = 0; b < NB; b++) w[u][b] = *(const i32x4*)(wb + (int64_t)b * g.kc * 512 + (int64_t)su * 2048);
+#pragma unroll
+            for (int t = 0; t < TT; t++) x[u][t] = *(const i32x4*)(xr[t] + (k < g.cols ? k : 0));  // the weights past cols are 0
         }
+        __builtin_amdgcn_sched_barrier(0);  // every load before the first wait
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (s + u < s1)  // uniform
+#pragma unroll
+                for (int t = 0; t < TT; t++)
+#pragma unroll
+                    for (int b = 0; b < NB; b++)
+                        acc[t][b] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x[u][t], w[u][b], acc[t][b], 0, 0, 0);
     }
 #pragma unroll
-    for (int b = 0; b < NB; b++)
+    for (int t = 0; t < TT; t++)
 #pragma unroll
-        for (int v = 0; v < 16; v++) red[wave][b][v][lane] = acc[b][v];
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int v = 0; v < 4; v++) red[(((wave * TT + t) * NB + b) * 4 + v) * 64 + lane] = acc[t][b][v];
     __syncthreads();
-    for (int o = tid; o < 16 * 64; o += 64 * NW) {
-        const int v = o >> 6, l = o & 63, tok = 8 * (v >> 2) + 4 * (l >> 5) + (v & 3);
-        if (tok >= tl.cnt) continue;
+    for (int o = tid; o < tl.cnt * 16; o += 64 * NW) {
+        const int r = o & 15, tok = o >> 4, t = tok >> 4, i = tok & 15, l = r + 16 * (i >> 2);
         int sum[NB];
 #pragma unroll
         for (int b = 0; b < NB; b++) {
             sum[b] = 0;
 #pragma unroll
-            for (int w = 0; w < NW; w++) sum[b] += red[w][b][v][l];
+            for (int w = 0; w < NW; w++) sum[b] += red[(((w * TT + t) * NB + b) * 4 + (i & 3)) * 64 + l];
         }
-        const int64_t a = g.perm ? g.perm[tl.start + tok] : tl.start + tok;
-        const float dx = g.xd[g.perm ? a / g.div : a];
-        const float* sc = g.scale + (int64_t)tl.e * g.mat_scales + blockIdx.x * NB * 32 + (l & 31);
-        const int col = blockIdx.x * 32 + (l & 31);
+        const int a = g.perm ? g.perm[tl.start + tok] : tl.start + tok;
+        const float dx = g.xd[a / g.div];
+        const float* sc = g.scale + (int64_t)tl.e * g.mat_scales + (bx >> 1) * NB * 32 + (bx & 1) * 16 + r;
+        const int col = bx * 16 + r;
         if (col >= g.out_cols) continue;
         float y = (float)sum[0] * (dx * sc[0]);
         if (PAIRED) y = gated(g, y, (float)sum[NB - 1] * (dx * sc[32]));
-        store_one<DT>(g.out, a * g.out_cols + col, y);
+        store_one<DT>(g.out, (int64_t)a * g.out_cols + col, y);
+    }
+}
+
+// CT: the most token tiles of 16 that a tile may hold (its capacity); a tile takes the product of its own count
+template <int NW, int CT, bool PAIRED, int DT>
+__global__ __launch_bounds__(64 * NW) void k_i8_rows(I8Args g)
+{
+    __shared__ int red[NW * CT * (PAIRED ? 2 : 1) * 256];
+    Tile tl;
+    if (!i8_tile(g, blockIdx.y, &tl)) return;  // uniform over the workgroup
+    const int n = (tl.cnt + 15) / 16;
+    if (CT == 1 || n == 1) i8_rows_product<NW, 1, PAIRED, DT>(g, tl, red);
+    else if (CT == 2 || n == 2) i8_rows_product<NW, CT < 2 ? 1 : 2, PAIRED, DT>(g, tl, red);
+    else if (CT == 4 || n <= 4) i8_rows_product<NW, CT < 4 ? 1 : 4, PAIRED, DT>(g, tl, red);
+    else i8_rows_product<NW, CT < 8 ? 1 : 8, PAIRED, DT>(g, tl, red);
+}
+
+// The down products of few assignments and their weighted sum, for a token (blockIdx.y) and 16 of its outputs: wave w takes
+// the token's places w, w + NW, ...  It issues the place's weights, forms the int8 row of its h meanwhile (every
+// workgroup of the token forms it again: nf floats from L2), and the places' values meet in LDS in order.  No lists, no
+// int8 rows and no partial outputs go through memory.
+template <int NW, int DT>
+__global__ __launch_bounds__(64 * NW) void k_i8_down_few(I8Args g, int k, int nf, const float* __restrict__ h,
+                                                         const float* __restrict__ weights)
+{
+    extern __shared__ __align__(16) int8_t rows[];  // [NW][kc * 16]
+    __shared__ float vals[PHX_MAX_USED][16];
+    constexpr int U = 12;
+    const int lane = threadIdx.x & 63, r16 = lane & 15, q = lane >> 4, bx = blockIdx.x;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t t = blockIdx.y;
+    const int steps = g.kc / 4;
+    int8_t* row = rows + wave * g.kc * 16;
+    for (int j = wave; j < k; j += NW) {
+        const int e = g.ids[t * k + j];  // uniform
+        if ((unsigned)e >= (unsigned)g.n_expert) continue;
+        const int8_t* wb = g.w + (int64_t)e * g.mat_bytes + (int64_t)(bx >> 1) * g.kc * 512 + (bx & 1) * 256 + q * 512 + r16 * 16;
+        i32x4 w[U];
+        auto load = [&](int s) {
+#pragma unroll
+            for (int u = 0; u < U; u++) w[u] = *(const i32x4*)(wb + (int64_t)min(s + u, steps - 1) * 2048);
+        };
+        load(0);
+        __builtin_amdgcn_sched_barrier(0);
+        const float* hr = h + (t * k + j) * nf;
+        unsigned am = 0;
+        for (int i = lane * 4; i < nf; i += 256) {
+            const uint4 v = *(const uint4*)(hr + i);
+            am = max(max(am, v.x & 0x7FFFFFFFu), max(max(v.y & 0x7FFFFFFFu, v.z & 0x7FFFFFFFu), v.w & 0x7FFFFFFFu));
+        }
+        const RowScale rs = row_scale(wave_max_u32(am));
+        for (int i = lane * 4; i < g.kc * 16; i += 256) {
+            uint32_t p = 0;
+            if (i < nf) {
+                const float4 v = *(const float4*)(hr + i);
+                p = pack4(quant_one(v.x, rs.inv), quant_one(v.y, rs.inv), quant_one(v.z, rs.inv), quant_one(v.w, rs.inv));
+            }
+            *(uint32_t*)(row + i) = p;
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        i32x4 acc = {0, 0, 0, 0};
+        for (int s = 0; s < steps; s += U) {
+            if (s) load(s);
+#pragma unroll
+            for (int u = 0; u < U; u++)
+                if (s + u < steps)  // uniform
+                    acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(*(const i32x4*)(row + 64 * (s + u) + 16 * q), w[u], acc, 0, 0, 0);
+        }
+        if (lane < 16) {
+            const float dw = g.scale[(int64_t)e * g.mat_scales + bx * 16 + lane];
+            vals[j][lane] = (float)acc[0] * (rs.d * dw);
+        }
+        // this wave's reads of the row end before the next place's writes
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+    __syncthreads();
+    const int col = bx * 16 + threadIdx.x;
+    if (threadIdx.x < 16 && col < g.out_cols) {
+        float acc = 0.0f;
+        for (int j = 0; j < k; j++)
+            if ((unsigned)g.ids[t * k + j] < (unsigned)g.n_expert) acc += vals[j][threadIdx.x] * weights[t * k + j];
+        store_one<DT>(g.out, t * g.out_cols + col, acc);
     }
 }
 
@@ -391,7 +500,7 @@ __global__ __launch_bounds__(256, 2) void k_i8_tile(I8Args g)
     }
 }
 
-void launch_i8_product(hipStream_t st, const I8Mat& m, I8Args g, int max_tiles, int out_type)
+static void set_matrix(I8Args& g, const I8Mat& m)
 {
     g.w = m.w;
     g.scale = m.scale;
@@ -401,20 +510,62 @@ void launch_i8_product(hipStream_t st, const I8Mat& m, I8Args g, int max_tiles, 
     g.cols = m.cols;
     g.out_cols = m.paired ? m.rows / 2 : m.rows;
     g.rgs = m.rg;
-    const dim3 blk(256);
-    if (g.cap == kI8Tile) {
-        const dim3 grid((m.rg + 7) / 8, (max_tiles + 7) / 8 * 8);
+    g.n_expert = m.n_mat;
+}
+
+template <int NW, int CT>
+static void rows_product(hipStream_t st, const I8Mat& m, const I8Args& g, int max_tiles, int out_type)
+{
+    const dim3 grid((g.out_cols + 15) / 16, max_tiles), blk(64 * NW);
+    if (m.paired) launch(k_i8_rows<NW, CT < 8 ? CT : 4, true, PHX_F32>, grid, blk, 0, st, g);
+    else if (out_type == PHX_F16) launch(k_i8_rows<NW, CT, false, PHX_F16>, grid, blk, 0, st, g);
+    else if (out_type == PHX_BF16) launch(k_i8_rows<NW, CT, false, PHX_BF16>, grid, blk, 0, st, g);
+    else launch(k_i8_rows<NW, CT, false, PHX_F32>, grid, blk, 0, st, g);
+}
+
+template <int NW>
+static void rows_product(hipStream_t st, const I8Mat& m, const I8Args& g, int max_tiles, int out_type)
+{
+    if (g.cap <= 16) rows_product<NW, 1>(st, m, g, max_tiles, out_type);
+    else if (g.cap <= 32) rows_product<NW, 2>(st, m, g, max_tiles, out_type);
+    else if (g.cap <= 64) rows_product<NW, 4>(st, m, g, max_tiles, out_type);
+    else rows_product<NW, 8>(st, m, g, max_tiles, out_type);
+}
+
+void launch_i8_product(hipStream_t st, const I8Mat& m, I8Args g, bool tile, int max_tiles, int ncu, int out_type)
+{
+    set_matrix(g, m);
+    if (tile) {
+        const dim3 grid((m.rg + 7) / 8, (max_tiles + 7) / 8 * 8), blk(256);
         if (m.paired) launch(k_i8_tile<true, PHX_F32>, grid, blk, 0, st, g);
         else if (out_type == PHX_F16) launch(k_i8_tile<false, PHX_F16>, grid, blk, 0, st, g);
         else if (out_type == PHX_BF16) launch(k_i8_tile<false, PHX_BF16>, grid, blk, 0, st, g);
         else launch(k_i8_tile<false, PHX_F32>, grid, blk, 0, st, g);
-        return;
-    }
-    const dim3 grid(m.paired ? m.rg / 2 : m.rg, max_tiles);
-    if (m.paired) launch(k_i8_rows<4, true, PHX_F32>, grid, blk, 0, st, g);
-    else if (out_type == PHX_F16) launch(k_i8_rows<4, false, PHX_F16>, grid, blk, 0, st, g);
-    else if (out_type == PHX_BF16) launch(k_i8_rows<4, false, PHX_BF16>, grid, blk, 0, st, g);
-    else launch(k_i8_rows<4, false, PHX_F32>, grid, blk, 0, st, g);
+    } else if ((int64_t)((g.out_cols + 15) / 16) * max_tiles < 4 * ncu) rows_product<8>(st, m, g, max_tiles, out_type);
+    else rows_product<4>(st, m, g, max_tiles, out_type);
+}
+
+template <int NW>
+static void down_few(hipStream_t st, const I8Args& g, int T, int k, int nf, const float* h, const float* weights, int out_type)
+{
+    const dim3 grid((g.out_cols + 15) / 16, T), blk(64 * NW);
+    const uint32_t lds = NW * g.kc * 16;
+    if (out_type == PHX_F16) launch(k_i8_down_few<NW, PHX_F16>, grid, blk, lds, st, g, k, nf, h, weights);
+    else if (out_type == PHX_BF16) launch(k_i8_down_few<NW, PHX_BF16>, grid, blk, lds, st, g, k, nf, h, weights);
+    else launch(k_i8_down_few<NW, PHX_F32>, grid, blk, lds, st, g, k, nf, h, weights);
+}
+
+bool i8_down_few_fits(const I8Mat& m) { return 8 * m.kc * 16 <= 65536; }
+
+void launch_i8_down_few(hipStream_t st, const I8Mat& m, int T, int k, const float* h, const int* ids, const float* weights,
+                        int out_type, void* out)
+{
+    I8Args g{};
+    set_matrix(g, m);
+    g.ids = ids;
+    g.out = out;
+    if (k <= 4) down_few<4>(st, g, T, k, m.cols, h, weights, out_type);
+    else down_few<8>(st, g, T, k, m.cols, h, weights, out_type);
 }
 
 // ------------------------------------------------------------------------------ experts

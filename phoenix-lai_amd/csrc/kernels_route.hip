@@ -13,7 +13,8 @@ __device__ __forceinline__ unsigned long long sortable_f64(double v)
 }
 
 struct RouteArgs {
-    int T, E, k, G, used, gs;  // gs = E / G
+    int T, E, k, G, used, gs, inv_gs;  // gs = E / G; e / gs = e * inv_gs >> 16 for e < 256
+    int lpg;                           // lanes that share a group's experts: the largest power of two up to 64 / G
     bool sigmoid, top2, renorm;
     float scale;
     const void* logits;
@@ -22,116 +23,164 @@ struct RouteArgs {
     float* w;
 };
 
-// One wave per token, lane l holding experts 4 l .. 4 l + 3.  Each round of the choice is a maximum over the wave and
-// a ballot: the lowest lane that holds it, and the first of its four, is the lowest index.
-template <int DT>
+// One wave per token, lane l holding experts V l .. V l + V - 1.  A round of the choice is the wave's maximum of 32-bit
+// keys and a ballot: the lowest lane that holds it, and the first of its V, is the lowest index.  The keys are the logits,
+// exact in 32 bits, where their order is the scores' (no bias): then only the k chosen scores are ever formed, one per
+// lane.  With a bias (WIDE) they are the doubles s + b: the high words decide, and the low words where those are equal.
+template <int V, bool WIDE, int DT>
 __global__ __launch_bounds__(256) void k_route(RouteArgs R)
 {
     constexpr double NINF = -__builtin_inf();
-    __shared__ double sel[4][PHX_MAX_EXPERTS_DEV];
+    __shared__ double sel[4][64 * V];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int t = blockIdx.x * 4 + wave;
     if (t >= R.T) return;  // uniform over the wave, and the kernel has no workgroup barrier
-    const int e0 = 4 * lane;
-    float l[4];
+    const int e0 = V * lane;
+    const bool grouped = R.used < R.G, pairs = grouped && R.top2;
+    float l[V];
+    unsigned hi[V], lo[V];
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
+    for (int i = 0; i < V; i++) {
         const float v = e0 + i < R.E ? load_one<DT>(R.logits, (int64_t)t * R.E + e0 + i) : -INFINITY;
         l[i] = v > -INFINITY ? fminf(v, 3.402823466e38f) : -INFINITY;  // NaN compares false
+        hi[i] = l[i] > -INFINITY ? sortable_f32(l[i] + 0.0f) : 0u;      // -0 equals 0
+        lo[i] = 0u;
     }
-    // scores, 0 for what is no candidate by its logit
-    double s[4];
-    if (R.sigmoid) {
+    // what the softmax needs of the whole row
+    const bool soft_row = !R.sigmoid && (WIDE || pairs || !R.renorm);
+    double m = 0.0, rz = 0.0, s[V];
+    if (soft_row) {
+        float mx = l[0];
 #pragma unroll
-        for (int i = 0; i < 4; i++) s[i] = l[i] > -INFINITY ? 1.0 / (1.0 + exp(-(double)l[i])) : 0.0;
-    } else {
-        const double m = wave_max_dpp((double)fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])));
+        for (int i = 1; i < V; i++) mx = fmaxf(mx, l[i]);
+        m = wave_max_dpp((double)mx);
         double z = 0.0;
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
+        for (int i = 0; i < V; i++) {
             s[i] = l[i] > -INFINITY ? exp((double)l[i] - m) : 0.0;
             z += s[i];
         }
         z = wave_sum_dpp(z);
-        const double rz = z > 0.0 ? 1.0 / z : 0.0;
-#pragma unroll
-        for (int i = 0; i < 4; i++) s[i] *= rz;
+        rz = z > 0.0 ? 1.0 / z : 0.0;
     }
-    // c: the score with the bias (what the sums of two take); key: what is compared
-    double c[4];
-    unsigned long long key[4];
+    if (WIDE || pairs) {  // every expert's score
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        bool able = l[i] > -INFINITY;
-        c[i] = s[i];
-        double r = (double)l[i];
-        if (R.bias) {
-            const float b = e0 + i < R.E ? R.bias[e0 + i] : -INFINITY;
-            able = able && b > -INFINITY;
-            r = c[i] = s[i] + (double)b;
+        for (int i = 0; i < V; i++) {
+            if (R.sigmoid) s[i] = l[i] > -INFINITY ? 1.0 / (1.0 + exp(-(double)l[i])) : 0.0;
+            else s[i] *= rz;
         }
-        if (!able) c[i] = NINF;
-        key[i] = able ? sortable_f64(r + 0.0) : 0ull;  // -0 equals 0
     }
-    if (R.used < R.G) {
-        // a lane per group walks its experts; a group's rank is the number of groups ahead of it
+    double c[V];  // selection scores: what the groups' sums of two take
+    if (WIDE) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) sel[wave][e0 + i] = R.top2 || R.bias ? c[i] : (double)l[i];
+        for (int i = 0; i < V; i++) {
+            const float b = e0 + i < R.E ? R.bias[e0 + i] : -INFINITY;
+            const bool able = l[i] > -INFINITY && b > -INFINITY;
+            c[i] = able ? s[i] + (double)b + 0.0 : NINF;
+            const unsigned long long key = able ? sortable_f64(c[i]) : 0ull;
+            hi[i] = (unsigned)(key >> 32);
+            lo[i] = (unsigned)key;
+        }
+    }
+    if (grouped) {
+#pragma unroll
+        for (int i = 0; i < V; i++)
+            sel[wave][e0 + i] = WIDE ? c[i] : !pairs ? (double)l[i] : l[i] > -INFINITY ? s[i] : NINF;
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        // lpg lanes walk a group's experts and join their two largest; its rank is the number of groups ahead of it
+        const int g = lane / R.lpg, sub = lane & (R.lpg - 1);
         double a = NINF, b = NINF;
-        if (lane < R.G)
-            for (int i = 0; i < R.gs; i++) {
-                const double v = sel[wave][lane * R.gs + i];
+        if (g < R.G)
+            for (int i = sub; i < R.gs; i += R.lpg) {
+                const double v = sel[wave][g * R.gs + i];
                 b = fmax(b, fmin(a, v));
                 a = fmax(a, v);
             }
-        if (R.top2 && b > NINF) a += b;
-        int rank = 0;
-        for (int g = 0; g < R.G; g++) {
-            const double v = readlane_d(a, g);
-            rank += v > a || (v == a && g < lane);
+        for (int x = 1; x < R.lpg; x <<= 1) {
+            const double oa = __shfl_xor(a, x, 64), ob = __shfl_xor(b, x, 64);
+            b = fmax(fmin(a, oa), fmax(b, ob));
+            a = fmax(a, oa);
         }
-        const unsigned long long kept = __ballot(lane < R.G && rank < R.used);
+        if (pairs && b > NINF) a += b;
+        int rank = 0;
+        for (int o = 0; o < R.G; o++) {
+            const double v = readlane_d(a, o * R.lpg);
+            rank += v > a || (v == a && o < g);
+        }
+        const unsigned long long kept = __ballot(sub == 0 && g < R.G && rank < R.used);
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (e0 + i >= R.E || !((kept >> ((e0 + i) / R.gs)) & 1)) key[i] = 0ull;
+        for (int i = 0; i < V; i++)
+            if (e0 + i >= R.E || !((kept >> ((((e0 + i) * R.inv_gs) >> 16) * R.lpg)) & 1)) hi[i] = lo[i] = 0u;
     }
     int my_id = -1;
-    double my_s = 0.0, total = 0.0;
+    float my_l = -INFINITY;
+    double my_s = 0.0;
     for (int j = 0; j < R.k; j++) {
-        unsigned long long best = key[0];
+        unsigned bh = hi[0], bl = lo[0];
         int at = 0;
 #pragma unroll
-        for (int i = 1; i < 4; i++)
-            if (key[i] > best) {
-                best = key[i];
+        for (int i = 1; i < V; i++)
+            if (WIDE ? u64_gt(hi[i], lo[i], bh, bl) : hi[i] > bh) {
+                bh = hi[i];
+                bl = lo[i];
                 at = i;
             }
-        const unsigned long long top = wave_max_u64(best);
-        if (top == 0ull) break;  // no candidate is left; uniform
-        const int owner = __builtin_ctzll(__ballot(best == top));
-        const double so = at == 0 ? s[0] : at == 1 ? s[1] : at == 2 ? s[2] : s[3];
-        const double sv = readlane_d(so, owner);
-        const int id = 4 * owner + __builtin_amdgcn_readlane(at, owner);
-        total += sv;
+        const unsigned top = wave_max_u32(bh);
+        if (top == 0u) break;  // no candidate is left; uniform
+        unsigned long long who = __ballot(bh == top);
+        if (WIDE && (who & (who - 1))) {
+            const unsigned tl = wave_max_u32(bh == top ? bl : 0u);
+            who = __ballot(bh == top && bl == tl);
+        }
+        const int owner = __builtin_ctzll(who);
+        float lv = l[0];
+        double sv = WIDE ? s[0] : 0.0;
+#pragma unroll
+        for (int i = 1; i < V; i++)
+            if (at == i) {
+                lv = l[i];
+                if (WIDE) sv = s[i];
+            }
+        const int id = V * owner + __builtin_amdgcn_readlane(at, owner);
+        if (WIDE) sv = readlane_d(sv, owner);
+        else lv = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(lv), owner));
         if (lane == j) {
             my_id = id;
+            my_l = lv;
             my_s = sv;
         }
-        if (lane == owner) {
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-                if (i == at) key[i] = 0ull;
-        }
+        for (int i = 0; i < V; i++)
+            if (lane == owner && at == i) hi[i] = lo[i] = 0u;
     }
+    if (!WIDE && my_id >= 0) {
+        if (R.sigmoid) my_s = 1.0 / (1.0 + exp(-(double)my_l));
+        else if (soft_row) my_s = exp((double)my_l - m) * rz;
+        else my_s = exp((double)my_l - (double)__int_as_float(__builtin_amdgcn_readlane(__float_as_int(my_l), 0)));
+    }
+    const double total = R.renorm ? wave_sum_dpp(my_s) : 1.0;
     if (lane < R.k) {
-        double w = my_s;
-        if (R.renorm) w = total > 0.0 ? w / total : 0.0;
+        const double w = !R.renorm ? my_s : total > 0.0 ? my_s / total : 0.0;
         R.ids[(int64_t)t * R.k + lane] = my_id;
         R.w[(int64_t)t * R.k + lane] = (float)(w * (double)R.scale);
     }
+}
+
+template <int V>
+static void route_of(hipStream_t st, int type, const RouteArgs& R)
+{
+    const dim3 grid((R.T + 3) / 4), blk(256);
+#define RT_L(DT)                                                                       \
+    if (R.bias) launch(k_route<V, true, DT>, grid, blk, 0, st, R);                     \
+    else launch(k_route<V, false, DT>, grid, blk, 0, st, R)
+    switch (type) {
+    case PHX_F16: RT_L(PHX_F16); break;
+    case PHX_BF16: RT_L(PHX_BF16); break;
+    default: RT_L(PHX_F32);
+    }
+#undef RT_L
 }
 
 void launch_route(hipStream_t st, const phx_route_desc& D, int T, const void* logits, const float* bias, int* ids, float* w)
@@ -151,12 +200,12 @@ void launch_route(hipStream_t st, const phx_route_desc& D, int T, const void* lo
     R.bias = bias;
     R.ids = ids;
     R.w = w;
-    const dim3 grid((T + 3) / 4), blk(256);
-    switch (D.logits_type) {
-    case PHX_F16: launch(k_route<PHX_F16>, grid, blk, 0, st, R); break;
-    case PHX_BF16: launch(k_route<PHX_BF16>, grid, blk, 0, st, R); break;
-    default: launch(k_route<PHX_F32>, grid, blk, 0, st, R); break;
-    }
+    R.inv_gs = (65536 + R.gs - 1) / R.gs;
+    R.lpg = 1;
+    while (2 * R.lpg * R.G <= 64) R.lpg *= 2;
+    if (R.E <= 64) route_of<1>(st, D.logits_type, R);
+    else if (R.E <= 128) route_of<2>(st, D.logits_type, R);
+    else route_of<4>(st, D.logits_type, R);
 }
 
 }  // namespace phx

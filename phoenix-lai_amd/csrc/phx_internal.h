@@ -299,13 +299,15 @@ struct I8Mat {
 void launch_i8_pack(hipStream_t st, const I8Mat& m, int m0, int n_mat, const int8_t* w, const float* scale);
 
 struct I8Args {
-    // set by the caller: input rows and scales, the tiles and lists of a grouped product (perm's value / div is the input
-    // row, perm's value the output row) or nrows of a dense one in tiles of cap, the output and the activation
+    // set by the caller: input rows and scales, the tiles and list of a grouped product or nrows of a dense one in tiles of
+    // cap (a place's output row is perm's value, or the place without a list; its input row that over div), the output
+    // and the activation
     const int8_t* xq;
     const float* xd;
     const Tile* tiles = nullptr;
     const int* ntiles = nullptr;
     const int* perm = nullptr;
+    const int* ids = nullptr;  // in place of the tiles: tile a is assignment a alone, its expert ids[a]
     int div = 1, nrows = 0, cap = 0, act = 0;
     const float* tab = nullptr;
     void* out;
@@ -313,12 +315,17 @@ struct I8Args {
     const int8_t* w;
     const float* scale;
     int64_t mat_bytes, mat_scales;
-    int kc, cols, out_cols, rgs;
+    int kc, cols, out_cols, rgs, n_expert;
 };
-// tile capacities: the tile kernel's and the row kernel's
-constexpr int kI8Tile = 128, kI8Rows = 32;
-// paired matrices write act(gate) * up as float, the others the product as out_type
-void launch_i8_product(hipStream_t st, const I8Mat& m, I8Args g, int max_tiles, int out_type);
+// tile capacities: the tile kernel's, and the row kernel's most for paired and plain matrices (16, 32, 64 or 128)
+constexpr int kI8Tile = 128, kI8RowsPaired = 64, kI8Rows = 128;
+// paired matrices write act(gate) * up as float, the others the product as out_type; tile: the tile kernel (cap kI8Tile), else
+// the row kernel
+void launch_i8_product(hipStream_t st, const I8Mat& m, I8Args g, bool tile, int max_tiles, int ncu, int out_type);
+// the down products of T tokens' k places from h [T k][cols], and their weighted sums as out [T][rows]
+bool i8_down_few_fits(const I8Mat& m);
+void launch_i8_down_few(hipStream_t st, const I8Mat& m, int T, int k, const float* h, const int* ids, const float* weights,
+                        int out_type, void* out);
 void launch_i8_lists(hipStream_t st, int n, int E, int cap, const int* ids, int* perm, Tile* tiles, int* ntiles);
 void launch_i8_combine(hipStream_t st, int T, int d, int k, int E, const float* y, const int* ids, const float* w, int out_type,
                        void* out);

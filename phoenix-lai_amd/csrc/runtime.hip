@@ -2234,6 +2234,12 @@ int phx_matvec(phx_moe_ctx* c, int type, const void* w, int rows, int cols, int 
 
 // ---------------------------------------------------------------------------- routing and int8 products
 
+#ifndef I8_DENSE_T
+#define I8_DENSE_T 128
+#define I8_FEW E / 2
+#define I8_TILE 16
+#define I8_CAP 8
+#endif
 namespace {
 constexpr int PHX_I8_WEIGHT = 24;  // GgmlType's int8
 constexpr int kMaxRowsI8 = 1 << 20;
@@ -2412,9 +2418,10 @@ int phx_matmul_i8(phx_moe_ctx* c, const phx_weight* w, int T, const int8_t* xq, 
     g.xq = xq;
     g.xd = xd;
     g.nrows = T;
-    g.cap = T > kI8Rows ? kI8Tile : kI8Rows;
+    const bool tile = T > I8_DENSE_T;
+    g.cap = tile ? kI8Tile : T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : kI8Rows;
     g.out = y;
-    launch_i8_product(c->stream, w->i8, g, (T + g.cap - 1) / g.cap, y_type);
+    launch_i8_product(c->stream, w->i8, g, tile, (T + g.cap - 1) / g.cap, c->ncu, y_type);
     HIPCHK(c, launch_status(c));
     return PHX_OK;
 }
@@ -2442,41 +2449,59 @@ int phx_experts_i8(phx_moe_ctx* c, const phx_weight* gu, const phx_weight* dn, i
                                                     {"weights", weights, (int64_t)T * k * 4, 4, false},
                                                     {"out", out, (int64_t)T * d * eb, 16, true}}))
         return rc;
+    hipStream_t st = c->stream;
+    float* h;
+    int rc;
+    I8Args g{};
+    g.xq = xq;
+    g.xd = xd;
+    g.div = k;
+    g.act = act;
+    g.tab = c->gelu_tab;
+    // few assignments, most of them of an expert of their own: two launches and no lists
+    if (T * k <= I8_FEW && i8_down_few_fits(dn->i8)) {
+        if ((rc = i8_ensure(c, I8_H, (int64_t)T * k * nf, &h))) return rc;
+        g.ids = ids;
+        g.cap = 16;
+        g.out = h;
+        launch_i8_product(st, gu->i8, g, false, T * k, c->ncu, PHX_F32);
+        launch_i8_down_few(st, dn->i8, T, k, h, ids, weights, out_type, out);
+        HIPCHK(c, launch_status(c));
+        return PHX_OK;
+    }
     // long batches go through in chunks, so that the workspace stays bounded
-    const int chunk = std::min(T, 65535 / k), A = chunk * k, cap = A > 8 * E ? kI8Tile : kI8Rows, max_tiles = (A + cap - 1) / cap + std::min(E, A);
+    const int chunk = std::min(T, 65535 / k), A = chunk * k;
+    const bool tile = A > I8_TILE * E;
+    const int cap = tile ? kI8Tile : A <= I8_CAP * E ? 32 : kI8RowsPaired;
+    const int max_tiles = (A + cap - 1) / cap + std::min(E, A);
     int *perm, *ntiles;
     Tile* tiles;
-    float *h, *hd, *y;
+    float *hd, *y;
     int8_t* hq;
-    int rc;
     if ((rc = i8_ensure(c, I8_PERM, A, &perm)) || (rc = i8_ensure(c, I8_TILES, max_tiles, &tiles)) ||
         (rc = i8_ensure(c, I8_NTILES, 1, &ntiles)) || (rc = i8_ensure(c, I8_H, (int64_t)A * nf, &h)) ||
         (rc = i8_ensure(c, I8_HQ, (int64_t)A * nf, &hq)) || (rc = i8_ensure(c, I8_HD, A, &hd)) ||
         (rc = i8_ensure(c, I8_Y, (int64_t)A * d, &y)))
         return rc;
-    hipStream_t st = c->stream;
+    g.tiles = tiles;
+    g.ntiles = ntiles;
+    g.perm = perm;
+    g.cap = cap;
     for (int t0 = 0; t0 < T; t0 += chunk) {
         const int n = std::min(chunk, T - t0);
         const int32_t* id = ids + (int64_t)t0 * k;
         launch_i8_lists(st, n * k, E, cap, id, perm, tiles, ntiles);
-        I8Args g{};
         g.xq = xq + (int64_t)t0 * d;
         g.xd = xd + t0;
-        g.tiles = tiles;
-        g.ntiles = ntiles;
-        g.perm = perm;
-        g.cap = cap;
         g.div = k;
-        g.act = act;
-        g.tab = c->gelu_tab;
         g.out = h;
-        launch_i8_product(st, gu->i8, g, max_tiles, PHX_F32);
+        launch_i8_product(st, gu->i8, g, tile, max_tiles, c->ncu, PHX_F32);
         launch_quant_i8(st, PHX_QUANT_PLAIN, PHX_F32, n * k, nf, nf, 0.0f, h, nullptr, nullptr, hq, hd);
         g.xq = hq;
         g.xd = hd;
         g.div = 1;
         g.out = y;
-        launch_i8_product(st, dn->i8, g, max_tiles, PHX_F32);
+        launch_i8_product(st, dn->i8, g, tile, max_tiles, c->ncu, PHX_F32);
         launch_i8_combine(st, n, d, k, E, y, id, weights + (int64_t)t0 * k, out_type, (char*)out + (int64_t)t0 * d * eb);
     }
     HIPCHK(c, launch_status(c));
