@@ -231,7 +231,7 @@ int phx_moe_profile_read(phx_moe_ctx* ctx, double* total_ms, int64_t* launches);
  * many-token router's error bound assumes); 10 the sequential double sum of squares of each row of
  * m = b[0] floats of a (n a multiple of m, 2 <= m <= 65536), the sum RmsNorm's certified means fall back
  * to, formed by one wave as the kernels form it: out[2 r] and out[2 r + 1] hold the low and high 32
- * bits of row r's double.  out is float (int results as their value). */
+ * bits of row r's double; 11 and 12 silu(a) * b and gelu(a) * b as phx_experts_i8 forms them.  out is float (int results as their value). */
 int phx_moe_selftest(phx_moe_ctx* ctx, int op, int n, const float* a, const float* b, float* out);
 
 /* Average time (ms) of `iters` coalesced streaming reads of a device buffer: the achievable HBM

@@ -186,10 +186,80 @@ __device__ __forceinline__ bool i8_tile(const I8Args& g, int tile, Tile* tl)
     return true;
 }
 
-// h = act(gate) * up as phx_quant_i8 forms it
-__device__ __forceinline__ float gated(const I8Args& g, float gate, float up)
+// Place i's output row as a byte offset from out_base (a tile's dense rows, or a list's whole output, lie within 2^32
+// bytes), and its input row's scale.  Past the tile's end the last row again: its product is then computed, and stored,
+// more than once, the same value to the same place.
+template <int DT>
+__device__ __forceinline__ void tile_rows(const I8Args& g, const Tile& tl, int i, uint32_t* orow, float* dxs)
 {
-    return (g.act == PHX_QUANT_SILU_MUL ? silu_ref(gate) : gelu_ref(gate, g.tab)) * up;
+    const int p = min(i, tl.cnt - 1), a = g.perm ? g.perm[tl.start + p] : tl.start + p;
+    orow[i] = (uint32_t)(g.perm ? a : p) * (uint32_t)g.out_cols * (DT == PHX_F32 ? 4u : 2u);
+    dxs[i] = g.xd[a / g.div];
+}
+template <int DT>
+__device__ __forceinline__ char* out_base(const I8Args& g, const Tile& tl)
+{
+    return (char*)g.out + (g.perm ? 0 : (int64_t)tl.start * g.out_cols * (DT == PHX_F32 ? 4 : 2));
+}
+
+// 2^f on [-1/2, 1/2] in double, the Taylor series of exp(f ln 2) to f^11: within 2^-46
+__device__ __forceinline__ double exp2_frac(double f)
+{
+    const double x = f * 0.69314718055994530942;
+    double p = 1.0 / 39916800.0;
+    p = __builtin_fma(p, x, 1.0 / 3628800.0);
+    p = __builtin_fma(p, x, 1.0 / 362880.0);
+    p = __builtin_fma(p, x, 1.0 / 40320.0);
+    p = __builtin_fma(p, x, 1.0 / 5040.0);
+    p = __builtin_fma(p, x, 1.0 / 720.0);
+    p = __builtin_fma(p, x, 1.0 / 120.0);
+    p = __builtin_fma(p, x, 1.0 / 24.0);
+    p = __builtin_fma(p, x, 1.0 / 6.0);
+    p = __builtin_fma(p, x, 0.5);
+    p = __builtin_fma(p, x, 1.0);
+    return __builtin_fma(p, x, 1.0);
+}
+// exp(x) in double for |x| <= 128, within 2^-45 of it: past the float it is rounded to by 21 bits
+__device__ __forceinline__ double exp_near(double x)
+{
+    const double t = x * 1.44269504088896340736, n = __builtin_rint(t);
+    return __builtin_amdgcn_ldexp(exp2_frac(t - n), (int)n);
+}
+// silu_ref and gelu_ref's table in the epilogues of the products, where the library's exponential and a gather per value
+// would cost as much as the product.  The same roundings: silu's quotient by the reciprocal, one refinement and two
+// corrections, which round it correctly while nothing leaves the normal numbers (|v| < 80); gelu_f16 equals
+// the table at every fp16 value (tests).
+__device__ __forceinline__ float silu_near(float v)
+{
+    if (fabsf(v) >= 80.0f || v != v) return silu_ref(v);
+    const float d = 1.0f + (float)exp_near(-(double)v);
+    float y = __builtin_amdgcn_rcpf(d);
+    y = __builtin_fmaf(__builtin_fmaf(-d, y, 1.0f), y, y);
+    float q = v * y;
+    q = __builtin_fmaf(__builtin_fmaf(-d, q, v), y, q);
+    return __builtin_fmaf(__builtin_fmaf(-d, q, v), y, q);
+}
+__device__ __forceinline__ float gelu_near(float x)
+{
+    if (!(x > -10.0f)) return 0.0f;  // and for a NaN, as the table has it
+    if (x >= 10.0f) return x;
+    const float h = h2f(f2h_bits(x));
+    if (h <= -10.0f) return 0.0f;
+    if (h >= 10.0f) return h;
+    const float inner = 0.79788456080286535587989211986876f * h * (1.0f + 0.044715f * h * h);
+    // tanh(z) = 1 - 2 / (1 + exp(2 z)), 1 from |z| = 22 on; the reciprocal from the hardware's by two refinements
+    const double z2 = 2.0 * (double)fminf(fmaxf(inner, -22.0f), 22.0f), e = 1.0 + exp_near(z2);
+    double y = __builtin_amdgcn_rcp(e);
+    y = __builtin_fma(__builtin_fma(-e, y, 1.0), y, y);
+    y = __builtin_fma(__builtin_fma(-e, y, 1.0), y, y);
+    const float t = (float)__builtin_fma(-2.0, y, 1.0);
+    return h2f(f2h_of(0.5f * h * (1.0f + t)));
+}
+
+// h = act(gate) * up as phx_quant_i8 forms it
+__device__ __forceinline__ float gated(int act, float gate, float up)
+{
+    return (act == PHX_QUANT_SILU_MUL ? silu_near(gate) : gelu_near(gate)) * up;
 }
 
 // v_mfma_i32_32x32x32_i8: lane l holds 16 bytes of A row l % 32 and of B row l % 32, both at k = 16 (l / 32); the
@@ -199,89 +269,113 @@ __device__ __forceinline__ float gated(const I8Args& g, float gate, float up)
 // v_mfma_i32_16x16x64_i8 is the same on 16 rows: lane l holds row l % 16 at k = 16 (l / 16), and D[i][j] sits in lane
 // j + 16 (i / 4), register i % 4.
 //
-// k_i8_rows: for few rows per matrix, where the weights' bytes are the time.  A workgroup takes 16 weight rows (PAIRED: 16
-// channels, their gate and up rows) and a tile of up to 16 TT tokens.  Its NW waves split the reduction, so that a matrix
-// of few rows still has every load in flight at once, U operands of 1 KB per wave before the first product; their
-// int32 sums meet in LDS (exact in any order).
-template <int NW, int TT, bool PAIRED, int DT>
-__device__ __forceinline__ void i8_rows_product(const I8Args& g, const Tile& tl, int* red)
+// k_i8_rows: for few rows per matrix, where the weights' bytes are the time.  A workgroup takes RT tiles of 16 weight rows
+// (PAIRED: of 16 channels, their gate and up rows) by a tile of up to 16 TT tokens, both straight from memory to registers:
+// its NW waves split the reduction, so no operand is wanted by two of them, and a matrix of few rows still has loads in
+// flight everywhere.  A wave keeps U steps of 64 columns ahead; the waves' int32 sums meet in LDS by atomic additions (exact
+// in any order).
+template <int NW, int RT, int TT, bool PAIRED, int DT>
+__device__ __forceinline__ void i8_rows_product(const I8Args& g, const Tile& tl, int* red, uint32_t* orow, float* dxs)
 {
-    constexpr int NB = PAIRED ? 2 : 1, U = PAIRED || TT > 2 ? 4 : 8;
+    constexpr int NB = PAIRED ? 2 : 1, NR = RT * NB, U = NR + TT <= 3 ? 8 : NR + TT <= 6 ? 4 : NR + TT <= 8 ? 3 : 2;
     const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, q = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int bx = blockIdx.x;
+    const int bx = blockIdx.x, tiles16 = g.rgs * 2 / NB;  // the matrix's row (channel) tiles of 16
     const int8_t* xr[TT];
 #pragma unroll
     for (int t = 0; t < TT; t++) {
         const int at = tl.start + min(16 * t + r16, tl.cnt - 1);
         xr[t] = g.xq + (int64_t)((g.perm ? g.perm[at] : at) / g.div) * g.cols;
     }
-    const int8_t* wb = g.w + (int64_t)tl.e * g.mat_bytes + (int64_t)(bx >> 1) * NB * g.kc * 512 + (bx & 1) * 256 + q * 512 + r16 * 16;
-    i32x4 acc[TT][NB];
+    const int8_t* wb[NR];
 #pragma unroll
-    for (int t = 0; t < TT; t++)
-#pragma unroll
-        for (int b = 0; b < NB; b++) acc[t][b] = i32x4{0, 0, 0, 0};
-    const int steps = g.kc / 4, s0 = wave * steps / NW, s1 = (wave + 1) * steps / NW;
-    for (int s = s0; s < s1; s += U) {
-        i32x4 w[U][NB], x[U][TT];
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int su = min(s + u, s1 - 1), k = 64 * su + 16 * q;
-#pragma unroll
-            for (int b = 0; b < NB; b++) w[u][b] = *(const i32x4*)(wb + (int64_t)b * g.kc * 512 + (int64_t)su * 2048);
-#pragma unroll
-            for (int t = 0; t < TT; t++) x[u][t] = *(const i32x4*)(xr[t] + (k < g.cols ? k : 0));  // the weights past cols are 0
-        }
-        __builtin_amdgcn_sched_barrier(0);  // every load before the first wait
-#pragma unroll
-        for (int u = 0; u < U; u++)
-            if (s + u < s1)  // uniform
-#pragma unroll
-                for (int t = 0; t < TT; t++)
-#pragma unroll
-                    for (int b = 0; b < NB; b++)
-                        acc[t][b] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x[u][t], w[u][b], acc[t][b], 0, 0, 0);
-    }
-#pragma unroll
-    for (int t = 0; t < TT; t++)
-#pragma unroll
-        for (int b = 0; b < NB; b++)
-#pragma unroll
-            for (int v = 0; v < 4; v++) red[(((wave * TT + t) * NB + b) * 4 + v) * 64 + lane] = acc[t][b][v];
-    __syncthreads();
-    for (int o = tid; o < tl.cnt * 16; o += 64 * NW) {
-        const int r = o & 15, tok = o >> 4, t = tok >> 4, i = tok & 15, l = r + 16 * (i >> 2);
-        int sum[NB];
+    for (int r = 0; r < RT; r++)
 #pragma unroll
         for (int b = 0; b < NB; b++) {
-            sum[b] = 0;
-#pragma unroll
-            for (int w = 0; w < NW; w++) sum[b] += red[(((w * TT + t) * NB + b) * 4 + (i & 3)) * 64 + l];
+            const int i = min(bx * RT + r, tiles16 - 1);
+            wb[r * NB + b] = g.w + (int64_t)tl.e * g.mat_bytes + ((int64_t)(i >> 1) * NB + b) * g.kc * 512 + (i & 1) * 256;
         }
-        const int a = g.perm ? g.perm[tl.start + tok] : tl.start + tok;
-        const float dx = g.xd[a / g.div];
-        const float* sc = g.scale + (int64_t)tl.e * g.mat_scales + (bx >> 1) * NB * 32 + (bx & 1) * 16 + r;
-        const int col = bx * 16 + r;
-        if (col >= g.out_cols) continue;
-        float y = (float)sum[0] * (dx * sc[0]);
-        if (PAIRED) y = gated(g, y, (float)sum[NB - 1] * (dx * sc[32]));
-        store_one<DT>(g.out, (int64_t)a * g.out_cols + col, y);
+    const int lo = q * 512 + r16 * 16;
+    // the epilogue's: a thread keeps one column, C threads a token, P tokens at a time
+    constexpr int C = RT * 16, P = 64 * NW / C;
+    const int c = tid % C, col = bx * C + c;
+    float sg = 0.0f, su = 0.0f;
+    if (col < g.out_cols) {
+        const float* sc = g.scale + (int64_t)tl.e * g.mat_scales + (col >> 5) * NB * 32 + (col & 31);
+        sg = sc[0];
+        if (PAIRED) su = sc[32];
+    }
+    if (tid < TT * 16) tile_rows<DT>(g, tl, tid, orow, dxs);
+    for (int o = tid; o < NR * TT * 256; o += 64 * NW) red[o] = 0;
+    i32x4 acc[TT][NR], w[U][NR], x[U][TT];
+#pragma unroll
+    for (int t = 0; t < TT; t++)
+#pragma unroll
+        for (int r = 0; r < NR; r++) acc[t][r] = i32x4{0, 0, 0, 0};
+    const int steps = g.kc / 4, s0 = wave * steps / NW, s1 = (wave + 1) * steps / NW;
+    auto load = [&](int u, int s) {
+        const int su = min(s, s1 - 1), k = 64 * su + 16 * q, kx = k < g.cols ? k : 0;  // the weights past cols are zero
+#pragma unroll
+        for (int r = 0; r < NR; r++) w[u][r] = *(const i32x4*)(wb[r] + (int64_t)su * 2048 + lo);
+#pragma unroll
+        for (int t = 0; t < TT; t++) x[u][t] = *(const i32x4*)(xr[t] + kx);
+    };
+    auto mma = [&](int u) {
+#pragma unroll
+        for (int t = 0; t < TT; t++)
+#pragma unroll
+            for (int r = 0; r < NR; r++)
+                acc[t][r] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x[u][t], w[u][r], acc[t][r], 0, 0, 0);
+    };
+    if (s0 < s1) {  // uniform over the wave
+#pragma unroll
+        for (int u = 0; u < U; u++) load(u, s0 + u);
+        int s = s0;
+        for (; s + U < s1; s += U)
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                mma(u);
+                load(u, s + u + U);
+            }
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (s + u < s1) mma(u);
+    }
+    __syncthreads();  // the zeros are there
+#pragma unroll
+    for (int t = 0; t < TT; t++)
+#pragma unroll
+        for (int r = 0; r < NR; r++)
+#pragma unroll
+            for (int v = 0; v < 4; v++) atomicAdd(&red[((t * NR + r) * 4 + v) * 64 + lane], acc[t][r][v]);
+    __syncthreads();
+    if (col >= g.out_cols) return;
+    char* out = out_base<DT>(g, tl);
+#pragma unroll
+    for (int it = 0; it < (TT * 16 + P - 1) / P; it++) {
+        const int tok = it * P + tid / C, i = tok & 15;
+        if (tok >= tl.cnt) break;
+        const int at = (((tok >> 4) * NR + (c >> 4) * NB) * 4 + (i & 3)) * 64 + (c & 15) + 16 * (i >> 2);
+        float y = (float)red[at] * (dxs[tok] * sg);
+        if (PAIRED) y = gated(g.act, y, (float)red[at + 256] * (dxs[tok] * su));
+        store_one<DT>(out + orow[tok], col, y);
     }
 }
 
 // CT: the most token tiles of 16 that a tile may hold (its capacity); a tile takes the product of its own count
-template <int NW, int CT, bool PAIRED, int DT>
+template <int NW, int RT, int CT, bool PAIRED, int DT>
 __global__ __launch_bounds__(64 * NW) void k_i8_rows(I8Args g)
 {
-    __shared__ int red[NW * CT * (PAIRED ? 2 : 1) * 256];
+    __shared__ int red[RT * CT * (PAIRED ? 2 : 1) * 256];
+    __shared__ uint32_t orow[CT * 16];
+    __shared__ float dxs[CT * 16];
     Tile tl;
     if (!i8_tile(g, blockIdx.y, &tl)) return;  // uniform over the workgroup
     const int n = (tl.cnt + 15) / 16;
-    if (CT == 1 || n == 1) i8_rows_product<NW, 1, PAIRED, DT>(g, tl, red);
-    else if (CT == 2 || n == 2) i8_rows_product<NW, CT < 2 ? 1 : 2, PAIRED, DT>(g, tl, red);
-    else if (CT == 4 || n <= 4) i8_rows_product<NW, CT < 4 ? 1 : 4, PAIRED, DT>(g, tl, red);
-    else i8_rows_product<NW, CT < 8 ? 1 : 8, PAIRED, DT>(g, tl, red);
+    if (CT == 1 || n == 1) i8_rows_product<NW, RT, 1, PAIRED, DT>(g, tl, red, orow, dxs);
+    else if (CT == 2 || n == 2) i8_rows_product<NW, RT, CT < 2 ? 1 : 2, PAIRED, DT>(g, tl, red, orow, dxs);
+    else if (CT == 4 || n <= 4) i8_rows_product<NW, RT, CT < 4 ? 1 : 4, PAIRED, DT>(g, tl, red, orow, dxs);
+    else i8_rows_product<NW, RT, CT < 8 ? 1 : 8, PAIRED, DT>(g, tl, red, orow, dxs);
 }
 
 // The down products of few assignments and their weighted sum, for a token (blockIdx.y) and 16 of its outputs: wave w takes
@@ -360,18 +454,20 @@ __global__ __launch_bounds__(64 * NW) void k_i8_down_few(I8Args g, int k, int nf
 // tokens.  The weights go straight from memory to each wave's registers (the layout has every operand as one run of
 // 1 KB, and no other wave of the workgroup wants it), one 128-column step ahead; the tokens, which all four waves read, go
 // through an LDS ring by direct loads two steps ahead, row-major runs of 128 bytes with the 16-byte chunks XOR-swizzled by
-// the row (an operand's 8 consecutive lanes hit all 32 banks).
-constexpr int TI_RING = 3;
+// half the row's number: LDS serves a 16-byte read in four turns of 16 lanes, {0-3, 12-15, 20-27}, {4-11, 16-19, 28-31} and the
+// same from lane 32, over 64 banks, and each turn then has 16 distinct bank groups (by the row's number itself, two rows of
+// a turn share one: 8 cycles a read against 4).
+constexpr int TI_RING = 3, TI_PITCH = 68;  // ring slots; ints between two tokens' rows of 64 in the epilogue
 
 template <int NT, bool PAIRED, int DT>
-__device__ __forceinline__ void i8_tile_product(const I8Args& g, const Tile& tl, int bx, unsigned char* ring, int* orow, float* dxs)
+__device__ __forceinline__ void i8_tile_product(const I8Args& g, const Tile& tl, int bx, unsigned char* ring, uint32_t* orow, float* dxs)
 {
     constexpr int STAGE = NT * 32 * 128;
     const int tid = threadIdx.x, lane = tid & 63, r32 = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int S = g.kc / 8;
     // this lane's rows of the direct loads: one per load, the last row again past the tile's end
-    const int chunk = ((lane & 7) ^ (lane >> 3)) * 16;
+    const int chunk = ((lane & 7) ^ (lane >> 4)) * 16;  // of the loads whose first row is a multiple of 16; 4 chunks on for 8
     const __amdgpu_buffer_rsrc_t rsrc = buf_rsrc(g.xq + (g.perm ? 0 : (int64_t)tl.start * g.cols));
     uint32_t xr[NT];  // a list's rows lie within 2^32 bytes of xq (phx_experts_i8's chunks), a dense tile's of its first
 #pragma unroll
@@ -379,31 +475,24 @@ __device__ __forceinline__ void i8_tile_product(const I8Args& g, const Tile& tl,
         const int at = min(8 * (wave * NT + i) + (lane >> 3), tl.cnt - 1);
         xr[i] = (uint32_t)(g.perm ? g.perm[tl.start + at] / g.div : at) * (uint32_t)g.cols;
     }
-    if (tid < NT * 32) {
-        const int at = tl.start + min(tid, tl.cnt - 1);
-        const int a = g.perm ? g.perm[at] : at;
-        orow[tid] = a;
-        dxs[tid] = g.xd[g.perm ? a / g.div : a];
-    }
-    auto dma = [&](int s) {
-        const uint32_t off = min(s, S - 1) * 128 + chunk, o = off < (uint32_t)g.cols ? off : 0;  // the weights past cols are 0
-        unsigned char* to = ring + (s % TI_RING) * STAGE + wave * NT * 1024;
-#pragma unroll
-        for (int i = 0; i < NT; i++)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void_t)(to + i * 1024), 16, xr[i] + o, 0, 0, 0);
+    if (tid < NT * 32) tile_rows<DT>(g, tl, tid, orow, dxs);
+    int slot = 0, slot1 = STAGE, slot2 = 2 * STAGE;  // the ring's slots of a step and the two after it
+    auto dma = [&](int s, int to, auto I) {          // load I of step s's rows
+        constexpr int i = decltype(I)::value;
+        const uint32_t off = min(s, S - 1) * 128 + (chunk ^ (64 * ((wave * NT + i) & 1)));
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void_t)(ring + to + (wave * NT + i) * 1024), 16,
+                                                 xr[i] + (off < (uint32_t)g.cols ? off : 0), 0, 0, 0);  // the weights past cols are zero
     };
     const int rg0 = (bx * 4 + wave) * 2, rgs = g.rgs;
     const int8_t* wb[2];
 #pragma unroll
     for (int b = 0; b < 2; b++)
         wb[b] = g.w + (int64_t)tl.e * g.mat_bytes + (int64_t)min(rg0 + b, rgs - 1) * g.kc * 512;
+    const uint32_t lane16 = lane * 16;
     i32x4 wv[2][2][4];
-    auto weights = [&](int s, auto P) {
-        const int64_t o = (int64_t)min(s, S - 1) * 4096;
-#pragma unroll
-        for (int b = 0; b < 2; b++)
-#pragma unroll
-            for (int kk = 0; kk < 4; kk++) wv[decltype(P)::value][b][kk] = *(const i32x4*)(wb[b] + o + kk * 1024 + lane * 16);
+    auto weight = [&](int s, int b, auto P, auto KK) {
+        const int8_t* at = wb[b] + (int64_t)min(s, S - 1) * 4096 + decltype(KK)::value * 1024;  // uniform
+        wv[decltype(P)::value][b][decltype(KK)::value] = *(const i32x4*)(at + lane16);
     };
     i32x16 acc[NT][2];
 #pragma unroll
@@ -412,91 +501,156 @@ __device__ __forceinline__ void i8_tile_product(const I8Args& g, const Tile& tl,
         for (int b = 0; b < 2; b++)
 #pragma unroll
             for (int v = 0; v < 16; v++) acc[j][b][v] = 0;
-    const uint32_t lds = (uint32_t)(uintptr_t)(lds_void_t)ring + r32 * 128, swz = (h ^ (r32 & 7)) * 16;
+    const uint32_t lds = (uint32_t)(uintptr_t)(lds_void_t)ring + r32 * 128, swz = (h ^ ((r32 >> 1) & 7)) * 16;
+    u32x4 a[2][NT];
+    auto read = [&](int from, auto KK) {
+        constexpr int kk = decltype(KK)::value;
+        const uint32_t ad = lds + from + (swz ^ (kk * 32));
+        static_for<NT>([&](auto J) { a[kk & 1][decltype(J)::value] = ds_r128<decltype(J)::value * 4096>(ad); });
+    };
+    auto landed = [&](auto Q) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int j = 0; j < NT; j++) tie(a[decltype(Q)::value][j]);
+    };
+    // A step is four groups of products on 32 columns.  A group first reads the next one's tokens (the last: the next step's,
+    // once its rows have landed in every wave, which also says that nobody reads this step's slot any more), and among its
+    // products issues the loads: the weights that the group before has just used the registers of, two steps on, and
+    // one load of the rows two steps on.  The order is fixed by scheduling barriers: the wait for the rows counts the loads
+    // issued after them.
+    constexpr int NEWER = 6 + (NT < 3 ? NT : 3) + 2 * (4 - NT);
     auto step = [&](int s, auto P) {
         constexpr int p = decltype(P)::value;
-        __builtin_amdgcn_s_waitcnt(vm_wait(NT + 8));  // step s's rows have landed (step s + 1's and its weights may not)
-        __builtin_amdgcn_s_barrier();                 // in every wave, and nobody reads slot s + 2 any more
-        __builtin_amdgcn_sched_barrier(0);
-        dma(s + 2);
-        weights(s + 1, ic<1 - p>{});
-        __builtin_amdgcn_sched_barrier(0);
-        const uint32_t at = lds + (s % TI_RING) * STAGE;
-        u32x4 a[2][NT];
-        auto read = [&](auto KK) {
-            constexpr int kk = decltype(KK)::value;
-            const uint32_t ad = at + (swz ^ (kk * 32));
-            static_for<NT>([&](auto J) { a[kk & 1][decltype(J)::value] = ds_r128<decltype(J)::value * 4096>(ad); });
-        };
-        read(ic<0>{});
         static_for<4>([&](auto KK) {
             constexpr int kk = decltype(KK)::value;
-            if constexpr (kk < 3) read(ic<kk + 1>{});
-            asm volatile("s_waitcnt lgkmcnt(%0)" ::"i"(kk < 3 ? NT : 0) : "memory");
-#pragma unroll
-            for (int j = 0; j < NT; j++) tie(a[kk & 1][j]);
-#pragma unroll
-            for (int j = 0; j < NT; j++)
-#pragma unroll
-                for (int b = 0; b < 2; b++)
-                    acc[j][b] = __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4, a[kk & 1][j]), wv[p][b][kk],
-                                                                      acc[j][b], 0, 0, 0);
+            if constexpr (kk < 3) read(slot, ic<kk + 1>{});
+            else {
+                __builtin_amdgcn_s_waitcnt(vm_wait(NEWER));
+                __builtin_amdgcn_s_barrier();
+                read(slot1, ic<0>{});
+            }
+            static_for<2 * NT>([&](auto M) {
+                constexpr int m = decltype(M)::value, j = m / 2, b = m % 2;
+                __builtin_amdgcn_sched_barrier(0);
+                acc[j][b] = __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4, a[kk & 1][j]), wv[p][b][kk], acc[j][b],
+                                                                  0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);
+                if constexpr (m == 0 || m == 1) {
+                    if constexpr (kk == 0) weight(s + 1, m, ic<1 - p>{}, ic<3>{});
+                    else weight(s + 2, m, ic<p>{}, ic<kk - 1>{});
+                }
+                if constexpr (m == (NT > 1 ? 3 : 1)) {
+                    if constexpr (kk < NT) dma(s + 2, slot2, ic<kk < NT ? kk : 0>{});
+                }
+            });
+            __builtin_amdgcn_sched_barrier(0);
+            landed(ic<(kk + 1) & 1>{});
         });
+        const int done = slot;
+        slot = slot1;
+        slot1 = slot2;
+        slot2 = done;
     };
-    dma(0);
-    dma(1);
-    weights(0, ic<0>{});
+    static_for<NT>([&](auto I) { dma(0, slot, I); });
+    static_for<NT>([&](auto I) { dma(1, slot1, I); });
+    static_for<4>([&](auto KK) {
+        weight(0, 0, ic<0>{}, KK);
+        weight(0, 1, ic<0>{}, KK);
+    });
+    static_for<3>([&](auto KK) {
+        weight(1, 0, ic<1>{}, KK);
+        weight(1, 1, ic<1>{}, KK);
+    });
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(vm_wait(NT + 14));
+    __builtin_amdgcn_s_barrier();
+    read(slot, ic<0>{});
+    landed(ic<0>{});
     for (int s = 0; s + 1 < S; s += 2) {
         step(s, ic<0>{});
         step(s + 1, ic<1>{});
     }
     if (S & 1) step(S - 1, ic<0>{});
-    const float* sc = g.scale + (int64_t)tl.e * g.mat_scales;
-    float dw[2];
-#pragma unroll
-    for (int b = 0; b < 2; b++) dw[b] = sc[min(rg0 + b, rgs - 1) * 32 + r32];
-    // the scales have landed before the first store (a later wait for them would wait for the stores too), and the direct
-    // loads past the last step before the workgroup's LDS goes
-    __builtin_amdgcn_s_waitcnt(0);
+    __builtin_amdgcn_s_waitcnt(0);  // the direct loads past the last step land before the workgroup's LDS goes
     __syncthreads();
+    char* out = out_base<DT>(g, tl);
+    const float* sc = g.scale + (int64_t)tl.e * g.mat_scales;
+    // Each 32 tokens' sums go through the wave's own part of the ring, so that a lane stores 16 bytes of one token's row: straight
+    // from the accumulators an instruction stores 4 or 2 bytes a lane, and the stores alone took a third of the time.
+    constexpr int V = DT == PHX_F32 ? 4 : 8, WC = PAIRED ? 32 : 64, LPT = WC / V, TPI = 64 / LPT;  // lanes a token, tokens a round
+    int* mine = (int*)ring + wave * 32 * TI_PITCH;
+    const int col0 = PAIRED ? (rg0 >> 1) * 32 : rg0 * 32, c = (lane % LPT) * V, col = col0 + c;
+    float dw[V], du[V];
 #pragma unroll
-    for (int j = 0; j < NT; j++)
+    for (int i = 0; i < V; i++) {
+        const int r = min(rg0 * 32 + c + i, rgs * 32 - 1);
+        dw[i] = sc[r];
+        du[i] = PAIRED ? sc[min(r + 32, rgs * 32 - 1)] : 0.0f;
+    }
+    const bool whole = g.out_cols % V == 0;  // rows and columns then start on 16 bytes
+    __builtin_amdgcn_s_waitcnt(0);           // the scales: a later wait for them would wait for the stores before it too
 #pragma unroll
-        for (int v = 0; v < 16; v++) {
-            const int tok = 32 * j + 8 * (v >> 2) + 4 * h + (v & 3);
-            if (tok >= tl.cnt) continue;
-            const float dx = dxs[tok];
-            const int64_t o = (int64_t)orow[tok] * g.out_cols;
-            if (PAIRED) {
-                const int col = (rg0 >> 1) * 32 + r32;
-                if (col < g.out_cols)
-                    store_one<DT>(g.out, o + col, gated(g, (float)acc[j][0][v] * (dx * dw[0]), (float)acc[j][1][v] * (dx * dw[1])));
+    for (int j = 0; j < NT; j++) {
+#pragma unroll
+        for (int b = 0; b < 2; b++)
+#pragma unroll
+            for (int v = 0; v < 16; v++) mine[(8 * (v >> 2) + 4 * h + (v & 3)) * TI_PITCH + 32 * b + r32] = acc[j][b][v];
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        // rolled: a workgroup runs this once, and the instructions of it unrolled took longer to fetch than to run
+#pragma unroll 1
+        for (int tok = lane / LPT; tok < 32; tok += TPI) {
+            const float dx = dxs[32 * j + tok];
+            char* o = out + orow[32 * j + tok];
+            int s[V], u[V];
+#pragma unroll
+            for (int i = 0; i < V; i += 4) {
+                *(int4*)(s + i) = *(const int4*)(mine + tok * TI_PITCH + c + i);
+                if (PAIRED) *(int4*)(u + i) = *(const int4*)(mine + tok * TI_PITCH + 32 + c + i);
+            }
+            float y[V];
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                y[i] = (float)s[i] * (dx * dw[i]);
+                if (PAIRED) y[i] = gated(g.act, y[i], (float)u[i] * (dx * du[i]));
+            }
+            if (whole) {
+                if (col < g.out_cols) store_16<DT>(o, col, y);
             } else {
 #pragma unroll
-                for (int b = 0; b < 2; b++) {
-                    const int col = (rg0 + b) * 32 + r32;
-                    if (col < g.out_cols) store_one<DT>(g.out, o + col, (float)acc[j][b][v] * (dx * dw[b]));
-                }
+                for (int i = 0; i < V; i++)
+                    if (col + i < g.out_cols) store_one<DT>(o, col + i, y[i]);
             }
         }
+        // this tile's reads end before the next one's writes
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
 }
 
 template <bool PAIRED, int DT>
 __global__ __launch_bounds__(256, 2) void k_i8_tile(I8Args g)
 {
     __shared__ __align__(16) unsigned char ring[TI_RING * 128 * 128];
-    __shared__ int orow[128];
-    __shared__ float dxs[128];
-    // workgroup L runs on XCD L % 8: it takes tile 8 (k / gridDim.x) + L % 8 and row block k % gridDim.x, k = L / 8, so a
-    // tile's row blocks share that XCD's L2 for the tile's rows
-    const int gx = gridDim.x, L = blockIdx.y * gx + blockIdx.x, k = L >> 3;
+    static_assert(sizeof(ring) >= 4 * 32 * TI_PITCH * 4, "the epilogue's part of each wave");
+    __shared__ __align__(16) uint32_t orow[128];
+    __shared__ __align__(16) float dxs[128];
+    // Workgroup L runs on XCD L % 8.  The XCDs share the tiles in xt parts and the row blocks in 8 / xt; an XCD takes runs of
+    // tiles of its part, and of a run's row blocks by tiles 8 row blocks at a time, tile by tile: what it runs together
+    // shares few rows of both operands in its L2.
+    const int L = blockIdx.x, k = L >> 3, xcd = L & 7, per = g.run * g.blocks, in = k % per;
+    const int band = in / (8 * g.run), wide = min(8, g.blocks - 8 * band), at = in - band * 8 * g.run;
+    const int tile = ((k / per) * g.xt + xcd % g.xt) * g.run + at / wide, bx = xcd / g.xt * g.blocks + band * 8 + at % wide;
+    if (bx * 8 >= g.rgs) return;
     Tile tl;
-    if (!i8_tile(g, 8 * (k / gx) + (L & 7), &tl)) return;  // uniform over the workgroup
+    if (!i8_tile(g, tile, &tl)) return;  // uniform over the workgroup
     switch ((tl.cnt + 31) / 32) {
-    case 1: i8_tile_product<1, PAIRED, DT>(g, tl, k % gx, ring, orow, dxs); break;
-    case 2: i8_tile_product<2, PAIRED, DT>(g, tl, k % gx, ring, orow, dxs); break;
-    case 3: i8_tile_product<3, PAIRED, DT>(g, tl, k % gx, ring, orow, dxs); break;
-    default: i8_tile_product<4, PAIRED, DT>(g, tl, k % gx, ring, orow, dxs);
+    case 1: i8_tile_product<1, PAIRED, DT>(g, tl, bx, ring, orow, dxs); break;
+    case 2: i8_tile_product<2, PAIRED, DT>(g, tl, bx, ring, orow, dxs); break;
+    case 3: i8_tile_product<3, PAIRED, DT>(g, tl, bx, ring, orow, dxs); break;
+    default: i8_tile_product<4, PAIRED, DT>(g, tl, bx, ring, orow, dxs);
     }
 }
 
@@ -513,36 +667,71 @@ static void set_matrix(I8Args& g, const I8Mat& m)
     g.n_expert = m.n_mat;
 }
 
-template <int NW, int CT>
-static void rows_product(hipStream_t st, const I8Mat& m, const I8Args& g, int max_tiles, int out_type)
+#ifndef I8_E_NW
+#define I8_E_NW 4
+#define I8_E_RT 2
+#endif
+template <int NW, int RT, int CT>
+static void rows_dense(hipStream_t st, const I8Args& g, int max_tiles, int out_type)
 {
-    const dim3 grid((g.out_cols + 15) / 16, max_tiles), blk(64 * NW);
-    if (m.paired) launch(k_i8_rows<NW, CT < 8 ? CT : 4, true, PHX_F32>, grid, blk, 0, st, g);
-    else if (out_type == PHX_F16) launch(k_i8_rows<NW, CT, false, PHX_F16>, grid, blk, 0, st, g);
-    else if (out_type == PHX_BF16) launch(k_i8_rows<NW, CT, false, PHX_BF16>, grid, blk, 0, st, g);
-    else launch(k_i8_rows<NW, CT, false, PHX_F32>, grid, blk, 0, st, g);
+    const dim3 grid((g.out_cols + 16 * RT - 1) / (16 * RT), max_tiles), blk(64 * NW);
+    if (out_type == PHX_F16) launch(k_i8_rows<NW, RT, CT, false, PHX_F16>, grid, blk, 0, st, g);
+    else if (out_type == PHX_BF16) launch(k_i8_rows<NW, RT, CT, false, PHX_BF16>, grid, blk, 0, st, g);
+    else launch(k_i8_rows<NW, RT, CT, false, PHX_F32>, grid, blk, 0, st, g);
 }
-
-template <int NW>
-static void rows_product(hipStream_t st, const I8Mat& m, const I8Args& g, int max_tiles, int out_type)
+template <int NW, int RT, int CT>
+static void rows_grouped(hipStream_t st, const I8Mat& m, const I8Args& g, int max_tiles)
 {
-    if (g.cap <= 16) rows_product<NW, 1>(st, m, g, max_tiles, out_type);
-    else if (g.cap <= 32) rows_product<NW, 2>(st, m, g, max_tiles, out_type);
-    else if (g.cap <= 64) rows_product<NW, 4>(st, m, g, max_tiles, out_type);
-    else rows_product<NW, 8>(st, m, g, max_tiles, out_type);
+    const dim3 grid((g.out_cols + 16 * RT - 1) / (16 * RT), max_tiles), blk(64 * NW);
+    if (m.paired) launch(k_i8_rows<NW, RT, CT, true, PHX_F32>, grid, blk, 0, st, g);
+    else launch(k_i8_rows<NW, RT, CT, false, PHX_F32>, grid, blk, 0, st, g);
 }
 
 void launch_i8_product(hipStream_t st, const I8Mat& m, I8Args g, bool tile, int max_tiles, int ncu, int out_type)
 {
     set_matrix(g, m);
     if (tile) {
-        const dim3 grid((m.rg + 7) / 8, (max_tiles + 7) / 8 * 8), blk(256);
+        // Lists: every XCD takes pairs of tiles (mostly of one expert: its second tile finds the weights in the L2) and all their
+        // row blocks.  A dense product: the split with the fewest workgroups on an XCD, and of those the one that brings
+        // the fewest bytes to the XCDs, each its tiles' tokens and its blocks' weights.
+        const int blocks = (m.rg + 7) / 8;
+        g.xt = 8;
+        g.run = 2;
+        if (!g.tiles) {
+            int64_t least = INT64_MAX;
+            for (int xt = 1; xt <= 8; xt *= 2) {
+                const int64_t t = (max_tiles + xt - 1) / xt, b = (blocks + 8 / xt - 1) / (8 / xt);
+                const int64_t cost = (t * b << 32) + t * xt * kI8Tile * (8 / xt) + b * (8 / xt) * 256 * xt;
+                if (cost < least) {
+                    least = cost;
+                    g.xt = xt;
+                    g.run = (int)t;
+                }
+            }
+        }
+        g.blocks = (blocks + 8 / g.xt - 1) / (8 / g.xt);
+        const int per = g.xt * g.run;
+        const dim3 grid((max_tiles + per - 1) / per * g.run * g.blocks * 8), blk(256);
         if (m.paired) launch(k_i8_tile<true, PHX_F32>, grid, blk, 0, st, g);
         else if (out_type == PHX_F16) launch(k_i8_tile<false, PHX_F16>, grid, blk, 0, st, g);
         else if (out_type == PHX_BF16) launch(k_i8_tile<false, PHX_BF16>, grid, blk, 0, st, g);
         else launch(k_i8_tile<false, PHX_F32>, grid, blk, 0, st, g);
-    } else if ((int64_t)((g.out_cols + 15) / 16) * max_tiles < 4 * ncu) rows_product<8>(st, m, g, max_tiles, out_type);
-    else rows_product<4>(st, m, g, max_tiles, out_type);
+    } else if (!g.tiles && !g.ids) {
+        if (g.cap <= 16) rows_dense<8, 1, 1>(st, g, max_tiles, out_type);
+        else if (g.cap <= 32) rows_dense<8, 1, 2>(st, g, max_tiles, out_type);
+        else {  // the widest row tile that still gives every compute unit a workgroup
+            const int64_t n = (int64_t)((g.out_cols + 15) / 16) * max_tiles;
+            if (g.cap <= 64) {
+                if (n < 2 * ncu) rows_dense<8, 1, 4>(st, g, max_tiles, out_type);
+                else rows_dense<8, 2, 4>(st, g, max_tiles, out_type);
+            } else if (n < 2 * ncu) rows_dense<8, 1, 8>(st, g, max_tiles, out_type);
+            else if (n < 4 * ncu) rows_dense<8, 2, 8>(st, g, max_tiles, out_type);
+            else rows_dense<8, 4, 8>(st, g, max_tiles, out_type);
+        }
+    } else if (g.ids) rows_grouped<8, 1, 1>(st, m, g, max_tiles);
+    else if (g.cap <= 16) rows_grouped<I8_E_NW, I8_E_RT, 1>(st, m, g, max_tiles);
+    else if (g.cap <= 32) rows_grouped<I8_E_NW, I8_E_RT, 2>(st, m, g, max_tiles);
+    else rows_grouped<I8_E_NW, I8_E_RT, 4>(st, m, g, max_tiles);
 }
 
 template <int NW>
@@ -569,19 +758,28 @@ void launch_i8_down_few(hipStream_t st, const I8Mat& m, int T, int k, const floa
 }
 
 // ------------------------------------------------------------------------------ experts
-// Each expert's assignments as one run of perm and as tiles of up to cap; ids outside [0, E) are in no run.  The order
-// inside a run is the atomics' and no result depends on it: a place of the list names its own input and output row.
+// Each expert's assignments as one run of perm and as tiles of up to cap; ids outside [0, E) are in no run.  One workgroup
+// takes up to 1024 IPT assignments: an id's place in its run is what its counter's atomic addition returns, kept in a
+// register, and the runs are put together in LDS and stored whole.  The order inside a run is the atomics' and no result
+// depends on it: a place of the list names its own input and output row.
+template <int IPT>
 __global__ __launch_bounds__(1024) void k_i8_lists(int n, int E, int cap, const int* __restrict__ ids, int* __restrict__ perm,
                                                    Tile* __restrict__ tiles, int* __restrict__ ntiles)
 {
-    __shared__ int count[PHX_MAX_EXPERTS_DEV], start[PHX_MAX_EXPERTS_DEV], first[PHX_MAX_EXPERTS_DEV];
+    __shared__ int count[PHX_MAX_EXPERTS_DEV], start[PHX_MAX_EXPERTS_DEV], first[PHX_MAX_EXPERTS_DEV], total;
+    __shared__ uint16_t list[1024 * IPT];
     const int tid = threadIdx.x;
     if (tid < PHX_MAX_EXPERTS_DEV) count[tid] = 0;
-    __syncthreads();
-    for (int a = tid; a < n; a += 1024) {
-        const int e = ids[a];
-        if ((unsigned)e < (unsigned)E) atomicAdd(&count[e], 1);
+    uint32_t place[IPT];  // expert << 16 | place in its run
+#pragma unroll
+    for (int i = 0; i < IPT; i++) {
+        const int a = i * 1024 + tid;
+        place[i] = a < n ? (uint32_t)min((unsigned)ids[a], 0xFFFFu) << 16 : 0xFFFF0000u;
     }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < IPT; i++)
+        if ((place[i] >> 16) < (unsigned)E) place[i] |= (uint32_t)atomicAdd(&count[place[i] >> 16], 1);
     __syncthreads();
     if (tid < 64) {  // prefix sums over the experts, four to a lane
         int c[4], t[4], sc = 0, stl = 0;
@@ -593,7 +791,10 @@ __global__ __launch_bounds__(1024) void k_i8_lists(int n, int E, int cap, const 
             stl += t[i];
         }
         int pc = wave_incl_scan_i(sc) - sc, pt = wave_incl_scan_i(stl) - stl;
-        if (tid == 63) *ntiles = pt + stl;
+        if (tid == 63) {
+            *ntiles = pt + stl;
+            total = pc + sc;
+        }
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             start[4 * tid + i] = pc;
@@ -607,16 +808,19 @@ __global__ __launch_bounds__(1024) void k_i8_lists(int n, int E, int cap, const 
         int at = start[tid], left = count[tid];
         for (int i = first[tid]; left > 0; i++, at += cap, left -= cap) tiles[i] = {tid, at, min(cap, left)};
     }
+#pragma unroll
+    for (int i = 0; i < IPT; i++)
+        if ((place[i] >> 16) < (unsigned)E) list[start[place[i] >> 16] + (place[i] & 0xFFFFu)] = (uint16_t)(i * 1024 + tid);
     __syncthreads();
-    for (int a = tid; a < n; a += 1024) {
-        const int e = ids[a];
-        if ((unsigned)e < (unsigned)E) perm[atomicAdd(&start[e], 1)] = a;
-    }
+    for (int p = tid; p < total; p += 1024) perm[p] = list[p];
 }
 
 void launch_i8_lists(hipStream_t st, int n, int E, int cap, const int* ids, int* perm, Tile* tiles, int* ntiles)
 {
-    launch(k_i8_lists, dim3(1), dim3(1024), 0, st, n, E, cap, ids, perm, tiles, ntiles);
+    const dim3 one(1), blk(1024);
+    if (n <= 2048) launch(k_i8_lists<2>, one, blk, 0, st, n, E, cap, ids, perm, tiles, ntiles);
+    else if (n <= 16384) launch(k_i8_lists<16>, one, blk, 0, st, n, E, cap, ids, perm, tiles, ntiles);
+    else launch(k_i8_lists<64>, one, blk, 0, st, n, E, cap, ids, perm, tiles, ntiles);
 }
 
 // out[t] = sum over the places j, in order, of w[t][j] * y[t k + j]; places without an expert are skipped
@@ -647,6 +851,18 @@ void launch_i8_combine(hipStream_t st, int T, int d, int k, int E, const float* 
     if (out_type == PHX_F16) launch(k_i8_combine<PHX_F16>, grid, blk, 0, st, d, k, E, y, ids, w, out);
     else if (out_type == PHX_BF16) launch(k_i8_combine<PHX_BF16>, grid, blk, 0, st, d, k, E, y, ids, w, out);
     else launch(k_i8_combine<PHX_F32>, grid, blk, 0, st, d, k, E, y, ids, w, out);
+}
+
+__global__ __launch_bounds__(256) void k_selftest_gated(int act, int n, const float* __restrict__ a, const float* __restrict__ b,
+                                                        float* __restrict__ out)
+{
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    if (i < n) out[i] = gated(act, a[i], b[i]);
+}
+
+void launch_selftest_gated(hipStream_t st, int act, int n, const float* a, const float* b, float* out)
+{
+    launch(k_selftest_gated, dim3((n + 255) / 256), dim3(256), 0, st, act, n, a, b, out);
 }
 
 }  // namespace phx

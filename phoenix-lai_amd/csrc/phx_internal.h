@@ -276,6 +276,7 @@ void launch_planar_act(hipStream_t st, int rows, int n, const int8_t* qs, const 
 void launch_planar_act_k(hipStream_t st, int rows, int n, const int8_t* qs, const float* d, Act a);
 void launch_selftest(hipStream_t st, int op, int n, const float* a, const float* b, float* out, const float* gelu_tab);
 void launch_selftest_seq(hipStream_t st, int m, int rows, const float* a, float* out);
+void launch_selftest_gated(hipStream_t st, int act, int n, const float* a, const float* b, float* out);
 
 
 // ---- routing and int8 products (kernels_route.hip, kernels_i8.hip)
@@ -316,6 +317,7 @@ struct I8Args {
     const float* scale;
     int64_t mat_bytes, mat_scales;
     int kc, cols, out_cols, rgs, n_expert;
+    int xt, run, blocks;  // the tile kernel's order: parts of the tiles, tiles of a run, row blocks of an XCD
 };
 // tile capacities: the tile kernel's, and the row kernel's most for paired and plain matrices (16, 32, 64 or 128)
 constexpr int kI8Tile = 128, kI8RowsPaired = 64, kI8Rows = 128;

@@ -7,11 +7,24 @@ namespace phx {
 
 __device__ __forceinline__ float bf2f(uint32_t h) { return __uint_as_float(h << 16); }
 
-// float -> bf16 bits, round to nearest even; a NaN keeps a set fraction bit
-__device__ __forceinline__ uint32_t f2bf(float v)
+typedef float rf2 __attribute__((ext_vector_type(2)));
+typedef __bf16 rbf2 __attribute__((ext_vector_type(2)));
+// two floats as bf16 bits, to nearest even
+__device__ __forceinline__ uint32_t f2bf_pair(float a, float b)
 {
-    const uint32_t b = __float_as_uint(v);
-    return v != v ? (b >> 16) | 0x40u : (b + 0x7FFFu + ((b >> 16) & 1u)) >> 16;
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((rf2{a, b}), rbf2));
+}
+// A float as fp16 bits, to nearest even.  The value is a float first: left to itself the compiler may round a product straight
+// to fp16, in one mixed instruction, in one kernel and not in another.
+__device__ __forceinline__ uint32_t f2h_of(float v)
+{
+    asm("" : "+v"(v));
+    return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v);
+}
+template <int DT>
+__device__ __forceinline__ uint32_t pair_of(float a, float b)
+{
+    return DT == PHX_F16 ? f2h_of(a) | (f2h_of(b) << 16) : f2bf_pair(a, b);
 }
 
 template <int DT>
@@ -40,19 +53,22 @@ __device__ __forceinline__ void load_eight(const void* p, int64_t i, float (&v)[
     }
 }
 
-// A product that is stored as fp16 is rounded to float first: left to itself the compiler may round it once, in one mixed
-// instruction, in one kernel and not in another.
-__device__ __forceinline__ uint32_t f2h_of(float v)
-{
-    asm("" : "+v"(v));
-    return f2h_bits(v);
-}
-
 template <int DT>
 __device__ __forceinline__ void store_one(void* p, int64_t i, float v)
 {
     if (DT == PHX_F32) ((float*)p)[i] = v;
-    else ((uint16_t*)p)[i] = (uint16_t)(DT == PHX_F16 ? f2h_of(v) : f2bf(v));
+    else ((uint16_t*)p)[i] = (uint16_t)(DT == PHX_F16 ? f2h_of(v) : f2bf_pair(v, 0.0f));
+}
+
+// 16 bytes of consecutive values (4 floats, 8 of the 16-bit types); p + i 16-byte aligned
+template <int DT, int V>
+__device__ __forceinline__ void store_16(void* p, int64_t i, const float (&v)[V])
+{
+    static_assert(V == (DT == PHX_F32 ? 4 : 8), "16 bytes");
+    if constexpr (DT == PHX_F32) *(float4*)((float*)p + i) = make_float4(v[0], v[1], v[2], v[3]);
+    else
+        *(uint4*)((uint16_t*)p + i) = make_uint4(pair_of<DT>(v[0], v[1]), pair_of<DT>(v[2], v[3]), pair_of<DT>(v[4], v[5]),
+                                                 pair_of<DT>(v[6], v[7]));
 }
 
 // four consecutive values; p + i aligned to four of them
@@ -60,9 +76,7 @@ template <int DT>
 __device__ __forceinline__ void store_four(void* p, int64_t i, float4 v)
 {
     if (DT == PHX_F32) *(float4*)((float*)p + i) = v;
-    else if (DT == PHX_F16)
-        *(uint2*)((uint16_t*)p + i) = make_uint2(f2h_of(v.x) | (f2h_of(v.y) << 16), f2h_of(v.z) | (f2h_of(v.w) << 16));
-    else *(uint2*)((uint16_t*)p + i) = make_uint2(f2bf(v.x) | (f2bf(v.y) << 16), f2bf(v.z) | (f2bf(v.w) << 16));
+    else *(uint2*)((uint16_t*)p + i) = make_uint2(pair_of<DT>(v.x, v.y), pair_of<DT>(v.z, v.w));
 }
 
 }  // namespace phx

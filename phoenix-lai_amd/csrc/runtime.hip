@@ -1913,7 +1913,7 @@ int phx_moe_profile_read(phx_moe_ctx* c, double* total_ms, int64_t* launches)
 
 int phx_moe_selftest(phx_moe_ctx* c, int op, int n, const float* a, const float* b, float* out)
 {
-    if (!c || n <= 0 || !a || !b || !out || op < 0 || op > 10 || ((op == 8 || op == 9) && n % 64)) return PHX_ERR_ARG;
+    if (!c || n <= 0 || !a || !b || !out || op < 0 || op > 12 || ((op == 8 || op == 9) && n % 64)) return PHX_ERR_ARG;
     int m = 0;  // op 10: the row length
     if (op == 10) {
         if (!(b[0] >= 2.0f && b[0] <= 65536.0f)) return PHX_ERR_ARG;
@@ -1929,6 +1929,7 @@ int phx_moe_selftest(phx_moe_ctx* c, int op, int n, const float* a, const float*
     HIPCHK(c, hipMemcpy(da, a, bytes, hipMemcpyHostToDevice));
     HIPCHK(c, hipMemcpy(db, b, bytes, hipMemcpyHostToDevice));
     if (op == 10) launch_selftest_seq(c->stream, m, n / m, da, dout);
+    else if (op > 10) launch_selftest_gated(c->stream, op == 11 ? PHX_QUANT_SILU_MUL : PHX_QUANT_GELU_MUL, n, da, db, dout);
     else launch_selftest(c->stream, op, n, da, db, dout, c->gelu_tab);
     HIPCHK(c, hipStreamSynchronize(c->stream));
     HIPCHK(c, hipMemcpy(out, dout, bytes, hipMemcpyDeviceToHost));
@@ -2238,7 +2239,7 @@ int phx_matvec(phx_moe_ctx* c, int type, const void* w, int rows, int cols, int 
 #define I8_DENSE_T 128
 #define I8_FEW E / 2
 #define I8_TILE 16
-#define I8_CAP 8
+#define I8_CAP 1
 #endif
 namespace {
 constexpr int PHX_I8_WEIGHT = 24;  // GgmlType's int8
@@ -2469,10 +2470,10 @@ int phx_experts_i8(phx_moe_ctx* c, const phx_weight* gu, const phx_weight* dn, i
         HIPCHK(c, launch_status(c));
         return PHX_OK;
     }
-    // long batches go through in chunks, so that the workspace stays bounded
-    const int chunk = std::min(T, 65535 / k), A = chunk * k;
+    // long batches go through in chunks, so that the workspace stays bounded and every row of it within 2^32 bytes
+    const int chunk = std::min<int64_t>(T, std::min<int64_t>(65535, ((1ll << 32) - 1) / (4ll * std::max(d, nf))) / k), A = chunk * k;
     const bool tile = A > I8_TILE * E;
-    const int cap = tile ? kI8Tile : A <= I8_CAP * E ? 32 : kI8RowsPaired;
+    const int cap = tile ? kI8Tile : A <= I8_CAP * E ? 16 : A <= 8 * E ? 32 : kI8RowsPaired;
     const int max_tiles = (A + cap - 1) / cap + std::min(E, A);
     int *perm, *ntiles;
     Tile* tiles;

@@ -211,6 +211,23 @@ def test_weights_from_device_memory(ctx):
     np.testing.assert_array_equal(ys[0], ys[2])
 
 
+# ---------------------------------------------------------------------------------------- activations
+def test_activations_of_the_experts(ctx, orc):
+    """The forms in the products' epilogues give the library's silu and gelu: gelu at every fp16 value and between them,
+    silu over the whole range with the places where its quotient leaves the normal numbers."""
+    every = np.arange(65536, dtype=np.uint16).view(np.float16).astype(F32)
+    rng = np.random.default_rng(12)
+    x = np.concatenate([every, (4 * rng.standard_normal(1 << 20)).astype(F32), rng.uniform(-110, 110, 1 << 18).astype(F32),
+                        np.array([0.0, -0.0, 1e-40, -1e-40, 79.99999, -79.99999, 80, -80, -88.7, -88.8, -104, 3e38, -3e38, 10, -10,
+                                  9.9999, -9.9999, 9.998, np.inf, -np.inf, np.nan], F32)])
+    one = np.ones_like(x)
+    with np.errstate(all="ignore"):
+        np.testing.assert_array_equal(ctx.selftest(11, x, one), orc.silu(x))
+        finite = x[~np.isnan(x)]
+        np.testing.assert_array_equal(ctx.selftest(12, finite, np.ones_like(finite)), orc.gelu(finite))
+    assert (ctx.selftest(12, np.full(64, np.nan, F32), np.ones(64, F32)) == 0).all()  # the table's value
+
+
 # ---------------------------------------------------------------------------------------- experts
 def expert_case(rng, E, d, nf):
     wg, sg = ref.weights_of(rng, E, 2 * nf, d)
