@@ -31,47 +31,48 @@ __device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d)
 }
 __device__ __forceinline__ float silu_ref(float v) { return v / (1.0f + (float)exp(-(double)v)); }
 
-// One workgroup per row, eight consecutive values per thread and step, the row held in registers between its
-// statistics and its integers: one pass over memory.
+// NT threads per row, eight consecutive values per thread and step, the row held in registers between its statistics and its
+// integers: one pass over memory.  A row of one wave needs no barrier, and a workgroup then takes four.
 template <int NT, int STEPS, int MODE, int DT>
-__global__ __launch_bounds__(NT) void k_quant_i8(int n, int64_t ld, float eps, const void* __restrict__ x,
-                                                 const void* __restrict__ aux, const float* __restrict__ tab,
-                                                 int8_t* __restrict__ qs, float* __restrict__ d)
+__global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_quant_i8(int rows, int n, int64_t ld, float eps,
+                                                                  const void* __restrict__ x, const void* __restrict__ aux,
+                                                                  const float* __restrict__ tab, int8_t* __restrict__ qs,
+                                                                  float* __restrict__ d)
 {
-    __shared__ double red[NT / 64];
-    __shared__ unsigned redu[NT / 64];
-    const int64_t row = blockIdx.x;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    constexpr int RPB = NT < 256 ? 256 / NT : 1, NW = NT / 64;
+    __shared__ double red[NW];
+    __shared__ unsigned redu[NW];
+    const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / NT;
+    if (NT == 64 && row >= rows) return;  // a whole wave, and no barrier with one wave a row
+    const int tid = threadIdx.x % NT, lane = tid & 63, wave = tid >> 6;
     float v[STEPS][8];
+    auto at = [&](int s) { return min((s * NT + tid) * 8, n - 8); };  // past the row its last values: every load in flight at once
 #pragma unroll
-    for (int s = 0; s < STEPS; s++) {
-        const int i = (s * NT + tid) * 8;
-#pragma unroll
-        for (int j = 0; j < 8; j++) v[s][j] = 0.0f;
-        if (i < n) load_eight<DT>(x, row * ld + i, v[s]);
-    }
+    for (int s = 0; s < STEPS; s++) load_eight<DT>(x, row * ld + at(s), v[s]);
     float scale = 0.0f;
     if (MODE == PHX_QUANT_RMS_NORM) {
         double sum = 0.0;
 #pragma unroll
         for (int s = 0; s < STEPS; s++)
+            if ((s * NT + tid) * 8 < n)
 #pragma unroll
-            for (int j = 0; j < 8; j++) sum += (double)v[s][j] * (double)v[s][j];
+                for (int j = 0; j < 8; j++) sum += (double)v[s][j] * (double)v[s][j];
         sum = wave_sum_dpp(sum);
-        if (lane == 0) red[wave] = sum;
-        __syncthreads();
-        sum = 0.0;
-        for (int w = 0; w < NT / 64; w++) sum += red[w];
+        if (NW > 1) {
+            if (lane == 0) red[wave] = sum;
+            __syncthreads();
+            sum = 0.0;
+            for (int w = 0; w < NW; w++) sum += red[w];
+        }
         scale = rms_scale_from_mean((float)(sum / (double)n), eps);
     }
     unsigned am = 0;
 #pragma unroll
     for (int s = 0; s < STEPS; s++) {
-        const int i = (s * NT + tid) * 8;
-        if (MODE != PHX_QUANT_PLAIN && i < n) {
+        if (MODE != PHX_QUANT_PLAIN) {
             float a[8];
-            if (MODE == PHX_QUANT_RMS_NORM) load_eight<PHX_F32>(aux, i, a);
-            else load_eight<DT>(aux, row * ld + i, a);
+            if (MODE == PHX_QUANT_RMS_NORM) load_eight<PHX_F32>(aux, at(s), a);
+            else load_eight<DT>(aux, row * ld + at(s), a);
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 const float u = v[s][j];
@@ -80,13 +81,15 @@ __global__ __launch_bounds__(NT) void k_quant_i8(int n, int64_t ld, float eps, c
             }
         }
 #pragma unroll
-        for (int j = 0; j < 8; j++) am = max(am, __float_as_uint(v[s][j]) & 0x7FFFFFFFu);
+        for (int j = 0; j < 8; j++) am = max(am, __float_as_uint(v[s][j]) & 0x7FFFFFFFu);  // the last values again are no more
     }
     am = wave_max_u32(am);
-    if (lane == 0) redu[wave] = am;
-    __syncthreads();
+    if (NW > 1) {
+        if (lane == 0) redu[wave] = am;
+        __syncthreads();
 #pragma unroll
-    for (int w = 0; w < NT / 64; w++) am = max(am, redu[w]);
+        for (int w = 0; w < NW; w++) am = max(am, redu[w]);
+    }
     const RowScale rs = row_scale(am);
     if (tid == 0) d[row] = rs.d;
 #pragma unroll
@@ -100,13 +103,27 @@ __global__ __launch_bounds__(NT) void k_quant_i8(int n, int64_t ld, float eps, c
     }
 }
 
+template <int NT, int STEPS, int MODE, int DT>
+static void quant_as(hipStream_t st, int rows, int n, int64_t ld, float eps, const void* x, const void* aux, const float* tab,
+                     int8_t* qs, float* d)
+{
+    constexpr int RPB = NT < 256 ? 256 / NT : 1;
+    launch(k_quant_i8<NT, STEPS, MODE, DT>, dim3((rows + RPB - 1) / RPB), dim3(NT * RPB), 0, st, rows, n, ld, eps, x, aux, tab, qs,
+           d);
+}
+
+#ifndef I8_Q_ROWS
+#define I8_Q_ROWS 1024
+#endif
 template <int MODE, int DT>
 static void quant_rows(hipStream_t st, int rows, int n, int64_t ld, float eps, const void* x, const void* aux,
                        const float* tab, int8_t* qs, float* d)
 {
-    if (n <= 2048) launch(k_quant_i8<256, 1, MODE, DT>, dim3(rows), dim3(256), 0, st, n, ld, eps, x, aux, tab, qs, d);
-    else if (n <= 8192) launch(k_quant_i8<512, 2, MODE, DT>, dim3(rows), dim3(512), 0, st, n, ld, eps, x, aux, tab, qs, d);
-    else launch(k_quant_i8<1024, 8, MODE, DT>, dim3(rows), dim3(1024), 0, st, n, ld, eps, x, aux, tab, qs, d);
+    if (n <= 1024) quant_as<64, 2, MODE, DT>(st, rows, n, ld, eps, x, aux, tab, qs, d);
+    else if (n <= 2048 && rows >= I8_Q_ROWS) quant_as<64, 4, MODE, DT>(st, rows, n, ld, eps, x, aux, tab, qs, d);
+    else if (n <= 4096) quant_as<256, 2, MODE, DT>(st, rows, n, ld, eps, x, aux, tab, qs, d);
+    else if (n <= 8192) quant_as<512, 2, MODE, DT>(st, rows, n, ld, eps, x, aux, tab, qs, d);
+    else quant_as<1024, 8, MODE, DT>(st, rows, n, ld, eps, x, aux, tab, qs, d);
 }
 
 template <int DT>
@@ -598,9 +615,10 @@ __device__ __forceinline__ void i8_tile_product(const I8Args& g, const Tile& tl,
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-        // rolled: a workgroup runs this once, and the instructions of it unrolled took longer to fetch than to run
-#pragma unroll 1
-        for (int tok = lane / LPT; tok < 32; tok += TPI) {
+        // two rounds at a time: a workgroup runs this once, and unrolled further the instructions take longer to fetch than to run
+#pragma unroll 2
+        for (int it = 0; it < 32 / TPI; it++) {
+            const int tok = it * TPI + lane / LPT;
             const float dx = dxs[32 * j + tok];
             char* o = out + orow[32 * j + tok];
             int s[V], u[V];
@@ -774,7 +792,8 @@ __global__ __launch_bounds__(1024) void k_i8_lists(int n, int E, int cap, const 
 #pragma unroll
     for (int i = 0; i < IPT; i++) {
         const int a = i * 1024 + tid;
-        place[i] = a < n ? (uint32_t)min((unsigned)ids[a], 0xFFFFu) << 16 : 0xFFFF0000u;
+        const uint32_t e = min((unsigned)ids[min(a, n - 1)], 0xFFFFu);  // every load before the first is waited for
+        place[i] = (a < n ? e : 0xFFFFu) << 16;
     }
     __syncthreads();
 #pragma unroll

@@ -37,12 +37,16 @@ __global__ __launch_bounds__(256) void k_route(RouteArgs R)
     if (t >= R.T) return;  // uniform over the wave, and the kernel has no workgroup barrier
     const int e0 = V * lane;
     const bool grouped = R.used < R.G, pairs = grouped && R.top2;
-    float l[V];
+    float l[V], bias[V];
     unsigned hi[V], lo[V];
+    if (WIDE) {
+#pragma unroll
+        for (int i = 0; i < V; i++) bias[i] = R.bias[min(e0 + i, R.E - 1)];  // what is past the last expert is no candidate
+    }
 #pragma unroll
     for (int i = 0; i < V; i++) {
-        const float v = e0 + i < R.E ? load_one<DT>(R.logits, (int64_t)t * R.E + e0 + i) : -INFINITY;
-        l[i] = v > -INFINITY ? fminf(v, 3.402823466e38f) : -INFINITY;  // NaN compares false
+        const float v = load_one<DT>(R.logits, (int64_t)t * R.E + min(e0 + i, R.E - 1));  // every load before a wait
+        l[i] = e0 + i < R.E && v > -INFINITY ? fminf(v, 3.402823466e38f) : -INFINITY;  // NaN compares false
         hi[i] = l[i] > -INFINITY ? sortable_f32(l[i] + 0.0f) : 0u;      // -0 equals 0
         lo[i] = 0u;
     }
@@ -74,7 +78,7 @@ __global__ __launch_bounds__(256) void k_route(RouteArgs R)
     if (WIDE) {
 #pragma unroll
         for (int i = 0; i < V; i++) {
-            const float b = e0 + i < R.E ? R.bias[e0 + i] : -INFINITY;
+            const float b = bias[i];
             const bool able = l[i] > -INFINITY && b > -INFINITY;
             c[i] = able ? s[i] + (double)b + 0.0 : NINF;
             const unsigned long long key = able ? sortable_f64(c[i]) : 0ull;
