@@ -31,13 +31,72 @@ __device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d)
 }
 __device__ __forceinline__ float silu_ref(float v) { return v / (1.0f + (float)exp(-(double)v)); }
 
+// 2^f on [-1/2, 1/2] in double, the Taylor series of exp(f ln 2) to f^11: within 2^-46
+__device__ __forceinline__ double exp2_frac(double f)
+{
+    const double x = f * 0.69314718055994530942;
+    double p = 1.0 / 39916800.0;
+    p = __builtin_fma(p, x, 1.0 / 3628800.0);
+    p = __builtin_fma(p, x, 1.0 / 362880.0);
+    p = __builtin_fma(p, x, 1.0 / 40320.0);
+    p = __builtin_fma(p, x, 1.0 / 5040.0);
+    p = __builtin_fma(p, x, 1.0 / 720.0);
+    p = __builtin_fma(p, x, 1.0 / 120.0);
+    p = __builtin_fma(p, x, 1.0 / 24.0);
+    p = __builtin_fma(p, x, 1.0 / 6.0);
+    p = __builtin_fma(p, x, 0.5);
+    p = __builtin_fma(p, x, 1.0);
+    return __builtin_fma(p, x, 1.0);
+}
+// exp(x) in double for |x| <= 128, within 2^-45 of it: past the float it is rounded to by 21 bits
+__device__ __forceinline__ double exp_near(double x)
+{
+    const double t = x * 1.44269504088896340736, n = __builtin_rint(t);
+    return __builtin_amdgcn_ldexp(exp2_frac(t - n), (int)n);
+}
+// silu_ref and gelu_ref without the library's exponential and the table: 26 and 45 instructions a value (a gate|up tile's
+// epilogue 24 us; by the exponential and a gather a value it took as long as the tile's products).  The same roundings:
+// silu's quotient by the reciprocal, one refinement and two corrections, which round it correctly while nothing leaves
+// the normal numbers (|v| < 80); gelu equals the table at every fp16 value (tests).
+__device__ __forceinline__ float silu_near(float v)
+{
+    if (fabsf(v) >= 80.0f || v != v) return silu_ref(v);
+    const float d = 1.0f + (float)exp_near(-(double)v);
+    float y = __builtin_amdgcn_rcpf(d);
+    y = __builtin_fmaf(__builtin_fmaf(-d, y, 1.0f), y, y);
+    float q = v * y;
+    q = __builtin_fmaf(__builtin_fmaf(-d, q, v), y, q);
+    return __builtin_fmaf(__builtin_fmaf(-d, q, v), y, q);
+}
+__device__ __forceinline__ float gelu_near(float x)
+{
+    if (!(x > -10.0f)) return 0.0f;  // and for a NaN, as the table has it
+    if (x >= 10.0f) return x;
+    const float h = h2f(f2h_bits(x));
+    if (h <= -10.0f) return 0.0f;
+    if (h >= 10.0f) return h;
+    const float inner = 0.79788456080286535587989211986876f * h * (1.0f + 0.044715f * h * h);
+    // tanh(z) = 1 - 2 / (1 + exp(2 z)), 1 from |z| = 22 on; the reciprocal from the hardware's by two refinements
+    const double z2 = 2.0 * (double)fminf(fmaxf(inner, -22.0f), 22.0f), e = 1.0 + exp_near(z2);
+    double y = __builtin_amdgcn_rcp(e);
+    y = __builtin_fma(__builtin_fma(-e, y, 1.0), y, y);
+    y = __builtin_fma(__builtin_fma(-e, y, 1.0), y, y);
+    const float t = (float)__builtin_fma(-2.0, y, 1.0);
+    return h2f(f2h_of(0.5f * h * (1.0f + t)));
+}
+
+// h = act(gate) * up as phx_quant_i8 forms it
+__device__ __forceinline__ float gated(int act, float gate, float up)
+{
+    return (act == PHX_QUANT_SILU_MUL ? silu_near(gate) : gelu_near(gate)) * up;
+}
+
 // NT threads per row, eight consecutive values per thread and step, the row held in registers between its statistics and its
 // integers: one pass over memory.  A row of one wave needs no barrier, and a workgroup then takes four.
 template <int NT, int STEPS, int MODE, int DT>
 __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_quant_i8(int rows, int n, int64_t ld, float eps,
                                                                   const void* __restrict__ x, const void* __restrict__ aux,
-                                                                  const float* __restrict__ tab, int8_t* __restrict__ qs,
-                                                                  float* __restrict__ d)
+                                                                  int8_t* __restrict__ qs, float* __restrict__ d)
 {
     constexpr int RPB = NT < 256 ? 256 / NT : 1, NW = NT / 64;
     __shared__ double red[NW];
@@ -76,8 +135,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_quant_i8(int rows, int 
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 const float u = v[s][j];
-                v[s][j] = MODE == PHX_QUANT_RMS_NORM ? u * scale * a[j] : MODE == PHX_QUANT_SILU_MUL ? silu_ref(u) * a[j]
-                                                                                                   : gelu_ref(u, tab) * a[j];
+                v[s][j] = MODE == PHX_QUANT_RMS_NORM ? u * scale * a[j] : gated(MODE, u, a[j]);
             }
         }
 #pragma unroll
@@ -104,47 +162,45 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_quant_i8(int rows, int 
 }
 
 template <int NT, int STEPS, int MODE, int DT>
-static void quant_as(hipStream_t st, int rows, int n, int64_t ld, float eps, const void* x, const void* aux, const float* tab,
-                     int8_t* qs, float* d)
+static void quant_as(hipStream_t st, int rows, int n, int64_t ld, float eps, const void* x, const void* aux, int8_t* qs,
+                     float* d)
 {
     constexpr int RPB = NT < 256 ? 256 / NT : 1;
-    launch(k_quant_i8<NT, STEPS, MODE, DT>, dim3((rows + RPB - 1) / RPB), dim3(NT * RPB), 0, st, rows, n, ld, eps, x, aux, tab, qs,
-           d);
+    launch(k_quant_i8<NT, STEPS, MODE, DT>, dim3((rows + RPB - 1) / RPB), dim3(NT * RPB), 0, st, rows, n, ld, eps, x, aux, qs, d);
 }
 
-#ifndef I8_Q_ROWS
-#define I8_Q_ROWS 1024
-#endif
+// a wave a row up to 1024 values, and up to 2048 where the rows are many (16384 of 1408: 63 us with the product behind it,
+// four waves a row 91; 256: 17 against 16)
 template <int MODE, int DT>
-static void quant_rows(hipStream_t st, int rows, int n, int64_t ld, float eps, const void* x, const void* aux,
-                       const float* tab, int8_t* qs, float* d)
+static void quant_rows(hipStream_t st, int rows, int n, int64_t ld, float eps, const void* x, const void* aux, int8_t* qs,
+                       float* d)
 {
-    if (n <= 1024) quant_as<64, 2, MODE, DT>(st, rows, n, ld, eps, x, aux, tab, qs, d);
-    else if (n <= 2048 && rows >= I8_Q_ROWS) quant_as<64, 4, MODE, DT>(st, rows, n, ld, eps, x, aux, tab, qs, d);
-    else if (n <= 4096) quant_as<256, 2, MODE, DT>(st, rows, n, ld, eps, x, aux, tab, qs, d);
-    else if (n <= 8192) quant_as<512, 2, MODE, DT>(st, rows, n, ld, eps, x, aux, tab, qs, d);
-    else quant_as<1024, 8, MODE, DT>(st, rows, n, ld, eps, x, aux, tab, qs, d);
+    if (n <= 1024) quant_as<64, 2, MODE, DT>(st, rows, n, ld, eps, x, aux, qs, d);
+    else if (n <= 2048 && rows >= 1024) quant_as<64, 4, MODE, DT>(st, rows, n, ld, eps, x, aux, qs, d);
+    else if (n <= 4096) quant_as<256, 2, MODE, DT>(st, rows, n, ld, eps, x, aux, qs, d);
+    else if (n <= 8192) quant_as<512, 2, MODE, DT>(st, rows, n, ld, eps, x, aux, qs, d);
+    else quant_as<1024, 8, MODE, DT>(st, rows, n, ld, eps, x, aux, qs, d);
 }
 
 template <int DT>
-static void quant_mode(hipStream_t st, int mode, int rows, int n, int64_t ld, float eps, const void* x, const void* aux,
-                       const float* tab, int8_t* qs, float* d)
+static void quant_mode(hipStream_t st, int mode, int rows, int n, int64_t ld, float eps, const void* x, const void* aux, int8_t* qs,
+                       float* d)
 {
     switch (mode) {
-    case PHX_QUANT_SILU_MUL: quant_rows<PHX_QUANT_SILU_MUL, DT>(st, rows, n, ld, eps, x, aux, tab, qs, d); break;
-    case PHX_QUANT_RMS_NORM: quant_rows<PHX_QUANT_RMS_NORM, DT>(st, rows, n, ld, eps, x, aux, tab, qs, d); break;
-    case PHX_QUANT_GELU_MUL: quant_rows<PHX_QUANT_GELU_MUL, DT>(st, rows, n, ld, eps, x, aux, tab, qs, d); break;
-    default: quant_rows<PHX_QUANT_PLAIN, DT>(st, rows, n, ld, eps, x, aux, tab, qs, d);
+    case PHX_QUANT_SILU_MUL: quant_rows<PHX_QUANT_SILU_MUL, DT>(st, rows, n, ld, eps, x, aux, qs, d); break;
+    case PHX_QUANT_RMS_NORM: quant_rows<PHX_QUANT_RMS_NORM, DT>(st, rows, n, ld, eps, x, aux, qs, d); break;
+    case PHX_QUANT_GELU_MUL: quant_rows<PHX_QUANT_GELU_MUL, DT>(st, rows, n, ld, eps, x, aux, qs, d); break;
+    default: quant_rows<PHX_QUANT_PLAIN, DT>(st, rows, n, ld, eps, x, aux, qs, d);
     }
 }
 
 void launch_quant_i8(hipStream_t st, int mode, int type, int rows, int n, int64_t ld, float eps, const void* x,
-                     const void* aux, const float* tab, int8_t* qs, float* d)
+                     const void* aux, int8_t* qs, float* d)
 {
     switch (type) {
-    case PHX_F16: quant_mode<PHX_F16>(st, mode, rows, n, ld, eps, x, aux, tab, qs, d); break;
-    case PHX_BF16: quant_mode<PHX_BF16>(st, mode, rows, n, ld, eps, x, aux, tab, qs, d); break;
-    default: quant_mode<PHX_F32>(st, mode, rows, n, ld, eps, x, aux, tab, qs, d);
+    case PHX_F16: quant_mode<PHX_F16>(st, mode, rows, n, ld, eps, x, aux, qs, d); break;
+    case PHX_BF16: quant_mode<PHX_BF16>(st, mode, rows, n, ld, eps, x, aux, qs, d); break;
+    default: quant_mode<PHX_F32>(st, mode, rows, n, ld, eps, x, aux, qs, d);
     }
 }
 
@@ -217,66 +273,6 @@ template <int DT>
 __device__ __forceinline__ char* out_base(const I8Args& g, const Tile& tl)
 {
     return (char*)g.out + (g.perm ? 0 : (int64_t)tl.start * g.out_cols * (DT == PHX_F32 ? 4 : 2));
-}
-
-// 2^f on [-1/2, 1/2] in double, the Taylor series of exp(f ln 2) to f^11: within 2^-46
-__device__ __forceinline__ double exp2_frac(double f)
-{
-    const double x = f * 0.69314718055994530942;
-    double p = 1.0 / 39916800.0;
-    p = __builtin_fma(p, x, 1.0 / 3628800.0);
-    p = __builtin_fma(p, x, 1.0 / 362880.0);
-    p = __builtin_fma(p, x, 1.0 / 40320.0);
-    p = __builtin_fma(p, x, 1.0 / 5040.0);
-    p = __builtin_fma(p, x, 1.0 / 720.0);
-    p = __builtin_fma(p, x, 1.0 / 120.0);
-    p = __builtin_fma(p, x, 1.0 / 24.0);
-    p = __builtin_fma(p, x, 1.0 / 6.0);
-    p = __builtin_fma(p, x, 0.5);
-    p = __builtin_fma(p, x, 1.0);
-    return __builtin_fma(p, x, 1.0);
-}
-// exp(x) in double for |x| <= 128, within 2^-45 of it: past the float it is rounded to by 21 bits
-__device__ __forceinline__ double exp_near(double x)
-{
-    const double t = x * 1.44269504088896340736, n = __builtin_rint(t);
-    return __builtin_amdgcn_ldexp(exp2_frac(t - n), (int)n);
-}
-// silu_ref and gelu_ref's table in the epilogues of the products, where the library's exponential and a gather per value
-// would cost as much as the product.  The same roundings: silu's quotient by the reciprocal, one refinement and two
-// corrections, which round it correctly while nothing leaves the normal numbers (|v| < 80); gelu_f16 equals
-// the table at every fp16 value (tests).
-__device__ __forceinline__ float silu_near(float v)
-{
-    if (fabsf(v) >= 80.0f || v != v) return silu_ref(v);
-    const float d = 1.0f + (float)exp_near(-(double)v);
-    float y = __builtin_amdgcn_rcpf(d);
-    y = __builtin_fmaf(__builtin_fmaf(-d, y, 1.0f), y, y);
-    float q = v * y;
-    q = __builtin_fmaf(__builtin_fmaf(-d, q, v), y, q);
-    return __builtin_fmaf(__builtin_fmaf(-d, q, v), y, q);
-}
-__device__ __forceinline__ float gelu_near(float x)
-{
-    if (!(x > -10.0f)) return 0.0f;  // and for a NaN, as the table has it
-    if (x >= 10.0f) return x;
-    const float h = h2f(f2h_bits(x));
-    if (h <= -10.0f) return 0.0f;
-    if (h >= 10.0f) return h;
-    const float inner = 0.79788456080286535587989211986876f * h * (1.0f + 0.044715f * h * h);
-    // tanh(z) = 1 - 2 / (1 + exp(2 z)), 1 from |z| = 22 on; the reciprocal from the hardware's by two refinements
-    const double z2 = 2.0 * (double)fminf(fmaxf(inner, -22.0f), 22.0f), e = 1.0 + exp_near(z2);
-    double y = __builtin_amdgcn_rcp(e);
-    y = __builtin_fma(__builtin_fma(-e, y, 1.0), y, y);
-    y = __builtin_fma(__builtin_fma(-e, y, 1.0), y, y);
-    const float t = (float)__builtin_fma(-2.0, y, 1.0);
-    return h2f(f2h_of(0.5f * h * (1.0f + t)));
-}
-
-// h = act(gate) * up as phx_quant_i8 forms it
-__device__ __forceinline__ float gated(int act, float gate, float up)
-{
-    return (act == PHX_QUANT_SILU_MUL ? silu_near(gate) : gelu_near(gate)) * up;
 }
 
 // v_mfma_i32_32x32x32_i8: lane l holds 16 bytes of A row l % 32 and of B row l % 32, both at k = 16 (l / 32); the
@@ -685,10 +681,6 @@ static void set_matrix(I8Args& g, const I8Mat& m)
     g.n_expert = m.n_mat;
 }
 
-#ifndef I8_E_NW
-#define I8_E_NW 4
-#define I8_E_RT 2
-#endif
 template <int NW, int RT, int CT>
 static void rows_dense(hipStream_t st, const I8Args& g, int max_tiles, int out_type)
 {
@@ -697,12 +689,14 @@ static void rows_dense(hipStream_t st, const I8Args& g, int max_tiles, int out_t
     else if (out_type == PHX_BF16) launch(k_i8_rows<NW, RT, CT, false, PHX_BF16>, grid, blk, 0, st, g);
     else launch(k_i8_rows<NW, RT, CT, false, PHX_F32>, grid, blk, 0, st, g);
 }
-template <int NW, int RT, int CT>
+// RT for paired matrices, RD for the others
+template <int NW, int RT, int RD, int CT>
 static void rows_grouped(hipStream_t st, const I8Mat& m, const I8Args& g, int max_tiles)
 {
-    const dim3 grid((g.out_cols + 16 * RT - 1) / (16 * RT), max_tiles), blk(64 * NW);
+    const int w = 16 * (m.paired ? RT : RD);
+    const dim3 grid((g.out_cols + w - 1) / w, max_tiles), blk(64 * NW);
     if (m.paired) launch(k_i8_rows<NW, RT, CT, true, PHX_F32>, grid, blk, 0, st, g);
-    else launch(k_i8_rows<NW, RT, CT, false, PHX_F32>, grid, blk, 0, st, g);
+    else launch(k_i8_rows<NW, RD, CT, false, PHX_F32>, grid, blk, 0, st, g);
 }
 
 void launch_i8_product(hipStream_t st, const I8Mat& m, I8Args g, bool tile, int max_tiles, int ncu, int out_type)
@@ -746,10 +740,12 @@ void launch_i8_product(hipStream_t st, const I8Mat& m, I8Args g, bool tile, int 
             else if (n < 4 * ncu) rows_dense<8, 2, 8>(st, g, max_tiles, out_type);
             else rows_dense<8, 4, 8>(st, g, max_tiles, out_type);
         }
-    } else if (g.ids) rows_grouped<8, 1, 1>(st, m, g, max_tiles);
-    else if (g.cap <= 16) rows_grouped<I8_E_NW, I8_E_RT, 1>(st, m, g, max_tiles);
-    else if (g.cap <= 32) rows_grouped<I8_E_NW, I8_E_RT, 2>(st, m, g, max_tiles);
-    else rows_grouped<I8_E_NW, I8_E_RT, 4>(st, m, g, max_tiles);
+    } else if (g.ids && (int64_t)((g.out_cols + 15) / 16) * max_tiles < 4 * ncu) rows_grouped<8, 1, 1, 1>(st, m, g, max_tiles);
+    // 32 channels, 64 outputs a workgroup: 64 experts of d = 4096, nf = 1408, T = 24 127 us; 64 channels 136, 32 outputs 125;
+    // 128 of 2816, 704, T = 128: 148; 16 channels 158, 32 outputs 156
+    else if (g.cap <= 16) rows_grouped<4, 2, 4, 1>(st, m, g, max_tiles);
+    else if (g.cap <= 32) rows_grouped<4, 2, 4, 2>(st, m, g, max_tiles);
+    else rows_grouped<4, 2, 4, 4>(st, m, g, max_tiles);
 }
 
 template <int NW>

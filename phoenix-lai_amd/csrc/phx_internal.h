@@ -282,7 +282,7 @@ void launch_selftest_gated(hipStream_t st, int act, int n, const float* a, const
 // ---- routing and int8 products (kernels_route.hip, kernels_i8.hip)
 void launch_route(hipStream_t st, const phx_route_desc& D, int T, const void* logits, const float* bias, int* ids, float* w);
 void launch_quant_i8(hipStream_t st, int mode, int type, int rows, int n, int64_t ld, float eps, const void* x,
-                     const void* aux, const float* tab, int8_t* qs, float* d);
+                     const void* aux, int8_t* qs, float* d);
 
 // int8 matrices on the device: groups of 32 stored rows, each [kc][32 rows][16 bytes] with kc = columns / 16 (padded to
 // whole 128-column steps with zeros), so the 16-byte operand of every lane of a 32 x 32 x 32 matrix product is one
@@ -310,7 +310,6 @@ struct I8Args {
     const int* perm = nullptr;
     const int* ids = nullptr;  // in place of the tiles: tile a is assignment a alone, its expert ids[a]
     int div = 1, nrows = 0, cap = 0, act = 0;
-    const float* tab = nullptr;
     void* out;
     // set by launch_i8_product from the matrix
     const int8_t* w;

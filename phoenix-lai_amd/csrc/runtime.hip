@@ -2235,12 +2235,6 @@ int phx_matvec(phx_moe_ctx* c, int type, const void* w, int rows, int cols, int 
 
 // ---------------------------------------------------------------------------- routing and int8 products
 
-#ifndef I8_DENSE_T
-#define I8_DENSE_T 128
-#define I8_FEW E / 2
-#define I8_TILE 16
-#define I8_CAP 1
-#endif
 namespace {
 constexpr int PHX_I8_WEIGHT = 24;  // GgmlType's int8
 constexpr int kMaxRowsI8 = 1 << 20;
@@ -2329,7 +2323,7 @@ int phx_quant_i8(phx_moe_ctx* c, int mode, int x_type, const void* x, const void
                        ? check_bufs(c, "quant_i8", {bx, bq, bd})
                        : check_bufs(c, "quant_i8", {bx, bq, bd, {"aux", aux, mode == PHX_QUANT_RMS_NORM ? n * 4ll : span, 16, false}});
     if (rc) return rc;
-    launch_quant_i8(c->stream, mode, x_type, rows, n, ld, eps, x, aux, c->gelu_tab, qs, d);
+    launch_quant_i8(c->stream, mode, x_type, rows, n, ld, eps, x, aux, qs, d);
     HIPCHK(c, launch_status(c));
     return PHX_OK;
 }
@@ -2419,7 +2413,7 @@ int phx_matmul_i8(phx_moe_ctx* c, const phx_weight* w, int T, const int8_t* xq, 
     g.xq = xq;
     g.xd = xd;
     g.nrows = T;
-    const bool tile = T > I8_DENSE_T;
+    const bool tile = T > kI8Rows;
     g.cap = tile ? kI8Tile : T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : kI8Rows;
     g.out = y;
     launch_i8_product(c->stream, w->i8, g, tile, (T + g.cap - 1) / g.cap, c->ncu, y_type);
@@ -2458,9 +2452,12 @@ int phx_experts_i8(phx_moe_ctx* c, const phx_weight* gu, const phx_weight* dn, i
     g.xd = xd;
     g.div = k;
     g.act = act;
-    g.tab = c->gelu_tab;
-    // few assignments, most of them of an expert of their own: two launches and no lists
-    if (T * k <= I8_FEW && i8_down_few_fits(dn->i8)) {
+    // Few assignments, most of them of an expert of their own: two launches without lists, which read an expert's matrices again
+    // for each of its assignments.  The lists' three further launches cost about what 48 MB of such reads do, or three times
+    // that where all experts stay in the caches (128 experts of d = 2816, nf = 704: T = 4 45 against 49 us, T = 8 72
+    // against 61; 32 of 1024, 512: T = 16 16 against 20, T = 32 23 against 22).
+    const double each = 3.0 * nf * d, A0 = (double)T * k, again = A0 - E * (1.0 - pow(1.0 - 1.0 / E, A0));
+    if (again * each <= (E * each <= 64e6 ? 144e6 : 48e6) && T <= 65535 && i8_down_few_fits(dn->i8)) {
         if ((rc = i8_ensure(c, I8_H, (int64_t)T * k * nf, &h))) return rc;
         g.ids = ids;
         g.cap = 16;
@@ -2472,8 +2469,8 @@ int phx_experts_i8(phx_moe_ctx* c, const phx_weight* gu, const phx_weight* dn, i
     }
     // long batches go through in chunks, so that the workspace stays bounded and every row of it within 2^32 bytes
     const int chunk = std::min<int64_t>(T, std::min<int64_t>(65535, ((1ll << 32) - 1) / (4ll * std::max(d, nf))) / k), A = chunk * k;
-    const bool tile = A > I8_TILE * E;
-    const int cap = tile ? kI8Tile : A <= I8_CAP * E ? 16 : A <= 8 * E ? 32 : kI8RowsPaired;
+    const bool tile = A > 14 * E;  // as T = 203 of 128 experts, k = 8: 172 us either way; 300: 188 against 192
+    const int cap = tile ? kI8Tile : A <= 2 * E ? 16 : A <= 8 * E ? 32 : kI8RowsPaired;
     const int max_tiles = (A + cap - 1) / cap + std::min(E, A);
     int *perm, *ntiles;
     Tile* tiles;
@@ -2497,7 +2494,7 @@ int phx_experts_i8(phx_moe_ctx* c, const phx_weight* gu, const phx_weight* dn, i
         g.div = k;
         g.out = h;
         launch_i8_product(st, gu->i8, g, tile, max_tiles, c->ncu, PHX_F32);
-        launch_quant_i8(st, PHX_QUANT_PLAIN, PHX_F32, n * k, nf, nf, 0.0f, h, nullptr, nullptr, hq, hd);
+        launch_quant_i8(st, PHX_QUANT_PLAIN, PHX_F32, n * k, nf, nf, 0.0f, h, nullptr, hq, hd);
         g.xq = hq;
         g.xd = hd;
         g.div = 1;
