@@ -7,7 +7,16 @@
 namespace phx {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x16 __attribute__((ext_vector_type(16)));
+
+// 16 bytes of weights; ONCE: no other workgroup reads them, so they need not stay in the caches
+template <bool ONCE>
+__device__ __forceinline__ i32x4 load_weights(const int8_t* p)
+{
+    if constexpr (ONCE) return __builtin_nontemporal_load((const i32x4*)p);
+    else return *(const i32x4*)p;
+}
 
 // ------------------------------------------------------------------------------ rows to int8
 // d = max |v| / 127, q = roundf(v * (1 / d)); a row whose d is under 2^-126 is zeros with d = 0, one that holds a NaN
@@ -287,7 +296,7 @@ __device__ __forceinline__ char* out_base(const I8Args& g, const Tile& tl)
 // its NW waves split the reduction, so no operand is wanted by two of them, and a matrix of few rows still has loads in
 // flight everywhere.  A wave keeps U steps of 64 columns ahead; the waves' int32 sums meet in LDS by atomic additions (exact
 // in any order).
-template <int NW, int RT, int TT, bool PAIRED, int DT>
+template <int NW, int RT, int TT, bool PAIRED, bool ONCE, int DT>
 __device__ __forceinline__ void i8_rows_product(const I8Args& g, const Tile& tl, int* red, uint32_t* orow, float* dxs)
 {
     constexpr int NB = PAIRED ? 2 : 1, NR = RT * NB, U = NR + TT <= 3 ? 8 : NR + TT <= 6 ? 4 : NR + TT <= 8 ? 3 : 2;
@@ -329,7 +338,7 @@ __device__ __forceinline__ void i8_rows_product(const I8Args& g, const Tile& tl,
     auto load = [&](int u, int s) {
         const int su = min(s, s1 - 1), k = 64 * su + 16 * q, kx = k < g.cols ? k : 0;  // the weights past cols are zero
 #pragma unroll
-        for (int r = 0; r < NR; r++) w[u][r] = *(const i32x4*)(wb[r] + (int64_t)su * 2048 + lo);
+        for (int r = 0; r < NR; r++) w[u][r] = load_weights<ONCE>(wb[r] + (int64_t)su * 2048 + lo);
 #pragma unroll
         for (int t = 0; t < TT; t++) x[u][t] = *(const i32x4*)(xr[t] + kx);
     };
@@ -376,7 +385,7 @@ __device__ __forceinline__ void i8_rows_product(const I8Args& g, const Tile& tl,
 }
 
 // CT: the most token tiles of 16 that a tile may hold (its capacity); a tile takes the product of its own count
-template <int NW, int RT, int CT, bool PAIRED, int DT>
+template <int NW, int RT, int CT, bool PAIRED, bool ONCE, int DT>
 __global__ __launch_bounds__(64 * NW) void k_i8_rows(I8Args g)
 {
     __shared__ int red[RT * CT * (PAIRED ? 2 : 1) * 256];
@@ -385,10 +394,10 @@ __global__ __launch_bounds__(64 * NW) void k_i8_rows(I8Args g)
     Tile tl;
     if (!i8_tile(g, blockIdx.y, &tl)) return;  // uniform over the workgroup
     const int n = (tl.cnt + 15) / 16;
-    if (CT == 1 || n == 1) i8_rows_product<NW, RT, 1, PAIRED, DT>(g, tl, red, orow, dxs);
-    else if (CT == 2 || n == 2) i8_rows_product<NW, RT, CT < 2 ? 1 : 2, PAIRED, DT>(g, tl, red, orow, dxs);
-    else if (CT == 4 || n <= 4) i8_rows_product<NW, RT, CT < 4 ? 1 : 4, PAIRED, DT>(g, tl, red, orow, dxs);
-    else i8_rows_product<NW, RT, CT < 8 ? 1 : 8, PAIRED, DT>(g, tl, red, orow, dxs);
+    if (CT == 1 || n == 1) i8_rows_product<NW, RT, 1, PAIRED, ONCE, DT>(g, tl, red, orow, dxs);
+    else if (CT == 2 || n == 2) i8_rows_product<NW, RT, CT < 2 ? 1 : 2, PAIRED, ONCE, DT>(g, tl, red, orow, dxs);
+    else if (CT == 4 || n <= 4) i8_rows_product<NW, RT, CT < 4 ? 1 : 4, PAIRED, ONCE, DT>(g, tl, red, orow, dxs);
+    else i8_rows_product<NW, RT, CT < 8 ? 1 : 8, PAIRED, ONCE, DT>(g, tl, red, orow, dxs);
 }
 
 // The down products of few assignments and their weighted sum, for a token (blockIdx.y) and 16 of its outputs: wave w takes
@@ -472,7 +481,7 @@ __global__ __launch_bounds__(64 * NW) void k_i8_down_few(I8Args g, int k, int nf
 // a turn share one: 8 cycles a read against 4).
 constexpr int TI_RING = 3, TI_PITCH = 68;  // ring slots; ints between two tokens' rows of 64 in the epilogue
 
-template <int NT, bool PAIRED, int DT>
+template <int NT, bool PAIRED, bool ONCE, int DT>
 __device__ __forceinline__ void i8_tile_product(const I8Args& g, const Tile& tl, int bx, unsigned char* ring, uint32_t* orow, float* dxs)
 {
     constexpr int STAGE = NT * 32 * 128;
@@ -505,7 +514,7 @@ __device__ __forceinline__ void i8_tile_product(const I8Args& g, const Tile& tl,
     i32x4 wv[2][2][4];
     auto weight = [&](int s, int b, auto P, auto KK) {
         const int8_t* at = wb[b] + (int64_t)min(s, S - 1) * 4096 + decltype(KK)::value * 1024;  // uniform
-        wv[decltype(P)::value][b][decltype(KK)::value] = *(const i32x4*)(at + lane16);
+        wv[decltype(P)::value][b][decltype(KK)::value] = load_weights<ONCE>(at + lane16);
     };
     i32x16 acc[NT][2];
 #pragma unroll
@@ -644,7 +653,7 @@ __device__ __forceinline__ void i8_tile_product(const I8Args& g, const Tile& tl,
     }
 }
 
-template <bool PAIRED, int DT>
+template <bool PAIRED, bool ONCE, int DT>
 __global__ __launch_bounds__(256, 2) void k_i8_tile(I8Args g)
 {
     __shared__ __align__(16) unsigned char ring[TI_RING * 128 * 128];
@@ -661,10 +670,10 @@ __global__ __launch_bounds__(256, 2) void k_i8_tile(I8Args g)
     Tile tl;
     if (!i8_tile(g, tile, &tl)) return;  // uniform over the workgroup
     switch ((tl.cnt + 31) / 32) {
-    case 1: i8_tile_product<1, PAIRED, DT>(g, tl, bx, ring, orow, dxs); break;
-    case 2: i8_tile_product<2, PAIRED, DT>(g, tl, bx, ring, orow, dxs); break;
-    case 3: i8_tile_product<3, PAIRED, DT>(g, tl, bx, ring, orow, dxs); break;
-    default: i8_tile_product<4, PAIRED, DT>(g, tl, bx, ring, orow, dxs);
+    case 1: i8_tile_product<1, PAIRED, ONCE, DT>(g, tl, bx, ring, orow, dxs); break;
+    case 2: i8_tile_product<2, PAIRED, ONCE, DT>(g, tl, bx, ring, orow, dxs); break;
+    case 3: i8_tile_product<3, PAIRED, ONCE, DT>(g, tl, bx, ring, orow, dxs); break;
+    default: i8_tile_product<4, PAIRED, ONCE, DT>(g, tl, bx, ring, orow, dxs);
     }
 }
 
@@ -685,18 +694,26 @@ template <int NW, int RT, int CT>
 static void rows_dense(hipStream_t st, const I8Args& g, int max_tiles, int out_type)
 {
     const dim3 grid((g.out_cols + 16 * RT - 1) / (16 * RT), max_tiles), blk(64 * NW);
-    if (out_type == PHX_F16) launch(k_i8_rows<NW, RT, CT, false, PHX_F16>, grid, blk, 0, st, g);
-    else if (out_type == PHX_BF16) launch(k_i8_rows<NW, RT, CT, false, PHX_BF16>, grid, blk, 0, st, g);
-    else launch(k_i8_rows<NW, RT, CT, false, PHX_F32>, grid, blk, 0, st, g);
+    if (out_type == PHX_F16) launch(k_i8_rows<NW, RT, CT, false, false, PHX_F16>, grid, blk, 0, st, g);
+    else if (out_type == PHX_BF16) launch(k_i8_rows<NW, RT, CT, false, false, PHX_BF16>, grid, blk, 0, st, g);
+    else launch(k_i8_rows<NW, RT, CT, false, false, PHX_F32>, grid, blk, 0, st, g);
 }
 // RT for paired matrices, RD for the others
-template <int NW, int RT, int RD, int CT>
+template <int NW, int RT, int RD, int CT, bool ONCE>
 static void rows_grouped(hipStream_t st, const I8Mat& m, const I8Args& g, int max_tiles)
 {
     const int w = 16 * (m.paired ? RT : RD);
     const dim3 grid((g.out_cols + w - 1) / w, max_tiles), blk(64 * NW);
-    if (m.paired) launch(k_i8_rows<NW, RT, CT, true, PHX_F32>, grid, blk, 0, st, g);
-    else launch(k_i8_rows<NW, RD, CT, false, PHX_F32>, grid, blk, 0, st, g);
+    if (m.paired) launch(k_i8_rows<NW, RT, CT, true, ONCE, PHX_F32>, grid, blk, 0, st, g);
+    else launch(k_i8_rows<NW, RD, CT, false, ONCE, PHX_F32>, grid, blk, 0, st, g);
+}
+
+template <bool ONCE>
+static void rows_lists(hipStream_t st, const I8Mat& m, const I8Args& g, int max_tiles)
+{
+    if (g.cap <= 16) rows_grouped<4, 2, 4, 1, ONCE>(st, m, g, max_tiles);
+    else if (g.cap <= 32) rows_grouped<4, 2, 4, 2, ONCE>(st, m, g, max_tiles);
+    else rows_grouped<4, 2, 4, 4, ONCE>(st, m, g, max_tiles);
 }
 
 void launch_i8_product(hipStream_t st, const I8Mat& m, I8Args g, bool tile, int max_tiles, int ncu, int out_type)
@@ -724,10 +741,12 @@ void launch_i8_product(hipStream_t st, const I8Mat& m, I8Args g, bool tile, int 
         g.blocks = (blocks + 8 / g.xt - 1) / (8 / g.xt);
         const int per = g.xt * g.run;
         const dim3 grid((max_tiles + per - 1) / per * g.run * g.blocks * 8), blk(256);
-        if (m.paired) launch(k_i8_tile<true, PHX_F32>, grid, blk, 0, st, g);
-        else if (out_type == PHX_F16) launch(k_i8_tile<false, PHX_F16>, grid, blk, 0, st, g);
-        else if (out_type == PHX_BF16) launch(k_i8_tile<false, PHX_BF16>, grid, blk, 0, st, g);
-        else launch(k_i8_tile<false, PHX_F32>, grid, blk, 0, st, g);
+        if (m.paired && g.once) launch(k_i8_tile<true, true, PHX_F32>, grid, blk, 0, st, g);
+        else if (m.paired) launch(k_i8_tile<true, false, PHX_F32>, grid, blk, 0, st, g);
+        else if (g.once) launch(k_i8_tile<false, true, PHX_F32>, grid, blk, 0, st, g);
+        else if (out_type == PHX_F16) launch(k_i8_tile<false, false, PHX_F16>, grid, blk, 0, st, g);
+        else if (out_type == PHX_BF16) launch(k_i8_tile<false, false, PHX_BF16>, grid, blk, 0, st, g);
+        else launch(k_i8_tile<false, false, PHX_F32>, grid, blk, 0, st, g);
     } else if (!g.tiles && !g.ids) {
         if (g.cap <= 16) rows_dense<8, 1, 1>(st, g, max_tiles, out_type);
         else if (g.cap <= 32) rows_dense<8, 1, 2>(st, g, max_tiles, out_type);
@@ -740,12 +759,14 @@ void launch_i8_product(hipStream_t st, const I8Mat& m, I8Args g, bool tile, int 
             else if (n < 4 * ncu) rows_dense<8, 2, 8>(st, g, max_tiles, out_type);
             else rows_dense<8, 4, 8>(st, g, max_tiles, out_type);
         }
-    } else if (g.ids && (int64_t)((g.out_cols + 15) / 16) * max_tiles < 4 * ncu) rows_grouped<8, 1, 1, 1>(st, m, g, max_tiles);
+    } else if (g.ids) {
+        if ((int64_t)((g.out_cols + 15) / 16) * max_tiles < 4 * ncu) rows_grouped<8, 1, 1, 1, false>(st, m, g, max_tiles);
+        else rows_grouped<4, 2, 4, 1, false>(st, m, g, max_tiles);
+    }
     // 32 channels, 64 outputs a workgroup: 64 experts of d = 4096, nf = 1408, T = 24 127 us; 64 channels 136, 32 outputs 125;
     // 128 of 2816, 704, T = 128: 148; 16 channels 158, 32 outputs 156
-    else if (g.cap <= 16) rows_grouped<4, 2, 4, 1>(st, m, g, max_tiles);
-    else if (g.cap <= 32) rows_grouped<4, 2, 4, 2>(st, m, g, max_tiles);
-    else rows_grouped<4, 2, 4, 4>(st, m, g, max_tiles);
+    else if (g.once) rows_lists<true>(st, m, g, max_tiles);
+    else rows_lists<false>(st, m, g, max_tiles);
 }
 
 template <int NW>
@@ -850,7 +871,7 @@ __global__ __launch_bounds__(256) void k_i8_combine(int d, int k, int E, const f
     for (int j = 0; j < k; j++) {
         if ((unsigned)ids[t * k + j] >= (unsigned)E) continue;  // uniform
         const float wj = w[t * k + j];
-        const float4 v = *(const float4*)(y + (t * k + j) * d + c);
+        const f32x4 v = __builtin_nontemporal_load((const f32x4*)(y + (t * k + j) * d + c));  // read once
         acc.x += v.x * wj;
         acc.y += v.y * wj;
         acc.z += v.z * wj;

@@ -310,6 +310,7 @@ struct I8Args {
     const int* perm = nullptr;
     const int* ids = nullptr;  // in place of the tiles: tile a is assignment a alone, its expert ids[a]
     int div = 1, nrows = 0, cap = 0, act = 0;
+    bool once = false;  // a grouped product whose weights nobody reads again soon (load_weights)
     void* out;
     // set by launch_i8_product from the matrix
     const int8_t* w;
