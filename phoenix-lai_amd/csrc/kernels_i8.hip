@@ -779,7 +779,7 @@ static void down_few(hipStream_t st, const I8Args& g, int T, int k, int nf, cons
     else launch(k_i8_down_few<NW, PHX_F32>, grid, blk, lds, st, g, k, nf, h, weights);
 }
 
-bool i8_down_few_fits(const I8Mat& m) { return 8 * m.kc * 16 <= 65536; }
+bool i8_down_few_fits(const I8Mat& m) { return 8 * m.kc * 16 <= 61440; }  // its rows and values in 64 KB of LDS
 
 void launch_i8_down_few(hipStream_t st, const I8Mat& m, int T, int k, const float* h, const int* ids, const float* weights,
                         int out_type, void* out)

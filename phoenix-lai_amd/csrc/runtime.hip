@@ -1296,9 +1296,9 @@ int check_ffn_args(phx_moe_ctx* c, int layer, int T, const float* x, float* out,
 
 // A device-pointer call's rows must be memory the GPU can address: hipMalloc'd, managed or pinned host.
 // A pageable host pointer would fault the device, so it is refused here.
-bool device_accessible(const void* p)
+bool device_accessible(const void* p, hipPointerAttribute_t* found = nullptr)
 {
-    hipPointerAttribute_t at{};
+    hipPointerAttribute_t mine{}, &at = found ? *found : mine;
     if (hipPointerGetAttributes(&at, p) != hipSuccess) {
         (void)hipGetLastError();  // the query's error is not the caller's
         return false;
@@ -2248,13 +2248,16 @@ struct CallBuf {
     bool out;
 };
 
-// Present, aligned, addressable by the GPU, and no output in any other buffer's bytes.
+// Present, aligned, addressable by the context's GPU, and no output in any other buffer's bytes.
 int check_bufs(phx_moe_ctx* c, const char* call, std::initializer_list<CallBuf> bufs)
 {
     for (const CallBuf& b : bufs) {
         if (!b.p) return set_err(c, PHX_ERR_ARG, "%s: null %s", call, b.what);
         if ((uintptr_t)b.p % b.align) return set_err(c, PHX_ERR_ARG, "%s: %s needs %d-byte alignment", call, b.what, b.align);
-        if (!device_accessible(b.p)) return set_err(c, PHX_ERR_ARG, "%s: %s is not device-accessible memory", call, b.what);
+        hipPointerAttribute_t at{};
+        if (!device_accessible(b.p, &at)) return set_err(c, PHX_ERR_ARG, "%s: %s is not device-accessible memory", call, b.what);
+        if (at.type == hipMemoryTypeDevice && at.device != c->device)
+            return set_err(c, PHX_ERR_ARG, "%s: %s is memory of device %d, the context's is %d", call, b.what, at.device, c->device);
     }
     for (const CallBuf& o : bufs)
         for (const CallBuf& b : bufs)
@@ -2457,7 +2460,7 @@ int phx_experts_i8(phx_moe_ctx* c, const phx_weight* gu, const phx_weight* dn, i
     // that where all experts stay in the caches (128 experts of d = 2816, nf = 704: T = 4 45 against 49 us, T = 8 72
     // against 61; 32 of 1024, 512: T = 16 16 against 20, T = 32 23 against 22).
     const double each = 3.0 * nf * d, A0 = (double)T * k, again = A0 - E * (1.0 - pow(1.0 - 1.0 / E, A0));
-    if (again * each <= (E * each <= 64e6 ? 144e6 : 48e6) && T <= 65535 && i8_down_few_fits(dn->i8)) {
+    if (A0 <= 1024 && again * each <= (E * each <= 64e6 ? 144e6 : 48e6) && i8_down_few_fits(dn->i8)) {
         if ((rc = i8_ensure(c, I8_H, (int64_t)T * k * nf, &h))) return rc;
         g.ids = ids;
         g.cap = 16;

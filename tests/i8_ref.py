@@ -93,15 +93,19 @@ def rms_norm(x, w, eps):
     return ((x * scale[:, None]).astype(F32) * np.asarray(w, F32)).astype(F32)
 
 
+def sums(xq, w):
+    """The whole-number sums, exact in float64."""
+    return xq.astype(np.float64) @ w.astype(np.float64).T
+
+
 def product(xq, xd, w, scale):
     """float64 of phx_matmul_i8's sum times the two scales."""
-    return (xq.astype(np.int64) @ w.astype(np.int64).T).astype(np.float64) * xd.astype(np.float64)[:, None] * \
-        scale.astype(np.float64)
+    return sums(xq, w) * xd.astype(np.float64)[:, None] * scale.astype(np.float64)
 
 
 def product_f32(xq, xd, w, scale):
     """phx_matmul_i8's float value: one rounding of the sum, one of the scales' product, one of the value."""
-    i = (xq.astype(np.int64) @ w.astype(np.int64).T).astype(F32)
+    i = sums(xq, w).astype(F32)
     return (i * (xd.astype(F32)[:, None] * scale.astype(F32)).astype(F32)).astype(F32)
 
 

@@ -1,6 +1,8 @@
 """int8 rows, products and experts (phx_quant_i8, phx_weight_upload_i8, phx_matmul_i8, phx_experts_i8) against plain
 implementations in 64 bits (tests/i8_ref.py): quants and scales equal, products within their stated roundings, at odd
 sizes, every type and mode, empty rows and skipped places, and the whole run from a router's logits."""
+import functools
+
 import numpy as np
 import pytest
 
@@ -159,6 +161,12 @@ def test_matmul(ctx, shape, type_):
     check_product(ctx, *shape, type_, seed=sum(shape))
 
 
+@pytest.mark.parametrize("shape", [(50, 8200, 96), (70, 8200, 64), (100, 16400, 64), (128, 16416, 160), (20, 8200, 32), (700, 8200, 96)])
+def test_matmul_many_outputs(ctx, shape):
+    """Outputs enough for the wider row tiles."""
+    check_product(ctx, *shape, 30, seed=sum(shape))
+
+
 def test_matmul_longest_rows(ctx):
     """65536 columns of the largest magnitudes: the sum's largest value, exact in int32."""
     T, rows, cols = 3, 40, 65536
@@ -235,6 +243,14 @@ def expert_case(rng, E, d, nf):
     return wg, sg, wd, sd
 
 
+@functools.lru_cache(maxsize=2)
+def big_experts(E, d, nf):
+    """Matrices of random bytes: quick to make where there are many."""
+    rng = np.random.default_rng(E + nf)
+    return (rng.integers(-90, 91, (E, 2 * nf, d), dtype=np.int8), (6e-4 * (1 + 0.3 * rng.random((E, 2 * nf)))).astype(F32),
+            rng.integers(-90, 91, (E, d, nf), dtype=np.int8), (6e-4 * (1 + 0.3 * rng.random((E, d)))).astype(F32))
+
+
 def upload(ctx, W):
     wg, sg, wd, sd = W
     E, n2, d = wg.shape
@@ -276,6 +292,29 @@ def test_experts(ctx, pkg, orc, dims, T, act):
     ids = np.argsort(rng.random((T, E)) ** 2, axis=1)[:, :k].astype(np.int32)
     weights = rng.random((T, k)).astype(F32)
     check_experts(ctx, pkg, orc, W, xq, xd, ids, weights, act, types=(0, 1, 30))
+
+
+@pytest.mark.parametrize("T", [20, 100, 200, 300, 600])
+def test_experts_past_the_caches(ctx, pkg, orc, T):
+    """Experts of 138 MB: lists of every tile capacity, with weights that are read once, and the tile kernel both ways."""
+    E, d, nf, k = 128, 1024, 352, 8
+    W = big_experts(E, d, nf)
+    rng = np.random.default_rng(T)
+    xq, xd = ref.rows_of(rng, T, d)
+    ids = np.argsort(rng.random((T, E)) ** 2, axis=1)[:, :k].astype(np.int32)
+    ids[T // 2, 1] = -1
+    check_experts(ctx, pkg, orc, W, xq, xd, ids, rng.random((T, k)).astype(F32), 1)
+
+
+@pytest.mark.parametrize("case", [(64, 512, 1024, 4, 24), (32, 512, 672, 4, 60), (32, 512, 672, 4, 100), (32, 512, 672, 4, 130)])
+def test_experts_in_the_caches(ctx, pkg, orc, case):
+    """Lists of every tile capacity, and the tile kernel, over fewer bytes."""
+    E, d, nf, k, T = case
+    W = big_experts(E, d, nf)
+    rng = np.random.default_rng(T)
+    xq, xd = ref.rows_of(rng, T, d)
+    ids = rng.integers(0, E, (T, k)).astype(np.int32)
+    check_experts(ctx, pkg, orc, W, xq, xd, ids, rng.random((T, k)).astype(F32), 3, types=(0, 30))
 
 
 @pytest.mark.parametrize("T", [1, 6, 150])
