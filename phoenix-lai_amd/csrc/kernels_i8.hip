@@ -1,4 +1,9 @@
 // int8 products with a scale per token and per output channel (phx_quant_i8, phx_matmul_i8, phx_experts_i8).
+//
+// Every sum of products is a whole number below 2^31 (65536 columns of at most 128 x 128), so the matrix cores' int32 sums
+// are exact in any order: reductions are split over waves and joined by integer additions without a word about order.  What
+// is rounded is stated at phx_matmul_i8: the sum to float, the scales' product, the value; nothing else between a row's
+// integers and an output.
 #include <algorithm>
 
 #include "device_common.h"
@@ -101,7 +106,8 @@ __device__ __forceinline__ float gated(int act, float gate, float up)
 }
 
 // NT threads per row, eight consecutive values per thread and step, the row held in registers between its statistics and its
-// integers: one pass over memory.  A row of one wave needs no barrier, and a workgroup then takes four.
+// integers: one pass over memory, which bounds it (8192 rows of 4096 fp16 values: 19 to 24 us, 4.2 to 5.2 TB/s; 2048 of
+// bf16, normed: 9 us).  A row of one wave needs no barrier, and a workgroup then takes four.
 template <int NT, int STEPS, int MODE, int DT>
 __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_quant_i8(int rows, int n, int64_t ld, float eps,
                                                                   const void* __restrict__ x, const void* __restrict__ aux,
@@ -144,7 +150,9 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_quant_i8(int rows, int 
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 const float u = v[s][j];
-                v[s][j] = MODE == PHX_QUANT_RMS_NORM ? u * scale * a[j] : gated(MODE, u, a[j]);
+                // silu by the library's exponential: the rows' bytes bound this kernel, and the shorter code is the faster one
+                // (77 rows of 2112: 4.2 us, by silu_near 5.1)
+                v[s][j] = MODE == PHX_QUANT_RMS_NORM ? u * scale * a[j] : (MODE == PHX_QUANT_SILU_MUL ? silu_ref(u) : gelu_near(u)) * a[j];
             }
         }
 #pragma unroll
@@ -403,7 +411,8 @@ __global__ __launch_bounds__(64 * NW) void k_i8_rows(I8Args g)
 // The down products of few assignments and their weighted sum, for a token (blockIdx.y) and 16 of its outputs: wave w takes
 // the token's places w, w + NW, ...  It issues the place's weights, forms the int8 row of its h meanwhile (every
 // workgroup of the token forms it again: nf floats from L2), and the places' values meet in LDS in order.  No lists, no
-// int8 rows and no partial outputs go through memory.
+// int8 rows and no partial outputs go through memory.  Bound by its chain of dependent trips (ids, h, the weights): 7.1 us
+// for one token of 8 x 704, d = 2816, whose 16 MB take 3.
 template <int NW, int DT>
 __global__ __launch_bounds__(64 * NW) void k_i8_down_few(I8Args g, int k, int nf, const float* __restrict__ h,
                                                          const float* __restrict__ weights)
@@ -479,6 +488,12 @@ __global__ __launch_bounds__(64 * NW) void k_i8_down_few(I8Args g, int k, int nf
 // half the row's number: LDS serves a 16-byte read in four turns of 16 lanes, {0-3, 12-15, 20-27}, {4-11, 16-19, 28-31} and the
 // same from lane 32, over 64 banks, and each turn then has 16 distinct bank groups (by the row's number itself, two rows of
 // a turn share one: 8 cycles a read against 4).
+//
+// What it reaches: 8192 x 5632 x 4096 169 us, 2.2 POP/s (a library product of that size 181); T = 2048 of 4096 x 4096 35 us.  The
+// matrix cores run in 60% of a tile's cycles at the 2.0 GHz that they leave the clock; without any load from memory a step
+// takes 1.13 us against 1.5, the rest is the issue and the wait of the loads.  Two 128-token halves on eight waves that share
+// the weights in the L1 (experts, T = 2048: gate|up 176 -> 197 us), four ring slots (the same), wave priorities (the same) and
+// experts' tiles longest first (297 -> 316 us: an expert's tiles no longer meet in the caches) were no faster.
 constexpr int TI_RING = 3, TI_PITCH = 68;  // ring slots; ints between two tokens' rows of 64 in the epilogue
 
 template <int NT, bool PAIRED, bool ONCE, int DT>
@@ -796,7 +811,8 @@ void launch_i8_down_few(hipStream_t st, const I8Mat& m, int T, int k, const floa
 // Each expert's assignments as one run of perm and as tiles of up to cap; ids outside [0, E) are in no run.  One workgroup
 // takes up to 1024 IPT assignments: an id's place in its run is what its counter's atomic addition returns, kept in a
 // register, and the runs are put together in LDS and stored whole.  The order inside a run is the atomics' and no result
-// depends on it: a place of the list names its own input and output row.
+// depends on it: a place of the list names its own input and output row.  One compute unit's latency bounds it: 4.5 us to
+// 2048 assignments, 8.8 for 16384, whose 16 loads a thread go out in one trip (waited for one by one: 14 us).
 template <int IPT>
 __global__ __launch_bounds__(1024) void k_i8_lists(int n, int E, int cap, const int* __restrict__ ids, int* __restrict__ perm,
                                                    Tile* __restrict__ tiles, int* __restrict__ ntiles)
@@ -859,7 +875,8 @@ void launch_i8_lists(hipStream_t st, int n, int E, int cap, const int* ids, int*
     else launch(k_i8_lists<64>, one, blk, 0, st, n, E, cap, ids, perm, tiles, ntiles);
 }
 
-// out[t] = sum over the places j, in order, of w[t][j] * y[t k + j]; places without an expert are skipped
+// out[t] = sum over the places j, in order, of w[t][j] * y[t k + j]; places without an expert are skipped.  Bound by y's bytes:
+// 2048 tokens of 8 x 2816 floats 33 us, 6.2 TB/s.
 template <int DT>
 __global__ __launch_bounds__(256) void k_i8_combine(int d, int k, int E, const float* __restrict__ y, const int* __restrict__ ids,
                                                     const float* __restrict__ w, void* __restrict__ out)

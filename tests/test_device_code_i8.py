@@ -48,7 +48,7 @@ def early_uses(text):
     return out
 
 
-def test_checker():
+def test_early_uses_are_found():
     read = ";;#ASMSTART\nds_read_b128 v[{}:{}], v1 offset:0\n;;#ASMEND\n"
     wait = ";;#ASMSTART\ns_waitcnt lgkmcnt({})\n;;#ASMEND\n"
     two = "_Zk:\n" + read.format(4, 7) + read.format(8, 11)
