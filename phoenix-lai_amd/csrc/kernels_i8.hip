@@ -713,31 +713,38 @@ static void rows_dense(hipStream_t st, const I8Args& g, int max_tiles, int out_t
     else if (out_type == PHX_BF16) launch(k_i8_rows<NW, RT, CT, false, false, PHX_BF16>, grid, blk, 0, st, g);
     else launch(k_i8_rows<NW, RT, CT, false, false, PHX_F32>, grid, blk, 0, st, g);
 }
-// RT for paired matrices, RD for the others
-template <int NW, int RT, int RD, int CT, bool ONCE>
-static void rows_grouped(hipStream_t st, const I8Mat& m, const I8Args& g, int max_tiles)
+
+template <int NW, int RT, int CT, bool PAIRED, bool ONCE>
+static void rows_float(hipStream_t st, const I8Args& g, int max_tiles)
 {
-    const int w = 16 * (m.paired ? RT : RD);
-    const dim3 grid((g.out_cols + w - 1) / w, max_tiles), blk(64 * NW);
-    if (m.paired) launch(k_i8_rows<NW, RT, CT, true, ONCE, PHX_F32>, grid, blk, 0, st, g);
-    else launch(k_i8_rows<NW, RD, CT, false, ONCE, PHX_F32>, grid, blk, 0, st, g);
+    const dim3 grid((g.out_cols + 16 * RT - 1) / (16 * RT), max_tiles), blk(64 * NW);
+    launch(k_i8_rows<NW, RT, CT, PAIRED, ONCE, PHX_F32>, grid, blk, 0, st, g);
+}
+
+// 32 channels, 64 outputs a workgroup: 64 experts of d = 4096, nf = 1408, T = 24 127 us; 64 channels 136, 32 outputs 125;
+// 128 of 2816, 704, T = 128: 148; 16 channels 158, 32 outputs 156
+template <int CT, bool ONCE>
+static void rows_lists(hipStream_t st, const I8Mat& m, const I8Args& g, int max_tiles)
+{
+    if (m.paired) rows_float<4, 2, CT, true, ONCE>(st, g, max_tiles);
+    else rows_float<4, 4, CT, false, ONCE>(st, g, max_tiles);
 }
 
 template <bool ONCE>
-static void rows_lists(hipStream_t st, const I8Mat& m, const I8Args& g, int max_tiles)
+static void rows_by_cap(hipStream_t st, const I8Mat& m, const I8Args& g, int max_tiles)
 {
-    if (g.cap <= 16) rows_grouped<4, 2, 4, 1, ONCE>(st, m, g, max_tiles);
-    else if (g.cap <= 32) rows_grouped<4, 2, 4, 2, ONCE>(st, m, g, max_tiles);
-    else rows_grouped<4, 2, 4, 4, ONCE>(st, m, g, max_tiles);
+    if (g.cap <= 16) rows_lists<1, ONCE>(st, m, g, max_tiles);
+    else if (g.cap <= 32) rows_lists<2, ONCE>(st, m, g, max_tiles);
+    else rows_lists<4, ONCE>(st, m, g, max_tiles);
 }
 
 void launch_i8_product(hipStream_t st, const I8Mat& m, I8Args g, bool tile, int max_tiles, int ncu, int out_type)
 {
     set_matrix(g, m);
     if (tile) {
-        // Lists: every XCD takes pairs of tiles (mostly of one expert: its second tile finds the weights in the L2) and all their
-        // row blocks.  A dense product: the split with the fewest workgroups on an XCD, and of those the one that brings
-        // the fewest bytes to the XCDs, each its tiles' tokens and its blocks' weights.
+        // Lists: every XCD takes pairs of tiles, mostly of one expert, and all their row blocks (64 experts of d = 4096,
+        // nf = 1408, T = 4096: gate|up 275 us, tile by tile 304).  A dense product: the split with the fewest workgroups on
+        // an XCD, and of those the one that brings the fewest bytes to the XCDs, each its tiles' tokens and its blocks' weights.
         const int blocks = (m.rg + 7) / 8;
         g.xt = 8;
         g.run = 2;
@@ -774,14 +781,11 @@ void launch_i8_product(hipStream_t st, const I8Mat& m, I8Args g, bool tile, int 
             else if (n < 4 * ncu) rows_dense<8, 2, 8>(st, g, max_tiles, out_type);
             else rows_dense<8, 4, 8>(st, g, max_tiles, out_type);
         }
-    } else if (g.ids) {
-        if ((int64_t)((g.out_cols + 15) / 16) * max_tiles < 4 * ncu) rows_grouped<8, 1, 1, 1, false>(st, m, g, max_tiles);
-        else rows_grouped<4, 2, 4, 1, false>(st, m, g, max_tiles);
-    }
-    // 32 channels, 64 outputs a workgroup: 64 experts of d = 4096, nf = 1408, T = 24 127 us; 64 channels 136, 32 outputs 125;
-    // 128 of 2816, 704, T = 128: 148; 16 channels 158, 32 outputs 156
-    else if (g.once) rows_lists<true>(st, m, g, max_tiles);
-    else rows_lists<false>(st, m, g, max_tiles);
+    } else if (g.ids) {  // single assignments: paired matrices only (launch_i8_down_few takes the others)
+        if ((int64_t)((g.out_cols + 15) / 16) * max_tiles < 4 * ncu) rows_float<8, 1, 1, true, false>(st, g, max_tiles);
+        else rows_float<4, 2, 1, true, false>(st, g, max_tiles);
+    } else if (g.once) rows_by_cap<true>(st, m, g, max_tiles);
+    else rows_by_cap<false>(st, m, g, max_tiles);
 }
 
 template <int NW>
