@@ -306,6 +306,9 @@ int phx_matvec(phx_moe_ctx* ctx, int type, const void* w, int rows, int cols, in
 typedef struct phx_weight phx_weight;
 int phx_weight_upload(phx_moe_ctx* ctx, int type, int rows, int cols, const void* gguf_rows, phx_weight** out);
 void phx_weight_free(phx_moe_ctx* ctx, phx_weight* w);
+/* The sizes a handle was uploaded with (n_mat: 1 but for phx_weight_upload_i8), for a caller that sizes buffers
+ * by it; the GPU is not touched.  Any pointer may be null; PHX_ERR_ARG without a handle. */
+int phx_weight_shape(const phx_weight* w, int* n_mat, int* rows, int* cols);
 int phx_matmul(phx_moe_ctx* ctx, const phx_weight* w, int T, const int8_t* xq, const uint16_t* xd, float* y);
 
 /* Dense K-quant matvec over T token rows: KernelsK.MatVec for Q4_K / Q5_K / Q6_K weights as GemmaGpu.MatVec

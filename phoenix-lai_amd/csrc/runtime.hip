@@ -2083,6 +2083,15 @@ void phx_weight_free(phx_moe_ctx* c, phx_weight* w)
     delete w;
 }
 
+int phx_weight_shape(const phx_weight* w, int* n_mat, int* rows, int* cols)
+{
+    if (!w) return PHX_ERR_ARG;
+    if (n_mat) *n_mat = w->i8.n_mat ? w->i8.n_mat : 1;
+    if (rows) *rows = w->rows;
+    if (cols) *cols = w->cols;
+    return PHX_OK;
+}
+
 // The VALU products read the caller's rows (qb bytes of integers, db of scales) while they write y: where y shares
 // bytes with them, they read a copy instead, enqueued first.
 static int rows_apart(phx_moe_ctx* c, const int8_t*& xq, int64_t qb, const void*& xd, int64_t db, const float* y, int64_t yb)

@@ -170,6 +170,7 @@ def load_lib():
         "phx_matvec": (i32, [vp, i32, vp, i32, i32, i32, vp, vp, vp]),
         "phx_weight_upload": (i32, [vp, i32, i32, i32, vp, C.POINTER(vp)]),
         "phx_weight_free": (None, [vp, vp]),
+        "phx_weight_shape": (i32, [vp, C.POINTER(i32), C.POINTER(i32), C.POINTER(i32)]),
         "phx_matmul": (i32, [vp, vp, i32, vp, vp, vp]),
         "phx_matmul_k": (i32, [vp, vp, i32, vp, vp, vp]),
         "phx_route_check": (i32, [C.POINTER(RouteDesc)]),
@@ -488,12 +489,26 @@ class MoeContext:
     def weight_free(self, handle: int):
         self.lib.phx_weight_free(self.h, handle)
 
+    def weight_shape(self, handle: int) -> tuple[int, int, int]:
+        """phx_weight_shape: (n_mat, rows, cols) that a handle was uploaded with."""
+        v = [C.c_int() for _ in range(3)]
+        rc = self.lib.phx_weight_shape(handle, *(C.byref(i) for i in v))
+        if rc:
+            _raise(rc, "null weight handle")
+        return tuple(i.value for i in v)
+
+    def _fits(self, handle: int, rows: int, cols: int):
+        """Refuse sizes that are not the handle's: the product reads and writes by the handle's own."""
+        if (have := self.weight_shape(handle)[1:]) != (rows, cols):
+            raise ArgumentError(PHX.ERR_ARG, f"a {rows} x {cols} product of a {have[0]} x {have[1]} weight")
+
     def matmul_device(self, handle: int, T: int, xq_ptr: int, xd_ptr: int, y_ptr: int):
         """phx_matmul (KernelsPrefill.MatMulQ4Q8Tile as GemmaGpu.Mm records it), asynchronous."""
         self._check(self.lib.phx_matmul(self.h, handle, T, xq_ptr, xd_ptr, y_ptr))
 
     def MatMul(self, handle: int, rows: int, cols: int, xq: np.ndarray, xd: np.ndarray) -> np.ndarray:
         """GemmaGpu.Mm on host arrays: y [T][rows] f32 from T Q8_0 rows (as Q80 returns them)."""
+        self._fits(handle, rows, cols)
         xq = np.ascontiguousarray(xq, dtype=np.int8).reshape(-1, cols)
         xd = np.ascontiguousarray(xd, dtype=np.uint16).reshape(xq.shape[0], cols // 32)
         T = xq.shape[0]
@@ -517,6 +532,7 @@ class MoeContext:
         d as Q8K returns them; the block sums are formed on the device)."""
         if cols <= 0 or cols % 256:
             raise ArgumentError(PHX.ERR_ARG, f"cols {cols} is not a multiple of 256")
+        self._fits(handle, rows, cols)
         xq = np.ascontiguousarray(xq, dtype=np.int8)
         xd = np.ascontiguousarray(xd, dtype=np.float32)
         if xq.size % cols or xd.size * 256 != xq.size:
@@ -617,6 +633,7 @@ class MoeContext:
 
     def MatMulI8(self, handle: int, rows: int, cols: int, xq: np.ndarray, xd: np.ndarray) -> np.ndarray:
         """phx_matmul_i8 on host arrays: y [T][rows] f32 from T int8 rows and their scales (as QuantI8 returns them)."""
+        self._fits(handle, rows, cols)
         xq = np.ascontiguousarray(xq, dtype=np.int8)
         xd = _f32(xd)
         if cols <= 0 or xq.size % cols or xd.size * cols != xq.size:
@@ -640,6 +657,7 @@ class MoeContext:
         xd, weights = _f32(xd), _f32(weights)
         if xq.ndim != 2 or ids.ndim != 2 or xd.shape != xq.shape[:1] or weights.shape != ids.shape or len(ids) != len(xq):
             raise ArgumentError(PHX.ERR_ARG, f"rows {xq.shape}, scales {xd.shape}, ids {ids.shape}, weights {weights.shape}")
+        self._fits(gate_up, self.weight_shape(gate_up)[1], xq.shape[1])  # down's sizes: phx_experts_i8
         return self._on_device([xq, xd, ids, weights], [(xq.shape, np.float32)],
                                lambda *p: self.experts_i8_device(gate_up, down, act, xq.shape[0], ids.shape[1], *p[:4], PHX.F32,
                                                                  p[4]))[0]
