@@ -192,6 +192,16 @@ def _f32(a) -> np.ndarray:
     return np.ascontiguousarray(a, dtype=np.float32)
 
 
+def _ints(a, dtype) -> np.ndarray:
+    """Whole numbers as dtype, refused where dtype does not hold one of them."""
+    a = np.asarray(a)
+    with np.errstate(invalid="ignore"):
+        out = np.ascontiguousarray(a, dtype=dtype)
+    if a.dtype != out.dtype and not np.array_equal(out, a):
+        raise ArgumentError(PHX.ERR_ARG, f"{a.dtype} values that {np.dtype(dtype)} does not hold")
+    return out
+
+
 class DeviceBuffer:
     def __init__(self, ctx: "MoeContext", nbytes: int):
         self.ctx, self.nbytes = ctx, nbytes
@@ -615,7 +625,7 @@ class MoeContext:
         (paired: gate rows, then up rows); w and scale numpy arrays or addresses (host or device memory).  Returns the
         handle for matmul_i8_device / experts_i8_device / weight_free."""
         if isinstance(w, np.ndarray):
-            w = np.ascontiguousarray(w, dtype=np.int8)
+            w = _ints(w, np.int8)
             if w.size != n_mat * rows * cols:
                 raise ArgumentError(PHX.ERR_ARG, f"{w.size} weights for {n_mat} matrices of {rows} x {cols}")
         if isinstance(scale, np.ndarray):
@@ -634,7 +644,7 @@ class MoeContext:
     def MatMulI8(self, handle: int, rows: int, cols: int, xq: np.ndarray, xd: np.ndarray) -> np.ndarray:
         """phx_matmul_i8 on host arrays: y [T][rows] f32 from T int8 rows and their scales (as QuantI8 returns them)."""
         self._fits(handle, rows, cols)
-        xq = np.ascontiguousarray(xq, dtype=np.int8)
+        xq = _ints(xq, np.int8)
         xd = _f32(xd)
         if cols <= 0 or xq.size % cols or xd.size * cols != xq.size:
             raise ArgumentError(PHX.ERR_ARG, f"input of {xq.size} quants and {xd.size} scales for {cols} columns")
@@ -652,8 +662,8 @@ class MoeContext:
                   weights: np.ndarray) -> np.ndarray:
         """phx_experts_i8 on host arrays: out [T][d] f32 from int8 rows (as QuantI8 returns them) and a routing (as Route
         returns it)."""
-        xq = np.ascontiguousarray(xq, dtype=np.int8)
-        ids = np.ascontiguousarray(ids, dtype=np.int32)
+        xq = _ints(xq, np.int8)
+        ids = _ints(ids, np.int32)
         xd, weights = _f32(xd), _f32(weights)
         if xq.ndim != 2 or ids.ndim != 2 or xd.shape != xq.shape[:1] or weights.shape != ids.shape or len(ids) != len(xq):
             raise ArgumentError(PHX.ERR_ARG, f"rows {xq.shape}, scales {xd.shape}, ids {ids.shape}, weights {weights.shape}")

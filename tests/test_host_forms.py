@@ -69,3 +69,27 @@ def test_experts_go_by_the_handles_sizes(host, pkg):
     assert "phx_experts_i8" not in host.lib.made
     assert experts(host, 256).shape == (3, 256)
     assert "phx_experts_i8" in host.lib.made
+
+
+@pytest.mark.parametrize("bad", [np.full((3, 256), 200, np.uint8), np.full((3, 256), -129, np.int64), np.full((3, 256), 0.5),
+                                 np.full((3, 256), 128.0, F32), np.full((3, 256), np.nan, F32)])
+def test_quants_that_int8_does_not_hold(host, pkg, bad):
+    ids, w = np.zeros((3, 2), np.int32), np.zeros((3, 2), F32)
+    with pytest.raises(pkg.ArgumentError):
+        host.MatMulI8(1, 64, 256, bad, np.zeros(3, F32))
+    with pytest.raises(pkg.ArgumentError):
+        host.ExpertsI8(2, 3, 1, bad, np.zeros(3, F32), ids, w)
+    with pytest.raises(pkg.ArgumentError):
+        host.weight_upload_i8(1, 3, 256, bad, np.zeros(3, F32))
+    assert not {"phx_matmul_i8", "phx_experts_i8", "phx_weight_upload_i8"} & set(host.lib.made)
+
+
+def test_ids_that_int32_does_not_hold(host, pkg):
+    """An id past 32 bits is no expert; cut to 32 bits it would be expert 0."""
+    xq, xd, w = np.zeros((3, 256), I8), np.zeros(3, F32), np.zeros((3, 2), F32)
+    for bad in (np.full((3, 2), 1 << 32), np.full((3, 2), 0xFFFFFFFF, np.uint32), np.full((3, 2), 0.5)):
+        with pytest.raises(pkg.ArgumentError):
+            host.ExpertsI8(2, 3, 1, xq, xd, bad, w)
+    assert "phx_experts_i8" not in host.lib.made
+    host.ExpertsI8(2, 3, 1, np.full((3, 256), 127.0), xd, np.full((3, 2), -1, np.int64), w)  # these they hold
+    assert "phx_experts_i8" in host.lib.made
