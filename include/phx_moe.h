@@ -328,9 +328,9 @@ int phx_matmul_k(phx_moe_ctx* ctx, const phx_weight* w, int T, const int8_t* xq,
  * output channel.  The reference has neither (its router is src/GemmaCpu.cs:385-407, its int8 weights
  * Q8_0 blocks): these stand beside phx_moe_ffn's router, phx_quant_q8_0, phx_matmul and the FFN itself.
  * Like those they take device pointers (memory the GPU can address: a pageable host pointer returns
- * PHX_ERR_ARG) and are asynchronous on the context's stream (phx_moe_sync waits); inputs are written, and
- * outputs free to overwrite, before the call.  An output that shares bytes with an input or another output
- * returns PHX_ERR_ARG. */
+ * PHX_ERR_ARG, and so does memory of another GPU or a handle uploaded to one) and are asynchronous on the
+ * context's stream (phx_moe_sync waits); inputs are written, and outputs free to overwrite, before the call.
+ * An output that shares bytes with an input or another output returns PHX_ERR_ARG. */
 
 /* How a router's scores become a choice of experts. */
 #define PHX_SCORE_SOFTMAX 0

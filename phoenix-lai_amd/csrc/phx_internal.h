@@ -33,12 +33,13 @@ struct LaunchTimer {
 };
 extern thread_local LaunchTimer* g_launch_timer;
 
-// Fault injection for tests of the error paths: PHX_FAULT="malloc:n" or "launch:n", read when a context
-// is created, fails that context's n-th device allocation with hipErrorOutOfMemory, or skips its n-th
+// Fault injection for tests of the error paths: PHX_FAULT="malloc:n", "launch:n" or "device:n", read when a
+// context is created, fails that context's n-th device allocation with hipErrorOutOfMemory, or skips its n-th
 // kernel launch and every later one of the same call and reports hipErrorLaunchFailure at the call's
-// launch check (as a lost device would); one fault per context.
+// launch check (as a lost device would), or takes the n-th buffer or handle that is checked for being another
+// GPU's for one (a refusal that a machine of one GPU cannot reach otherwise); one fault per context.
 struct FaultPlan {
-    enum Site { NONE = 0, MALLOC = 1, LAUNCH = 2 };
+    enum Site { NONE = 0, MALLOC = 1, LAUNCH = 2, DEVICE = 3 };
     int site = NONE;
     int64_t n = 0, count = 0;
     hipError_t pending = hipSuccess;

@@ -1250,6 +1250,7 @@ struct phx_weight {
     QMat q;
     I8Mat i8;
     int type = 0, rows = 0, cols = 0;
+    int device = 0;  // of the int8 matrices
 };
 
 // Workspace of phx_moe_ffn_noalloc: one array per device, which each GPU the library runs on holds
@@ -1334,10 +1335,11 @@ int phx_moe_create(int hip_device, phx_moe_ctx** out)
     if (hip_device < 0 || hip_device >= n) return PHX_ERR_ARG;
     phx_moe_ctx* c = new phx_moe_ctx();
     c->device = hip_device;
-    if (const char* f = getenv("PHX_FAULT")) {  // "malloc:n" | "launch:n" (tests of the error paths)
+    if (const char* f = getenv("PHX_FAULT")) {  // "malloc:n" | "launch:n" | "device:n" (tests of the error paths)
         long long n = 0;
         if (sscanf(f, "malloc:%lld", &n) == 1) c->fault.site = FaultPlan::MALLOC;
         else if (sscanf(f, "launch:%lld", &n) == 1) c->fault.site = FaultPlan::LAUNCH;
+        else if (sscanf(f, "device:%lld", &n) == 1) c->fault.site = FaultPlan::DEVICE;
         c->fault.n = n;
     }
     int rc = PHX_OK;
@@ -2257,6 +2259,14 @@ struct CallBuf {
     bool out;
 };
 
+// Memory, or a weight handle's matrices, of a GPU that is not the context's.
+bool foreign(phx_moe_ctx* c, int device) { return c->fault.fire(FaultPlan::DEVICE) || device != c->device; }
+
+int refuse_foreign(phx_moe_ctx* c, const char* call, const char* what, int device)
+{
+    return set_err(c, PHX_ERR_ARG, "%s: %s is memory of device %d, the context's is %d", call, what, device, c->device);
+}
+
 // Present, aligned, addressable by the context's GPU, and no output in any other buffer's bytes.
 int check_bufs(phx_moe_ctx* c, const char* call, std::initializer_list<CallBuf> bufs)
 {
@@ -2265,8 +2275,7 @@ int check_bufs(phx_moe_ctx* c, const char* call, std::initializer_list<CallBuf> 
         if ((uintptr_t)b.p % b.align) return set_err(c, PHX_ERR_ARG, "%s: %s needs %d-byte alignment", call, b.what, b.align);
         hipPointerAttribute_t at{};
         if (!device_accessible(b.p, &at)) return set_err(c, PHX_ERR_ARG, "%s: %s is not device-accessible memory", call, b.what);
-        if (at.type == hipMemoryTypeDevice && at.device != c->device)
-            return set_err(c, PHX_ERR_ARG, "%s: %s is memory of device %d, the context's is %d", call, b.what, at.device, c->device);
+        if (at.type == hipMemoryTypeDevice && foreign(c, at.device)) return refuse_foreign(c, call, b.what, at.device);
     }
     for (const CallBuf& o : bufs)
         for (const CallBuf& b : bufs)
@@ -2344,7 +2353,11 @@ namespace {
 int upload_i8(phx_moe_ctx* c, I8Mat& m, const int8_t* w, const float* scale)
 {
     const int64_t src = (int64_t)m.rows * m.cols;
-    const bool dev_w = device_accessible(w), dev_s = device_accessible(scale);
+    hipPointerAttribute_t aw{}, as{};
+    const bool dev_w = device_accessible(w, &aw), dev_s = device_accessible(scale, &as);
+    if (dev_w && aw.type == hipMemoryTypeDevice && foreign(c, aw.device)) return refuse_foreign(c, "weight upload", "w", aw.device);
+    if (dev_s && as.type == hipMemoryTypeDevice && foreign(c, as.device))
+        return refuse_foreign(c, "weight upload", "scale", as.device);
     HIPCHK(c, dev_malloc(c, (void**)&m.w, (size_t)(m.n_mat * m.mat_bytes())));
     HIPCHK(c, dev_malloc(c, (void**)&m.scale, (size_t)m.n_mat * m.rg * 32 * 4));
     // host matrices go through a buffer of one of them
@@ -2391,6 +2404,7 @@ int phx_weight_upload_i8(phx_moe_ctx* c, int n_mat, int rows, int cols, int pair
     h->type = PHX_I8_WEIGHT;
     h->rows = rows;
     h->cols = cols;
+    h->device = c->device;
     I8Mat& m = h->i8;
     m.n_mat = n_mat;
     m.rows = rows;
@@ -2417,6 +2431,7 @@ int phx_matmul_i8(phx_moe_ctx* c, const phx_weight* w, int T, const int8_t* xq, 
     if (!eb) return set_err(c, PHX_ERR_UNSUPPORTED, "matmul_i8: type %d (PHX_F32, PHX_F16 and PHX_BF16 only)", y_type);
     if (T <= 0 || T > kMaxRowsI8) return set_err(c, PHX_ERR_ARG, "matmul_i8: T=%d out of range", T);
     ENTER(c);
+    if (foreign(c, w->device)) return refuse_foreign(c, "matmul_i8", "the weight", w->device);
     if (const int rc = check_bufs(c, "matmul_i8", {{"xq", xq, (int64_t)T * w->cols, 16, false},
                                                    {"xd", xd, T * 4ll, 4, false},
                                                    {"y", y, (int64_t)T * w->rows * eb, 16, true}}))
@@ -2450,6 +2465,8 @@ int phx_experts_i8(phx_moe_ctx* c, const phx_weight* gu, const phx_weight* dn, i
     if (T <= 0 || T > kMaxRowsI8 || k <= 0 || k > PHX_MAX_USED)
         return set_err(c, PHX_ERR_ARG, "experts_i8: T=%d, k=%d out of range", T, k);
     ENTER(c);
+    if (foreign(c, gu->device)) return refuse_foreign(c, "experts_i8", "gate_up", gu->device);
+    if (foreign(c, dn->device)) return refuse_foreign(c, "experts_i8", "down", dn->device);
     if (const int rc = check_bufs(c, "experts_i8", {{"xq", xq, (int64_t)T * d, 16, false},
                                                     {"xd", xd, T * 4ll, 4, false},
                                                     {"ids", ids, (int64_t)T * k * 4, 4, false},
