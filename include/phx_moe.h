@@ -231,7 +231,8 @@ int phx_moe_profile_read(phx_moe_ctx* ctx, double* total_ms, int64_t* launches);
  * many-token router's error bound assumes); 10 the sequential double sum of squares of each row of
  * m = b[0] floats of a (n a multiple of m, 2 <= m <= 65536), the sum RmsNorm's certified means fall back
  * to, formed by one wave as the kernels form it: out[2 r] and out[2 r + 1] hold the low and high 32
- * bits of row r's double; 11 and 12 silu(a) * b and gelu(a) * b as phx_experts_i8 forms them.  out is float (int results as their value). */
+ * bits of row r's double; 11 and 12 silu(a) * b and gelu(a) * b as phx_experts_i8 forms them, but for a NaN a
+ * in 12, which the experts keep and the table form has 0 for.  out is float (int results as their value). */
 int phx_moe_selftest(phx_moe_ctx* ctx, int op, int n, const float* a, const float* b, float* out);
 
 /* Average time (ms) of `iters` coalesced streaming reads of a device buffer: the achievable HBM
@@ -370,8 +371,9 @@ int phx_route(phx_moe_ctx* ctx, const phx_route_desc* desc, int T, const void* l
  * values v = x, silu(x) * aux, rmsnorm(x) * aux or gelu(x) * aux (mode PHX_QUANT_*, each value rounded to
  * float as phx_quant_q8_0 forms it; the norm's sum of squares in double), then
  *   d[r] = max |v| / 127,  qs[r][i] = roundf(v * (1 / d[r]))   (halves away from zero, within +-127)
- * A row whose d would be under 2^-126 gets d = 0 and zeros; one that holds a NaN or an infinity gets d = NaN
- * and zeros.  x: rows x n of x_type (PHX_F32, PHX_F16, PHX_BF16), ld values apart (ld >= n); aux as x with
+ * A row whose d would be under 2^-126 gets d = 0 and zeros; one whose v hold a NaN or an infinity gets d = NaN
+ * and zeros.  A NaN in x or aux makes its v a NaN in every mode (phx_quant_q8_0's gelu has 0 for a NaN); gelu of
+ * -infinity is 0.  x: rows x n of x_type (PHX_F32, PHX_F16, PHX_BF16), ld values apart (ld >= n); aux as x with
  * the gated modes (so gate and up may lie side by side in one buffer), float [n] in PHX_QUANT_RMS_NORM, NULL
  * in PHX_QUANT_PLAIN.  qs [rows][n], d [rows].  n a multiple of 32, at most 65536; ld a multiple of 8; rows <= 2^24;
  * x and aux 16-byte, qs 8-byte aligned. */

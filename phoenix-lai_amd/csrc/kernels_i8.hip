@@ -99,10 +99,17 @@ __device__ __forceinline__ float gelu_near(float x)
     return h2f(f2h_of(0.5f * h * (1.0f + t)));
 }
 
-// h = act(gate) * up as phx_quant_i8 forms it
+// act(gate) * up
 __device__ __forceinline__ float gated(int act, float gate, float up)
 {
     return (act == PHX_QUANT_SILU_MUL ? silu_near(gate) : gelu_near(gate)) * up;
+}
+// h as phx_quant_i8 forms it: a NaN gate stays one, so that the row which held it says so in its scale (gelu_near, like
+// the table, has 0 there)
+__device__ __forceinline__ float gated_kept(int act, float gate, float up)
+{
+    const float h = gated(act, gate, up);
+    return gate != gate ? gate : h;
 }
 
 // NT threads per row, eight consecutive values per thread and step, the row held in registers between its statistics and its
@@ -153,6 +160,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_quant_i8(int rows, int 
                 // silu by the library's exponential: the rows' bytes bound this kernel, and the shorter code is the faster one
                 // (77 rows of 2112: 4.2 us, by silu_near 5.1)
                 v[s][j] = MODE == PHX_QUANT_RMS_NORM ? u * scale * a[j] : (MODE == PHX_QUANT_SILU_MUL ? silu_ref(u) : gelu_near(u)) * a[j];
+                if (MODE == PHX_QUANT_GELU_MUL && u != u) v[s][j] = u;  // gelu_near has 0 there
             }
         }
 #pragma unroll
@@ -387,7 +395,7 @@ __device__ __forceinline__ void i8_rows_product(const I8Args& g, const Tile& tl,
         if (tok >= tl.cnt) break;
         const int at = (((tok >> 4) * NR + (c >> 4) * NB) * 4 + (i & 3)) * 64 + (c & 15) + 16 * (i >> 2);
         float y = (float)red[at] * (dxs[tok] * sg);
-        if (PAIRED) y = gated(g.act, y, (float)red[at + 256] * (dxs[tok] * su));
+        if (PAIRED) y = gated_kept(g.act, y, (float)red[at + 256] * (dxs[tok] * su));
         store_one<DT>(out + orow[tok], col, y);
     }
 }
@@ -651,7 +659,7 @@ __device__ __forceinline__ void i8_tile_product(const I8Args& g, const Tile& tl,
 #pragma unroll
             for (int i = 0; i < V; i++) {
                 y[i] = (float)s[i] * (dx * dw[i]);
-                if (PAIRED) y[i] = gated(g.act, y[i], (float)u[i] * (dx * du[i]));
+                if (PAIRED) y[i] = gated_kept(g.act, y[i], (float)u[i] * (dx * du[i]));
             }
             if (whole) {
                 if (col < g.out_cols) store_16<DT>(o, col, y);
