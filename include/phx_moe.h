@@ -339,6 +339,11 @@ int phx_matmul_k(phx_moe_ctx* ctx, const phx_weight* w, int T, const int8_t* xq,
 #define PHX_GROUP_MAX 0  /* a group's score: its largest selection score */
 #define PHX_GROUP_TOP2 1 /* the sum of its two largest (of its one, where it has but one) */
 #define PHX_MAX_GROUPS 64
+/* Limits of a call: rows of phx_route, phx_quant_i8, phx_matmul_i8 and phx_experts_i8, or of an int8 matrix (2^20); values of
+ * a row (2^16); elements of one int8 matrix (2^34). */
+#define PHX_MAX_ROWS_I8 1048576
+#define PHX_MAX_COLS_I8 65536
+#define PHX_MAX_MATRIX_I8 17179869184
 typedef struct phx_route_desc {
     int32_t n_expert;     /* E, 1 .. PHX_MAX_EXPERTS */
     int32_t n_used;       /* k, 1 .. PHX_MAX_USED */
@@ -355,7 +360,7 @@ typedef struct phx_route_desc {
  * for sizes past the limits and unknown types. */
 int phx_route_check(const phx_route_desc* desc);
 
-/* Routing of T rows of logits [T][E] (1 <= T <= 2^20):
+/* Routing of T rows of logits [T][E] (1 <= T <= PHX_MAX_ROWS_I8):
  *   s = softmax(logits[t]) or sigmoid(logits[t]);  c = s + bias (bias [E] f32 or NULL)
  * keeps the n_group_used groups of largest score, then the k experts of largest c in them, best first, ties to
  * the lower index throughout; ids [T][k], and weights [T][k] = s of the chosen (not c), divided by their
@@ -375,23 +380,24 @@ int phx_route(phx_moe_ctx* ctx, const phx_route_desc* desc, int T, const void* l
  * and zeros.  A NaN in x or aux makes its v a NaN in every mode (phx_quant_q8_0's gelu has 0 for a NaN); gelu of
  * -infinity is 0.  x: rows x n of x_type (PHX_F32, PHX_F16, PHX_BF16), ld values apart (ld >= n); aux as x with
  * the gated modes (so gate and up may lie side by side in one buffer), float [n] in PHX_QUANT_RMS_NORM, NULL
- * in PHX_QUANT_PLAIN.  qs [rows][n], d [rows].  n a multiple of 32, at most 65536; ld a multiple of 8; rows <= 2^24;
- * x and aux 16-byte, qs 8-byte aligned. */
+ * in PHX_QUANT_PLAIN.  qs [rows][n], d [rows].  n a multiple of 32, at most PHX_MAX_COLS_I8; ld a multiple of
+ * 8, at most 2^40; 1 <= rows <= PHX_MAX_ROWS_I8; x and aux 16-byte, qs 8-byte aligned. */
 int phx_quant_i8(phx_moe_ctx* ctx, int mode, int x_type, const void* x, const void* aux, int rows, int n, int64_t ld,
                  float eps, int8_t* qs, float* d);
 
 /* int8 matrices to the device, laid out once for the products: n_mat matrices (1 for a dense projection,
  * n_expert for experts, <= 256) of `rows` rows of `cols`, w [n_mat][rows][cols] and a scale per output
  * channel, scale [n_mat][rows] (host or device memory, read before the call returns).  cols a multiple of
- * 32, at most 65536; rows <= 2^20.  paired: the rows are gate (first half) and up of a gated FFN, for
- * phx_experts_i8 (rows a multiple of 64).  phx_weight_free releases the handle. */
+ * 32, at most PHX_MAX_COLS_I8; rows <= PHX_MAX_ROWS_I8; rows * cols <= PHX_MAX_MATRIX_I8.  paired: the rows
+ * are gate (first half) and up of a gated FFN, for phx_experts_i8 (rows a multiple of 64).  phx_weight_free
+ * releases the handle. */
 int phx_weight_upload_i8(phx_moe_ctx* ctx, int n_mat, int rows, int cols, int paired, const int8_t* w,
                          const float* scale, phx_weight** out);
 
 /* y[t][r] = (float)(sum_i xq[t][i] * w[r][i]) * (xd[t] * scale[r]) for T rows as phx_quant_i8 makes them: the sum
  * exact in int32, one rounding to float, one for the product of the scales, one for the value, and one more to
- * y_type (PHX_F32, PHX_F16, PHX_BF16).  w: a handle of one matrix, not paired.  1 <= T <= 2^20; xq 16-byte, y
- * 16-byte aligned. */
+ * y_type (PHX_F32, PHX_F16, PHX_BF16).  w: a handle of one matrix, not paired.  1 <= T <= PHX_MAX_ROWS_I8; xq
+ * and y 16-byte aligned. */
 int phx_matmul_i8(phx_moe_ctx* ctx, const phx_weight* w, int T, const int8_t* xq, const float* xd, int y_type, void* y);
 
 /* The gated FFN of int8 experts for T rows and a routing (phx_route's, or any ids):
@@ -400,8 +406,8 @@ int phx_matmul_i8(phx_moe_ctx* ctx, const phx_weight* w, int T, const int8_t* xq
  *   out[t] = sum over j, in order, of weights[t][j] * (the product of that row with down matrix e)
  * the sum in float, rounded to out_type at the end.  A place whose id is outside [0, n_expert) is skipped; a
  * row without experts is zero.  An id may come more than once in a row.  gate_up: paired, [n_expert][2 nf][d]; down:
- * [n_expert][d][nf]; xq [T][d], xd [T], ids and weights [T][k], out [T][d]; 1 <= T <= 2^20, 1 <= k <= PHX_MAX_USED;
- * xq and out 16-byte aligned. */
+ * [n_expert][d][nf]; xq [T][d], xd [T], ids and weights [T][k], out [T][d]; 1 <= T <= PHX_MAX_ROWS_I8,
+ * 1 <= k <= PHX_MAX_USED; xq and out 16-byte aligned. */
 int phx_experts_i8(phx_moe_ctx* ctx, const phx_weight* gate_up, const phx_weight* down, int act, int T, int k,
                    const int8_t* xq, const float* xd, const int32_t* ids, const float* weights, int out_type, void* out);
 

@@ -2248,7 +2248,6 @@ int phx_matvec(phx_moe_ctx* c, int type, const void* w, int rows, int cols, int 
 
 namespace {
 constexpr int PHX_I8_WEIGHT = 24;  // GgmlType's int8
-constexpr int kMaxRowsI8 = 1 << 20;
 
 // A buffer of a device-pointer call: what it is, its bytes, its alignment, and whether the call writes it.
 struct CallBuf {
@@ -2312,7 +2311,7 @@ int phx_route(phx_moe_ctx* c, const phx_route_desc* R, int T, const void* logits
 {
     if (!c) return PHX_ERR_ARG;
     if (const int rc = phx_route_check(R)) return set_err(c, rc, "route: descriptor refused (phx_route_check)");
-    if (T <= 0 || T > kMaxRowsI8) return set_err(c, PHX_ERR_ARG, "route: T=%d out of range", T);
+    if (T <= 0 || T > PHX_MAX_ROWS_I8) return set_err(c, PHX_ERR_ARG, "route: T=%d out of range", T);
     const int eb = elem_bytes(R->logits_type);
     const int64_t n = (int64_t)T * R->n_used * 4;
     const CallBuf lo{"logits", logits, (int64_t)T * R->n_expert * eb, eb, false}, id{"ids", ids, n, 4, true},
@@ -2333,9 +2332,9 @@ int phx_quant_i8(phx_moe_ctx* c, int mode, int x_type, const void* x, const void
     const int eb = elem_bytes(x_type);
     if (!eb) return set_err(c, PHX_ERR_UNSUPPORTED, "quant_i8: type %d (PHX_F32, PHX_F16 and PHX_BF16 only)", x_type);
     if (mode < PHX_QUANT_PLAIN || mode > PHX_QUANT_GELU_MUL) return set_err(c, PHX_ERR_ARG, "quant_i8: mode %d", mode);
-    if (rows <= 0 || rows > kMaxRowsI8 || n <= 0 || n % 32 || n > 65536 || ld < n || ld % 8 || ld > (int64_t)1 << 40)
-        return set_err(c, PHX_ERR_ARG, "quant_i8: %d rows of %d, %lld apart (n a multiple of 32, <= 65536; ld of 8, >= n)", rows,
-                       n, (long long)ld);
+    if (rows <= 0 || rows > PHX_MAX_ROWS_I8 || n <= 0 || n % 32 || n > PHX_MAX_COLS_I8 || ld < n || ld % 8 || ld > (int64_t)1 << 40)
+        return set_err(c, PHX_ERR_ARG, "quant_i8: %d rows of %d, %lld apart (rows <= %d; n a multiple of 32, <= %d; ld of 8, >= n)",
+                       rows, n, (long long)ld, PHX_MAX_ROWS_I8, PHX_MAX_COLS_I8);
     if (mode == PHX_QUANT_RMS_NORM && !(eps >= 0.0f)) return set_err(c, PHX_ERR_ARG, "quant_i8: eps");
     const int64_t span = ((rows - 1) * ld + n) * eb;
     const CallBuf bx{"x", x, span, 16, false}, bq{"qs", qs, (int64_t)rows * n, 8, true}, bd{"d", d, rows * 4ll, 4, true};
@@ -2394,10 +2393,14 @@ int phx_weight_upload_i8(phx_moe_ctx* c, int n_mat, int rows, int cols, int pair
 {
     if (!c || !out) return PHX_ERR_ARG;
     *out = nullptr;
-    if (n_mat <= 0 || n_mat > PHX_MAX_EXPERTS || rows <= 0 || rows > kMaxRowsI8 || cols <= 0 || cols % 32 || cols > 65536 ||
-        (int64_t)rows * cols > (int64_t)1 << 34 || (paired && rows % 64) || !w || !scale || (uintptr_t)scale % 4)
-        return set_err(c, PHX_ERR_ARG, "weight upload: %d int8 matrices of %d x %d (cols a multiple of 32, <= 65536)", n_mat, rows,
-                       cols);
+    if (n_mat <= 0 || n_mat > PHX_MAX_EXPERTS || rows <= 0 || rows > PHX_MAX_ROWS_I8 || cols <= 0 || cols % 32 ||
+        cols > PHX_MAX_COLS_I8 || (paired && rows % 64))
+        return set_err(c, PHX_ERR_ARG, "weight upload: %d int8 matrices of %d x %d (at most %d; rows <= %d, a multiple of 64 where paired; "
+                       "cols a multiple of 32, <= %d)", n_mat, rows, cols, PHX_MAX_EXPERTS, PHX_MAX_ROWS_I8, PHX_MAX_COLS_I8);
+    if ((int64_t)rows * cols > PHX_MAX_MATRIX_I8)
+        return set_err(c, PHX_ERR_ARG, "weight upload: an int8 matrix of %d x %d (rows * cols <= %lld)", rows, cols,
+                       (long long)PHX_MAX_MATRIX_I8);
+    if (!w || !scale || (uintptr_t)scale % 4) return set_err(c, PHX_ERR_ARG, "weight upload: null w or scale, or scale off 4 bytes");
     ENTER(c);
     phx_weight* h = new (std::nothrow) phx_weight();
     if (!h) return set_err(c, PHX_ERR_OOM, "weight upload: host memory");
@@ -2429,7 +2432,7 @@ int phx_matmul_i8(phx_moe_ctx* c, const phx_weight* w, int T, const int8_t* xq, 
         return set_err(c, PHX_ERR_UNSUPPORTED, "matmul_i8: the weight is not one plain int8 matrix (phx_weight_upload_i8)");
     const int eb = elem_bytes(y_type);
     if (!eb) return set_err(c, PHX_ERR_UNSUPPORTED, "matmul_i8: type %d (PHX_F32, PHX_F16 and PHX_BF16 only)", y_type);
-    if (T <= 0 || T > kMaxRowsI8) return set_err(c, PHX_ERR_ARG, "matmul_i8: T=%d out of range", T);
+    if (T <= 0 || T > PHX_MAX_ROWS_I8) return set_err(c, PHX_ERR_ARG, "matmul_i8: T=%d out of range", T);
     ENTER(c);
     if (foreign(c, w->device)) return refuse_foreign(c, "matmul_i8", "the weight", w->device);
     if (const int rc = check_bufs(c, "matmul_i8", {{"xq", xq, (int64_t)T * w->cols, 16, false},
@@ -2462,7 +2465,7 @@ int phx_experts_i8(phx_moe_ctx* c, const phx_weight* gu, const phx_weight* dn, i
     const int eb = elem_bytes(out_type);
     if (!eb) return set_err(c, PHX_ERR_UNSUPPORTED, "experts_i8: type %d (PHX_F32, PHX_F16 and PHX_BF16 only)", out_type);
     if (act != PHX_QUANT_SILU_MUL && act != PHX_QUANT_GELU_MUL) return set_err(c, PHX_ERR_ARG, "experts_i8: act %d", act);
-    if (T <= 0 || T > kMaxRowsI8 || k <= 0 || k > PHX_MAX_USED)
+    if (T <= 0 || T > PHX_MAX_ROWS_I8 || k <= 0 || k > PHX_MAX_USED)
         return set_err(c, PHX_ERR_ARG, "experts_i8: T=%d, k=%d out of range", T, k);
     ENTER(c);
     if (foreign(c, gu->device)) return refuse_foreign(c, "experts_i8", "gate_up", gu->device);

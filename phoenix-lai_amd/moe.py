@@ -28,6 +28,7 @@ class PHX:
     QUANT_PLAIN, QUANT_SILU_MUL, QUANT_RMS_NORM, QUANT_GELU_MUL = 0, 1, 2, 3
     SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
     GROUP_MAX, GROUP_TOP2, MAX_GROUPS = 0, 1, 64
+    MAX_ROWS_I8, MAX_COLS_I8, MAX_MATRIX_I8 = 1 << 20, 1 << 16, 1 << 34
 
 
 class MoeError(RuntimeError):
