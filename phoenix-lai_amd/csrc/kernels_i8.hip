@@ -68,7 +68,7 @@ __device__ __forceinline__ double exp_near(double x)
     const double t = x * 1.44269504088896340736, n = __builtin_rint(t);
     return __builtin_amdgcn_ldexp(exp2_frac(t - n), (int)n);
 }
-// silu_ref and gelu_ref without the library's exponential and the table: 26 and 45 instructions a value (a gate|up tile's
+// silu_ref and gelu_ref without the library's exponential and the table: 27 and 45 instructions a value (a gate|up tile's
 // epilogue 24 us; by the exponential and a gather a value it took as long as the tile's products).  The same roundings:
 // silu's quotient by the reciprocal, one refinement and two corrections, which round it correctly while nothing leaves
 // the normal numbers (|v| < 80); gelu equals the table at every fp16 value (tests).
@@ -80,7 +80,8 @@ __device__ __forceinline__ float silu_near(float v)
     y = __builtin_fmaf(__builtin_fmaf(-d, y, 1.0f), y, y);
     float q = v * y;
     q = __builtin_fmaf(__builtin_fmaf(-d, q, v), y, q);
-    return __builtin_fmaf(__builtin_fmaf(-d, q, v), y, q);
+    q = __builtin_fmaf(__builtin_fmaf(-d, q, v), y, q);
+    return __builtin_copysignf(q, v);  // of -0 the corrections make +0
 }
 __device__ __forceinline__ float gelu_near(float x)
 {
