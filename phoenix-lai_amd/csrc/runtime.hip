@@ -374,6 +374,8 @@ struct Buf {
     size_t bytes = 0;
 };
 
+enum I8Ws { I8_PERM, I8_TILES, I8_NTILES, I8_H, I8_HQ, I8_HD, I8_Y, I8_WS_COUNT };
+
 }  // namespace
 
 struct phx_moe_ctx {
@@ -433,8 +435,9 @@ struct phx_moe_ctx {
     };
     std::vector<FfnGraph> ffn_graphs;
     uint64_t upload_gen = 0;
-    // workspace of the int8 experts (I8Ws): a table of its own, which no captured graph names
-    std::vector<Buf> ws_i8;
+    // workspace of the int8 experts (I8Ws): a table of its own, which no captured graph names; an array, as the C entry points
+    // that fill it have nothing to catch a container's exception
+    Buf ws_i8[I8_WS_COUNT];
 };
 
 namespace {
@@ -2285,12 +2288,9 @@ int check_bufs(phx_moe_ctx* c, const char* call, std::initializer_list<CallBuf> 
 
 int elem_bytes(int type) { return type == PHX_F32 ? 4 : type == PHX_F16 || type == PHX_BF16 ? 2 : 0; }
 
-enum I8Ws { I8_PERM, I8_TILES, I8_NTILES, I8_H, I8_HQ, I8_HD, I8_Y, I8_WS_COUNT };
-
 template <class T>
 int i8_ensure(phx_moe_ctx* c, int id, int64_t n, T** out)
 {
-    if (c->ws_i8.empty()) c->ws_i8.resize(I8_WS_COUNT);
     Buf& b = c->ws_i8[id];
     const size_t bytes = std::max<size_t>((size_t)n * sizeof(T), 256);
     if (b.bytes < bytes) {
