@@ -114,8 +114,10 @@ __device__ __forceinline__ float gated_kept(int act, float gate, float up)
 }
 
 // NT threads per row, eight consecutive values per thread and step, the row held in registers between its statistics and its
-// integers: one pass over memory, which bounds it (8192 rows of 4096 fp16 values: 19 to 24 us, 4.2 to 5.2 TB/s; 2048 of
-// bf16, normed: 9 us).  A row of one wave needs no barrier, and a workgroup then takes four.
+// integers: one pass over memory, which bounds it (8192 rows of 4096 fp16 values: 20 to 24 us, 4.2 to 5.0 TB/s).  The row's own
+// loads all go out before the first wait; a norm's weights are loaded after the sum's barrier, a second trip (2048 rows of 4096
+// bf16, normed: 9 us, of which their bytes take 6).  A row of one wave needs no barrier, and a workgroup then takes four.  A
+// thread's steps past its row load and form the row's last values again: 2112 values pay for 4096, 14336 for 65536.
 template <int NT, int STEPS, int MODE, int DT>
 __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_quant_i8(int rows, int n, int64_t ld, float eps,
                                                                   const void* __restrict__ x, const void* __restrict__ aux,
@@ -128,7 +130,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_quant_i8(int rows, int 
     if (NT == 64 && row >= rows) return;  // a whole wave, and no barrier with one wave a row
     const int tid = threadIdx.x % NT, lane = tid & 63, wave = tid >> 6;
     float v[STEPS][8];
-    auto at = [&](int s) { return min((s * NT + tid) * 8, n - 8); };  // past the row its last values: every load in flight at once
+    auto at = [&](int s) { return min((s * NT + tid) * 8, n - 8); };  // past the row its last values
 #pragma unroll
     for (int s = 0; s < STEPS; s++) load_eight<DT>(x, row * ld + at(s), v[s]);
     float scale = 0.0f;
@@ -159,7 +161,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_quant_i8(int rows, int 
             for (int j = 0; j < 8; j++) {
                 const float u = v[s][j];
                 // silu by the library's exponential: the rows' bytes bound this kernel, and the shorter code is the faster one
-                // (77 rows of 2112: 4.2 us, by silu_near 5.1)
+                // (77 rows of 2112: 4.1 us, by silu_near 5.1)
                 v[s][j] = MODE == PHX_QUANT_RMS_NORM ? u * scale * a[j] : (MODE == PHX_QUANT_SILU_MUL ? silu_ref(u) : gelu_near(u)) * a[j];
                 if (MODE == PHX_QUANT_GELU_MUL && u != u) v[s][j] = u;  // gelu_near has 0 there
             }
@@ -420,8 +422,8 @@ __global__ __launch_bounds__(64 * NW) void k_i8_rows(I8Args g)
 // The down products of few assignments and their weighted sum, for a token (blockIdx.y) and 16 of its outputs: wave w takes
 // the token's places w, w + NW, ...  It issues the place's weights, forms the int8 row of its h meanwhile (every
 // workgroup of the token forms it again: nf floats from L2), and the places' values meet in LDS in order.  No lists, no
-// int8 rows and no partial outputs go through memory.  Bound by its chain of dependent trips (ids, h, the weights): 7.1 us
-// for one token of 8 x 704, d = 2816, whose 16 MB take 3.
+// int8 rows and no partial outputs go through memory.  Bound by its chains of dependent trips (ids, h twice, the weights; at the
+// end the id and the weight of each place in turn): 6.8 to 8.1 us for one token of 8 x 704, d = 2816, whose 16 MB take 2.5.
 template <int NW, int DT>
 __global__ __launch_bounds__(64 * NW) void k_i8_down_few(I8Args g, int k, int nf, const float* __restrict__ h,
                                                          const float* __restrict__ weights)
@@ -498,7 +500,8 @@ __global__ __launch_bounds__(64 * NW) void k_i8_down_few(I8Args g, int k, int nf
 // same from lane 32, over 64 banks, and each turn then has 16 distinct bank groups (by the row's number itself, two rows of
 // a turn share one: 8 cycles a read against 4).
 //
-// What it reaches: 8192 x 5632 x 4096 169 us, 2.2 POP/s (a library product of that size 181); T = 2048 of 4096 x 4096 35 us.  The
+// What it reaches: 8192 x 5632 x 4096 173 to 195 us by the clock, 1.9 to 2.2 POP/s (a library product of that size 181); T = 2048 of
+// 4096 x 4096 30 to 35 us.  Under 256 workgroups the time is one workgroup's chain: 4096 x 4096 takes 24 us from T = 129 to 512.  The
 // matrix cores run in 60% of a tile's cycles at the 2.0 GHz that they leave the clock; without any load from memory a step
 // takes 1.13 us against 1.5, the rest is the issue and the wait of the loads.  Two 128-token halves on eight waves that share
 // the weights in the L1 (experts, T = 2048: gate|up 176 -> 197 us), four ring slots (the same), wave priorities (the same) and
@@ -731,7 +734,8 @@ static void rows_float(hipStream_t st, const I8Args& g, int max_tiles)
 }
 
 // 32 channels, 64 outputs a workgroup: 64 experts of d = 4096, nf = 1408, T = 24 127 us; 64 channels 136, 32 outputs 125;
-// 128 of 2816, 704, T = 128: 148; 16 channels 158, 32 outputs 156
+// 128 of 2816, 704, T = 128: 148; 16 channels 158, 32 outputs 156 (all before weights read once passed the caches by, with
+// which the two kept forms take 114 and 139)
 template <int CT, bool ONCE>
 static void rows_lists(hipStream_t st, const I8Mat& m, const I8Args& g, int max_tiles)
 {
@@ -751,9 +755,11 @@ void launch_i8_product(hipStream_t st, const I8Mat& m, I8Args g, bool tile, int 
 {
     set_matrix(g, m);
     if (tile) {
-        // Lists: every XCD takes pairs of tiles, mostly of one expert, and all their row blocks (64 experts of d = 4096,
-        // nf = 1408, T = 4096: gate|up 275 us, tile by tile 304).  A dense product: the split with the fewest workgroups on
-        // an XCD, and of those the one that brings the fewest bytes to the XCDs, each its tiles' tokens and its blocks' weights.
+        // Lists: every XCD takes pairs of tiles and all their row blocks (64 experts of d = 4096, nf = 1408, T = 4096: gate|up
+        // 275 us, tile by tile 304).  A pair starts at an even tile whatever its expert: of the tiles that follow one of the same
+        // expert about half fall into the next pair, on another XCD, and read the expert's weights from memory again.  A dense
+        // product: the split with the fewest workgroups on an XCD, and of those the one that brings the fewest bytes to the
+        // XCDs, each its tiles' tokens and its blocks' weights.
         const int blocks = (m.rg + 7) / 8;
         g.xt = 8;
         g.run = 2;
@@ -781,7 +787,11 @@ void launch_i8_product(hipStream_t st, const I8Mat& m, I8Args g, bool tile, int 
     } else if (!g.tiles && !g.ids) {
         if (g.cap <= 16) rows_dense<8, 1, 1>(st, g, max_tiles, out_type);
         else if (g.cap <= 32) rows_dense<8, 1, 2>(st, g, max_tiles, out_type);
-        else {  // the widest row tile that still gives every compute unit a workgroup
+        else {
+            // Row tiles of 16 until their workgroups number two per compute unit, of 32 to four, then of 64 where the tokens are
+            // past 64 (us by tiles of 16, 32, 64; 2816 columns, T = 96): 4096 outputs 12.7, 13.4, 17.3; 8192 23.6, 13.7, 17.6;
+            // 16384 45.0, 25.4, 19.1.  T = 64: 4096 10.6, 11.3; 8192 19.6, 11.6.  In between the rule is not the best: 12288
+            // outputs, T = 96, take tiles of 32 and 25.2 us, of 64 18.1.
             const int64_t n = (int64_t)((g.out_cols + 15) / 16) * max_tiles;
             if (g.cap <= 64) {
                 if (n < 2 * ncu) rows_dense<8, 1, 4>(st, g, max_tiles, out_type);
@@ -790,7 +800,10 @@ void launch_i8_product(hipStream_t st, const I8Mat& m, I8Args g, bool tile, int 
             else if (n < 4 * ncu) rows_dense<8, 2, 8>(st, g, max_tiles, out_type);
             else rows_dense<8, 4, 8>(st, g, max_tiles, out_type);
         }
-    } else if (g.ids) {  // single assignments: paired matrices only (launch_i8_down_few takes the others)
+    } else if (g.ids) {
+        // Single assignments: paired matrices only (launch_i8_down_few takes the others).  8 waves on 16 channels until these
+        // workgroups number four per compute unit, then 4 waves on 32 (us, 8 waves first): 128 experts of d = 2816, nf = 704,
+        // T = 1 16.0, 15.8; T = 2 22.9, 24.3; T = 4 42.0 either way; 32 of 1024, 512, k = 4: T = 4 11.6, 10.7; T = 8 15.5, 12.7.
         if ((int64_t)((g.out_cols + 15) / 16) * max_tiles < 4 * ncu) rows_float<8, 1, 1, true, false>(st, g, max_tiles);
         else rows_float<4, 2, 1, true, false>(st, g, max_tiles);
     } else if (g.once) rows_by_cap<true>(st, m, g, max_tiles);

@@ -27,8 +27,9 @@ struct RouteArgs {
 // keys and a ballot: the lowest lane that holds it, and the first of its V, is the lowest index.  The keys are the logits,
 // exact in 32 bits, where their order is the scores' (no bias): then only the k chosen scores are ever formed, one per
 // lane.  With a bias (WIDE) they are the doubles s + b: the high words decide, and the low words where those are equal.
-// A token's chain of rounds bounds it, not memory: one token 3.2 us, all of it latency; 13001 of 128 bf16 logits 8.7 us
-// (4.2 MB); 2048 of 256 with bias and groups 7.2 us.  Double scores and 64-bit keys for every expert, each lane four of
+// One token takes 3.2 us, the latency of its chain of rounds.  Many are bound by instructions, not memory: a round over 64
+// lanes serves one token, and 13001 tokens are 13 waves a SIMD: of 128 bf16 logits 8.5 us (4.2 MB); 2048 of 256 with bias and
+// groups 7.3 us.  Double scores and 64-bit keys for every expert, each lane four of
 // them, took 24.3 and 9.2.
 template <int V, bool WIDE, int DT>
 __global__ __launch_bounds__(256) void k_route(RouteArgs R)

@@ -2443,6 +2443,10 @@ int phx_matmul_i8(phx_moe_ctx* c, const phx_weight* w, int T, const int8_t* xq, 
     g.xq = xq;
     g.xd = xd;
     g.nrows = T;
+    // The tile kernel past one tile of the row kernel, without a look at how many workgroups that makes (us, row kernel and tile
+    // kernel).  4096 x 4096: T = 128 18.6, 23.8; 256 19.5, 23.9; 512 24.4, 24.3; 1024 46.1, 25.7.
+    // 16384 x 4096: 128 26.1, 24.4; 256 49.5, 25.8; 1024 199.9, 58.3.  Few outputs would take the row kernel longer: 512 x 1024,
+    // T = 256 7.1, 10.8; 2048 9.2, 11.1; 2816 x 2112, T = 300 10.9, 16.0.
     const bool tile = T > kI8Rows;
     g.cap = tile ? kI8Tile : T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : kI8Rows;
     g.out = y;
@@ -2486,8 +2490,8 @@ int phx_experts_i8(phx_moe_ctx* c, const phx_weight* gu, const phx_weight* dn, i
     g.act = act;
     // Few assignments, most of them of an expert of their own: two launches without lists, which read an expert's matrices again
     // for each of its assignments.  The lists' three further launches cost about what 48 MB of such reads do, or three times
-    // that where all experts stay in the caches (128 experts of d = 2816, nf = 704: T = 4 45 against 49 us, T = 8 72
-    // against 61; 32 of 1024, 512: T = 16 16 against 20, T = 32 23 against 22).
+    // that where all experts stay in the caches (128 experts of d = 2816, nf = 704: T = 4 42 against 43 us, T = 8 72
+    // against 58; 64 of 4096, 1408, k = 4: T = 2 28 against 37; 32 of 1024, 512: T = 16 16 against 20, T = 32 23 against 21).
     const double each = 3.0 * nf * d, A0 = (double)T * k, again = A0 - E * (1.0 - pow(1.0 - 1.0 / E, A0));
     if (A0 <= 1024 && again * each <= (E * each <= 64e6 ? 144e6 : 48e6) && i8_down_few_fits(dn->i8)) {
         if ((rc = i8_ensure(c, I8_H, (int64_t)T * k * nf, &h))) return rc;
@@ -2501,7 +2505,12 @@ int phx_experts_i8(phx_moe_ctx* c, const phx_weight* gu, const phx_weight* dn, i
     }
     // long batches go through in chunks, so that the workspace stays bounded and every row of it within 2^32 bytes
     const int chunk = std::min<int64_t>(T, std::min<int64_t>(65535, ((1ll << 32) - 1) / (4ll * std::max(d, nf))) / k), A = chunk * k;
-    const bool tile = A > 14 * E;  // as T = 203 of 128 experts, k = 8: 172 us either way; 300: 188 against 192
+    // The tile kernel past 14 places an expert (us, lists of 64 and tile kernel): 128 experts of d = 2816, nf = 704, k = 8: T = 160
+    // 149, 148; 203 162, 160; 300 192, 176; 64 of 4096, 1408, k = 4: T = 128 184, 186; 200 207, 201; 300 238, 216.  Small experts
+    // would take the lists longer: 32 of 1024, 512, k = 4: T = 120 28, 33; 300 37, 47.  The lists' tiles: 16 places to two an
+    // expert, 32 to eight (us by 16, 32, 64; the 128 experts): T = 32 88.9, 90.2, 93.8; 64 111.1, 109.6, 112.9; 128 149, 138, 138;
+    // 160 172, 152, 149.
+    const bool tile = A > 14 * E;
     const int cap = tile ? kI8Tile : A <= 2 * E ? 16 : A <= 8 * E ? 32 : kI8RowsPaired;
     const int max_tiles = (A + cap - 1) / cap + std::min(E, A);
     int *perm, *ntiles;
@@ -2518,8 +2527,8 @@ int phx_experts_i8(phx_moe_ctx* c, const phx_weight* gu, const phx_weight* dn, i
     g.perm = perm;
     g.cap = cap;
     // Weights that nobody reads again soon pass the caches by: where the experts exceed half of the 256 MB that hold what was read
-    // last, and most have one tile (128 of d = 2816, nf = 704: T = 128 148 -> 142 us, T = 300 188 -> 179; T = 1000, 62 places an
-    // expert, 245 -> 258, T = 2048 317 -> 381; 32 of 1024, 512, 50 MB in all: T = 40 22.3 -> 23.3).
+    // last, and most have one tile (64 of d = 4096, nf = 1408: T = 24 124 -> 114 us; 128 of 2816, 704: T = 128 145 -> 139, T = 400
+    // 197 -> 190; T = 600, 38 places an expert, 218 -> 221, T = 2048 313 -> 374; 32 of 1024, 512, 50 MB in all: T = 40 21.9 -> 22.5).
     g.once = E * each > 128e6 && A <= 32 * E;
     for (int t0 = 0; t0 < T; t0 += chunk) {
         const int n = std::min(chunk, T - t0);
