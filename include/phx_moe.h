@@ -340,7 +340,7 @@ int phx_matmul_k(phx_moe_ctx* ctx, const phx_weight* w, int T, const int8_t* xq,
 #define PHX_GROUP_TOP2 1 /* the sum of its two largest (of its one, where it has but one) */
 #define PHX_MAX_GROUPS 64
 /* Limits of a call: rows of phx_route, phx_quant_i8, phx_matmul_i8 and phx_experts_i8, or of an int8 matrix (2^20); values of
- * a row (2^16); elements of one int8 matrix (2^34). */
+ * a row (2^16); elements of one int8 matrix (2^34).  The calls of the next section have the same ones. */
 #define PHX_MAX_ROWS_I8 1048576
 #define PHX_MAX_COLS_I8 65536
 #define PHX_MAX_MATRIX_I8 17179869184
@@ -410,6 +410,80 @@ int phx_matmul_i8(phx_moe_ctx* ctx, const phx_weight* w, int T, const int8_t* xq
  * 1 <= k <= PHX_MAX_USED; xq and out 16-byte aligned. */
 int phx_experts_i8(phx_moe_ctx* ctx, const phx_weight* gate_up, const phx_weight* down, int act, int T, int k,
                    const int8_t* xq, const float* xd, const int32_t* ids, const float* weights, int out_type, void* out);
+
+/* ---------------------------------------------------------------- float experts, adapters, the residual's norm
+ * For models whose experts are fp16 or bf16, and for projections that many requests share, each with an adapter of
+ * its own.  The reference has none of these: they stand beside phx_experts_i8, phx_matmul_i8 and phx_norm_add /
+ * phx_quant_i8, with the section above's rules for device pointers, streams and overlaps (where a call says that an
+ * output may be an input, it may be exactly that buffer).  Sums are in 32-bit floats, on the matrix cores for the products. */
+
+/* fp16 or bf16 matrices (type PHX_F16 or PHX_BF16) to the device, laid out once for phx_matmul_grouped and
+ * phx_experts_half: n_mat matrices (<= PHX_MAX_EXPERTS) of `rows` rows of `cols`, w [n_mat][rows][cols] (host or device
+ * memory, 2-byte aligned, read before the call returns).  cols a multiple of 8, at most PHX_MAX_COLS_I8; rows at most
+ * PHX_MAX_ROWS_I8; rows * cols <= PHX_MAX_MATRIX_I8 / 2.  paired: the rows are gate (first half) and up of a gated
+ * FFN (rows even).  phx_weight_free releases the handle, phx_weight_shape says its sizes. */
+int phx_weight_upload_half(phx_moe_ctx* ctx, int type, int n_mat, int rows, int cols, int paired, const void* w,
+                           phx_weight** out);
+
+/* Products in runs of ragged length, one matrix a run: for the places i of group e, offsets[e] <= i < offsets[e + 1],
+ *   y[i] = W[e] x[src[i]]                                     (act PHX_QUANT_PLAIN, a plain handle: y [n][rows])
+ *   y[i] = act(Wgate[e] x[src[i]]) * (Wup[e] x[src[i]])       (PHX_QUANT_SILU_MUL, PHX_QUANT_GELU_MUL, a paired handle:
+ *                                                              y [n][rows / 2])
+ * with src[i] = i where src is NULL.  silu(g) = g / (1 + exp(-g)); gelu(g) = g / (1 + exp(-2 z)), z = sqrt(2 / pi) (g +
+ * 0.044715 g^3), the tanh form, in float (phx_quant_i8's gelu goes through fp16, this one does not); both are 0 for
+ * -infinity, and a NaN stays one.  One rounding, to y_type (PHX_F32, PHX_F16, PHX_BF16).  x: n_x rows of cols of the
+ * weights' type.  offsets [n_mat + 1] ascend from any value on, in 0 .. n; a value outside counts as the nearest of
+ * these, and a group that ends where it begins is empty.  Rows of y outside every group, and places whose src is outside
+ * [0, n_x), are left as they were.  (Offsets that do not ascend give some places to two groups: which of the two is
+ * then stored is not defined.)  1 <= n <= PHX_MAX_ROWS_I8, 1 <= n_x <= PHX_MAX_ROWS_I8, n_x >= n without src; with src
+ * x spans less than 2^32 bytes.  x and y 16-byte, offsets and src 4-byte aligned.  n_mat = 1 is a dense product. */
+int phx_matmul_grouped(phx_moe_ctx* ctx, const phx_weight* w, int act, int n, const int32_t* offsets, const void* x, int n_x,
+                       const int32_t* src, int y_type, void* y);
+
+/* The gated FFN of fp16 or bf16 experts for T rows and a routing (phx_route's, or any ids):
+ *   h = act(Wgate[e] x[t]) * (Wup[e] x[t]),  e = ids[t][j], as phx_matmul_grouped forms it, rounded to the weights' type
+ *   out[t] = sum over j, in order, of weights[t][j] * (Wdown[e] h)
+ * the products and the sum in float, rounded to out_type at the end.  A place whose id is outside [0, n_expert) is
+ * skipped; a row without experts is zero.  An id may come more than once in a row.  gate_up: paired, [n_expert][2 nf][d];
+ * down: [n_expert][d][nf], of the same type; x [T][d] of that type, ids and weights [T][k], out [T][d];
+ * 1 <= T <= PHX_MAX_ROWS_I8, 1 <= k <= PHX_MAX_USED; x and out 16-byte aligned. */
+int phx_experts_half(phx_moe_ctx* ctx, const phx_weight* gate_up, const phx_weight* down, int act, int T, int k, const void* x,
+                     const int32_t* ids, const float* weights, int out_type, void* out);
+
+/* Low-rank adapters of one projection (rows x cols): n_slot slots (<= PHX_MAX_ADAPTERS), each empty or an adapter of rank
+ * up to max_rank (<= PHX_MAX_RANK): A [rank][cols], B [rows][rank] of `type` (PHX_F16 or PHX_BF16), and a scale.  cols a
+ * multiple of 8, at most PHX_MAX_COLS_I8; rows at most PHX_MAX_ROWS_I8; all slots are allocated at once, empty.  phx_lora_set
+ * puts an adapter into a slot (a and b host or device memory, 2-byte aligned, read before the call returns; calls enqueued
+ * earlier see the slot as it was); rank 0 empties it (a and b unused).  The scale is finite. */
+#define PHX_MAX_ADAPTERS 256
+#define PHX_MAX_RANK 128
+typedef struct phx_lora phx_lora;
+int phx_lora_create(phx_moe_ctx* ctx, int type, int n_slot, int max_rank, int rows, int cols, phx_lora** out);
+int phx_lora_set(phx_moe_ctx* ctx, phx_lora* lora, int slot, int rank, const void* a, const void* b, float scale);
+void phx_lora_free(phx_moe_ctx* ctx, phx_lora* lora);
+
+/* The adapters of T rows' requests, added to the rows of the projection that they share (phx_matmul_i8's y, say):
+ *   y[t] = y_in[t] + scale * B (A x[t])      with the adapter of slot ids[t]
+ *   y[t] = y_in[t]                           where ids[t] is outside [0, n_slot) or the slot is empty
+ * A x and its scale in float; B's products take that value in two terms of the adapters' type (16 bits of it with
+ * bf16, 22 with fp16), in four where y is float; one rounding, to y_type (PHX_F32, PHX_F16, PHX_BF16).  x [T][cols] of the
+ * adapters' type; y_in and y of y_type, rows ld values apart (ld >= rows: both may be a section of a wider matrix), y may
+ * be y_in.  1 <= T <= PHX_MAX_ROWS_I8, ld <= 2^40; x 16-byte aligned, y_in and y to their values, ids 4-byte. */
+int phx_lora_add(phx_moe_ctx* ctx, const phx_lora* lora, int T, const void* x, const int32_t* ids, int y_type, int64_t ld,
+                 const void* y_in, void* y);
+
+/* The residual's addition and the norm of the sum, in one pass over the rows:
+ *   sum[r] = x[r] + branch[r]                  added in float, rounded to type
+ *   v = CpuRef.RmsNorm(sum[r], w, eps)         as phx_quant_i8 forms it in PHX_QUANT_RMS_NORM, of the rounded sum
+ *   qs[r], d[r]                                v as an int8 row with its scale (phx_quant_i8's, bit for bit)
+ *   out[r] = v                                 rounded to out_type; NULL: not stored
+ * the int8 rows for phx_matmul_i8 and phx_experts_i8, the float rows for a router, phx_lora_add or phx_experts_half.  x and sum
+ * [rows][n] of type (PHX_F32, PHX_F16, PHX_BF16), sum may be x; branch of type, rows ld values apart (ld >= n); w [n] float; out
+ * [rows][n] of out_type; qs [rows][n], d [rows].  A row that holds a NaN or an infinity after the addition has d = NaN and zeros
+ * in qs.  n a multiple of 32, at most PHX_MAX_COLS_I8; ld a multiple of 8, at most 2^40; 1 <= rows <= PHX_MAX_ROWS_I8; x, branch, w,
+ * sum and out 16-byte, qs 8-byte aligned. */
+int phx_add_norm_i8(phx_moe_ctx* ctx, int type, const void* x, const void* branch, const float* w, int rows, int n, int64_t ld,
+                    float eps, void* sum, int out_type, void* out, int8_t* qs, float* d);
 
 #ifdef __cplusplus
 }

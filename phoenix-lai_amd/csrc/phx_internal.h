@@ -333,4 +333,71 @@ void launch_i8_lists(hipStream_t st, int n, int E, int cap, const int* ids, int*
 void launch_i8_combine(hipStream_t st, int T, int d, int k, int E, const float* y, const int* ids, const float* w, int out_type,
                        void* out);
 
+// ---- float experts, adapters, the residual's norm (kernels_half.hip, kernels_lora.hip, kernels_add_norm.hip)
+// fp16 or bf16 matrices on the device, laid out by bytes as I8Mat: groups of 32 stored rows, each [kc][32 rows][16 bytes] with
+// kc = columns / 8, padded to whole steps of 64 columns with zeros; paired, group 2 g holds gate rows 32 g .. + 31 and
+// group 2 g + 1 the up rows of the same channels.
+struct HalfMat {
+    int n_mat = 0, rows = 0, cols = 0, type = 0;
+    bool paired = false;
+    int rg = 0, kc = 0;
+    uint8_t* w = nullptr;
+    __host__ __device__ int64_t mat_bytes() const { return (int64_t)rg * kc * 512; }
+};
+// matrices m0 .. m0 + n_mat - 1 of m from w (device-readable)
+void launch_half_pack(hipStream_t st, const HalfMat& m, int m0, int n_mat, const uint16_t* w);
+
+struct HalfArgs {
+    // set by the caller.  Groups: offsets [n_mat + 1] over n places, or tiles of them (capacity cap), or one place each whose group
+    // is ids[place].  A place's row of x is src[place] / div (none outside n_x rows), without src the place's own number (with ids
+    // over div); its output row is dst[place], without dst its own number.
+    const uint16_t* x = nullptr;
+    const int *src = nullptr, *dst = nullptr, *offsets = nullptr, *ids = nullptr;
+    const Tile* tiles = nullptr;
+    const int* ntiles = nullptr;
+    int n = 0, n_x = 0, div = 1, cap = 0, act = 0, type = 0;  // type: the output's
+    void* out = nullptr;
+    // set by launch_half_product from the matrix
+    const uint8_t* w;
+    int64_t mat_bytes;
+    int kc, cols, out_cols, rgs, n_mat;
+};
+constexpr int kHalfRows = 64;  // the row kernel's most places a tile (16, 32 or 64)
+void launch_half_product(hipStream_t st, const HalfMat& m, HalfArgs g, int max_tiles);
+// the down products of T tokens' k places from h [T k][cols], and their weighted sums as out [T][rows]
+void launch_half_down_few(hipStream_t st, const HalfMat& m, int T, int k, const uint16_t* h, const int* ids, const float* weights,
+                          int out_type, void* out);
+
+// The slots of an adapter handle: A [slot][rt][kc][16 ranks][16 bytes] (kc = columns / 8, padded to steps of 32 columns), B
+// [slot][64 rows' group][rt][4 tiles of 16 rows][2][16 rows][16 bytes]: ranks in rt tiles of 16, zeros past a slot's own rank; B's tile m
+// holds row 16 (i / 4) + 4 m + i % 4 of its group at i, so that a lane's sums are 16 consecutive outputs.
+struct LoraSlots {
+    int type = 0, n_slot = 0, rows = 0, cols = 0, rt = 0, kc = 0, groups = 0;
+    uint8_t *a = nullptr, *b = nullptr;
+    int* rank = nullptr;
+    float* scale = nullptr;
+    __host__ __device__ int64_t a_bytes() const { return (int64_t)rt * kc * 256; }
+    __host__ __device__ int64_t b_bytes() const { return (int64_t)groups * rt * 2048; }
+};
+void launch_lora_set(hipStream_t st, const LoraSlots& L, int slot, int rank, const uint16_t* a, const uint16_t* b, float scale);
+// the parts that A's reduction is split in for T rows; part [parts][T][16 rt] floats
+int lora_parts(const LoraSlots& L, int T, int ncu);
+void launch_lora_down(hipStream_t st, const LoraSlots& L, int T, const uint16_t* x, const int* ids, int parts, float* part);
+void launch_lora_up(hipStream_t st, const LoraSlots& L, int T, const int* ids, int parts, const float* part, int y_type, int64_t ld,
+                    const void* y_in, void* y);
+
+struct AddNormArgs {
+    const void *x, *branch;
+    const float* w;
+    int rows, n;
+    int64_t ld;
+    float eps;
+    void* sum;
+    int out_type;
+    void* out;
+    int8_t* qs;
+    float* d;
+};
+void launch_add_norm_i8(hipStream_t st, int type, const AddNormArgs& a);
+
 }  // namespace phx

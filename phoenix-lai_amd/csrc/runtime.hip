@@ -374,7 +374,7 @@ struct Buf {
     size_t bytes = 0;
 };
 
-enum I8Ws { I8_PERM, I8_TILES, I8_NTILES, I8_H, I8_HQ, I8_HD, I8_Y, I8_WS_COUNT };
+enum I8Ws { I8_PERM, I8_TILES, I8_NTILES, I8_H, I8_HQ, I8_HD, I8_Y, LORA_PART, I8_WS_COUNT };
 
 }  // namespace
 
@@ -435,7 +435,7 @@ struct phx_moe_ctx {
     };
     std::vector<FfnGraph> ffn_graphs;
     uint64_t upload_gen = 0;
-    // workspace of the int8 experts (I8Ws): a table of its own, which no captured graph names; an array, as the C entry points
+    // workspace of the int8 and float experts and of the adapters (I8Ws): a table of its own, which no captured graph names; an array, as the C entry points
     // that fill it have nothing to catch a container's exception
     Buf ws_i8[I8_WS_COUNT];
 };
@@ -1248,12 +1248,18 @@ int drain_profile(phx_moe_ctx* c)
 
 // One dense quantized matrix on the device (GemmaGpu's GW, src/GemmaGpu.cs:344-352), repacked into row
 // groups like the experts, for phx_matmul; or the int8 matrices of phx_weight_upload_i8 (type PHX_I8_WEIGHT, the
-// other fields in i8).
+// other fields in i8), or the float ones of phx_weight_upload_half (type PHX_F16 or PHX_BF16, in half).
 struct phx_weight {
     QMat q;
     I8Mat i8;
+    HalfMat half;
     int type = 0, rows = 0, cols = 0;
-    int device = 0;  // of the int8 matrices
+    int device = 0;  // of the int8 and float matrices
+};
+
+struct phx_lora {
+    LoraSlots s;
+    int max_rank = 0, device = 0;
 };
 
 // Workspace of phx_moe_ffn_noalloc: one array per device, which each GPU the library runs on holds
@@ -2085,13 +2091,14 @@ void phx_weight_free(phx_moe_ctx* c, phx_weight* w)
     free_qmat(w->q);
     if (w->i8.w) (void)hipFree(w->i8.w);
     if (w->i8.scale) (void)hipFree(w->i8.scale);
+    if (w->half.w) (void)hipFree(w->half.w);
     delete w;
 }
 
 int phx_weight_shape(const phx_weight* w, int* n_mat, int* rows, int* cols)
 {
     if (!w) return PHX_ERR_ARG;
-    if (n_mat) *n_mat = w->i8.n_mat ? w->i8.n_mat : 1;
+    if (n_mat) *n_mat = w->i8.n_mat ? w->i8.n_mat : w->half.n_mat ? w->half.n_mat : 1;
     if (rows) *rows = w->rows;
     if (cols) *cols = w->cols;
     return PHX_OK;
@@ -2547,6 +2554,354 @@ int phx_experts_i8(phx_moe_ctx* c, const phx_weight* gu, const phx_weight* dn, i
         launch_i8_product(st, dn->i8, g, tile, max_tiles, c->ncu, PHX_F32);
         launch_i8_combine(st, n, d, k, E, y, id, weights + (int64_t)t0 * k, out_type, (char*)out + (int64_t)t0 * d * eb);
     }
+    HIPCHK(c, launch_status(c));
+    return PHX_OK;
+}
+
+// ---------------------------------------------------------------------------- float experts, adapters, the residual's norm
+
+namespace {
+// A host buffer on its way to the device.
+struct Staging {
+    void* p = nullptr;
+    ~Staging()
+    {
+        if (p) (void)hipFree(p);
+    }
+};
+
+// Whether p is device-accessible, refusing memory of another GPU.
+int where_is(phx_moe_ctx* c, const char* call, const char* what, const void* p, bool* on_device)
+{
+    hipPointerAttribute_t at{};
+    *on_device = device_accessible(p, &at);
+    if (*on_device && at.type == hipMemoryTypeDevice && foreign(c, at.device)) return refuse_foreign(c, call, what, at.device);
+    return PHX_OK;
+}
+
+int upload_half(phx_moe_ctx* c, HalfMat& m, const uint16_t* w)
+{
+    const int64_t src = (int64_t)m.rows * m.cols;
+    bool on_device;
+    if (const int rc = where_is(c, "weight upload", "w", w, &on_device)) return rc;
+    HIPCHK(c, dev_malloc(c, (void**)&m.w, (size_t)(m.n_mat * m.mat_bytes())));
+    Staging sw;  // host matrices go through a buffer of one of them
+    if (!on_device) HIPCHK(c, dev_malloc(c, &sw.p, (size_t)src * 2));
+    for (int i = 0; i < m.n_mat; i++) {
+        const uint16_t* wi = w + i * src;
+        if (!on_device) {
+            HIPCHK(c, hipMemcpyAsync(sw.p, wi, (size_t)src * 2, hipMemcpyHostToDevice, c->stream));
+            wi = (const uint16_t*)sw.p;
+        }
+        launch_half_pack(c->stream, m, i, 1, wi);
+    }
+    HIPCHK(c, launch_status(c));
+    HIPCHK(c, hipStreamSynchronize(c->stream));
+    return PHX_OK;
+}
+
+bool half_type(int type) { return type == PHX_F16 || type == PHX_BF16; }
+
+// The workgroups' tiles of n places in n_mat groups, at most.
+int most_tiles(int n, int n_mat, int cap) { return n / cap + std::min(n, n_mat); }
+int rows_cap(int n, int n_mat) { return n <= 2 * n_mat ? 16 : n <= 8 * n_mat ? 32 : kHalfRows; }
+}  // namespace
+
+int phx_weight_upload_half(phx_moe_ctx* c, int type, int n_mat, int rows, int cols, int paired, const void* w, phx_weight** out)
+{
+    if (!c || !out) return PHX_ERR_ARG;
+    *out = nullptr;
+    if (!half_type(type)) return set_err(c, PHX_ERR_UNSUPPORTED, "weight upload: type %d (PHX_F16 and PHX_BF16 only)", type);
+    if (n_mat <= 0 || n_mat > PHX_MAX_EXPERTS || rows <= 0 || rows > PHX_MAX_ROWS_I8 || cols <= 0 || cols % 8 ||
+        cols > PHX_MAX_COLS_I8 || (paired && rows % 2))
+        return set_err(c, PHX_ERR_ARG, "weight upload: %d fp16 or bf16 matrices of %d x %d (at most %d; rows <= %d, even where paired; "
+                       "cols a multiple of 8, <= %d)", n_mat, rows, cols, PHX_MAX_EXPERTS, PHX_MAX_ROWS_I8, PHX_MAX_COLS_I8);
+    if ((int64_t)rows * cols > PHX_MAX_MATRIX_I8 / 2)
+        return set_err(c, PHX_ERR_ARG, "weight upload: an fp16 or bf16 matrix of %d x %d (rows * cols <= %lld)", rows, cols,
+                       (long long)PHX_MAX_MATRIX_I8 / 2);
+    if (!w || (uintptr_t)w % 2) return set_err(c, PHX_ERR_ARG, "weight upload: null w, or w off 2 bytes");
+    ENTER(c);
+    phx_weight* h = new (std::nothrow) phx_weight();
+    if (!h) return set_err(c, PHX_ERR_OOM, "weight upload: host memory");
+    h->type = type;
+    h->rows = rows;
+    h->cols = cols;
+    h->device = c->device;
+    HalfMat& m = h->half;
+    m.n_mat = n_mat;
+    m.rows = rows;
+    m.cols = cols;
+    m.type = type;
+    m.paired = paired != 0;
+    m.rg = paired ? (rows / 2 + 31) / 32 * 2 : (rows + 31) / 32;
+    m.kc = (cols + 63) / 64 * 8;
+    const int rc = upload_half(c, m, (const uint16_t*)w);
+    if (rc) {
+        phx_weight_free(c, h);
+        return rc;
+    }
+    *out = h;
+    return PHX_OK;
+}
+
+int phx_matmul_grouped(phx_moe_ctx* c, const phx_weight* w, int act, int n, const int32_t* offsets, const void* x, int n_x,
+                       const int32_t* src, int y_type, void* y)
+{
+    if (!c) return PHX_ERR_ARG;
+    if (!w) return set_err(c, PHX_ERR_ARG, "matmul_grouped: null weight");
+    if (!half_type(w->type))
+        return set_err(c, PHX_ERR_UNSUPPORTED, "matmul_grouped: the weight is not fp16 or bf16 (phx_weight_upload_half)");
+    const HalfMat& m = w->half;
+    if (act != PHX_QUANT_PLAIN && act != PHX_QUANT_SILU_MUL && act != PHX_QUANT_GELU_MUL)
+        return set_err(c, PHX_ERR_ARG, "matmul_grouped: act %d", act);
+    if (m.paired != (act != PHX_QUANT_PLAIN))
+        return set_err(c, PHX_ERR_UNSUPPORTED, "matmul_grouped: an activation takes a paired weight, PHX_QUANT_PLAIN one that is not");
+    const int eb = elem_bytes(y_type), out = m.paired ? m.rows / 2 : m.rows;
+    if (!eb) return set_err(c, PHX_ERR_UNSUPPORTED, "matmul_grouped: type %d (PHX_F32, PHX_F16 and PHX_BF16 only)", y_type);
+    if (n <= 0 || n > PHX_MAX_ROWS_I8 || n_x <= 0 || n_x > PHX_MAX_ROWS_I8 || (!src && n_x < n))
+        return set_err(c, PHX_ERR_ARG, "matmul_grouped: %d places of %d rows (at most %d; without src a row each)", n, n_x, PHX_MAX_ROWS_I8);
+    const int64_t xb = (int64_t)n_x * m.cols * 2;
+    if (src && xb >= 1ll << 32) return set_err(c, PHX_ERR_ARG, "matmul_grouped: with src x spans %lld bytes (under 2^32)", (long long)xb);
+    ENTER(c);
+    if (foreign(c, w->device)) return refuse_foreign(c, "matmul_grouped", "the weight", w->device);
+    const CallBuf bo{"offsets", offsets, (m.n_mat + 1) * 4ll, 4, false}, bx{"x", x, xb, 16, false},
+        by{"y", y, (int64_t)n * out * eb, 16, true};
+    const int rc = src ? check_bufs(c, "matmul_grouped", {bo, bx, by, {"src", src, n * 4ll, 4, false}})
+                       : check_bufs(c, "matmul_grouped", {bo, bx, by});
+    if (rc) return rc;
+    HalfArgs g{};
+    g.x = (const uint16_t*)x;
+    g.src = src;
+    g.offsets = offsets;
+    g.n = n;
+    g.n_x = n_x;
+    g.act = act;
+    g.type = y_type;
+    g.out = y;
+    g.cap = rows_cap(n, m.n_mat);
+    launch_half_product(c->stream, m, g, most_tiles(n, m.n_mat, g.cap));
+    HIPCHK(c, launch_status(c));
+    return PHX_OK;
+}
+
+int phx_experts_half(phx_moe_ctx* c, const phx_weight* gu, const phx_weight* dn, int act, int T, int k, const void* x,
+                     const int32_t* ids, const float* weights, int out_type, void* out)
+{
+    if (!c) return PHX_ERR_ARG;
+    if (!gu || !dn) return set_err(c, PHX_ERR_ARG, "experts_half: null weight");
+    if (!half_type(gu->type) || dn->type != gu->type || !gu->half.paired || dn->half.paired)
+        return set_err(c, PHX_ERR_UNSUPPORTED, "experts_half: takes a paired gate_up and a plain down, both fp16 or both bf16");
+    const int E = gu->half.n_mat, d = gu->cols, nf = gu->rows / 2;
+    if (dn->half.n_mat != E || dn->rows != d || dn->cols != nf)
+        return set_err(c, PHX_ERR_ARG, "experts_half: gate_up [%d][%d][%d] and down [%d][%d][%d] do not fit", E, gu->rows, d,
+                       dn->half.n_mat, dn->rows, dn->cols);
+    const int eb = elem_bytes(out_type);
+    if (!eb) return set_err(c, PHX_ERR_UNSUPPORTED, "experts_half: type %d (PHX_F32, PHX_F16 and PHX_BF16 only)", out_type);
+    if (act != PHX_QUANT_SILU_MUL && act != PHX_QUANT_GELU_MUL) return set_err(c, PHX_ERR_ARG, "experts_half: act %d", act);
+    if (T <= 0 || T > PHX_MAX_ROWS_I8 || k <= 0 || k > PHX_MAX_USED)
+        return set_err(c, PHX_ERR_ARG, "experts_half: T=%d, k=%d out of range", T, k);
+    ENTER(c);
+    if (foreign(c, gu->device)) return refuse_foreign(c, "experts_half", "gate_up", gu->device);
+    if (foreign(c, dn->device)) return refuse_foreign(c, "experts_half", "down", dn->device);
+    if (const int rc = check_bufs(c, "experts_half", {{"x", x, (int64_t)T * d * 2, 16, false},
+                                                      {"ids", ids, (int64_t)T * k * 4, 4, false},
+                                                      {"weights", weights, (int64_t)T * k * 4, 4, false},
+                                                      {"out", out, (int64_t)T * d * eb, 16, true}}))
+        return rc;
+    hipStream_t st = c->stream;
+    uint16_t* h;
+    int rc;
+    HalfArgs g{};
+    g.x = (const uint16_t*)x;
+    g.act = act;
+    // few assignments, most of them of an expert of their own: two launches without lists, which read an expert's matrices again
+    // for each of its assignments
+    const double each = 6.0 * nf * d, A0 = (double)T * k, again = A0 - E * (1.0 - pow(1.0 - 1.0 / E, A0));
+    if (A0 <= 1024 && again * each <= (E * each <= 64e6 ? 144e6 : 48e6)) {
+        if ((rc = i8_ensure(c, I8_H, (int64_t)T * k * nf, &h))) return rc;
+        g.ids = ids;
+        g.div = k;
+        g.n_x = T;
+        g.cap = 16;
+        g.type = gu->type;
+        g.out = h;
+        launch_half_product(st, gu->half, g, T * k);
+        launch_half_down_few(st, dn->half, T, k, h, ids, weights, out_type, out);
+        HIPCHK(c, launch_status(c));
+        return PHX_OK;
+    }
+    // long batches go through in chunks, so that the workspace stays bounded and every row of it, and of x, within 2^32 bytes
+    const int chunk = std::min<int64_t>(T, std::min<int64_t>(65535, ((1ll << 32) - 1) / (4ll * std::max(d, nf))) / k), A = chunk * k;
+    const int cap = rows_cap(A, E), max_tiles = most_tiles(A, E, cap);
+    int *perm, *ntiles;
+    Tile* tiles;
+    float* y;
+    if ((rc = i8_ensure(c, I8_PERM, A, &perm)) || (rc = i8_ensure(c, I8_TILES, max_tiles, &tiles)) ||
+        (rc = i8_ensure(c, I8_NTILES, 1, &ntiles)) || (rc = i8_ensure(c, I8_H, (int64_t)A * nf, &h)) ||
+        (rc = i8_ensure(c, I8_Y, (int64_t)A * d, &y)))
+        return rc;
+    g.tiles = tiles;
+    g.ntiles = ntiles;
+    g.cap = cap;
+    for (int t0 = 0; t0 < T; t0 += chunk) {
+        const int n = std::min(chunk, T - t0);
+        const int32_t* id = ids + (int64_t)t0 * k;
+        launch_i8_lists(st, n * k, E, cap, id, perm, tiles, ntiles);
+        // gate and up in the lists' order, down back to the assignments' own
+        g.x = (const uint16_t*)x + (int64_t)t0 * d;
+        g.n_x = n;
+        g.src = perm;
+        g.div = k;
+        g.dst = nullptr;
+        g.type = gu->type;
+        g.out = h;
+        launch_half_product(st, gu->half, g, max_tiles);
+        g.x = h;
+        g.src = nullptr;
+        g.div = 1;
+        g.dst = perm;
+        g.type = PHX_F32;
+        g.out = y;
+        launch_half_product(st, dn->half, g, max_tiles);
+        launch_i8_combine(st, n, d, k, E, y, id, weights + (int64_t)t0 * k, out_type, (char*)out + (int64_t)t0 * d * eb);
+    }
+    HIPCHK(c, launch_status(c));
+    return PHX_OK;
+}
+
+int phx_lora_create(phx_moe_ctx* c, int type, int n_slot, int max_rank, int rows, int cols, phx_lora** out)
+{
+    if (!c || !out) return PHX_ERR_ARG;
+    *out = nullptr;
+    if (!half_type(type)) return set_err(c, PHX_ERR_UNSUPPORTED, "lora: type %d (PHX_F16 and PHX_BF16 only)", type);
+    if (n_slot <= 0 || n_slot > PHX_MAX_ADAPTERS || max_rank <= 0 || max_rank > PHX_MAX_RANK || rows <= 0 || rows > PHX_MAX_ROWS_I8 ||
+        cols <= 0 || cols % 8 || cols > PHX_MAX_COLS_I8)
+        return set_err(c, PHX_ERR_ARG, "lora: %d slots of rank %d for %d x %d (slots <= %d, rank <= %d; rows <= %d; cols a multiple of 8, <= %d)",
+                       n_slot, max_rank, rows, cols, PHX_MAX_ADAPTERS, PHX_MAX_RANK, PHX_MAX_ROWS_I8, PHX_MAX_COLS_I8);
+    ENTER(c);
+    phx_lora* h = new (std::nothrow) phx_lora();
+    if (!h) return set_err(c, PHX_ERR_OOM, "lora: host memory");
+    h->max_rank = max_rank;
+    h->device = c->device;
+    LoraSlots& L = h->s;
+    L.type = type;
+    L.n_slot = n_slot;
+    L.rows = rows;
+    L.cols = cols;
+    L.rt = (max_rank + 15) / 16;
+    L.kc = (cols + 31) / 32 * 4;
+    L.groups = (rows + 63) / 64;
+    const int rc = [&] {
+        HIPCHK(c, dev_malloc(c, (void**)&L.a, (size_t)(n_slot * L.a_bytes())));
+        HIPCHK(c, dev_malloc(c, (void**)&L.b, (size_t)(n_slot * L.b_bytes())));
+        HIPCHK(c, dev_malloc(c, (void**)&L.rank, n_slot * 4));
+        HIPCHK(c, dev_malloc(c, (void**)&L.scale, n_slot * 4));
+        HIPCHK(c, hipMemsetAsync(L.rank, 0, n_slot * 4, c->stream));  // an empty slot's matrices are not read
+        HIPCHK(c, hipStreamSynchronize(c->stream));
+        return PHX_OK;
+    }();
+    if (rc) {
+        phx_lora_free(c, h);
+        return rc;
+    }
+    *out = h;
+    return PHX_OK;
+}
+
+int phx_lora_set(phx_moe_ctx* c, phx_lora* l, int slot, int rank, const void* a, const void* b, float scale)
+{
+    if (!c) return PHX_ERR_ARG;
+    if (!l) return set_err(c, PHX_ERR_ARG, "lora_set: null handle");
+    const LoraSlots& L = l->s;
+    if (slot < 0 || slot >= L.n_slot || rank < 0 || rank > l->max_rank || !std::isfinite(scale))
+        return set_err(c, PHX_ERR_ARG, "lora_set: slot %d of %d, rank %d (at most %d), scale %g", slot, L.n_slot, rank, l->max_rank, scale);
+    if (rank && (!a || !b || (uintptr_t)a % 2 || (uintptr_t)b % 2)) return set_err(c, PHX_ERR_ARG, "lora_set: null a or b, or off 2 bytes");
+    ENTER(c);
+    if (foreign(c, l->device)) return refuse_foreign(c, "lora_set", "the adapters", l->device);
+    Staging sa, sb;
+    if (rank) {
+        bool on_a, on_b;
+        int rc;
+        if ((rc = where_is(c, "lora_set", "a", a, &on_a)) || (rc = where_is(c, "lora_set", "b", b, &on_b))) return rc;
+        const size_t na = (size_t)rank * L.cols * 2, nb = (size_t)rank * L.rows * 2;
+        if (!on_a) {
+            HIPCHK(c, dev_malloc(c, &sa.p, na));
+            HIPCHK(c, hipMemcpyAsync(sa.p, a, na, hipMemcpyHostToDevice, c->stream));
+            a = sa.p;
+        }
+        if (!on_b) {
+            HIPCHK(c, dev_malloc(c, &sb.p, nb));
+            HIPCHK(c, hipMemcpyAsync(sb.p, b, nb, hipMemcpyHostToDevice, c->stream));
+            b = sb.p;
+        }
+    }
+    launch_lora_set(c->stream, L, slot, rank, (const uint16_t*)a, (const uint16_t*)b, scale);
+    HIPCHK(c, launch_status(c));
+    HIPCHK(c, hipStreamSynchronize(c->stream));
+    return PHX_OK;
+}
+
+void phx_lora_free(phx_moe_ctx* c, phx_lora* l)
+{
+    if (!l) return;
+    if (c) {
+        (void)hipSetDevice(c->device);
+        (void)hipStreamSynchronize(c->stream);
+    }
+    for (void* p : {(void*)l->s.a, (void*)l->s.b, (void*)l->s.rank, (void*)l->s.scale})
+        if (p) (void)hipFree(p);
+    delete l;
+}
+
+int phx_lora_add(phx_moe_ctx* c, const phx_lora* l, int T, const void* x, const int32_t* ids, int y_type, int64_t ld, const void* y_in,
+                 void* y)
+{
+    if (!c) return PHX_ERR_ARG;
+    if (!l) return set_err(c, PHX_ERR_ARG, "lora_add: null handle");
+    const LoraSlots& L = l->s;
+    const int eb = elem_bytes(y_type);
+    if (!eb) return set_err(c, PHX_ERR_UNSUPPORTED, "lora_add: type %d (PHX_F32, PHX_F16 and PHX_BF16 only)", y_type);
+    if (T <= 0 || T > PHX_MAX_ROWS_I8 || ld < L.rows || ld > (int64_t)1 << 40)
+        return set_err(c, PHX_ERR_ARG, "lora_add: %d rows of %d, %lld apart (rows <= %d)", T, L.rows, (long long)ld, PHX_MAX_ROWS_I8);
+    ENTER(c);
+    if (foreign(c, l->device)) return refuse_foreign(c, "lora_add", "the adapters", l->device);
+    const int64_t span = ((T - 1) * ld + L.rows) * eb;
+    const CallBuf bx{"x", x, (int64_t)T * L.cols * 2, 16, false}, bi{"ids", ids, T * 4ll, 4, false}, by{"y", y, span, eb, true};
+    int rc = y_in == y ? check_bufs(c, "lora_add", {bx, bi, by}) : check_bufs(c, "lora_add", {bx, bi, by, {"y_in", y_in, span, eb, false}});
+    if (rc) return rc;
+    const int chunk = std::min(T, 65536), parts = lora_parts(L, chunk, c->ncu);
+    float* part;
+    if ((rc = i8_ensure(c, LORA_PART, (int64_t)parts * chunk * 16 * L.rt, &part))) return rc;
+    for (int t0 = 0; t0 < T; t0 += chunk) {
+        const int n = std::min(chunk, T - t0);
+        launch_lora_down(c->stream, L, n, (const uint16_t*)x + (int64_t)t0 * L.cols, ids + t0, parts, part);
+        launch_lora_up(c->stream, L, n, ids + t0, parts, part, y_type, ld, (const char*)y_in + t0 * ld * eb, (char*)y + t0 * ld * eb);
+    }
+    HIPCHK(c, launch_status(c));
+    return PHX_OK;
+}
+
+int phx_add_norm_i8(phx_moe_ctx* c, int type, const void* x, const void* branch, const float* w, int rows, int n, int64_t ld, float eps,
+                    void* sum, int out_type, void* out, int8_t* qs, float* d)
+{
+    if (!c) return PHX_ERR_ARG;
+    const int eb = elem_bytes(type), ob = elem_bytes(out_type);
+    if (!eb || !ob)
+        return set_err(c, PHX_ERR_UNSUPPORTED, "add_norm_i8: type %d, out_type %d (PHX_F32, PHX_F16 and PHX_BF16 only)", type, out_type);
+    if (rows <= 0 || rows > PHX_MAX_ROWS_I8 || n <= 0 || n % 32 || n > PHX_MAX_COLS_I8 || ld < n || ld % 8 || ld > (int64_t)1 << 40)
+        return set_err(c, PHX_ERR_ARG, "add_norm_i8: %d rows of %d, %lld apart (rows <= %d; n a multiple of 32, <= %d; ld of 8, >= n)",
+                       rows, n, (long long)ld, PHX_MAX_ROWS_I8, PHX_MAX_COLS_I8);
+    if (!(eps >= 0.0f)) return set_err(c, PHX_ERR_ARG, "add_norm_i8: eps");
+    ENTER(c);
+    const int64_t all = (int64_t)rows * n;
+    const CallBuf bs{"sum", sum, all * eb, 16, true}, bb{"branch", branch, ((rows - 1) * ld + n) * eb, 16, false},
+        bw{"w", w, n * 4ll, 16, false}, bq{"qs", qs, all, 8, true}, bd{"d", d, rows * 4ll, 4, true},
+        bx{"x", x, all * eb, 16, false}, bo{"out", out, all * ob, 16, true};
+    int rc;
+    if (x == sum) rc = out ? check_bufs(c, "add_norm_i8", {bs, bb, bw, bq, bd, bo}) : check_bufs(c, "add_norm_i8", {bs, bb, bw, bq, bd});
+    else rc = out ? check_bufs(c, "add_norm_i8", {bx, bs, bb, bw, bq, bd, bo}) : check_bufs(c, "add_norm_i8", {bx, bs, bb, bw, bq, bd});
+    if (rc) return rc;
+    launch_add_norm_i8(c->stream, type, {x, branch, w, rows, n, ld, eps, sum, out_type, out, qs, d});
     HIPCHK(c, launch_status(c));
     return PHX_OK;
 }

@@ -29,6 +29,7 @@ class PHX:
     SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
     GROUP_MAX, GROUP_TOP2, MAX_GROUPS = 0, 1, 64
     MAX_ROWS_I8, MAX_COLS_I8, MAX_MATRIX_I8 = 1 << 20, 1 << 16, 1 << 34
+    MAX_ADAPTERS, MAX_RANK = 256, 128
 
 
 class MoeError(RuntimeError):
@@ -180,6 +181,14 @@ def load_lib():
         "phx_weight_upload_i8": (i32, [vp, i32, i32, i32, i32, vp, vp, C.POINTER(vp)]),
         "phx_matmul_i8": (i32, [vp, vp, i32, vp, vp, i32, vp]),
         "phx_experts_i8": (i32, [vp, vp, vp, i32, i32, i32, vp, vp, vp, vp, i32, vp]),
+        "phx_weight_upload_half": (i32, [vp, i32, i32, i32, i32, i32, vp, C.POINTER(vp)]),
+        "phx_matmul_grouped": (i32, [vp, vp, i32, i32, vp, vp, i32, vp, i32, vp]),
+        "phx_experts_half": (i32, [vp, vp, vp, i32, i32, i32, vp, vp, vp, i32, vp]),
+        "phx_lora_create": (i32, [vp, i32, i32, i32, i32, i32, C.POINTER(vp)]),
+        "phx_lora_set": (i32, [vp, vp, i32, i32, vp, vp, C.c_float]),
+        "phx_lora_free": (None, [vp, vp]),
+        "phx_lora_add": (i32, [vp, vp, i32, vp, vp, i32, C.c_int64, vp, vp]),
+        "phx_add_norm_i8": (i32, [vp, i32, vp, vp, vp, i32, i32, C.c_int64, C.c_float, vp, i32, vp, vp, vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
@@ -672,6 +681,110 @@ class MoeContext:
         return self._on_device([xq, xd, ids, weights], [(xq.shape, np.float32)],
                                lambda *p: self.experts_i8_device(gate_up, down, act, xq.shape[0], ids.shape[1], *p[:4], PHX.F32,
                                                                  p[4]))[0]
+
+    # ------------------------------------------------------------------ float experts, adapters, the residual's norm
+    def weight_upload_half(self, type_: int, n_mat: int, rows: int, cols: int, w, paired: bool = False) -> int:
+        """phx_weight_upload_half: n_mat fp16 (PHX.F16) or bf16 (PHX.BF16) matrices [rows][cols] laid out on the device once
+        (paired: gate rows, then up rows); w a numpy array (float16, or uint16 holding bf16 bits) or an address (host or
+        device memory).  Returns the handle for matmul_grouped_device / experts_half_device / weight_free."""
+        w = self._halves(type_, w, n_mat * rows * cols)
+        h = C.c_void_p()
+        self._check(self.lib.phx_weight_upload_half(self.h, type_, n_mat, rows, cols, 1 if paired else 0,
+                                                    w.ctypes.data if isinstance(w, np.ndarray) else w, C.byref(h)))
+        return h.value
+
+    @staticmethod
+    def _halves(type_: int, a, n: int):
+        """An array of n 16-bit values of a type (bf16: their bits); an address stays one."""
+        if not isinstance(a, np.ndarray):
+            return a
+        if a.dtype != {PHX.F16: np.float16, PHX.BF16: np.uint16}.get(type_, a.dtype) or a.size != n:
+            raise ArgumentError(PHX.ERR_ARG, f"{a.size} values of {a.dtype} for {n} of type {type_}")
+        return np.ascontiguousarray(a)
+
+    def matmul_grouped_device(self, handle: int, act: int, n: int, offsets_ptr: int, x_ptr: int, n_x: int, src_ptr, y_type: int,
+                              y_ptr: int):
+        """Enqueue phx_matmul_grouped on device buffers (sync() waits)."""
+        self._check(self.lib.phx_matmul_grouped(self.h, handle, act, n, offsets_ptr, x_ptr, n_x, src_ptr, y_type, y_ptr))
+
+    def MatMulGrouped(self, handle: int, act: int, offsets: np.ndarray, x: np.ndarray, src: np.ndarray | None = None) -> np.ndarray:
+        """phx_matmul_grouped on host arrays: y f32 [n][rows, or rows / 2 where the handle is paired] of x [n_x][cols]
+        (float16, or uint16 holding bf16 bits, as the handle's type is); n is src's length, or n_x without it.  Rows
+        outside the groups, and places whose src is outside x, are zero."""
+        n_mat, rows, cols = self.weight_shape(handle)
+        offsets = _ints(offsets, np.int32)
+        src = None if src is None else _ints(src, np.int32)
+        if offsets.shape != (n_mat + 1,) or x.ndim != 2 or x.shape[1] != cols or x.itemsize != 2:
+            raise ArgumentError(PHX.ERR_ARG, f"offsets {offsets.shape} and rows {x.shape} {x.dtype} for {n_mat} matrices of {rows} x {cols}")
+        n = len(x) if src is None else src.size
+        out = rows if act == PHX.QUANT_PLAIN else rows // 2
+        y = np.zeros((n, out), np.float32)
+        bufs = [self.alloc(max(a.nbytes, 16)) for a in (offsets, x, y)] + ([] if src is None else [self.alloc(max(src.nbytes, 16))])
+        try:
+            for b, a in zip(bufs, (offsets, x, y) if src is None else (offsets, x, y, src)):
+                b.upload(a)
+            self.matmul_grouped_device(handle, act, n, bufs[0].ptr, bufs[1].ptr, len(x), None if src is None else bufs[3].ptr,
+                                       PHX.F32, bufs[2].ptr)
+            self.sync()
+            return bufs[2].download((n, out))
+        finally:
+            for b in bufs:
+                b.free()
+
+    def experts_half_device(self, gate_up: int, down: int, act: int, T: int, k: int, x_ptr: int, ids_ptr: int, weights_ptr: int,
+                            out_type: int, out_ptr: int):
+        """Enqueue phx_experts_half on device buffers (sync() waits)."""
+        self._check(self.lib.phx_experts_half(self.h, gate_up, down, act, T, k, x_ptr, ids_ptr, weights_ptr, out_type, out_ptr))
+
+    def ExpertsHalf(self, gate_up: int, down: int, act: int, x: np.ndarray, ids: np.ndarray, weights: np.ndarray) -> np.ndarray:
+        """phx_experts_half on host arrays: out [T][d] f32 from rows x (float16, or uint16 holding bf16 bits) and a routing
+        (as Route returns it)."""
+        ids, weights = _ints(ids, np.int32), _f32(weights)
+        if x.ndim != 2 or x.itemsize != 2 or ids.ndim != 2 or weights.shape != ids.shape or len(ids) != len(x):
+            raise ArgumentError(PHX.ERR_ARG, f"rows {x.shape} {x.dtype}, ids {ids.shape}, weights {weights.shape}")
+        self._fits(gate_up, self.weight_shape(gate_up)[1], x.shape[1])  # down's sizes: phx_experts_half
+        return self._on_device([np.ascontiguousarray(x), ids, weights], [(x.shape, np.float32)],
+                               lambda *p: self.experts_half_device(gate_up, down, act, x.shape[0], ids.shape[1], *p[:3], PHX.F32,
+                                                                   p[3]))[0]
+
+    def lora_create(self, type_: int, n_slot: int, max_rank: int, rows: int, cols: int) -> int:
+        """phx_lora_create: empty slots for adapters of a rows x cols projection; returns the handle for lora_set /
+        lora_add_device / lora_free."""
+        h = C.c_void_p()
+        self._check(self.lib.phx_lora_create(self.h, type_, n_slot, max_rank, rows, cols, C.byref(h)))
+        return h.value
+
+    def lora_set(self, handle: int, slot: int, rank: int, a, b, scale: float = 1.0):
+        """phx_lora_set: A [rank][cols] and B [rows][rank] (numpy arrays of 16-bit values, or addresses of host or device
+        memory) into a slot; rank 0 empties it."""
+        at = [np.ascontiguousarray(m).ctypes.data if isinstance(m, np.ndarray) else m for m in (a, b)]
+        self._check(self.lib.phx_lora_set(self.h, handle, slot, rank, *at, scale))
+
+    def lora_free(self, handle: int):
+        self.lib.phx_lora_free(self.h, handle)
+
+    def lora_add_device(self, handle: int, T: int, x_ptr: int, ids_ptr: int, y_type: int, ld: int, y_in_ptr: int, y_ptr: int):
+        """Enqueue phx_lora_add on device buffers (sync() waits)."""
+        self._check(self.lib.phx_lora_add(self.h, handle, T, x_ptr, ids_ptr, y_type, ld, y_in_ptr, y_ptr))
+
+    def add_norm_i8_device(self, type_: int, x_ptr: int, branch_ptr: int, w_ptr: int, rows: int, n: int, ld: int, eps: float,
+                           sum_ptr: int, out_type: int, out_ptr, qs_ptr: int, d_ptr: int):
+        """Enqueue phx_add_norm_i8 on device buffers (sync() waits)."""
+        self._check(self.lib.phx_add_norm_i8(self.h, type_, x_ptr, branch_ptr, w_ptr, rows, n, ld, eps, sum_ptr, out_type, out_ptr,
+                                             qs_ptr, d_ptr))
+
+    def AddNormI8(self, x: np.ndarray, branch: np.ndarray, w: np.ndarray, eps: float = 1e-6):
+        """phx_add_norm_i8 on host arrays: x and branch [rows][n] float32 or float16, w [n]; returns (sum of x's type, the
+        normed rows f32, qs int8 [rows][n], d f32 [rows])."""
+        x = np.ascontiguousarray(x) if x.dtype == np.float16 else _f32(x)
+        branch, w = np.ascontiguousarray(branch, dtype=x.dtype), _f32(w)
+        if x.ndim != 2 or branch.shape != x.shape or w.shape != x.shape[1:]:
+            raise ArgumentError(PHX.ERR_ARG, f"rows {x.shape}, branch {branch.shape}, weight {w.shape}")
+        rows, n = x.shape
+        return self._on_device(
+            [x, branch, w], [((rows, n), x.dtype), ((rows, n), np.float32), ((rows, n), np.int8), ((rows,), np.float32)],
+            lambda px, pb, pw, ps, po, pq, pd: self.add_norm_i8_device(PHX.F32 if x.dtype == np.float32 else PHX.F16, px, pb, pw,
+                                                                       rows, n, n, eps, ps, PHX.F32, po, pq, pd))
 
     def stack_run_device(self, x_ptr: int, T: int):
         """Replay the captured stack on a device-resident x (async; sync() waits)."""
