@@ -823,7 +823,7 @@ void launch_i8_down_few(hipStream_t st, const I8Mat& m, int T, int k, const floa
 // 2048 assignments, 8.8 for 16384, whose 16 loads a thread go out in one trip (waited for one by one: 14 us).
 template <int IPT>
 __global__ __launch_bounds__(1024) void k_i8_lists(int n, int E, int cap, const int* __restrict__ ids, int* __restrict__ perm,
-                                                   Tile* __restrict__ tiles, int* __restrict__ ntiles)
+                                                   Tile* __restrict__ tiles, int* __restrict__ ntiles, int* __restrict__ offsets)
 {
     __shared__ int count[PHX_MAX_EXPERTS_DEV], start[PHX_MAX_EXPERTS_DEV], first[PHX_MAX_EXPERTS_DEV], total;
     __shared__ uint16_t list[1024 * IPT];
@@ -852,7 +852,7 @@ __global__ __launch_bounds__(1024) void k_i8_lists(int n, int E, int cap, const 
         }
         int pc = wave_incl_scan_i(sc) - sc, pt = wave_incl_scan_i(stl) - stl;
         if (tid == 63) {
-            *ntiles = pt + stl;
+            if (ntiles) *ntiles = pt + stl;
             total = pc + sc;
         }
 #pragma unroll
@@ -864,7 +864,8 @@ __global__ __launch_bounds__(1024) void k_i8_lists(int n, int E, int cap, const 
         }
     }
     __syncthreads();
-    if (tid < E) {
+    if (offsets && tid <= E) offsets[tid] = tid < E ? start[tid] : total;
+    if (tiles && tid < E) {
         int at = start[tid], left = count[tid];
         for (int i = first[tid]; left > 0; i++, at += cap, left -= cap) tiles[i] = {tid, at, min(cap, left)};
     }
@@ -875,12 +876,12 @@ __global__ __launch_bounds__(1024) void k_i8_lists(int n, int E, int cap, const 
     for (int p = tid; p < total; p += 1024) perm[p] = list[p];
 }
 
-void launch_i8_lists(hipStream_t st, int n, int E, int cap, const int* ids, int* perm, Tile* tiles, int* ntiles)
+void launch_i8_lists(hipStream_t st, int n, int E, int cap, const int* ids, int* perm, Tile* tiles, int* ntiles, int* offsets)
 {
     const dim3 one(1), blk(1024);
-    if (n <= 2048) launch(k_i8_lists<2>, one, blk, 0, st, n, E, cap, ids, perm, tiles, ntiles);
-    else if (n <= 16384) launch(k_i8_lists<16>, one, blk, 0, st, n, E, cap, ids, perm, tiles, ntiles);
-    else launch(k_i8_lists<64>, one, blk, 0, st, n, E, cap, ids, perm, tiles, ntiles);
+    if (n <= 2048) launch(k_i8_lists<2>, one, blk, 0, st, n, E, cap, ids, perm, tiles, ntiles, offsets);
+    else if (n <= 16384) launch(k_i8_lists<16>, one, blk, 0, st, n, E, cap, ids, perm, tiles, ntiles, offsets);
+    else launch(k_i8_lists<64>, one, blk, 0, st, n, E, cap, ids, perm, tiles, ntiles, offsets);
 }
 
 // out[t] = sum over the places j, in order, of w[t][j] * y[t k + j]; places without an expert are skipped.  Bound by y's bytes:

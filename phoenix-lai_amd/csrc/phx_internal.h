@@ -329,14 +329,16 @@ void launch_i8_product(hipStream_t st, const I8Mat& m, I8Args g, bool tile, int 
 bool i8_down_few_fits(const I8Mat& m);
 void launch_i8_down_few(hipStream_t st, const I8Mat& m, int T, int k, const float* h, const int* ids, const float* weights,
                         int out_type, void* out);
-void launch_i8_lists(hipStream_t st, int n, int E, int cap, const int* ids, int* perm, Tile* tiles, int* ntiles);
+// offsets [E + 1], where given, gets each expert's bounds in perm
+void launch_i8_lists(hipStream_t st, int n, int E, int cap, const int* ids, int* perm, Tile* tiles, int* ntiles, int* offsets = nullptr);
 void launch_i8_combine(hipStream_t st, int T, int d, int k, int E, const float* y, const int* ids, const float* w, int out_type,
                        void* out);
 
 // ---- float experts, adapters, the residual's norm (kernels_half.hip, kernels_lora.hip, kernels_add_norm.hip)
 // fp16 or bf16 matrices on the device, laid out by bytes as I8Mat: groups of 32 stored rows, each [kc][32 rows][16 bytes] with
 // kc = columns / 8, padded to whole steps of 64 columns with zeros; paired, group 2 g holds gate rows 32 g .. + 31 and
-// group 2 g + 1 the up rows of the same channels.
+// group 2 g + 1 the up rows of the same channels.  Within a group the rows are in the order of the matrix product's results
+// (slot_row in kernels_half.hip).
 struct HalfMat {
     int n_mat = 0, rows = 0, cols = 0, type = 0;
     bool paired = false;
@@ -348,13 +350,11 @@ struct HalfMat {
 void launch_half_pack(hipStream_t st, const HalfMat& m, int m0, int n_mat, const uint16_t* w);
 
 struct HalfArgs {
-    // set by the caller.  Groups: offsets [n_mat + 1] over n places, or tiles of them (capacity cap), or one place each whose group
-    // is ids[place].  A place's row of x is src[place] / div (none outside n_x rows), without src the place's own number (with ids
+    // set by the caller.  Groups: offsets [n_mat + 1] over n places, taken in tiles of cap, or one place each whose group is
+    // ids[place].  A place's row of x is src[place] / div (none outside n_x rows), without src the place's own number (with ids
     // over div); its output row is dst[place], without dst its own number.
     const uint16_t* x = nullptr;
     const int *src = nullptr, *dst = nullptr, *offsets = nullptr, *ids = nullptr;
-    const Tile* tiles = nullptr;
-    const int* ntiles = nullptr;
     int n = 0, n_x = 0, div = 1, cap = 0, act = 0, type = 0;  // type: the output's
     void* out = nullptr;
     // set by launch_half_product from the matrix
@@ -362,7 +362,7 @@ struct HalfArgs {
     int64_t mat_bytes;
     int kc, cols, out_cols, rgs, n_mat;
 };
-constexpr int kHalfRows = 64;  // the row kernel's most places a tile (16, 32 or 64)
+constexpr int kHalfRows = 64, kHalfTile = 256;  // places a tile: the row kernel's most (16, 32 or 64), the tile kernel's
 void launch_half_product(hipStream_t st, const HalfMat& m, HalfArgs g, int max_tiles);
 // the down products of T tokens' k places from h [T k][cols], and their weighted sums as out [T][rows]
 void launch_half_down_few(hipStream_t st, const HalfMat& m, int T, int k, const uint16_t* h, const int* ids, const float* weights,

@@ -374,7 +374,7 @@ struct Buf {
     size_t bytes = 0;
 };
 
-enum I8Ws { I8_PERM, I8_TILES, I8_NTILES, I8_H, I8_HQ, I8_HD, I8_Y, LORA_PART, I8_WS_COUNT };
+enum I8Ws { I8_PERM, I8_TILES, I8_NTILES, I8_H, I8_HQ, I8_HD, I8_Y, HALF_OFFSETS, LORA_PART, I8_WS_COUNT };
 
 }  // namespace
 
@@ -2604,7 +2604,11 @@ bool half_type(int type) { return type == PHX_F16 || type == PHX_BF16; }
 
 // The workgroups' tiles of n places in n_mat groups, at most.
 int most_tiles(int n, int n_mat, int cap) { return n / cap + std::min(n, n_mat); }
-int rows_cap(int n, int n_mat) { return n <= 2 * n_mat ? 16 : n <= 8 * n_mat ? 32 : kHalfRows; }
+int half_cap(int n, int n_mat)
+{
+    if (const char* f = getenv("PHX_CAP")) return atoi(f);
+    return n <= 2 * n_mat ? 16 : n <= 8 * n_mat ? 32 : n <= 12 * n_mat ? kHalfRows : kHalfTile;
+}
 }  // namespace
 
 int phx_weight_upload_half(phx_moe_ctx* c, int type, int n_mat, int rows, int cols, int paired, const void* w, phx_weight** out)
@@ -2678,7 +2682,7 @@ int phx_matmul_grouped(phx_moe_ctx* c, const phx_weight* w, int act, int n, cons
     g.act = act;
     g.type = y_type;
     g.out = y;
-    g.cap = rows_cap(n, m.n_mat);
+    g.cap = half_cap(n, m.n_mat);
     launch_half_product(c->stream, m, g, most_tiles(n, m.n_mat, g.cap));
     HIPCHK(c, launch_status(c));
     return PHX_OK;
@@ -2732,23 +2736,21 @@ int phx_experts_half(phx_moe_ctx* c, const phx_weight* gu, const phx_weight* dn,
     }
     // long batches go through in chunks, so that the workspace stays bounded and every row of it, and of x, within 2^32 bytes
     const int chunk = std::min<int64_t>(T, std::min<int64_t>(65535, ((1ll << 32) - 1) / (4ll * std::max(d, nf))) / k), A = chunk * k;
-    const int cap = rows_cap(A, E), max_tiles = most_tiles(A, E, cap);
-    int *perm, *ntiles;
-    Tile* tiles;
+    int *perm, *offsets;
     float* y;
-    if ((rc = i8_ensure(c, I8_PERM, A, &perm)) || (rc = i8_ensure(c, I8_TILES, max_tiles, &tiles)) ||
-        (rc = i8_ensure(c, I8_NTILES, 1, &ntiles)) || (rc = i8_ensure(c, I8_H, (int64_t)A * nf, &h)) ||
-        (rc = i8_ensure(c, I8_Y, (int64_t)A * d, &y)))
+    if ((rc = i8_ensure(c, I8_PERM, A, &perm)) || (rc = i8_ensure(c, HALF_OFFSETS, E + 1, &offsets)) ||
+        (rc = i8_ensure(c, I8_H, (int64_t)A * nf, &h)) || (rc = i8_ensure(c, I8_Y, (int64_t)A * d, &y)))
         return rc;
-    g.tiles = tiles;
-    g.ntiles = ntiles;
-    g.cap = cap;
+    g.offsets = offsets;
+    g.cap = half_cap(A, E);
+    const int max_tiles = most_tiles(A, E, g.cap);
     for (int t0 = 0; t0 < T; t0 += chunk) {
         const int n = std::min(chunk, T - t0);
         const int32_t* id = ids + (int64_t)t0 * k;
-        launch_i8_lists(st, n * k, E, cap, id, perm, tiles, ntiles);
+        launch_i8_lists(st, n * k, E, g.cap, id, perm, nullptr, nullptr, offsets);
         // gate and up in the lists' order, down back to the assignments' own
         g.x = (const uint16_t*)x + (int64_t)t0 * d;
+        g.n = n * k;
         g.n_x = n;
         g.src = perm;
         g.div = k;
