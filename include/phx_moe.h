@@ -432,10 +432,9 @@ int phx_weight_upload_half(phx_moe_ctx* ctx, int type, int n_mat, int rows, int 
  * with src[i] = i where src is NULL.  silu(g) = g / (1 + exp(-g)); gelu(g) = g / (1 + exp(-2 z)), z = sqrt(2 / pi) (g +
  * 0.044715 g^3), the tanh form, in float (phx_quant_i8's gelu goes through fp16, this one does not); both are 0 for
  * -infinity, and a NaN stays one.  One rounding, to y_type (PHX_F32, PHX_F16, PHX_BF16).  x: n_x rows of cols of the
- * weights' type.  offsets [n_mat + 1] ascend from any value on, in 0 .. n; a value outside counts as the nearest of
- * these, and a group that ends where it begins is empty.  Rows of y outside every group, and places whose src is outside
- * [0, n_x), are left as they were.  (Offsets that do not ascend give some places to two groups: which of the two is
- * then stored is not defined.)  1 <= n <= PHX_MAX_ROWS_I8, 1 <= n_x <= PHX_MAX_ROWS_I8, n_x >= n without src; with src
+ * weights' type.  offsets [n_mat + 1] ascend in 0 .. n (a value outside counts as the nearest of these, one below
+ * the one before it as that one); a group that ends where it begins is empty.  Rows of y outside every group, and places
+ * whose src is outside [0, n_x), are left as they were.  1 <= n <= PHX_MAX_ROWS_I8, 1 <= n_x <= PHX_MAX_ROWS_I8, n_x >= n without src; with src
  * x spans less than 2^32 bytes.  x and y 16-byte, offsets and src 4-byte aligned.  n_mat = 1 is a dense product. */
 int phx_matmul_grouped(phx_moe_ctx* ctx, const phx_weight* w, int act, int n, const int32_t* offsets, const void* x, int n_x,
                        const int32_t* src, int y_type, void* y);

@@ -99,22 +99,32 @@ void launch_half_pack(hipStream_t st, const HalfMat& m, int m0, int n_mat, const
 template <bool EVEN>
 struct Groups {
     int at[5], t[4], first, sum;  // the lane's groups' bounds and tiles, the tiles before them and in them
-    __device__ Groups(const HalfArgs& g)
+    __device__ __forceinline__ Groups(const HalfArgs& g)
     {
+        // the offsets held to 0 .. n, and each to at least the one before it, so that no two groups share a place; past the last
+        // group all are its end
         const int lane = threadIdx.x & 63;
         sum = 0;
 #pragma unroll
         for (int i = 0; i < 5; i++) at[i] = min(max(g.offsets[min(4 * lane + i, g.n_mat)], 0), g.n);
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            t[i] = max(at[i + 1] - at[i] + g.cap - 1, 0) / g.cap;  // past the last group both ends are its end
-            sum += t[i];
+        for (int i = 1; i < 5; i++) at[i] = max(at[i], at[i - 1]);
+        int most = at[3];
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const int before = __shfl_up(most, d);
+            most = lane >= d ? max(most, before) : most;
         }
+        const int before = __shfl_up(most, 1);  // lane 0: its own
+#pragma unroll
+        for (int i = 0; i < 5; i++) at[i] = lane ? max(at[i], before) : at[i];
+#pragma unroll
+        for (int i = 0; i < 4; i++) sum += t[i] = (at[i + 1] - at[i] + g.cap - 1) / g.cap;
         first = wave_incl_scan_i(sum) - sum;
     }
-    __device__ int total() const { return __builtin_amdgcn_readlane(first + sum, 63); }
+    __device__ __forceinline__ int total() const { return __builtin_amdgcn_readlane(first + sum, 63); }
     // Item `item` of `per` items a tile, a group's tiles following each other for each of its items: the tile, and which item.
-    __device__ bool find(const HalfArgs& g, int item, int per, Tile* tl, int* which) const
+    __device__ __forceinline__ bool find(const HalfArgs& g, int item, int per, Tile* tl, int* which) const
     {
         const unsigned long long here = __ballot(item >= first * per && item < (first + sum) * per);
         if (!here) return false;
@@ -388,7 +398,7 @@ __device__ __forceinline__ void half_tile_product(const HalfArgs& g, const Tile&
                     constexpr int i = decltype(I)::value, d = kk * DPG + i - 2;
                     if constexpr (m == NT + i * NT / (2 + DPG)) {
                         if constexpr (i < 2 && kk == 0) weight(s + 1, i, ic<1 - p>{}, ic<3>{});
-                        else if constexpr (i < 2) weight(s + 2, i, ic<p>{}, ic<kk - 1>{});
+                        else if constexpr (i < 2) weight(s + 2, i, ic<p>{}, ic<(kk + 3) % 4>{});
                         else if constexpr (d < NT) dma(s + RING - 1, far, ic<d>{});
                     }
                 });
@@ -408,7 +418,7 @@ __device__ __forceinline__ void half_tile_product(const HalfArgs& g, const Tile&
         static_for<4>([&](auto KK) {
             constexpr int kk = decltype(KK)::value;
             __builtin_amdgcn_sched_barrier(0);
-            if constexpr (kk > 0) weight(p, 0, ic<p>{}, ic<kk - 1>{}), weight(p, 1, ic<p>{}, ic<kk - 1>{});
+            if constexpr (kk > 0) weight(p, 0, ic<p>{}, ic<(kk + 3) % 4>{}), weight(p, 1, ic<p>{}, ic<(kk + 3) % 4>{});
             else if constexpr (p == 1) weight(0, 0, ic<0>{}, ic<3>{}), weight(0, 1, ic<0>{}, ic<3>{});
             __builtin_amdgcn_sched_barrier(0);
             static_for<DPG>([&](auto D) {

@@ -28,14 +28,14 @@ __device__ __forceinline__ f32x4 mma16(w4 a, w4 b, f32x4 c)
 struct TileSlots {
     int mine;
     unsigned left;
-    __device__ TileSlots(const int* ids, int n_slot, int T, int t0)
+    __device__ __forceinline__ TileSlots(const int* ids, int n_slot, int T, int t0)
     {
         const int r = t0 + (int)(threadIdx.x & 15), id = ids[min(r, T - 1)];
         mine = (unsigned)id < (unsigned)n_slot ? id : -1;
         left = (1u << min(16, T - t0)) - 1;
     }
     // the next slot's number and rows; false when no row is left
-    __device__ bool next(int* slot, unsigned* rows)
+    __device__ __forceinline__ bool next(int* slot, unsigned* rows)
     {
         if (!left) return false;
         *slot = __builtin_amdgcn_readlane(mine, __builtin_ctz(left));

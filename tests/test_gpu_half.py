@@ -46,7 +46,7 @@ def check(ctx, type_, y_type, E, n, rows, cols, act=0, gather=None, offsets=None
     finally:
         ctx.weight_free(h)
     assert (raw[n * out * item:] == before[n * out * item:]).all()
-    at = np.clip(offsets, 0, n)
+    at = np.maximum.accumulate(np.clip(offsets, 0, n))
     stored = np.zeros(n, bool)
     for e in range(E):
         p = np.arange(at[e], max(at[e], at[e + 1]))
@@ -103,6 +103,26 @@ def test_offsets_outside(ctx, n, E):
     check(ctx, 30, 30, E, n, 48, 64, offsets=np.full(E + 1, n // 2, np.int32))
     check(ctx, 30, 30, E, n, 48, 64, offsets=np.full(E + 1, 2 ** 31 - 1, np.int32))
     check(ctx, 30, 30, E, n, 48, 64, offsets=np.array([n - 1] * E + [n], np.int32))
+
+
+@pytest.mark.parametrize("n,E", [(60, 5), (400, 200), (900, 3), (3000, 256)])
+def test_offsets_that_fall(ctx, n, E):
+    """A value below the one before it counts as that one: no place has two groups."""
+    check(ctx, 1, 1, E, n, 48, 64, offsets=np.random.default_rng(n).integers(-20, n + 20, E + 1).astype(np.int32))
+    check(ctx, 30, 30, E, n, 48, 64, offsets=np.linspace(n, 0, E + 1).astype(np.int32))
+
+
+# long reductions and odd ones, more and fewer tiles than compute units
+@pytest.mark.parametrize("E,n,rows,cols", [(1, 200, 64, 8192), (1, 1000, 300, 4096), (2, 700, 2000, 2048), (9, 2500, 1030, 1536), (3, 97, 700, 16384),
+                                           (40, 6000, 520, 1024), (5, 2100, 4096, 1608), (1, 3000, 2816, 2056)])
+def test_reductions(ctx, E, n, rows, cols):
+    check(ctx, 30, 30, E, n, rows, cols)
+    check(ctx, 1, 0, E, n, rows // 2 * 2, cols, act=1, gather=n // 2)
+
+
+@pytest.mark.parametrize("places", range(30, 290, 20))
+def test_tile_widths(ctx, places):
+    check(ctx, 30, 0, 2, 2 * places + 5, 600, 1032, offsets=np.array([2, 2 + places, 2 * places + 3], np.int32))
 
 
 @pytest.mark.parametrize("n", [9, 40, 300])
