@@ -290,8 +290,7 @@ __global__ __launch_bounds__(64 * NW) void k_half_rows(HalfArgs g)
     if (!half_tile(g, blockIdx.y, &tl)) return;  // uniform over the workgroup
     const int n = (tl.cnt + 15) / 16;
     if (CT == 1 || n == 1) half_rows_product<NW, RT, 1, PAIRED, ONCE, BF>(g, tl, red, orow);
-    else if (CT == 2 || n == 2) half_rows_product<NW, RT, CT < 2 ? 1 : 2, PAIRED, ONCE, BF>(g, tl, red, orow);
-    else half_rows_product<NW, RT, CT < 4 ? 1 : 4, PAIRED, ONCE, BF>(g, tl, red, orow);
+    else half_rows_product<NW, RT, CT < 2 ? 1 : 2, PAIRED, ONCE, BF>(g, tl, red, orow);
 }
 
 // k_half_tile: four waves, each 64 stored weight rows (PAIRED: the gate and up rows of 32 channels), by a tile of up to 256 places.
@@ -300,12 +299,13 @@ __global__ __launch_bounds__(64 * NW) void k_half_rows(HalfArgs g)
 // ring by direct loads three to five steps ahead, row-major runs of 128 bytes with the 16-byte chunks XOR-swizzled by half the row's number
 // (16 lanes of a 16-byte read then have 16 distinct bank groups).
 constexpr int TI_WAVE = 32 * (64 * 4 + 16);  // a wave's part of the ring in the epilogue: 32 places' rows of 64 floats
-constexpr int ti_ring(int nt) { return nt >= 7 ? 4 : nt >= 5 ? 5 : 6; }  // slots: as many steps as 128 KB hold, up to six
+// slots: as many steps as the ring holds, up to six (MT: the row tiles it is made for, 16 KB each)
+constexpr int ti_ring(int nt, int mt) { return std::min(mt * 4 / nt, 6); }
 
-template <int NT, bool PAIRED, bool ONCE, bool BF>
+template <int NT, int MT, bool PAIRED, bool ONCE, bool BF>
 __device__ __forceinline__ void half_tile_product(const HalfArgs& g, const Tile& tl, int bx, unsigned char* ring, uint32_t* orow)
 {
-    constexpr int STAGE = NT * 32 * 128, RING = ti_ring(NT);
+    constexpr int STAGE = NT * 32 * 128, RING = ti_ring(NT, MT);
     const int tid = threadIdx.x, lane = tid & 63, r32 = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int S = g.kc / 8, row_bytes = g.cols * 2;
@@ -505,12 +505,12 @@ __device__ __forceinline__ void half_tile_product(const HalfArgs& g, const Tile&
 // Workgroup L runs on XCD L % 8.  The items (a tile's block of 256 stored rows) are in the order of groups, blocks, tiles, and
 // each XCD takes an eighth of them as one run: a group's tiles meet a block's weights in one L2 at about one time, and the weights
 // leave memory once.
-template <bool PAIRED, bool ONCE, bool BF>
-__global__ __launch_bounds__(256, 1) void k_half_tile(HalfArgs g)
+template <int MT, bool PAIRED, bool ONCE, bool BF>
+__global__ __launch_bounds__(256, MT > 4 ? 1 : 2) void k_half_tile(HalfArgs g)
 {
-    __shared__ __align__(16) unsigned char ring[128 * 1024];
+    __shared__ __align__(16) unsigned char ring[MT * 16 * 1024];
     static_assert(sizeof(ring) >= 4 * TI_WAVE, "the epilogue's part of each wave");
-    __shared__ __align__(16) uint32_t orow[kHalfTile];
+    __shared__ __align__(16) uint32_t orow[MT * 32];
     const Groups<true> G(g);
     const int blocks = (g.rgs + 7) / 8, all = G.total() * blocks, run = (all + 7) / 8, k = blockIdx.x >> 3;
     const int item = (blockIdx.x & 7) * run + k;
@@ -520,15 +520,25 @@ __global__ __launch_bounds__(256, 1) void k_half_tile(HalfArgs g)
     // said once more, so that addresses stay in scalar registers: a buffer in vector ones costs a loop for each load
     tl = {__builtin_amdgcn_readfirstlane(tl.e), __builtin_amdgcn_readfirstlane(tl.start), __builtin_amdgcn_readfirstlane(tl.cnt)};
     bx = __builtin_amdgcn_readfirstlane(bx);
-    switch ((tl.cnt + 31) / 32) {
-    case 1: half_tile_product<1, PAIRED, ONCE, BF>(g, tl, bx, ring, orow); break;
-    case 2: half_tile_product<2, PAIRED, ONCE, BF>(g, tl, bx, ring, orow); break;
-    case 3: half_tile_product<3, PAIRED, ONCE, BF>(g, tl, bx, ring, orow); break;
-    case 4: half_tile_product<4, PAIRED, ONCE, BF>(g, tl, bx, ring, orow); break;
-    case 5: half_tile_product<5, PAIRED, ONCE, BF>(g, tl, bx, ring, orow); break;
-    case 6: half_tile_product<6, PAIRED, ONCE, BF>(g, tl, bx, ring, orow); break;
-    case 7: half_tile_product<7, PAIRED, ONCE, BF>(g, tl, bx, ring, orow); break;
-    default: half_tile_product<8, PAIRED, ONCE, BF>(g, tl, bx, ring, orow);
+    const int n = (tl.cnt + 31) / 32;
+    if constexpr (MT == 4) {
+        switch (n) {
+        case 1: half_tile_product<1, MT, PAIRED, ONCE, BF>(g, tl, bx, ring, orow); break;
+        case 2: half_tile_product<2, MT, PAIRED, ONCE, BF>(g, tl, bx, ring, orow); break;
+        case 3: half_tile_product<3, MT, PAIRED, ONCE, BF>(g, tl, bx, ring, orow); break;
+        default: half_tile_product<4, MT, PAIRED, ONCE, BF>(g, tl, bx, ring, orow);
+        }
+    } else {
+        switch (n) {
+        case 1: half_tile_product<1, MT, PAIRED, ONCE, BF>(g, tl, bx, ring, orow); break;
+        case 2: half_tile_product<2, MT, PAIRED, ONCE, BF>(g, tl, bx, ring, orow); break;
+        case 3: half_tile_product<3, MT, PAIRED, ONCE, BF>(g, tl, bx, ring, orow); break;
+        case 4: half_tile_product<4, MT, PAIRED, ONCE, BF>(g, tl, bx, ring, orow); break;
+        case 5: half_tile_product<5, MT, PAIRED, ONCE, BF>(g, tl, bx, ring, orow); break;
+        case 6: half_tile_product<6, MT, PAIRED, ONCE, BF>(g, tl, bx, ring, orow); break;
+        case 7: half_tile_product<7, MT, PAIRED, ONCE, BF>(g, tl, bx, ring, orow); break;
+        default: half_tile_product<8, MT, PAIRED, ONCE, BF>(g, tl, bx, ring, orow);
+        }
     }
 }
 
@@ -558,22 +568,24 @@ static void rows_by_pair(hipStream_t st, const HalfMat& m, const HalfArgs& g, in
     else half_rows<4, 4, CT, false, ONCE>(st, m, g, max_tiles);
 }
 
-template <bool PAIRED>
+template <int MT, bool PAIRED>
 static void half_tiles(hipStream_t st, const HalfMat& m, const HalfArgs& g, int max_tiles)
 {
     const dim3 grid((max_tiles * ((m.rg + 7) / 8) + 7) / 8 * 8), blk(256);
-    if (m.type == PHX_BF16) launch(k_half_tile<PAIRED, false, true>, grid, blk, 0, st, g);
-    else launch(k_half_tile<PAIRED, false, false>, grid, blk, 0, st, g);
+    if (m.type == PHX_BF16) launch(k_half_tile<MT, PAIRED, false, true>, grid, blk, 0, st, g);
+    else launch(k_half_tile<MT, PAIRED, false, false>, grid, blk, 0, st, g);
 }
 
 void launch_half_product(hipStream_t st, const HalfMat& m, HalfArgs g, int max_tiles)
 {
     set_matrix(g, m);
     if (g.cap <= 16) rows_by_pair<1, false>(st, m, g, max_tiles);
-    else if (g.cap <= 32) rows_by_pair<2, false>(st, m, g, max_tiles);
-    else if (g.cap <= 64) rows_by_pair<4, false>(st, m, g, max_tiles);
-    else if (m.paired) half_tiles<true>(st, m, g, max_tiles);
-    else half_tiles<false>(st, m, g, max_tiles);
+    else if (g.cap <= kHalfRows) rows_by_pair<2, false>(st, m, g, max_tiles);
+    else if (g.cap <= kHalfNarrow) {
+        if (m.paired) half_tiles<4, true>(st, m, g, max_tiles);
+        else half_tiles<4, false>(st, m, g, max_tiles);
+    } else if (m.paired) half_tiles<8, true>(st, m, g, max_tiles);
+    else half_tiles<8, false>(st, m, g, max_tiles);
 }
 
 // ------------------------------------------------------------------------------ experts

@@ -1,9 +1,9 @@
 // Low-rank adapters of many requests at once (phx_lora_add): y[t] = y_in[t] + scale * B (A x[t]) with the adapter of slot ids[t].
 //
-// Two launches: k_lora_down forms A x in parts of the reduction, as floats, and k_lora_up joins the parts in order, scales them and adds
-// B's products to the rows.  Both take tiles of 16 consecutive rows and, of a tile, one slot after another: the matrix
-// cores form the slot's products with all 16 rows, and the rows of that slot keep theirs.  No sorting, no order that depends on
-// timing; rows of one request that follow each other, as a prompt's do, cost one pass.
+// Two launches: k_lora_down forms A x as floats, scales it and writes it down as terms of the adapters' type, the second
+// product's operands; k_lora_up adds B's products to the rows.  Both take tiles of 16 consecutive rows and, of a tile, one slot after
+// another: the matrix cores form the slot's products with all 16 rows, and the rows of that slot keep theirs.  No sorting, no order
+// that depends on timing; rows of one request that follow each other, as a prompt's do, cost one pass.
 #include <algorithm>
 
 #include "device_common.h"
@@ -28,11 +28,11 @@ __device__ __forceinline__ f32x4 mma16(w4 a, w4 b, f32x4 c)
 struct TileSlots {
     int mine;
     unsigned left;
-    __device__ __forceinline__ TileSlots(const int* ids, int n_slot, int T, int t0)
+    __device__ __forceinline__ void load(const int* ids, int n_slot, int T, int t0)
     {
         const int r = t0 + (int)(threadIdx.x & 15), id = ids[min(r, T - 1)];
         mine = (unsigned)id < (unsigned)n_slot ? id : -1;
-        left = (1u << min(16, T - t0)) - 1;
+        left = t0 < T ? (1u << min(16, T - t0)) - 1 : 0;
     }
     // the next slot's number and rows; false when no row is left
     __device__ __forceinline__ bool next(int* slot, unsigned* rows)
@@ -42,6 +42,12 @@ struct TileSlots {
         *rows = (unsigned)__ballot(mine == *slot) & left;
         left &= ~*rows;
         return true;
+    }
+    // row r's slot alone, if r is the first of its rows; else nothing
+    __device__ __forceinline__ void only(int r)
+    {
+        const unsigned rows = (unsigned)__ballot(mine == __builtin_amdgcn_readlane(mine, r)) & left;
+        left = rows && __builtin_ctz(rows) == r ? rows : 0;
     }
 };
 
@@ -80,37 +86,64 @@ void launch_lora_set(hipStream_t st, const LoraSlots& L, int slot, int rank, con
 }
 
 // ------------------------------------------------------------------------------ A x
-// A workgroup takes 16 rows (x), every gridDim.y-th slot of theirs (y), and a rank tile of 16 by a part of the reduction (z), which its
-// four waves split again; their sums meet in LDS, added in the waves' order.
-constexpr int LD_WAVES = 4;
-template <bool BF>
-__global__ __launch_bounds__(64 * LD_WAVES) void k_lora_down(LoraSlots L, int T, const uint16_t* __restrict__ x,
-                                                             const int* __restrict__ ids, int parts, float* __restrict__ part)
+// A value as the sum of TERMS terms of the adapters' type, each the rounding of what the ones before leave: 16 bits of it with two
+// bf16 terms, 22 with two of fp16, more than a float's with four.  An infinity or a NaN is in the first alone.
+template <bool BF, int TERMS>
+__device__ __forceinline__ void split(float v, uint16_t (&t)[TERMS])
 {
-    __shared__ float red[LD_WAVES * 256];
-    constexpr int U = 4;
+#pragma unroll
+    for (int i = 0; i < TERMS; i++) {
+        t[i] = (uint16_t)(BF ? f2bf_pair(v, 0.0f) : f2h_of(v));
+        const float rest = v - (BF ? bf2f(t[i]) : h2f(t[i]));
+        v = fabsf(rest) < 3.0e38f ? rest : 0.0f;
+    }
+}
+
+// A workgroup takes 16 rows (x) and RT rank tiles of 16 (z), FEW: for the slot of row y of them alone; its NW waves split the
+// reduction, all of a wave's loads in flight at once for rows of up to NW U steps, and their sums meet in LDS, added in the waves'
+// order.  low [T][rt][TERMS][16 ranks]; fp16's terms are of the value over 2^exps
+// [T][rt], which brings a row's 16 to below 2, so that none leaves the type's range.
+template <int NW, int RT, int TERMS, bool FEW, bool BF>
+__global__ __launch_bounds__(64 * NW) void k_lora_down(LoraSlots L, int T, const uint16_t* __restrict__ x,
+                                                       const int* __restrict__ ids, uint16_t* __restrict__ low,
+                                                       int* __restrict__ exps)
+{
+    __shared__ float red[NW * RT * 256];
+    constexpr int U = RT <= 2 ? 8 : 4;
     const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, q = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int t0 = blockIdx.x * 16, p = blockIdx.z % parts, rt = blockIdx.z / parts;
-    const int steps = L.kc / 4, n = parts * LD_WAVES, w = p * LD_WAVES + wave;
-    const int s0 = (int)((int64_t)w * steps / n), s1 = (int)((int64_t)(w + 1) * steps / n);
+    const int t0 = blockIdx.x * 16, rt0 = blockIdx.z * RT;
+    const int steps = L.kc / 4, s0 = wave * steps / NW, s1 = (wave + 1) * steps / NW;
     const uint16_t* xr = x + (int64_t)min(t0 + r16, T - 1) * L.cols;
-    TileSlots S(ids, L.n_slot, T, t0);
+    TileSlots S;
+    S.load(ids, L.n_slot, T, t0);
+    if (FEW) S.only(blockIdx.y);
     int slot;
     unsigned rows;
-    for (int j = 0; S.next(&slot, &rows); j++) {
-        if (j % gridDim.y != blockIdx.y || slot < 0 || L.rank[slot] <= rt * 16) continue;  // uniform over the workgroup
-        const uint8_t* a = L.a + slot * L.a_bytes() + (int64_t)rt * L.kc * 256 + q * 256 + r16 * 16;
-        f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-        w4 av[U], xv[U];
+    while (S.next(&slot, &rows)) {
+        if (slot < 0) continue;  // uniform over the workgroup
+        const bool here = rows >> r16 & 1;
+        const int rank = L.rank[slot];
+        if (rank <= rt0 * 16) continue;
+        const float scale = L.scale[slot];
+        const uint8_t* a[RT];
+#pragma unroll
+        for (int r = 0; r < RT; r++) a[r] = L.a + slot * L.a_bytes() + (int64_t)min(rt0 + r, L.rt - 1) * L.kc * 256 + q * 256 + r16 * 16;
+        f32x4 acc[RT];
+        w4 av[U][RT], xv[U];
+#pragma unroll
+        for (int r = 0; r < RT; r++) acc[r] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         auto load = [&](int u, int s) {
             const int su = min(s, s1 - 1);
-            av[u] = *(const w4*)(a + (int64_t)su * 1024);
-            xv[u] = *(const w4*)(xr + min(32 * su + 8 * q, L.cols - 8));
+#pragma unroll
+            for (int r = 0; r < RT; r++) av[u][r] = *(const w4*)(a[r] + (int64_t)su * 1024);
+            xv[u] = w4{0, 0, 0, 0};
+            if (here) xv[u] = *(const w4*)(xr + min(32 * su + 8 * q, L.cols - 8));
         };
         auto mma = [&](int u, int s) {
             if (32 * s + 32 > L.cols && 32 * s + 8 * q >= L.cols) xv[u] = w4{0, 0, 0, 0};  // against zero weights an infinity is none
-            acc = mma16<BF>(xv[u], av[u], acc);
+#pragma unroll
+            for (int r = 0; r < RT; r++) acc[r] = mma16<BF>(xv[u], av[u][r], acc[r]);
         };
         if (s0 < s1) {
 #pragma unroll
@@ -127,188 +160,208 @@ __global__ __launch_bounds__(64 * LD_WAVES) void k_lora_down(LoraSlots L, int T,
                 if (s + u < s1) mma(u, s + u);
         }
 #pragma unroll
-        for (int v = 0; v < 4; v++) red[wave * 256 + (4 * q + v) * 16 + r16] = acc[v];  // [row][rank]
+        for (int r = 0; r < RT; r++)
+#pragma unroll
+            for (int v = 0; v < 4; v++) red[(wave * RT + r) * 256 + (4 * q + v) * 16 + r16] = acc[r][v];  // [row][rank]
         __syncthreads();
-        const int row = tid >> 4;
-        if (rows >> row & 1) {
+        const int row = (tid >> 4) & 15, i = tid & 15;
+#pragma unroll
+        for (int r = 0; r < RT; r++) {
+            if (tid >= 256 || rt0 + r >= L.rt) continue;
             float s = 0.0f;
 #pragma unroll
-            for (int i = 0; i < LD_WAVES; i++) s += red[i * 256 + tid];
-            part[((int64_t)p * T + t0 + row) * (16 * L.rt) + rt * 16 + (tid & 15)] = s;
+            for (int w = 0; w < NW; w++) s += red[(w * RT + r) * 256 + (tid & 255)];
+            s = (rt0 + r) * 16 + i < rank ? s * scale : 0.0f;  // past the rank A's zeros may have met an infinity
+            const int64_t at = (int64_t)(t0 + row) * L.rt + rt0 + r;
+            int ex = 0;
+            if (!BF) {
+                unsigned m = __float_as_uint(s) & 0x7FFFFFFFu;
+                m = m >= 0x7F800000u ? 0u : m;
+#pragma unroll
+                for (int d = 1; d < 16; d *= 2) m = max(m, (unsigned)__shfl_xor((int)m, d));
+                ex = m ? (int)(m >> 23) - 127 : 0;  // |values| < 2^(ex + 1)
+                s = __builtin_amdgcn_ldexpf(s, -ex);
+            }
+            if (rows >> row & 1) {
+                uint16_t t[TERMS];
+                split<BF, TERMS>(s, t);
+#pragma unroll
+                for (int k = 0; k < TERMS; k++) low[(at * TERMS + k) * 16 + i] = t[k];
+                if (!BF && i == 0) exps[at] = ex;
+            }
         }
         __syncthreads();
     }
-}
-
-int lora_parts(const LoraSlots& L, int T, int ncu)
-{
-    const int tiles = (T + 15) / 16 * L.rt * std::min(L.n_slot, std::min(T, 16));
-    return std::max(1, std::min(std::min(8, L.kc / 4 / (4 * LD_WAVES)), ncu / std::max(tiles, 1)));
 }
 
 // the slots of a tile side by side where the rows are few, else one after another
-static int slots_apart(const LoraSlots& L, int T) { return T <= 256 ? std::min(L.n_slot + 1, std::min(T, 16)) : 1; }
+static bool few_rows(int T) { return T <= 256; }
 
-void launch_lora_down(hipStream_t st, const LoraSlots& L, int T, const uint16_t* x, const int* ids, int parts, float* part)
+template <int NW, int RT, bool FEW, bool BF>
+static void lora_down(hipStream_t st, const LoraSlots& L, int T, const uint16_t* x, const int* ids, int terms, uint16_t* low, int* exps)
 {
-    const dim3 grid((T + 15) / 16, slots_apart(L, T), L.rt * parts), blk(64 * LD_WAVES);
-    if (L.type == PHX_BF16) launch(k_lora_down<true>, grid, blk, 0, st, L, T, x, ids, parts, part);
-    else launch(k_lora_down<false>, grid, blk, 0, st, L, T, x, ids, parts, part);
+    const dim3 grid((T + 15) / 16, FEW ? std::min(T, 16) : 1, (L.rt + RT - 1) / RT), blk(64 * NW);
+    if (terms == 2) launch(k_lora_down<NW, RT, 2, FEW, BF>, grid, blk, 0, st, L, T, x, ids, low, exps);
+    else launch(k_lora_down<NW, RT, 4, FEW, BF>, grid, blk, 0, st, L, T, x, ids, low, exps);
+}
+
+template <bool BF>
+static void lora_down_type(hipStream_t st, const LoraSlots& L, int T, const uint16_t* x, const int* ids, int terms, uint16_t* low,
+                           int* exps)
+{
+    if (few_rows(T)) lora_down<16, 1, true, BF>(st, L, T, x, ids, terms, low, exps);
+    else if (L.rt == 1) lora_down<8, 1, false, BF>(st, L, T, x, ids, terms, low, exps);
+    else lora_down<8, 2, false, BF>(st, L, T, x, ids, terms, low, exps);
+}
+
+void launch_lora_down(hipStream_t st, const LoraSlots& L, int T, const uint16_t* x, const int* ids, int terms, uint16_t* low, int* exps)
+{
+    if (L.type == PHX_BF16) lora_down_type<true>(st, L, T, x, ids, terms, low, exps);
+    else lora_down_type<false>(st, L, T, x, ids, terms, low, exps);
 }
 
 // ------------------------------------------------------------------------------ y
-// Eight floats as two terms of the adapters' type, hi + lo; an infinity or a NaN is in hi alone.
-template <bool BF>
-__device__ __forceinline__ uint32_t pair16(float a, float b) { return pair_of<BF ? PHX_BF16 : PHX_F16>(a, b); }
-template <bool BF>
-__device__ __forceinline__ float value16(uint32_t h) { return BF ? bf2f(h & 0xFFFF) : h2f(h & 0xFFFF); }
-template <bool BF>
-__device__ __forceinline__ w4 term(float (&v)[8])
+// Four waves, each 64 outputs of TT tiles of 16 rows (FEW: of one tile, for the slot of row z of it alone).  The matrix instruction's 32
+// columns are 16 ranks twice: lanes 0 - 31 bring a value's first term, lanes 32 - 63 its second, B's ranks the same for both; for
+// float rows a second instruction takes the third and the fourth.  Weights are the first operand, so that a lane's sums are 16
+// consecutive outputs of one row; they stay in registers from tile to tile while the slot does (RM: the rank tiles there can be).
+// All tiles' ids and rows are loaded before the first is waited for.
+template <int DT, int RM, int TT, bool FEW, bool BF>
+__global__ __launch_bounds__(256) void k_lora_up(LoraSlots L, int T, const int* __restrict__ ids, const uint16_t* __restrict__ low,
+                                                 const int* __restrict__ exps, int64_t ld, const void* y_in, void* y)
 {
-    w4 t;
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-        t[j] = pair16<BF>(v[2 * j], v[2 * j + 1]);
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const float rest = v[2 * j + h] - value16<BF>(t[j] >> (16 * h));
-            v[2 * j + h] = fabsf(rest) < 3.0e38f ? rest : 0.0f;
-        }
-    }
-    return t;
-}
-
-// Four waves, each 64 outputs of 16 rows.  The matrix instruction's 32 columns are 16 ranks twice: lanes 0 - 31 bring the value's first
-// term, lanes 32 - 63 its second, B's ranks the same for both; for float rows a second instruction takes a third and a fourth.
-// A row's values are scaled by a power of two to below 2, so that neither term leaves the type's range, and its sums scaled
-// back.  Weights are the first operand, so that a lane's sums are 16 consecutive outputs of one row.
-template <int DT, bool BF>
-__global__ __launch_bounds__(256) void k_lora_up(LoraSlots L, int T, const int* __restrict__ ids, int parts,
-                                                 const float* __restrict__ part, int64_t ld, const void* y_in, void* y)
-{
-    constexpr int V = DT == PHX_F32 ? 4 : 8;  // values of 16 bytes
+    constexpr int ES = DT == PHX_F32 ? 4 : 2, V = 16 / ES, TERMS = DT == PHX_F32 ? 4 : 2;  // V: values of 16 bytes
     const int lane = threadIdx.x & 63, r16 = lane & 15, q = lane >> 4;
     const int grp = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (grp >= L.groups) return;
-    const int t0 = blockIdx.x * 16, row = t0 + r16;
-    const int64_t at = min(row, T - 1) * ld + grp * 64 + q * 16;
     const int cols = L.rows - grp * 64 - q * 16;  // this lane's outputs that there are
-    const bool wide = ld % V == 0 && ((uintptr_t)y_in | (uintptr_t)y) % 16 == 0;
-    TileSlots S(ids, L.n_slot, T, t0);
-    int slot;
-    unsigned rows;
-    for (int j = 0; S.next(&slot, &rows); j++) {
-        if (j % gridDim.z != blockIdx.z) continue;
-        const int rank = slot < 0 ? 0 : L.rank[slot];
-        if (rank == 0 && y_in == y) continue;
-        float v[16];
-        const bool here = rows >> r16 & 1;
-        if (here) {
+    const bool wide = cols >= 16 && ld % V == 0 && ((uintptr_t)y_in | (uintptr_t)y) % 16 == 0;
+    const int first = blockIdx.x * TT * 16;
+    auto place = [&](int tt) { return min(first + tt * 16 + r16, T - 1) * ld + grp * 64 + q * 16; };
+    TileSlots S[TT];
+    w4 yr[TT][16 / V];
 #pragma unroll
-            for (int i = 0; i < 16; i += V) {
-                if (wide && i + V <= cols) {
-                    if constexpr (DT == PHX_F32) *(float4*)(v + i) = *(const float4*)((const float*)y_in + at + i);
-                    else {
-                        float e[8];
-                        load_eight<DT>(y_in, at + i, e);
+    for (int tt = 0; tt < TT; tt++) S[tt].load(ids, L.n_slot, T, first + tt * 16);
+    if (FEW) S[0].only(blockIdx.z);
 #pragma unroll
-                        for (int k = 0; k < 8; k++) v[i + k] = e[k];
-                    }
-                } else {
+    for (int tt = 0; tt < TT; tt++)
+        if (wide && (!FEW || (S[tt].left >> r16 & 1)))
 #pragma unroll
-                    for (int k = 0; k < V; k++) v[i + k] = i + k < cols ? load_one<DT>(y_in, at + i + k) : 0.0f;
-                }
+            for (int i = 0; i < 16 / V; i++) yr[tt][i] = *(const w4*)((const char*)y_in + (place(tt) + i * V) * ES);
+    w4 bv[RM][4];
+    int held = -1, tiles = 0;  // the slot in bv, and its rank tiles
+#pragma unroll
+    for (int tt = 0; tt < TT; tt++) {
+        if (!S[tt].left) break;  // uniform
+        const int row = min(first + tt * 16 + r16, T - 1);
+        const int64_t at = place(tt);
+        float sum[16];
+#pragma unroll
+        for (int i = 0; i < 16; i++) sum[i] = 0.0f;
+        int slot;
+        unsigned rows, mine = 0;  // mine: the rows that are stored
+        while (S[tt].next(&slot, &rows)) {
+            if (slot >= 0 && slot != held) {
+                held = slot;
+                tiles = (L.rank[slot] + 15) / 16;
+                const uint8_t* b = L.b + slot * L.b_bytes() + (int64_t)grp * L.rt * 2048 + (q & 1) * 256 + r16 * 16;
+#pragma unroll
+                for (int r = 0; r < RM; r++)
+#pragma unroll
+                    for (int m = 0; m < 4; m++) bv[r][m] = *(const w4*)(b + min(r, L.rt - 1) * 2048 + m * 512);
             }
-        }
-        if (rank > 0) {
-            const int tiles = (rank + 15) / 16;
-            const float scale = L.scale[slot];
-            const float* s = part + (int64_t)min(row, T - 1) * (16 * L.rt) + 8 * (q & 1);
-            auto values = [&](int rt, float (&c)[8]) {
-#pragma unroll
-                for (int k = 0; k < 8; k++) c[k] = 0.0f;
-                if (here)
-                    for (int p = 0; p < parts; p++) {
-                        float e[8];
-                        load_eight<PHX_F32>(s, (int64_t)p * T * (16 * L.rt) + rt * 16, e);
-#pragma unroll
-                        for (int k = 0; k < 8; k++) c[k] += e[k];
-                    }
-#pragma unroll
-                for (int k = 0; k < 8; k++) c[k] = rt * 16 + 8 * (q & 1) + k < rank ? c[k] * scale : 0.0f;  // a NaN past the rank: 0 * infinity
-            };
-            // the row's largest exponent, over its ranks: lanes r16 and r16 + 16 hold the halves of a rank tile
-            unsigned most = 0;
-            for (int rt = 0; rt < tiles; rt++) {
-                float c[8];
-                values(rt, c);
-#pragma unroll
-                for (int k = 0; k < 8; k++) {
-                    const unsigned m = __float_as_uint(c[k]) & 0x7FFFFFFFu;
-                    most = max(most, m >= 0x7F800000u ? 0u : m);
-                }
-            }
-            most = max(most, (unsigned)__shfl_xor((int)most, 16));
-            const int ex = most ? (int)(most >> 23) - 127 : 0;  // |values| < 2^(ex + 1)
+            const int n = slot >= 0 ? tiles : 0;
+            if (n > 0 || y_in != y) mine |= rows;
+            if (n == 0) continue;
+            const bool here = rows >> r16 & 1;
             f32x4 acc[4];
 #pragma unroll
             for (int m = 0; m < 4; m++) acc[m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-            const uint8_t* b = L.b + slot * L.b_bytes() + (int64_t)grp * L.rt * 2048 + (q & 1) * 256 + r16 * 16;
-            for (int rt = 0; rt < tiles; rt++) {
-                float c[8];
-                values(rt, c);
+            const uint16_t* lo = low + (int64_t)row * L.rt * (TERMS * 16) + (q >> 1) * 16 + (q & 1) * 8;
 #pragma unroll
-                for (int k = 0; k < 8; k++) c[k] = __builtin_amdgcn_ldexpf(c[k], -ex);
-                w4 bv[4];
+            for (int r = 0; r < RM; r++) {
+                if (r >= n) break;  // uniform
+                w4 t[TERMS / 2];
 #pragma unroll
-                for (int m = 0; m < 4; m++) bv[m] = *(const w4*)(b + (int64_t)rt * 2048 + m * 512);
+                for (int k = 0; k < TERMS / 2; k++) t[k] = *(const w4*)(lo + (r * TERMS + 2 * k) * 16);
+                if (BF) {
 #pragma unroll
-                for (int k = 0; k < (DT == PHX_F32 ? 2 : 1); k++) {
-                    const w4 hi = term<BF>(c), lo = term<BF>(c);
-                    w4 mine;
+                    for (int k = 0; k < TERMS / 2; k++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) mine[i] = q < 2 ? hi[i] : lo[i];
+                        for (int m = 0; m < 4; m++) acc[m] = mma16<BF>(bv[r][m], t[k], acc[m]);
+                } else {
+                    const int ex = here ? exps[(int64_t)row * L.rt + r] : 0;
 #pragma unroll
-                    for (int m = 0; m < 4; m++) acc[m] = mma16<BF>(bv[m], mine, acc[m]);
+                    for (int m = 0; m < 4; m++) {
+                        f32x4 p = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                        for (int k = 0; k < TERMS / 2; k++) p = mma16<BF>(bv[r][m], t[k], p);
+#pragma unroll
+                        for (int i = 0; i < 4; i++) acc[m][i] += __builtin_amdgcn_ldexpf(p[i], ex);
+                    }
                 }
             }
 #pragma unroll
             for (int m = 0; m < 4; m++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) v[4 * m + i] += __builtin_amdgcn_ldexpf(acc[m][i], ex);
+                for (int i = 0; i < 4; i++) sum[4 * m + i] = here ? acc[m][i] : sum[4 * m + i];
         }
-        if (!here) continue;
+        if (!(mine >> r16 & 1)) continue;
+        if (wide) {
 #pragma unroll
-        for (int i = 0; i < 16; i += V) {
-            if (wide && i + V <= cols) {
+            for (int i = 0; i < 16 / V; i++) {
                 float e[V];
 #pragma unroll
-                for (int k = 0; k < V; k++) e[k] = v[i + k];
-                store_16<DT>(y, at + i, e);
-            } else {
-#pragma unroll
-                for (int k = 0; k < V; k++)
-                    if (i + k < cols) store_one<DT>(y, at + i + k, v[i + k]);
+                for (int k = 0; k < V; k++) {
+                    const uint32_t u = yr[tt][i][k * ES / 4], h = k & 1 ? u >> 16 : u & 0xFFFFu;
+                    e[k] = (DT == PHX_F32 ? __uint_as_float(u) : DT == PHX_F16 ? h2f(h) : bf2f(h)) + sum[i * V + k];
+                }
+                store_16<DT>(y, at + i * V, e);
             }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; i++)
+                if (i < cols) store_one<DT>(y, at + i, load_one<DT>(y_in, at + i) + sum[i]);
         }
     }
 }
 
-template <int DT>
-static void lora_up(hipStream_t st, const LoraSlots& L, int T, const int* ids, int parts, const float* part, int64_t ld,
+template <int DT, int RM, bool BF>
+static void lora_up(hipStream_t st, const LoraSlots& L, int T, const int* ids, const uint16_t* low, const int* exps, int64_t ld,
                     const void* y_in, void* y)
 {
-    const dim3 grid((T + 15) / 16, (L.groups + 3) / 4, slots_apart(L, T)), blk(256);
-    if (L.type == PHX_BF16) launch(k_lora_up<DT, true>, grid, blk, 0, st, L, T, ids, parts, part, ld, y_in, y);
-    else launch(k_lora_up<DT, false>, grid, blk, 0, st, L, T, ids, parts, part, ld, y_in, y);
+    const dim3 blk(256);
+    if (few_rows(T)) {
+        const dim3 grid((T + 15) / 16, (L.groups + 3) / 4, std::min(T, 16));
+        launch(k_lora_up<DT, RM, 1, true, BF>, grid, blk, 0, st, L, T, ids, low, exps, ld, y_in, y);
+    } else {
+        constexpr int TT = 4;
+        const dim3 grid((T + 16 * TT - 1) / (16 * TT), (L.groups + 3) / 4);
+        launch(k_lora_up<DT, RM, TT, false, BF>, grid, blk, 0, st, L, T, ids, low, exps, ld, y_in, y);
+    }
 }
 
-void launch_lora_up(hipStream_t st, const LoraSlots& L, int T, const int* ids, int parts, const float* part, int y_type, int64_t ld,
-                    const void* y_in, void* y)
+template <int DT>
+static void lora_up_type(hipStream_t st, const LoraSlots& L, int T, const int* ids, const uint16_t* low, const int* exps, int64_t ld,
+                         const void* y_in, void* y)
 {
-    if (y_type == PHX_F16) lora_up<PHX_F16>(st, L, T, ids, parts, part, ld, y_in, y);
-    else if (y_type == PHX_BF16) lora_up<PHX_BF16>(st, L, T, ids, parts, part, ld, y_in, y);
-    else lora_up<PHX_F32>(st, L, T, ids, parts, part, ld, y_in, y);
+    const bool bf = L.type == PHX_BF16;
+    if (L.rt == 1 && bf) lora_up<DT, 1, true>(st, L, T, ids, low, exps, ld, y_in, y);
+    else if (L.rt == 1) lora_up<DT, 1, false>(st, L, T, ids, low, exps, ld, y_in, y);
+    else if (L.rt == 2 && bf) lora_up<DT, 2, true>(st, L, T, ids, low, exps, ld, y_in, y);
+    else if (L.rt == 2) lora_up<DT, 2, false>(st, L, T, ids, low, exps, ld, y_in, y);
+    else if (L.rt <= 4 && bf) lora_up<DT, 4, true>(st, L, T, ids, low, exps, ld, y_in, y);
+    else if (L.rt <= 4) lora_up<DT, 4, false>(st, L, T, ids, low, exps, ld, y_in, y);
+    else if (bf) lora_up<DT, 8, true>(st, L, T, ids, low, exps, ld, y_in, y);
+    else lora_up<DT, 8, false>(st, L, T, ids, low, exps, ld, y_in, y);
+}
+
+void launch_lora_up(hipStream_t st, const LoraSlots& L, int T, const int* ids, const uint16_t* low, const int* exps, int y_type,
+                    int64_t ld, const void* y_in, void* y)
+{
+    if (y_type == PHX_F16) lora_up_type<PHX_F16>(st, L, T, ids, low, exps, ld, y_in, y);
+    else if (y_type == PHX_BF16) lora_up_type<PHX_BF16>(st, L, T, ids, low, exps, ld, y_in, y);
+    else lora_up_type<PHX_F32>(st, L, T, ids, low, exps, ld, y_in, y);
 }
 
 }  // namespace phx

@@ -362,7 +362,7 @@ struct HalfArgs {
     int64_t mat_bytes;
     int kc, cols, out_cols, rgs, n_mat;
 };
-constexpr int kHalfRows = 64, kHalfTile = 256;  // places a tile: the row kernel's most (16, 32 or 64), the tile kernel's
+constexpr int kHalfRows = 32, kHalfNarrow = 128, kHalfTile = 256;  // places a tile: the row kernel's (16 or 32), the tile kernel's two
 void launch_half_product(hipStream_t st, const HalfMat& m, HalfArgs g, int max_tiles);
 // the down products of T tokens' k places from h [T k][cols], and their weighted sums as out [T][rows]
 void launch_half_down_few(hipStream_t st, const HalfMat& m, int T, int k, const uint16_t* h, const int* ids, const float* weights,
@@ -380,11 +380,11 @@ struct LoraSlots {
     __host__ __device__ int64_t b_bytes() const { return (int64_t)groups * rt * 2048; }
 };
 void launch_lora_set(hipStream_t st, const LoraSlots& L, int slot, int rank, const uint16_t* a, const uint16_t* b, float scale);
-// the parts that A's reduction is split in for T rows; part [parts][T][16 rt] floats
-int lora_parts(const LoraSlots& L, int T, int ncu);
-void launch_lora_down(hipStream_t st, const LoraSlots& L, int T, const uint16_t* x, const int* ids, int parts, float* part);
-void launch_lora_up(hipStream_t st, const LoraSlots& L, int T, const int* ids, int parts, const float* part, int y_type, int64_t ld,
-                    const void* y_in, void* y);
+// scale A x as `terms` terms of the adapters' type (2, or 4 for float rows), low [T][rt][terms][16], and for fp16 the exponents that
+// they are over, exps [T][rt]; then its products with B added to y_in's rows
+void launch_lora_down(hipStream_t st, const LoraSlots& L, int T, const uint16_t* x, const int* ids, int terms, uint16_t* low, int* exps);
+void launch_lora_up(hipStream_t st, const LoraSlots& L, int T, const int* ids, const uint16_t* low, const int* exps, int y_type,
+                    int64_t ld, const void* y_in, void* y);
 
 struct AddNormArgs {
     const void *x, *branch;

@@ -374,7 +374,7 @@ struct Buf {
     size_t bytes = 0;
 };
 
-enum I8Ws { I8_PERM, I8_TILES, I8_NTILES, I8_H, I8_HQ, I8_HD, I8_Y, HALF_OFFSETS, LORA_PART, I8_WS_COUNT };
+enum I8Ws { I8_PERM, I8_TILES, I8_NTILES, I8_H, I8_HQ, I8_HD, I8_Y, HALF_OFFSETS, LORA_LOW, LORA_EXPS, I8_WS_COUNT };
 
 }  // namespace
 
@@ -2602,12 +2602,31 @@ int upload_half(phx_moe_ctx* c, HalfMat& m, const uint16_t* w)
 
 bool half_type(int type) { return type == PHX_F16 || type == PHX_BF16; }
 
-// The workgroups' tiles of n places in n_mat groups, at most.
+// The tiles of n places in n_mat groups, at most.
 int most_tiles(int n, int n_mat, int cap) { return n / cap + std::min(n, n_mat); }
-int half_cap(int n, int n_mat)
+
+// The kernel of a product over n places, by its tiles' capacity.
+// Row kernel to 10 places a group, and where its workgroups number under three per compute unit (us, row kernel and tile kernel; 128
+// groups of 1408 x 2816: 8.8 places 157, 157; 12.7 167, 164; 64 of 4096 x 1408: 6.3 109, 114; 15 137, 133; 32 of 1024 x 1024: 12.5
+// 14.1, 15.0; 25 16.4, 17.5; 50 21.3, 19.3; one of 4096 x 4096: 128 places 17.6, 40; 256 29, 41; 512 51, 42; 1024 92, 44).  Its tiles
+// of 16 places to two a group and to 64 in all, else of 32 (one of 4096 x 4096: 64 places 12.7, 16.7; 128 20.5, 17.6; 128 groups, 8.8
+// places 167, 157).
+// Tiles of 256 places, one workgroup a compute unit, past 192 places a group where they number two per compute unit, else of 128, two
+// workgroups (us, tiles of 128 and 256; 32 groups of 2816 x 4096, 513 places 393, 381; 128 of 1408 x 2816, 128 places 249, 252; one of
+// 4096 x 4096, 2048 places 60, 78; 512 42, 71).
+int half_cap(phx_moe_ctx* c, const HalfMat& m, int n)
 {
-    if (const char* f = getenv("PHX_CAP")) return atoi(f);
-    return n <= 2 * n_mat ? 16 : n <= 8 * n_mat ? 32 : n <= 12 * n_mat ? kHalfRows : kHalfTile;
+    const int64_t groups = std::min(n, m.n_mat);
+    if (n <= 10 * m.n_mat || (n / 32 + groups / 2) * (m.rg / 2) < 3 * c->ncu) return n <= 64 || n <= 2 * m.n_mat ? 16 : kHalfRows;
+    return n > 192 * m.n_mat && (int64_t)(n / kHalfTile) * (m.rg / 8) >= 2 * c->ncu ? kHalfTile : kHalfNarrow;
+}
+
+// One product over n places.
+void half_product(phx_moe_ctx* c, const HalfMat& m, HalfArgs g, int n)
+{
+    g.n = n;
+    g.cap = half_cap(c, m, n);
+    launch_half_product(c->stream, m, g, most_tiles(n, m.n_mat, g.cap));
 }
 }  // namespace
 
@@ -2677,13 +2696,11 @@ int phx_matmul_grouped(phx_moe_ctx* c, const phx_weight* w, int act, int n, cons
     g.x = (const uint16_t*)x;
     g.src = src;
     g.offsets = offsets;
-    g.n = n;
     g.n_x = n_x;
     g.act = act;
     g.type = y_type;
     g.out = y;
-    g.cap = half_cap(n, m.n_mat);
-    launch_half_product(c->stream, m, g, most_tiles(n, m.n_mat, g.cap));
+    half_product(c, m, g, n);
     HIPCHK(c, launch_status(c));
     return PHX_OK;
 }
@@ -2742,29 +2759,26 @@ int phx_experts_half(phx_moe_ctx* c, const phx_weight* gu, const phx_weight* dn,
         (rc = i8_ensure(c, I8_H, (int64_t)A * nf, &h)) || (rc = i8_ensure(c, I8_Y, (int64_t)A * d, &y)))
         return rc;
     g.offsets = offsets;
-    g.cap = half_cap(A, E);
-    const int max_tiles = most_tiles(A, E, g.cap);
     for (int t0 = 0; t0 < T; t0 += chunk) {
         const int n = std::min(chunk, T - t0);
         const int32_t* id = ids + (int64_t)t0 * k;
-        launch_i8_lists(st, n * k, E, g.cap, id, perm, nullptr, nullptr, offsets);
+        launch_i8_lists(st, n * k, E, 1, id, perm, nullptr, nullptr, offsets);
         // gate and up in the lists' order, down back to the assignments' own
         g.x = (const uint16_t*)x + (int64_t)t0 * d;
-        g.n = n * k;
         g.n_x = n;
         g.src = perm;
         g.div = k;
         g.dst = nullptr;
         g.type = gu->type;
         g.out = h;
-        launch_half_product(st, gu->half, g, max_tiles);
+        half_product(c, gu->half, g, n * k);
         g.x = h;
         g.src = nullptr;
         g.div = 1;
         g.dst = perm;
         g.type = PHX_F32;
         g.out = y;
-        launch_half_product(st, dn->half, g, max_tiles);
+        half_product(c, dn->half, g, n * k);
         launch_i8_combine(st, n, d, k, E, y, id, weights + (int64_t)t0 * k, out_type, (char*)out + (int64_t)t0 * d * eb);
     }
     HIPCHK(c, launch_status(c));
@@ -2871,13 +2885,16 @@ int phx_lora_add(phx_moe_ctx* c, const phx_lora* l, int T, const void* x, const 
     const CallBuf bx{"x", x, (int64_t)T * L.cols * 2, 16, false}, bi{"ids", ids, T * 4ll, 4, false}, by{"y", y, span, eb, true};
     int rc = y_in == y ? check_bufs(c, "lora_add", {bx, bi, by}) : check_bufs(c, "lora_add", {bx, bi, by, {"y_in", y_in, span, eb, false}});
     if (rc) return rc;
-    const int chunk = std::min(T, 65536), parts = lora_parts(L, chunk, c->ncu);
-    float* part;
-    if ((rc = i8_ensure(c, LORA_PART, (int64_t)parts * chunk * 16 * L.rt, &part))) return rc;
+    const int chunk = std::min(T, 65536), terms = y_type == PHX_F32 ? 4 : 2;  // the workspace stays bounded
+    uint16_t* low;
+    int* exps;
+    if ((rc = i8_ensure(c, LORA_LOW, (int64_t)chunk * L.rt * terms * 16, &low)) ||
+        (rc = i8_ensure(c, LORA_EXPS, (int64_t)chunk * L.rt, &exps)))
+        return rc;
     for (int t0 = 0; t0 < T; t0 += chunk) {
         const int n = std::min(chunk, T - t0);
-        launch_lora_down(c->stream, L, n, (const uint16_t*)x + (int64_t)t0 * L.cols, ids + t0, parts, part);
-        launch_lora_up(c->stream, L, n, ids + t0, parts, part, y_type, ld, (const char*)y_in + t0 * ld * eb, (char*)y + t0 * ld * eb);
+        launch_lora_down(c->stream, L, n, (const uint16_t*)x + (int64_t)t0 * L.cols, ids + t0, terms, low, exps);
+        launch_lora_up(c->stream, L, n, ids + t0, low, exps, y_type, ld, (const char*)y_in + t0 * ld * eb, (char*)y + t0 * ld * eb);
     }
     HIPCHK(c, launch_status(c));
     return PHX_OK;
