@@ -3,36 +3,9 @@
 //
 // Sums are the matrix cores' floats.  Where waves split a reduction they meet in LDS in the waves' order, so no result depends
 // on timing.  A place's products involve its own row alone: an infinity or a NaN in another row of a tile reaches nothing.
-#include <algorithm>
-
-#include "device_common.h"
-#include "rows_io.h"
+#include "half_common.h"
 
 namespace phx {
-
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef uint32_t w4 __attribute__((ext_vector_type(4)));  // 16 bytes: eight values
-typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-typedef __bf16 b8 __attribute__((ext_vector_type(8)));
-
-// v_mfma_f32_16x16x32: lane l holds eight values of A row l % 16 and of B row l % 16, both at k = 8 (l / 16); D[i][j] sits
-// in lane j + 16 (i / 4), register i % 4.
-template <bool BF>
-__device__ __forceinline__ f32x4 mma16(w4 a, w4 b, f32x4 c)
-{
-    if constexpr (BF) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
-    else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
-}
-
-// v_mfma_f32_32x32x16: lane l holds eight values of A row l % 32 and of B row l % 32, both at k = 8 (l / 32); D[i][j] sits in
-// lane j + 32 ((i / 4) % 2), register 4 (i / 8) + i % 4.
-template <bool BF>
-__device__ __forceinline__ f32x16 mma32(w4 a, u32x4 b, f32x16 c)
-{
-    if constexpr (BF) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
-    else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
-}
 
 // 16 bytes of weights; ONCE: no other workgroup reads them, so they need not stay in the caches
 template <bool ONCE>
@@ -42,28 +15,7 @@ __device__ __forceinline__ w4 load_weights(const uint8_t* p)
     else return *(const w4*)p;
 }
 
-// act(g) * u, both activations g * sigmoid(z), the exponential and the reciprocal the hardware's (1 ulp each): a few units of
-// 2^-24, and the exponential's argument.  Far below, where the quotient is under every number, the reciprocal is 0; the gate
-// is then held to a number, so that no infinity meets it.
-__device__ __forceinline__ float gated_half(int act, float g, float u)
-{
-    const float z = act == PHX_QUANT_SILU_MUL ? g : 1.5957691216057308f * (g + 0.044715f * g * g * g);
-    const float r = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504088896340736f * z));
-    return fmaxf(g, -3.402823466e38f) * r * u;
-}
-
-__device__ __forceinline__ void store_as(int type, void* p, int64_t i, float v)
-{
-    if (type == PHX_F32) store_one<PHX_F32>(p, i, v);
-    else if (type == PHX_BF16) store_one<PHX_BF16>(p, i, v);
-    else store_one<PHX_F16>(p, i, v);
-}
-
 // ------------------------------------------------------------------------------ weights
-// The row of its group of 32 that is stored at slot s: what a lane holds of a 32 x 32 product, slots 8 g + 4 h + 0 .. 3 for
-// half h, are then 16 consecutive rows.
-__device__ __forceinline__ int slot_row(int s) { return 16 * ((s >> 2) & 1) + 4 * (s >> 3) + (s & 3); }
-
 // HalfMat's layout from matrices as the caller holds them: a thread writes 8 columns of one stored row, zeros past the
 // last row or column.
 __global__ __launch_bounds__(256) void k_half_pack(HalfMat m, int m0, int64_t n16, const uint16_t* __restrict__ w)
@@ -93,100 +45,6 @@ void launch_half_pack(hipStream_t st, const HalfMat& m, int m0, int n_mat, const
 }
 
 // ------------------------------------------------------------------------------ products
-// The groups that the offsets give, each in tiles of up to cap places, four groups to a lane: every wave looks a tile up for itself.
-// EVEN: a group's tiles are of one size, whole 32s (513 places as 192, 192 and 129 cost what 256, 256 and 1 do, and the longest
-// tile is what a launch ends with).
-template <bool EVEN>
-struct Groups {
-    int at[5], t[4], first, sum;  // the lane's groups' bounds and tiles, the tiles before them and in them
-    __device__ __forceinline__ Groups(const HalfArgs& g)
-    {
-        // the offsets held to 0 .. n, and each to at least the one before it, so that no two groups share a place; past the last
-        // group all are its end
-        const int lane = threadIdx.x & 63;
-        sum = 0;
-#pragma unroll
-        for (int i = 0; i < 5; i++) at[i] = min(max(g.offsets[min(4 * lane + i, g.n_mat)], 0), g.n);
-#pragma unroll
-        for (int i = 1; i < 5; i++) at[i] = max(at[i], at[i - 1]);
-        int most = at[3];
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const int before = __shfl_up(most, d);
-            most = lane >= d ? max(most, before) : most;
-        }
-        const int before = __shfl_up(most, 1);  // lane 0: its own
-#pragma unroll
-        for (int i = 0; i < 5; i++) at[i] = lane ? max(at[i], before) : at[i];
-#pragma unroll
-        for (int i = 0; i < 4; i++) sum += t[i] = (at[i + 1] - at[i] + g.cap - 1) / g.cap;
-        first = wave_incl_scan_i(sum) - sum;
-    }
-    __device__ __forceinline__ int total() const { return __builtin_amdgcn_readlane(first + sum, 63); }
-    // Item `item` of `per` items a tile, a group's tiles following each other for each of its items: the tile, and which item.
-    __device__ __forceinline__ bool find(const HalfArgs& g, int item, int per, Tile* tl, int* which) const
-    {
-        const unsigned long long here = __ballot(item >= first * per && item < (first + sum) * per);
-        if (!here) return false;
-        int e = 0, tile = 0, w = 0, f = first;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            if (item >= f * per && item < (f + t[i]) * per) {
-                e = i;
-                w = (item - f * per) / t[i];
-                tile = (item - f * per) % t[i];
-            }
-            f += t[i];
-        }
-        const int l = __builtin_ctzll(here);
-        int start = at[0], end = at[1], n = t[0];
-#pragma unroll
-        for (int i = 1; i < 4; i++)
-            if (e == i) start = at[i], end = at[i + 1], n = t[i];
-        tl->e = 4 * l + __builtin_amdgcn_readlane(e, l);
-        start = __builtin_amdgcn_readlane(start, l);
-        end = __builtin_amdgcn_readlane(end, l);
-        n = __builtin_amdgcn_readlane(n, l);
-        const int size = EVEN ? ((end - start + n - 1) / n + 31) & ~31 : g.cap;
-        tl->start = start + __builtin_amdgcn_readlane(tile, l) * size;
-        tl->cnt = min(end - tl->start, size);
-        *which = __builtin_amdgcn_readlane(w, l);
-        return true;
-    }
-};
-
-// The tile of a workgroup: cnt places of one group from start.  False where there is none.
-__device__ __forceinline__ bool half_tile(const HalfArgs& g, int tile, Tile* tl)
-{
-    if (g.ids) {  // a tile per assignment, those without an expert empty
-        *tl = {g.ids[tile], tile, 1};
-        return (unsigned)tl->e < (unsigned)g.n_mat;
-    }
-    int one;
-    return Groups<false>(g).find(g, tile, 1, tl, &one);
-}
-
-// Place p's row of x, -1 where src has none.
-__device__ __forceinline__ int x_row(const HalfArgs& g, int p)
-{
-    if (!g.src) return g.ids ? p / g.div : p;
-    const int r = g.src[p];
-    return (unsigned)r < (unsigned)(g.n_x * g.div) ? r / g.div : -1;
-}
-
-// Tile place i's output row, in bytes from out_base (a tile's own rows, or a whole output that dst points into, lie within 2^32
-// bytes); NO_ROW where it has none.
-constexpr uint32_t NO_ROW = 0xFFFFFFFFu;
-__device__ __forceinline__ uint32_t out_row(const HalfArgs& g, const Tile& tl, int i)
-{
-    if (i >= tl.cnt || x_row(g, tl.start + i) < 0) return NO_ROW;
-    return (uint32_t)(g.dst ? g.dst[tl.start + i] : i) * (uint32_t)g.out_cols * (g.type == PHX_F32 ? 4u : 2u);
-}
-__device__ __forceinline__ char* out_base(const HalfArgs& g, const Tile& tl)
-{
-    return (char*)g.out + (g.dst ? 0 : (int64_t)tl.start * g.out_cols * (g.type == PHX_F32 ? 4 : 2));
-}
-
 // k_half_rows: for few rows per matrix, where the weights' bytes are the time.  A workgroup takes RT tiles of 16 weight rows
 // (PAIRED: of 16 channels, their gate and up rows) by a tile of up to 16 TT places, both straight from memory to registers:
 // its NW waves split the reduction, so no operand is wanted by two of them, and a matrix of few rows still has loads in
@@ -293,255 +151,6 @@ __global__ __launch_bounds__(64 * NW) void k_half_rows(HalfArgs g)
     else half_rows_product<NW, RT, CT < 2 ? 1 : 2, PAIRED, ONCE, BF>(g, tl, red, orow);
 }
 
-// k_half_tile: four waves, each 64 stored weight rows (PAIRED: the gate and up rows of 32 channels), by a tile of up to 256 places.
-// The weights go straight from memory to each wave's registers (the layout has every operand as one run of 1 KB, and no other wave
-// of the workgroup wants it), nearly two steps of 64 columns ahead; the places' rows, which all four waves read, go through an LDS
-// ring by direct loads three to five steps ahead, row-major runs of 128 bytes with the 16-byte chunks XOR-swizzled by half the row's number
-// (16 lanes of a 16-byte read then have 16 distinct bank groups).
-constexpr int TI_WAVE = 32 * (64 * 4 + 16);  // a wave's part of the ring in the epilogue: 32 places' rows of 64 floats
-// slots: as many steps as the ring holds, up to six (MT: the row tiles it is made for, 16 KB each)
-constexpr int ti_ring(int nt, int mt) { return std::min(mt * 4 / nt, 6); }
-
-template <int NT, int MT, bool PAIRED, bool ONCE, bool BF>
-__device__ __forceinline__ void half_tile_product(const HalfArgs& g, const Tile& tl, int bx, unsigned char* ring, uint32_t* orow)
-{
-    constexpr int STAGE = NT * 32 * 128, RING = ti_ring(NT, MT);
-    const int tid = threadIdx.x, lane = tid & 63, r32 = lane & 31, h = lane >> 5;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int S = g.kc / 8, row_bytes = g.cols * 2;
-    // this lane's rows of the direct loads: one per load, the last row again past the tile's end
-    const int chunk = ((lane & 7) ^ (lane >> 4)) * 16;  // of the loads whose first row is a multiple of 16; 4 chunks on for 8
-    const __amdgpu_buffer_rsrc_t rsrc = buf_rsrc(g.x + (g.src ? 0 : (int64_t)tl.start * g.cols));
-    uint32_t xr[NT];  // rows that src names lie within 2^32 bytes of x, a tile's own of its first
-#pragma unroll
-    for (int i = 0; i < NT; i++) {
-        const int at = min(8 * (wave * NT + i) + (lane >> 3), tl.cnt - 1);
-        xr[i] = (uint32_t)(g.src ? max(x_row(g, tl.start + at), 0) : at) * (uint32_t)row_bytes;
-    }
-    for (int i = tid; i < NT * 32; i += 256) orow[i] = out_row(g, tl, i);
-    int slot = 0;  // the ring's slot of a step; the one before it takes the rows of the step RING - 1 on
-    auto after = [&](int at) { return at == (RING - 1) * STAGE ? 0 : at + STAGE; };
-    auto before = [&](int at) { return at == 0 ? (RING - 1) * STAGE : at - STAGE; };
-    auto column = [&](int s, int i) { return s * 128 + (chunk ^ (64 * ((wave * NT + i) & 1))); };  // the lane's byte of load i's rows
-    auto dma = [&](int s, int to, auto I) {          // load I of step s's rows
-        constexpr int i = decltype(I)::value;
-        const int off = column(min(s, S - 1), i);
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void_t)(ring + to + (wave * NT + i) * 1024), 16,
-                                                 xr[i] + (off < row_bytes ? off : 0), 0, 0, 0);
-    };
-    // zeros where a last step's loads, landed, hold columns past the row: against zero weights an infinity is none
-    auto clear = [&](int s, int to) {
-        if (s != S - 1 || row_bytes == S * 128) return;  // uniform
-#pragma unroll
-        for (int i = 0; i < NT; i++)
-            if (column(s, i) >= row_bytes) *(uint4*)(ring + to + (wave * NT + i) * 1024 + lane * 16) = make_uint4(0u, 0u, 0u, 0u);
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    };
-    const int rg0 = (bx * 4 + wave) * 2, rgs = g.rgs;
-    const uint8_t* wb[2];
-#pragma unroll
-    for (int b = 0; b < 2; b++)
-        wb[b] = g.w + (int64_t)tl.e * g.mat_bytes + (int64_t)min(rg0 + b, rgs - 1) * g.kc * 512;
-    const uint32_t lane16 = lane * 16;
-    w4 wv[2][2][4];
-    auto weight = [&](int s, int b, auto P, auto KK) {
-        const uint8_t* at = wb[b] + (int64_t)min(s, S - 1) * 4096 + decltype(KK)::value * 1024;  // uniform
-        wv[decltype(P)::value][b][decltype(KK)::value] = load_weights<ONCE>(at + lane16);
-    };
-    f32x16 acc[NT][2];
-#pragma unroll
-    for (int j = 0; j < NT; j++)
-#pragma unroll
-        for (int b = 0; b < 2; b++)
-#pragma unroll
-            for (int v = 0; v < 16; v++) acc[j][b][v] = 0.0f;
-    const uint32_t lds = (uint32_t)(uintptr_t)(lds_void_t)ring + r32 * 128, swz = (h ^ ((r32 >> 1) & 7)) * 16;
-    u32x4 a[2][NT];
-    auto read = [&](int from, auto KK, auto J) {  // row tile J's columns of group KK
-        constexpr int kk = decltype(KK)::value, j = decltype(J)::value;
-        a[kk & 1][j] = ds_r128<j * 4096>(lds + from + (swz ^ (kk * 32)));
-    };
-    auto landed = [&](auto Q) {
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-#pragma unroll
-        for (int j = 0; j < NT; j++) tie(a[decltype(Q)::value][j]);
-    };
-    // A step is four groups of products on 16 columns.  Behind each of a group's first products goes a read of the next group's
-    // rows (the last group: of the next step's, once they have landed in every wave, which also says that nobody reads this step's
-    // slot any more): all at the group's start, the four waves' reads held up each other and the products behind them (8192 x
-    // 8192 x 8192 READS_AT_START us).  Behind the others go the loads: the weights that the group before has just used the
-    // registers of, two steps on, and the group's share of the rows RING - 1 steps on.  The order is fixed by scheduling barriers:
-    // the wait for the rows counts the loads issued after them.
-    constexpr int DPG = (NT + 3) / 4;                                     // direct loads of a group
-    constexpr int LAST = (NT - 1) / DPG, AFTER = 2 * (3 - LAST);          // the group of a step's last one, the weights after it
-    constexpr int NEWER = AFTER + (RING - 3) * (8 + NT) + 6 + (NT < 3 * DPG ? NT : 3 * DPG);
-    // the loads behind the first step's rows
-    constexpr int NEWER_AT_START = (RING - 2) * NT + 14;
-    static_assert(NEWER < 64 && NEWER_AT_START < 64 && RING > 3, "vmcnt's range, and the first step's rows before any weights");
-    auto step = [&](int s, auto P) {
-        constexpr int p = decltype(P)::value;
-        const int next = after(slot), far = before(slot);
-        static_for<4>([&](auto KK) {
-            constexpr int kk = decltype(KK)::value;
-            static_for<2 * NT>([&](auto M) {
-                constexpr int m = decltype(M)::value, j = m / 2, b = m % 2;
-                __builtin_amdgcn_sched_barrier(0);
-                acc[j][b] = mma32<BF>(wv[p][b][kk], a[kk & 1][j], acc[j][b]);
-                __builtin_amdgcn_sched_barrier(0);
-                if constexpr (m == 0 && kk == 3) {
-                    __builtin_amdgcn_s_waitcnt(vm_wait(NEWER));
-                    clear(s + 1, next);
-                    __builtin_amdgcn_s_barrier();
-                }
-                if constexpr (m < NT) read(kk < 3 ? slot : next, ic<(kk + 1) % 4>{}, ic<(m < NT ? m : 0)>{});
-                static_for<2 + DPG>([&](auto I) {
-                    constexpr int i = decltype(I)::value, d = kk * DPG + i - 2;
-                    if constexpr (m == NT + i * NT / (2 + DPG)) {
-                        if constexpr (i < 2 && kk == 0) weight(s + 1, i, ic<1 - p>{}, ic<3>{});
-                        else if constexpr (i < 2) weight(s + 2, i, ic<p>{}, ic<(kk + 3) % 4>{});
-                        else if constexpr (d < NT) dma(s + RING - 1, far, ic<d>{});
-                    }
-                });
-            });
-            __builtin_amdgcn_sched_barrier(0);
-            landed(ic<(kk + 1) & 1>{});
-        });
-        slot = next;
-    };
-    // The loads before the first step in the order of the steps that would have issued them: the waits for weights inside the loop
-    // hold for its first pass too, and in another order would have to count fewer loads ever after.
-    static_for<RING - 3>([&](auto R) {
-        static_for<NT>([&](auto I) { dma(decltype(R)::value, decltype(R)::value * STAGE, I); });
-    });
-    static_for<2>([&](auto P) {
-        constexpr int p = decltype(P)::value, r = RING - 3 + p;  // step p - 2, its rows those of step r
-        static_for<4>([&](auto KK) {
-            constexpr int kk = decltype(KK)::value;
-            __builtin_amdgcn_sched_barrier(0);
-            if constexpr (kk > 0) weight(p, 0, ic<p>{}, ic<(kk + 3) % 4>{}), weight(p, 1, ic<p>{}, ic<(kk + 3) % 4>{});
-            else if constexpr (p == 1) weight(0, 0, ic<0>{}, ic<3>{}), weight(0, 1, ic<0>{}, ic<3>{});
-            __builtin_amdgcn_sched_barrier(0);
-            static_for<DPG>([&](auto D) {
-                constexpr int d = kk * DPG + decltype(D)::value;
-                if constexpr (d < NT) dma(r, r * STAGE, ic<d>{});
-            });
-        });
-    });
-    __builtin_amdgcn_sched_barrier(0);
-    __builtin_amdgcn_s_waitcnt(vm_wait(NEWER_AT_START));
-    clear(0, slot);
-    __builtin_amdgcn_s_barrier();
-    static_for<NT>([&](auto J) { read(slot, ic<0>{}, J); });
-    landed(ic<0>{});
-    for (int s = 0; s + 1 < S; s += 2) {
-        step(s, ic<0>{});
-        step(s + 1, ic<1>{});
-    }
-    if (S & 1) step(S - 1, ic<0>{});
-    __builtin_amdgcn_s_waitcnt(0);  // the direct loads past the last step land before the workgroup's LDS goes
-    __syncthreads();
-    char* out = out_base(g, tl);
-    // A lane holds 16 consecutive channels of one place (twice, or gate and up).  Each 32 places' values go through the wave's own part
-    // of the ring as they are stored, so that an instruction stores whole runs of a place's row: 128 bytes where the lane alone
-    // has 32.  A row's 16 bytes more than its values keep 16 lanes of a write or read on distinct banks.
-    constexpr int WC = PAIRED ? 32 : 64;
-    unsigned char* mine = ring + wave * TI_WAVE;
-    const int col0 = PAIRED ? (rg0 >> 1) * 32 : rg0 * 32;
-    const bool bf = g.type == PHX_BF16;
-    auto store = [&](auto ESC, auto J) {
-        constexpr int j = decltype(J)::value, ES = decltype(ESC)::value, V = 16 / ES, LPT = WC / V, TPI = 64 / LPT, PITCH = WC * ES + 16;
-#pragma unroll
-        for (int b = 0; b < (PAIRED ? 1 : 2); b++)
-#pragma unroll
-            for (int i = 0; i < 16; i += V) {
-                float y[V];
-#pragma unroll
-                for (int v = 0; v < V; v++) y[v] = PAIRED ? gated_half(g.act, acc[j][0][i + v], acc[j][1][i + v]) : acc[j][b][i + v];
-                unsigned char* to = mine + r32 * PITCH + (32 * b + 16 * h + i) * ES;
-                if constexpr (ES == 4) *(float4*)to = make_float4(y[0], y[1], y[2], y[3]);
-                else {
-                    uint32_t u[4];
-#pragma unroll
-                    for (int v = 0; v < 4; v++) {
-                        const uint32_t as_bf = pair_of<PHX_BF16>(y[2 * v], y[2 * v + 1]), as_f16 = pair_of<PHX_F16>(y[2 * v], y[2 * v + 1]);
-                        u[v] = bf ? as_bf : as_f16;
-                    }
-                    *(uint4*)to = make_uint4(u[0], u[1], u[2], u[3]);
-                }
-            }
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-        const int c = (lane % LPT) * V, col = col0 + c;  // LPT lanes a place, TPI places a round
-        const bool whole = g.out_cols % V == 0;          // rows and columns then start on 16 bytes
-#pragma unroll
-        for (int it = 0; it < 32 / TPI; it++) {
-            const int tok = it * TPI + lane / LPT;
-            const uint32_t o = orow[32 * j + tok];
-            const uint4 y = *(const uint4*)(mine + tok * PITCH + c * ES);
-            if (o == NO_ROW) continue;
-            if (whole) {
-                if (col < g.out_cols) *(uint4*)(out + o + (int64_t)col * ES) = y;
-            } else {
-                const uint32_t u[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-                for (int i = 0; i < V; i++)
-                    if (col + i < g.out_cols) {
-                        if constexpr (ES == 4) *(uint32_t*)(out + o + (int64_t)(col + i) * 4) = u[i];
-                        else *(uint16_t*)(out + o + (int64_t)(col + i) * 2) = (uint16_t)(u[i >> 1] >> (16 * (i & 1)));
-                    }
-            }
-        }
-        // this tile's reads end before the next one's writes
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-        __builtin_amdgcn_sched_barrier(0);
-    };
-    if (g.type == PHX_F32) static_for<NT>([&](auto J) { store(ic<4>{}, J); });
-    else static_for<NT>([&](auto J) { store(ic<2>{}, J); });
-}
-
-// Workgroup L runs on XCD L % 8.  The items (a tile's block of 256 stored rows) are in the order of groups, blocks, tiles, and
-// each XCD takes an eighth of them as one run: a group's tiles meet a block's weights in one L2 at about one time, and the weights
-// leave memory once.
-template <int MT, bool PAIRED, bool ONCE, bool BF>
-__global__ __launch_bounds__(256, MT > 4 ? 1 : 2) void k_half_tile(HalfArgs g)
-{
-    __shared__ __align__(16) unsigned char ring[MT * 16 * 1024];
-    static_assert(sizeof(ring) >= 4 * TI_WAVE, "the epilogue's part of each wave");
-    __shared__ __align__(16) uint32_t orow[MT * 32];
-    const Groups<true> G(g);
-    const int blocks = (g.rgs + 7) / 8, all = G.total() * blocks, run = (all + 7) / 8, k = blockIdx.x >> 3;
-    const int item = (blockIdx.x & 7) * run + k;
-    Tile tl;
-    int bx;
-    if (k >= run || item >= all || !G.find(g, item, blocks, &tl, &bx)) return;  // uniform over the workgroup
-    // said once more, so that addresses stay in scalar registers: a buffer in vector ones costs a loop for each load
-    tl = {__builtin_amdgcn_readfirstlane(tl.e), __builtin_amdgcn_readfirstlane(tl.start), __builtin_amdgcn_readfirstlane(tl.cnt)};
-    bx = __builtin_amdgcn_readfirstlane(bx);
-    const int n = (tl.cnt + 31) / 32;
-    if constexpr (MT == 4) {
-        switch (n) {
-        case 1: half_tile_product<1, MT, PAIRED, ONCE, BF>(g, tl, bx, ring, orow); break;
-        case 2: half_tile_product<2, MT, PAIRED, ONCE, BF>(g, tl, bx, ring, orow); break;
-        case 3: half_tile_product<3, MT, PAIRED, ONCE, BF>(g, tl, bx, ring, orow); break;
-        default: half_tile_product<4, MT, PAIRED, ONCE, BF>(g, tl, bx, ring, orow);
-        }
-    } else {
-        switch (n) {
-        case 1: half_tile_product<1, MT, PAIRED, ONCE, BF>(g, tl, bx, ring, orow); break;
-        case 2: half_tile_product<2, MT, PAIRED, ONCE, BF>(g, tl, bx, ring, orow); break;
-        case 3: half_tile_product<3, MT, PAIRED, ONCE, BF>(g, tl, bx, ring, orow); break;
-        case 4: half_tile_product<4, MT, PAIRED, ONCE, BF>(g, tl, bx, ring, orow); break;
-        case 5: half_tile_product<5, MT, PAIRED, ONCE, BF>(g, tl, bx, ring, orow); break;
-        case 6: half_tile_product<6, MT, PAIRED, ONCE, BF>(g, tl, bx, ring, orow); break;
-        case 7: half_tile_product<7, MT, PAIRED, ONCE, BF>(g, tl, bx, ring, orow); break;
-        default: half_tile_product<8, MT, PAIRED, ONCE, BF>(g, tl, bx, ring, orow);
-        }
-    }
-}
-
 static void set_matrix(HalfArgs& g, const HalfMat& m)
 {
     g.w = m.w;
@@ -568,24 +177,14 @@ static void rows_by_pair(hipStream_t st, const HalfMat& m, const HalfArgs& g, in
     else half_rows<4, 4, CT, false, ONCE>(st, m, g, max_tiles);
 }
 
-template <int MT, bool PAIRED>
-static void half_tiles(hipStream_t st, const HalfMat& m, const HalfArgs& g, int max_tiles)
-{
-    const dim3 grid((max_tiles * ((m.rg + 7) / 8) + 7) / 8 * 8), blk(256);
-    if (m.type == PHX_BF16) launch(k_half_tile<MT, PAIRED, false, true>, grid, blk, 0, st, g);
-    else launch(k_half_tile<MT, PAIRED, false, false>, grid, blk, 0, st, g);
-}
-
 void launch_half_product(hipStream_t st, const HalfMat& m, HalfArgs g, int max_tiles)
 {
     set_matrix(g, m);
-    if (g.cap <= 16) rows_by_pair<1, false>(st, m, g, max_tiles);
+    if (g.cap <= 16 && g.once) rows_by_pair<1, true>(st, m, g, max_tiles);
+    else if (g.cap <= 16) rows_by_pair<1, false>(st, m, g, max_tiles);
+    else if (g.cap <= kHalfRows && g.once) rows_by_pair<2, true>(st, m, g, max_tiles);
     else if (g.cap <= kHalfRows) rows_by_pair<2, false>(st, m, g, max_tiles);
-    else if (g.cap <= kHalfNarrow) {
-        if (m.paired) half_tiles<4, true>(st, m, g, max_tiles);
-        else half_tiles<4, false>(st, m, g, max_tiles);
-    } else if (m.paired) half_tiles<8, true>(st, m, g, max_tiles);
-    else half_tiles<8, false>(st, m, g, max_tiles);
+    else launch_half_tiles(st, m, g, max_tiles);
 }
 
 // ------------------------------------------------------------------------------ experts
@@ -610,7 +209,7 @@ __global__ __launch_bounds__(64 * NW) void k_half_down_few(HalfArgs g, int k, co
         for (int s = 0; s < steps; s += U) {
             w4 w[U], x[U];
 #pragma unroll
-            for (int u = 0; u < U; u++) w[u] = *(const w4*)(wb + (int64_t)min(s + u, steps - 1) * 2048);
+            for (int u = 0; u < U; u++) w[u] = load_weights<false>(wb + (int64_t)min(s + u, steps - 1) * 2048);
 #pragma unroll
             for (int u = 0; u < U; u++) x[u] = *(const w4*)(row + min(32 * (s + u) + 8 * q, g.cols - 8));
 #pragma unroll

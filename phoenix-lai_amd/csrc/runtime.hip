@@ -2621,11 +2621,17 @@ int half_cap(phx_moe_ctx* c, const HalfMat& m, int n)
     return n > 192 * m.n_mat && (int64_t)(n / kHalfTile) * (m.rg / 8) >= 2 * c->ncu ? kHalfTile : kHalfNarrow;
 }
 
+// Whether the weights pass the caches by: more than the last cache keeps to the next call, and hardly a group of two tiles (us, through
+// the caches and past them; 96 places in 64 groups of 4096 x 1408 67, 60; 512 in 128 of 1408 x 2816 146, 134; 1120 there 179, 179;
+// 192 in 32 of 1408 x 2816 52, 48; 192 in 32 of 1024 x 1024 12.6, 13.9; one group of 16384 x 4096: 12 places 32, 28; 24 49, 50).
+bool half_once(const HalfMat& m, int n) { return m.n_mat * m.mat_bytes() > 128e6 && n <= std::max(8 * m.n_mat, 16); }
+
 // One product over n places.
 void half_product(phx_moe_ctx* c, const HalfMat& m, HalfArgs g, int n)
 {
     g.n = n;
     g.cap = half_cap(c, m, n);
+    g.once = half_once(m, n);
     launch_half_product(c->stream, m, g, most_tiles(n, m.n_mat, g.cap));
 }
 }  // namespace
@@ -2736,7 +2742,9 @@ int phx_experts_half(phx_moe_ctx* c, const phx_weight* gu, const phx_weight* dn,
     g.x = (const uint16_t*)x;
     g.act = act;
     // few assignments, most of them of an expert of their own: two launches without lists, which read an expert's matrices again
-    // for each of its assignments
+    // for each of its assignments (us, with and without lists; 128 of 2816, 704, eight a token: T = 1 29, 22; 4 67, 67; 8 93, 122;
+    // 32 of 4096, 2816, four a token: T = 1 63, 59; 2 102, 104; 4 147, 194; 16 of 1024, 512, two a token: T = 8 16.6, 11.8; 24 18.4,
+    // 17.7; 64 21.7, 34.7; 32 of them, four a token: T = 8 20.8, 14.9; 24 24.5, 28.0)
     const double each = 6.0 * nf * d, A0 = (double)T * k, again = A0 - E * (1.0 - pow(1.0 - 1.0 / E, A0));
     if (A0 <= 1024 && again * each <= (E * each <= 64e6 ? 144e6 : 48e6)) {
         if ((rc = i8_ensure(c, I8_H, (int64_t)T * k * nf, &h))) return rc;
@@ -2744,6 +2752,7 @@ int phx_experts_half(phx_moe_ctx* c, const phx_weight* gu, const phx_weight* dn,
         g.div = k;
         g.n_x = T;
         g.cap = 16;
+        g.once = half_once(gu->half, T * k);
         g.type = gu->type;
         g.out = h;
         launch_half_product(st, gu->half, g, T * k);
