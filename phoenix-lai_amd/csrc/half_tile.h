@@ -1,5 +1,7 @@
-// The tile kernel of products with fp16 and bf16 matrices in runs of ragged length.  In a file of its own: its sums need both halves
-// of the register file, for which the matrix instructions' results have to be left in accumulation registers.
+// The tile kernel of products with fp16 and bf16 matrices in runs of ragged length.  Built apart from the row kernel, since its sums
+// need both halves of the register file, for which the matrix instructions' results have to be left in accumulation registers,
+// and each type by itself, since the widths of a tile are many and long to compile.
+#pragma once
 #include <algorithm>
 
 #include "half_common.h"
@@ -255,21 +257,20 @@ __global__ __launch_bounds__(256, MT > 4 ? 1 : 2) void k_half_tile(HalfArgs g)
     }
 }
 
-template <int MT, bool PAIRED>
+template <int MT, bool PAIRED, bool BF>
 static void half_tiles(hipStream_t st, const HalfMat& m, const HalfArgs& g, int max_tiles)
 {
-    const dim3 grid((max_tiles * ((m.rg + 7) / 8) + 7) / 8 * 8), blk(256);
-    if (m.type == PHX_BF16) launch(k_half_tile<MT, PAIRED, true>, grid, blk, 0, st, g);
-    else launch(k_half_tile<MT, PAIRED, false>, grid, blk, 0, st, g);
+    const dim3 grid((max_tiles * ((m.rg + 7) / 8) + 7) / 8 * 8);
+    launch(k_half_tile<MT, PAIRED, BF>, grid, dim3(256), 0, st, g);
 }
 
+template <bool BF>
 void launch_half_tiles(hipStream_t st, const HalfMat& m, const HalfArgs& g, int max_tiles)
 {
-    if (g.cap <= kHalfNarrow) {
-        if (m.paired) half_tiles<4, true>(st, m, g, max_tiles);
-        else half_tiles<4, false>(st, m, g, max_tiles);
-    } else if (m.paired) half_tiles<8, true>(st, m, g, max_tiles);
-    else half_tiles<8, false>(st, m, g, max_tiles);
+    if (g.cap <= kHalfNarrow && m.paired) half_tiles<4, true, BF>(st, m, g, max_tiles);
+    else if (g.cap <= kHalfNarrow) half_tiles<4, false, BF>(st, m, g, max_tiles);
+    else if (m.paired) half_tiles<8, true, BF>(st, m, g, max_tiles);
+    else half_tiles<8, false, BF>(st, m, g, max_tiles);
 }
 
 }  // namespace phx

@@ -184,7 +184,8 @@ void launch_half_product(hipStream_t st, const HalfMat& m, HalfArgs g, int max_t
     else if (g.cap <= 16) rows_by_pair<1, false>(st, m, g, max_tiles);
     else if (g.cap <= kHalfRows && g.once) rows_by_pair<2, true>(st, m, g, max_tiles);
     else if (g.cap <= kHalfRows) rows_by_pair<2, false>(st, m, g, max_tiles);
-    else launch_half_tiles(st, m, g, max_tiles);
+    else if (m.type == PHX_BF16) launch_half_tiles<true>(st, m, g, max_tiles);
+    else launch_half_tiles<false>(st, m, g, max_tiles);
 }
 
 // ------------------------------------------------------------------------------ experts

@@ -194,8 +194,10 @@ __global__ __launch_bounds__(64 * NW) void k_lora_down(LoraSlots L, int T, const
     }
 }
 
-// the slots of a tile side by side where the rows are few, else one after another
-static bool few_rows(int T) { return T <= 256; }
+// The slots of a tile side by side where the rows are few, else one after another with weights held and more rows in flight (us, side
+// by side and one after another; 4096 x 4096, eight adapters of rank 16, rows of one request in runs of 100: T = 512 13.7, 17.2; 1024
+// 19.4, 18.4; each row another request than the last: 512 20, 44; 1000 30, 45; 2000 53, 50; rank 128: 500 94, 105; 1000 140, 114).
+static bool few_rows(const LoraSlots& L, int T) { return T <= (L.rt <= 2 ? 1024 : 512); }
 
 template <int NW, int RT, bool FEW, bool BF>
 static void lora_down(hipStream_t st, const LoraSlots& L, int T, const uint16_t* x, const int* ids, int terms, uint16_t* low, int* exps)
@@ -209,7 +211,7 @@ template <bool BF>
 static void lora_down_type(hipStream_t st, const LoraSlots& L, int T, const uint16_t* x, const int* ids, int terms, uint16_t* low,
                            int* exps)
 {
-    if (few_rows(T)) lora_down<16, 1, true, BF>(st, L, T, x, ids, terms, low, exps);
+    if (few_rows(L, T)) lora_down<16, 1, true, BF>(st, L, T, x, ids, terms, low, exps);
     else if (L.rt == 1) lora_down<8, 1, false, BF>(st, L, T, x, ids, terms, low, exps);
     else lora_down<8, 2, false, BF>(st, L, T, x, ids, terms, low, exps);
 }
@@ -331,7 +333,7 @@ static void lora_up(hipStream_t st, const LoraSlots& L, int T, const int* ids, c
                     const void* y_in, void* y)
 {
     const dim3 blk(256);
-    if (few_rows(T)) {
+    if (few_rows(L, T)) {
         const dim3 grid((T + 15) / 16, (L.groups + 3) / 4, std::min(T, 16));
         launch(k_lora_up<DT, RM, 1, true, BF>, grid, blk, 0, st, L, T, ids, low, exps, ld, y_in, y);
     } else {

@@ -334,7 +334,7 @@ void launch_i8_lists(hipStream_t st, int n, int E, int cap, const int* ids, int*
 void launch_i8_combine(hipStream_t st, int T, int d, int k, int E, const float* y, const int* ids, const float* w, int out_type,
                        void* out);
 
-// ---- float experts, adapters, the residual's norm (kernels_half.hip, kernels_half_tile.hip, kernels_lora.hip, kernels_add_norm.hip)
+// ---- float experts, adapters, the residual's norm (kernels_half.hip, half_tile.h, kernels_lora.hip, kernels_add_norm.hip)
 // fp16 or bf16 matrices on the device, laid out by bytes as I8Mat: groups of 32 stored rows, each [kc][32 rows][16 bytes] with
 // kc = columns / 8, padded to whole steps of 64 columns with zeros; paired, group 2 g holds gate rows 32 g .. + 31 and
 // group 2 g + 1 the up rows of the same channels.  Within a group the rows are in the order of the matrix product's results
@@ -365,6 +365,7 @@ struct HalfArgs {
 };
 constexpr int kHalfRows = 32, kHalfNarrow = 128, kHalfTile = 256;  // places a tile: the row kernel's (16 or 32), the tile kernel's two
 void launch_half_product(hipStream_t st, const HalfMat& m, HalfArgs g, int max_tiles);
+template <bool BF>
 void launch_half_tiles(hipStream_t st, const HalfMat& m, const HalfArgs& g, int max_tiles);  // its tile kernel, g's matrix set
 // the down products of T tokens' k places from h [T k][cols], and their weighted sums as out [T][rows]
 void launch_half_down_few(hipStream_t st, const HalfMat& m, int T, int k, const uint16_t* h, const int* ids, const float* weights,

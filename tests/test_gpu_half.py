@@ -201,6 +201,15 @@ def test_upload_from_device_and_unaligned(ctx):
     np.testing.assert_array_equal(got[0], got[2])
 
 
+@pytest.mark.parametrize("n,paired", [(9, False), (16, True), (17, False), (70, False), (72, True), (73, False)])
+def test_weights_past_the_caches(ctx, n, paired):
+    """Matrices of more than 128 MB, few places a group: the row kernel's loads that pass the caches by, and the sizes beside them."""
+    def alter(raw_x, x, raw_w, w):  # the same values from matrix to matrix, in other places
+        for e in range(1, len(w)):
+            raw_w[e], w[e] = np.roll(raw_w[0], e, 1), np.roll(w[0], e, 1)
+    check(ctx, 30, 0, 9, n, 4096, 1800, act=1 if paired else 0, alter=alter)
+
+
 def test_same_call_same_bits(ctx):
     """A call's result does not depend on timing, nor on the calls beside it."""
     rng = np.random.default_rng(5)
@@ -389,6 +398,12 @@ def test_host_forms_refuse_sizes_that_are_not_the_handles(ctx, pkg):
                 ctx.MatMulGrouped(h, 0, np.array(at), x)
     finally:
         ctx.weight_free(h)
+
+
+def test_experts_past_the_caches(ctx):
+    """One token's experts, and a decode step's, of matrices of more than 128 MB."""
+    for T in (1, 12):
+        check_experts(ctx, 30, 0, 1, T, 4, 20, 1024, 1704)
 
 
 @pytest.mark.parametrize("n,what", enumerate(("the weight", "offsets", "x", "y", "src"), 1))

@@ -106,6 +106,29 @@ def test_many_slots(ctx):
     check(ctx, 1, 1, 256, 40, 64, 4, {s: 1 + s % 4 for s in range(0, 255)}, ids)
 
 
+@pytest.mark.parametrize("type_,y_type", [(1, 0), (30, 30)])
+@pytest.mark.parametrize("rank,T", [(16, 1023), (16, 1024), (16, 1025), (32, 1100), (33, 512), (40, 513), (128, 600)])
+def test_many_rows_of_mixed_slots(ctx, rank, T, type_, y_type):
+    """About the sizes where the slots of a tile go one after another in place of side by side; every tile of many slots."""
+    ids = np.random.default_rng(rank + T).integers(-1, 5, T)
+    check(ctx, type_, y_type, T, 136, 72, rank, {0: rank, 2: rank - 1, 3: 1, 4: min(rank, 17)}, ids, in_place=T % 2 == 0)
+
+
+@pytest.mark.parametrize("T", [9, 700, 1100])
+def test_same_call_same_bits(ctx, T):
+    rng = np.random.default_rng(T)
+    h, _ = adapters(ctx, rng, 30, 4, 24, 520, 1024, {0: 24, 1: 3, 2: 16})
+    raw_x, _ = ref.held(rng.standard_normal((T, 1024)), 30)
+    raw_y, _ = ref.held(rng.standard_normal((T, 520)), 30)
+    ids = rng.integers(-1, 4, T)
+    try:
+        first = run(ctx, h, T, raw_x, ids, 30, 520, 520, raw_y)
+        for _ in range(3):
+            np.testing.assert_array_equal(run(ctx, h, T, raw_x, ids, 30, 520, 520, raw_y), first)
+    finally:
+        ctx.lora_free(h)
+
+
 def test_long_batch(ctx):
     """More rows than one chunk of the workspace takes."""
     check(ctx, 30, 30, 70001, 8, 8, 3, {0: 3, 1: 2}, np.arange(70001) // 5 % 3)
