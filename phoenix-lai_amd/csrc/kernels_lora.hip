@@ -268,9 +268,11 @@ __global__ __launch_bounds__(256) void k_lora_up(LoraSlots L, int T, const int* 
                 tiles = (L.rank[slot] + 15) / 16;
                 const uint8_t* b = L.b + slot * L.b_bytes() + (int64_t)grp * L.rt * 2048 + (q & 1) * 256 + r16 * 16;
 #pragma unroll
-                for (int r = 0; r < RM; r++)
+                for (int r = 0; r < RM; r++) {
+                    if (r > 0 && r >= tiles) break;  // the first while the rank is on its way
 #pragma unroll
-                    for (int m = 0; m < 4; m++) bv[r][m] = *(const w4*)(b + min(r, L.rt - 1) * 2048 + m * 512);
+                    for (int m = 0; m < 4; m++) bv[r][m] = *(const w4*)(b + r * 2048 + m * 512);
+                }
             }
             const int n = slot >= 0 ? tiles : 0;
             if (n > 0 || y_in != y) mine |= rows;
