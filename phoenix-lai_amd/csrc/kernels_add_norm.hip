@@ -35,32 +35,42 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_add_norm_i8(int rows, i
                                                                      float* __restrict__ d)
 {
     constexpr int RPB = NT < 256 ? 256 / NT : 1, NW = NT / 64;
+    constexpr bool EARLY = STEPS * NT <= 2048;
     __shared__ double red[NW];
     __shared__ unsigned redu[NW];
     const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / NT;
     if (NT == 64 && row >= rows) return;  // a whole wave, and no barrier with one wave a row
     const int tid = threadIdx.x % NT, lane = tid & 63, wave = tid >> 6;
-    float v[STEPS][8], b[STEPS][8];
-#pragma unroll
-    for (int s = 0; s < STEPS; s++) {
-        const int i = (s * NT + tid) * 8;
-#pragma unroll
-        for (int j = 0; j < 8; j++) v[s][j] = b[s][j] = 0.0f;
-        if (i < n) {
-            load_eight<DT>(x, row * n + i, v[s]);
-            load_eight<DT>(branch, row * ld + i, b[s]);
-        }
-    }
+    float v[STEPS][8];
+    float a[STEPS][8];  // the norm's weights on their way while the row is summed, where registers hold them
     double sq = 0.0;
+    constexpr int AT = STEPS < 4 ? STEPS : 4;  // steps whose loads are in flight together: all eight would spill
 #pragma unroll
-    for (int s = 0; s < STEPS; s++) {
-        const int i = (s * NT + tid) * 8;
+    for (int s0 = 0; s0 < STEPS; s0 += AT) {
+        float b[AT][8];
 #pragma unroll
-        for (int j = 0; j < 8; j++) v[s][j] = held<DT>(v[s][j] + b[s][j]);
-        if (i < n) {
-            store_eight<DT>(sum, row * n + i, v[s]);
+        for (int s = s0; s < s0 + AT; s++) {
+            const int i = (s * NT + tid) * 8;
 #pragma unroll
-            for (int j = 0; j < 8; j++) sq += (double)v[s][j] * (double)v[s][j];
+            for (int j = 0; j < 8; j++) v[s][j] = b[s - s0][j] = 0.0f;
+            if (i < n) {
+                load_eight<DT>(x, row * n + i, v[s]);
+                load_eight<DT>(branch, row * ld + i, b[s - s0]);
+            }
+        }
+        if (EARLY)
+#pragma unroll
+            for (int s = 0; s < STEPS; s++) load_eight<PHX_F32>(w, min((s * NT + tid) * 8, n - 8), a[s]);
+#pragma unroll
+        for (int s = s0; s < s0 + AT; s++) {
+            const int i = (s * NT + tid) * 8;
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[s][j] = held<DT>(v[s][j] + b[s - s0][j]);
+            if (i < n) {
+                store_eight<DT>(sum, row * n + i, v[s]);
+#pragma unroll
+                for (int j = 0; j < 8; j++) sq += (double)v[s][j] * (double)v[s][j];
+            }
         }
     }
     sq = wave_sum_dpp(sq);
@@ -76,11 +86,10 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_add_norm_i8(int rows, i
     for (int s = 0; s < STEPS; s++) {
         const int i = (s * NT + tid) * 8;
         if (i >= n) continue;
-        float a[8];
-        load_eight<PHX_F32>(w, i, a);
+        if (!EARLY) load_eight<PHX_F32>(w, i, a[s]);
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            v[s][j] = v[s][j] * scale * a[j];
+            v[s][j] = v[s][j] * scale * a[s][j];
             am = max(am, __float_as_uint(v[s][j]) & 0x7FFFFFFFu);
         }
     }
@@ -125,6 +134,8 @@ static void add_norm_type(hipStream_t st, const AddNormArgs& a)
     else if (a.n <= 2048 && a.rows >= 1024) add_norm_as<64, 4, DT>(st, a);
     else if (a.n <= 4096) add_norm_as<256, 2, DT>(st, a);
     else if (a.n <= 8192) add_norm_as<512, 2, DT>(st, a);
+    else if (a.n <= 16384) add_norm_as<1024, 2, DT>(st, a);  // the last one's threads and values, and fewer registers
+    else if (a.n <= 32768) add_norm_as<1024, 4, DT>(st, a);
     else add_norm_as<1024, 8, DT>(st, a);
 }
 

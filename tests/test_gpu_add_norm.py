@@ -59,6 +59,12 @@ def test_rows(ctx, n, type_, out_type):
     check(ctx, 3, n, type_, out_type, in_place=True)
 
 
+@pytest.mark.parametrize("n", [16384, 16416, 32768, 32800, 65504, 65536])
+def test_long_rows(ctx, n):
+    check(ctx, 4, n, 30, 0, extra=8)
+    check(ctx, 2, n, 0, 1, in_place=True)
+
+
 @pytest.mark.parametrize("rows,n", [(1, 2816), (1200, 1088), (70001, 32), (1 << 20, 32)])
 def test_many_rows(ctx, rows, n):
     check(ctx, rows, n, 30, 30, in_place=True)
