@@ -8,11 +8,16 @@
 
 namespace phx {
 
-// k_half_tile: four waves, each 64 stored weight rows (PAIRED: the gate and up rows of 32 channels), by a tile of up to 256 places.
+// k_half_tile: four waves, each 64 stored weight rows (PAIRED: the gate and up rows of 32 channels), by a tile of up to 256 places with
+// one workgroup a compute unit, all of whose registers hold sums, or of up to 128 with two (MT 8 and 4: the row tiles of 32 it holds).
 // The weights go straight from memory to each wave's registers (the layout has every operand as one run of 1 KB, and no other wave
 // of the workgroup wants it), nearly two steps of 64 columns ahead; the places' rows, which all four waves read, go through an LDS
 // ring by direct loads three to five steps ahead, row-major runs of 128 bytes with the 16-byte chunks XOR-swizzled by half the row's number
 // (16 lanes of a 16-byte read then have 16 distinct bank groups).
+// Measured: one 8192 x 8192 matrix by 8192 places 840 us, 1.31 PF (a library product 757), the matrix cores busy in 76% of the cycles: the
+// last round and the epilogue of 8 us a tile are the rest.  16384 places in 128 uneven groups of 1408 x 2816 250 us at 5.8 TB/s: 1.46 GB read
+// for 1.02 GB, since a group's second tile finds only a third of the weights still in the L2.  Few items are bound by whole rounds:
+// 16412 places in 32 groups of 2816 x 4096 380 us, 1.0 PF, 918 items on 256 compute units.
 constexpr int TI_WAVE = 32 * (64 * 4 + 16);  // a wave's part of the ring in the epilogue: 32 places' rows of 64 floats
 // slots: as many steps as the ring holds, up to six (MT: the row tiles it is made for, 16 KB each)
 constexpr int ti_ring(int nt, int mt) { return std::min(mt * 4 / nt, 6); }
@@ -84,8 +89,9 @@ __device__ __forceinline__ void half_tile_product(const HalfArgs& g, const Tile&
     // A step is four groups of products on 16 columns.  Behind each of a group's first products goes a read of the next group's
     // rows (the last group: of the next step's, once they have landed in every wave, which also says that nobody reads this step's
     // slot any more): all at the group's start, the four waves' reads held up each other and the products behind them (an 8192 x
-    // 8192 matrix by 8192 places, before the buffers were in scalar registers: 952 us, among the products 928).  Behind the others go the loads: the weights that the group before has just used the
-    // registers of, two steps on, and the group's share of the rows RING - 1 steps on.  The order is fixed by scheduling barriers:
+    // 8192 matrix by 8192 places, before the buffers were in scalar registers: 952 us, among the products 928).  Behind the others go
+    // the loads: the weights that the group before has just used the registers of, two steps on, and the group's share of the rows
+    // RING - 1 steps on.  The order is fixed by scheduling barriers:
     // the wait for the rows counts the loads issued after them.
     constexpr int DPG = (NT + 3) / 4;                                     // direct loads of a group
     constexpr int LAST = (NT - 1) / DPG, AFTER = 2 * (3 - LAST);          // the group of a step's last one, the weights after it

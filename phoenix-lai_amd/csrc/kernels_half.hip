@@ -170,10 +170,16 @@ static void half_rows(hipStream_t st, const HalfMat& m, const HalfArgs& g, int m
     else launch(k_half_rows<NW, RT, CT, PAIRED, ONCE, false>, grid, blk, 0, st, g);
 }
 
+// Four waves and 32 channels or 64 outputs; plain matrices with at most a workgroup a compute unit then, eight waves and 32 outputs (us, four
+// waves with 64 outputs, with 32, eight with 64, with 32; 96 places in 64 groups of 4096 x 1408: 60, 68, 80, 80; one matrix of 4096 x
+// 4096: 1 place 10.4, 9.3, 10.4, 8.9; 16 places 12.9, 10.7, 12.4, 10.2; 128 places 17.5, 23.5, 18.1, 23.5; 16384 x 4096, 12 places 29,
+// 28, 28, 27; paired, of 32 or 16 channels: 512 places in 128 groups of 1408 x 2816 134, 139, 135, 155; 192 in 32 of 1024 x 1024 12.9,
+// 13.4, 14.1, 15.2).
 template <int CT, bool ONCE>
 static void rows_by_pair(hipStream_t st, const HalfMat& m, const HalfArgs& g, int max_tiles)
 {
     if (m.paired) half_rows<4, 2, CT, true, ONCE>(st, m, g, max_tiles);
+    else if (CT == 1 && max_tiles * ((m.rg + 1) / 2) <= 256) half_rows<8, 2, 1, false, ONCE>(st, m, g, max_tiles);
     else half_rows<4, 4, CT, false, ONCE>(st, m, g, max_tiles);
 }
 
@@ -191,7 +197,7 @@ void launch_half_product(hipStream_t st, const HalfMat& m, HalfArgs g, int max_t
 // ------------------------------------------------------------------------------ experts
 // The down products of few assignments and their weighted sum, for a token (blockIdx.y) and 16 of its outputs: wave w takes
 // the token's places w, w + NW, ..., and the places' values meet in LDS in order.  No lists and no partial outputs go through
-// memory.
+// memory.  One token's eight experts of 2816 x 704 take 7.2 us (a launch 3.4, two dependent trips to memory).
 template <int NW, bool BF>
 __global__ __launch_bounds__(64 * NW) void k_half_down_few(HalfArgs g, int k, const float* __restrict__ weights)
 {

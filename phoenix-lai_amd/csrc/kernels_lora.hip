@@ -102,7 +102,8 @@ __device__ __forceinline__ void split(float v, uint16_t (&t)[TERMS])
 // A workgroup takes 16 rows (x) and RT rank tiles of 16 (z), FEW: for the slot of row y of them alone; its NW waves split the
 // reduction, all of a wave's loads in flight at once for rows of up to NW U steps, and their sums meet in LDS, added in the waves'
 // order.  low [T][rt][TERMS][16 ranks]; fp16's terms are of the value over 2^exps
-// [T][rt], which brings a row's 16 to below 2, so that none leaves the type's range.
+// [T][rt], which brings a row's 16 to below 2, so that none leaves the type's range.  One row of 4096, rank 16: 4.9 us, a launch and two
+// dependent trips to memory; 4096 rows, rank 32: 17.4, the rows' 34 MB in 6 and the trips of a workgroup a compute unit behind each other.
 template <int NW, int RT, int TERMS, bool FEW, bool BF>
 __global__ __launch_bounds__(64 * NW) void k_lora_down(LoraSlots L, int T, const uint16_t* __restrict__ x,
                                                        const int* __restrict__ ids, uint16_t* __restrict__ low,
@@ -227,7 +228,8 @@ void launch_lora_down(hipStream_t st, const LoraSlots& L, int T, const uint16_t*
 // columns are 16 ranks twice: lanes 0 - 31 bring a value's first term, lanes 32 - 63 its second, B's ranks the same for both; for
 // float rows a second instruction takes the third and the fourth.  Weights are the first operand, so that a lane's sums are 16
 // consecutive outputs of one row; they stay in registers from tile to tile while the slot does (RM: the rank tiles there can be).
-// All tiles' ids and rows are loaded before the first is waited for.
+// All tiles' ids and rows are loaded before the first is waited for.  One row, 4096 outputs: 3.6 us; 67 rows of as many adapters of ranks to
+// 64, 4224 float outputs: 9.9, B read once a tile and slot (20 MB from the caches); 4096 rows of 5632: 27, 92 MB read and written, 3.4 TB/s.
 template <int DT, int RM, int TT, bool FEW, bool BF>
 __global__ __launch_bounds__(256) void k_lora_up(LoraSlots L, int T, const int* __restrict__ ids, const uint16_t* __restrict__ low,
                                                  const int* __restrict__ exps, int64_t ld, const void* y_in, void* y)
