@@ -452,8 +452,9 @@ int phx_experts_half(phx_moe_ctx* ctx, const phx_weight* gate_up, const phx_weig
 /* Low-rank adapters of one projection (rows x cols): n_slot slots (<= PHX_MAX_ADAPTERS), each empty or an adapter of rank
  * up to max_rank (<= PHX_MAX_RANK): A [rank][cols], B [rows][rank] of `type` (PHX_F16 or PHX_BF16), and a scale.  cols a
  * multiple of 8, at most PHX_MAX_COLS_I8; rows at most PHX_MAX_ROWS_I8; all slots are allocated at once, empty.  phx_lora_set
- * puts an adapter into a slot (a and b host or device memory, 2-byte aligned, read before the call returns; calls enqueued
- * earlier see the slot as it was); rank 0 empties it (a and b unused).  The scale is finite. */
+ * puts an adapter into a slot (a and b host or device memory, 2-byte aligned, read before the call returns; this context's calls
+ * enqueued earlier see the slot as it was, while those of another context that uses the handle have to be done); rank 0 empties
+ * it (a and b unused).  The scale is finite. */
 #define PHX_MAX_ADAPTERS 256
 #define PHX_MAX_RANK 128
 typedef struct phx_lora phx_lora;

@@ -47,6 +47,14 @@ __device__ __forceinline__ void store_as(int type, void* p, int64_t i, float v)
     else store_one<PHX_F16>(p, i, v);
 }
 
+// 16 bytes of weights; ONCE: no other workgroup reads them, so they need not stay in the caches
+template <bool ONCE>
+__device__ __forceinline__ w4 load_weights(const uint8_t* p)
+{
+    if constexpr (ONCE) return __builtin_nontemporal_load((const w4*)p);
+    else return *(const w4*)p;
+}
+
 // The row of its group of 32 that is stored at slot s: what a lane holds of a 32 x 32 product, slots 8 g + 4 h + 0 .. 3 for
 // half h, are then 16 consecutive rows.
 __device__ __forceinline__ int slot_row(int s) { return 16 * ((s >> 2) & 1) + 4 * (s >> 3) + (s & 3); }
@@ -82,8 +90,9 @@ struct Groups {
         first = wave_incl_scan_i(sum) - sum;
     }
     __device__ __forceinline__ int total() const { return __builtin_amdgcn_readlane(first + sum, 63); }
-    // Item `item` of `per` items a tile, a group's tiles following each other for each of its items: the tile, and which item.
-    __device__ __forceinline__ bool find(const HalfArgs& g, int item, int per, Tile* tl, int* which) const
+    // Item `item` of `per` items a tile, a group's tiles following each other for each of its items: the tile, which item, and whether the
+    // group has no other tile.
+    __device__ __forceinline__ bool find(const HalfArgs& g, int item, int per, Tile* tl, int* which, bool* alone) const
     {
         const unsigned long long here = __ballot(item >= first * per && item < (first + sum) * per);
         if (!here) return false;
@@ -110,6 +119,7 @@ struct Groups {
         tl->start = start + __builtin_amdgcn_readlane(tile, l) * size;
         tl->cnt = min(end - tl->start, size);
         *which = __builtin_amdgcn_readlane(w, l);
+        *alone = n == 1;
         return true;
     }
 };
@@ -122,7 +132,8 @@ __device__ __forceinline__ bool half_tile(const HalfArgs& g, int tile, Tile* tl)
         return (unsigned)tl->e < (unsigned)g.n_mat;
     }
     int one;
-    return Groups<false>(g).find(g, tile, 1, tl, &one);
+    bool alone;
+    return Groups<false>(g).find(g, tile, 1, tl, &one, &alone);
 }
 
 // Place p's row of x, -1 where src has none.

@@ -22,7 +22,7 @@ constexpr int TI_WAVE = 32 * (64 * 4 + 16);  // a wave's part of the ring in the
 // slots: as many steps as the ring holds, up to six (MT: the row tiles it is made for, 16 KB each)
 constexpr int ti_ring(int nt, int mt) { return std::min(mt * 4 / nt, 6); }
 
-template <int NT, int MT, bool PAIRED, bool BF>
+template <int NT, int MT, bool PAIRED, bool ONCE, bool BF>
 __device__ __forceinline__ void half_tile_product(const HalfArgs& g, const Tile& tl, int bx, unsigned char* ring, uint32_t* orow)
 {
     constexpr int STAGE = NT * 32 * 128, RING = ti_ring(NT, MT);
@@ -66,7 +66,7 @@ __device__ __forceinline__ void half_tile_product(const HalfArgs& g, const Tile&
     w4 wv[2][2][4];
     auto weight = [&](int s, int b, auto P, auto KK) {
         const uint8_t* at = wb[b] + (int64_t)min(s, S - 1) * 4096 + decltype(KK)::value * 1024;  // uniform
-        wv[decltype(P)::value][b][decltype(KK)::value] = *(const w4*)(at + lane16);
+        wv[decltype(P)::value][b][decltype(KK)::value] = load_weights<ONCE>(at + lane16);
     };
     f32x16 acc[NT][2];
 #pragma unroll
@@ -237,28 +237,36 @@ __global__ __launch_bounds__(256, MT > 4 ? 1 : 2) void k_half_tile(HalfArgs g)
     const int item = (blockIdx.x & 7) * run + k;
     Tile tl;
     int bx;
-    if (k >= run || item >= all || !G.find(g, item, blocks, &tl, &bx)) return;  // uniform over the workgroup
+    bool alone;
+    if (k >= run || item >= all || !G.find(g, item, blocks, &tl, &bx, &alone)) return;  // uniform over the workgroup
     // said once more, so that addresses stay in scalar registers: a buffer in vector ones costs a loop for each load
     tl = {__builtin_amdgcn_readfirstlane(tl.e), __builtin_amdgcn_readfirstlane(tl.start), __builtin_amdgcn_readfirstlane(tl.cnt)};
     bx = __builtin_amdgcn_readfirstlane(bx);
     const int n = (tl.cnt + 31) / 32;
     if constexpr (MT == 4) {
-        switch (n) {
-        case 1: half_tile_product<1, MT, PAIRED, BF>(g, tl, bx, ring, orow); break;
-        case 2: half_tile_product<2, MT, PAIRED, BF>(g, tl, bx, ring, orow); break;
-        case 3: half_tile_product<3, MT, PAIRED, BF>(g, tl, bx, ring, orow); break;
-        default: half_tile_product<4, MT, PAIRED, BF>(g, tl, bx, ring, orow);
+        // a group's only tile reads its weights alone: past the caches, where the call's are more than they keep to the next (us,
+        // through and past them; places in 128 groups of 1408 x 2816: 1624 170, 154; 4000 212, 193; 8000 214, 206; 16384 255, 252;
+        // 4000 in 64 of 4096 x 1408 168, 173; past them for every tile, 16384 places: 295)
+        switch (g.once && alone ? n + 4 : n) {
+        case 1: half_tile_product<1, MT, PAIRED, false, BF>(g, tl, bx, ring, orow); break;
+        case 2: half_tile_product<2, MT, PAIRED, false, BF>(g, tl, bx, ring, orow); break;
+        case 3: half_tile_product<3, MT, PAIRED, false, BF>(g, tl, bx, ring, orow); break;
+        case 4: half_tile_product<4, MT, PAIRED, false, BF>(g, tl, bx, ring, orow); break;
+        case 5: half_tile_product<1, MT, PAIRED, true, BF>(g, tl, bx, ring, orow); break;
+        case 6: half_tile_product<2, MT, PAIRED, true, BF>(g, tl, bx, ring, orow); break;
+        case 7: half_tile_product<3, MT, PAIRED, true, BF>(g, tl, bx, ring, orow); break;
+        default: half_tile_product<4, MT, PAIRED, true, BF>(g, tl, bx, ring, orow);
         }
     } else {
         switch (n) {
-        case 1: half_tile_product<1, MT, PAIRED, BF>(g, tl, bx, ring, orow); break;
-        case 2: half_tile_product<2, MT, PAIRED, BF>(g, tl, bx, ring, orow); break;
-        case 3: half_tile_product<3, MT, PAIRED, BF>(g, tl, bx, ring, orow); break;
-        case 4: half_tile_product<4, MT, PAIRED, BF>(g, tl, bx, ring, orow); break;
-        case 5: half_tile_product<5, MT, PAIRED, BF>(g, tl, bx, ring, orow); break;
-        case 6: half_tile_product<6, MT, PAIRED, BF>(g, tl, bx, ring, orow); break;
-        case 7: half_tile_product<7, MT, PAIRED, BF>(g, tl, bx, ring, orow); break;
-        default: half_tile_product<8, MT, PAIRED, BF>(g, tl, bx, ring, orow);
+        case 1: half_tile_product<1, MT, PAIRED, false, BF>(g, tl, bx, ring, orow); break;
+        case 2: half_tile_product<2, MT, PAIRED, false, BF>(g, tl, bx, ring, orow); break;
+        case 3: half_tile_product<3, MT, PAIRED, false, BF>(g, tl, bx, ring, orow); break;
+        case 4: half_tile_product<4, MT, PAIRED, false, BF>(g, tl, bx, ring, orow); break;
+        case 5: half_tile_product<5, MT, PAIRED, false, BF>(g, tl, bx, ring, orow); break;
+        case 6: half_tile_product<6, MT, PAIRED, false, BF>(g, tl, bx, ring, orow); break;
+        case 7: half_tile_product<7, MT, PAIRED, false, BF>(g, tl, bx, ring, orow); break;
+        default: half_tile_product<8, MT, PAIRED, false, BF>(g, tl, bx, ring, orow);
         }
     }
 }

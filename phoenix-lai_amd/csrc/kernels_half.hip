@@ -7,14 +7,6 @@
 
 namespace phx {
 
-// 16 bytes of weights; ONCE: no other workgroup reads them, so they need not stay in the caches
-template <bool ONCE>
-__device__ __forceinline__ w4 load_weights(const uint8_t* p)
-{
-    if constexpr (ONCE) return __builtin_nontemporal_load((const w4*)p);
-    else return *(const w4*)p;
-}
-
 // ------------------------------------------------------------------------------ weights
 // HalfMat's layout from matrices as the caller holds them: a thread writes 8 columns of one stored row, zeros past the
 // last row or column.

@@ -356,7 +356,7 @@ struct HalfArgs {
     const uint16_t* x = nullptr;
     const int *src = nullptr, *dst = nullptr, *offsets = nullptr, *ids = nullptr;
     int n = 0, n_x = 0, div = 1, cap = 0, act = 0, type = 0;  // type: the output's
-    bool once = false;  // the row kernel's: weights that nobody reads again soon (load_weights)
+    bool once = false;  // weights that nobody reads again soon: all of the row kernel's, the tile kernel's of groups with one tile
     void* out = nullptr;
     // set by launch_half_product from the matrix
     const uint8_t* w;

@@ -2606,18 +2606,18 @@ bool half_type(int type) { return type == PHX_F16 || type == PHX_BF16; }
 int most_tiles(int n, int n_mat, int cap) { return n / cap + std::min(n, n_mat); }
 
 // The kernel of a product over n places, by its tiles' capacity.
-// Row kernel to 10 places a group, and where its workgroups number under three per compute unit (us, row kernel and tile kernel; 128
-// groups of 1408 x 2816: 8.8 places 157, 157; 12.7 167, 164; 64 of 4096 x 1408: 6.3 109, 114; 15 137, 133; 32 of 1024 x 1024: 12.5
-// 14.1, 15.0; 25 16.4, 17.5; 50 21.3, 19.3; one of 4096 x 4096: 128 places 17.6, 40; 256 29, 41; 512 51, 42; 1024 92, 44).  Its tiles
-// of 16 places to two a group and to 64 in all, else of 32 (one of 4096 x 4096: 64 places 12.7, 16.7; 128 20.5, 17.6; 128 groups, 8.8
-// places 167, 157).
+// Row kernel to 6 places a group, and where its workgroups number under three per compute unit (us, row kernel and tile kernel; 128
+// groups of 1408 x 2816: 4 places 120, 131; 6 153, 153; 7 163, 155; 9.7 181, 161; 64 of 4096 x 1408: 5 102, 110; 6.9 115, 115; 9.4 127,
+// 121; 32 of 1024 x 1024: 12.5 14.1, 15.0; 25 16.4, 17.5; 50 21.3, 19.3; one of 4096 x 4096: 128 places 17.6, 40; 256 29, 41; 512 51,
+// 42; 1024 92, 44).  Its tiles of 16 places to two a group and to 64 in all, else of 32 (one of 4096 x 4096: 64 places 12.7, 16.7; 128
+// 20.5, 17.6; 128 groups, 8.8 places 167, 157).
 // Tiles of 256 places, one workgroup a compute unit, past 192 places a group where they number two per compute unit, else of 128, two
 // workgroups (us, tiles of 128 and 256; 32 groups of 2816 x 4096, 513 places 393, 381; 128 of 1408 x 2816, 128 places 249, 252; one of
 // 4096 x 4096, 2048 places 60, 78; 512 42, 71).
 int half_cap(phx_moe_ctx* c, const HalfMat& m, int n)
 {
     const int64_t groups = std::min(n, m.n_mat);
-    if (n <= 10 * m.n_mat || (n / 32 + groups / 2) * (m.rg / 2) < 3 * c->ncu) return n <= 64 || n <= 2 * m.n_mat ? 16 : kHalfRows;
+    if (n <= 6 * m.n_mat || (n / 32 + groups / 2) * (m.rg / 2) < 3 * c->ncu) return n <= 64 || n <= 2 * m.n_mat ? 16 : kHalfRows;
     return n > 192 * m.n_mat && (int64_t)(n / kHalfTile) * (m.rg / 8) >= 2 * c->ncu ? kHalfTile : kHalfNarrow;
 }
 
@@ -2631,7 +2631,7 @@ void half_product(phx_moe_ctx* c, const HalfMat& m, HalfArgs g, int n)
 {
     g.n = n;
     g.cap = half_cap(c, m, n);
-    g.once = half_once(m, n);
+    g.once = g.cap <= kHalfRows ? half_once(m, n) : m.n_mat * m.mat_bytes() > 128e6;
     launch_half_product(c->stream, m, g, most_tiles(n, m.n_mat, g.cap));
 }
 }  // namespace
