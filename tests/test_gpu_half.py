@@ -210,6 +210,18 @@ def test_weights_past_the_caches(ctx, n, paired):
     check(ctx, 30, 0, 9, n, 4096, 1800, act=1 if paired else 0, alter=alter)
 
 
+@pytest.mark.parametrize("type_,paired", [(1, True), (30, False)])
+@pytest.mark.parametrize("lengths", [(1, 32, 33, 64, 65, 96, 97, 128, 129), (0, 300, 5, 0, 128, 90, 257, 0, 31)])
+def test_only_tiles_past_the_caches(ctx, lengths, type_, paired):
+    """Matrices of more than 128 MB on the tile kernel: groups of one tile, whose weights pass the caches by, of each width, beside
+    groups of several."""
+    def alter(raw_x, x, raw_w, w):
+        for e in range(1, len(w)):
+            raw_w[e], w[e] = np.roll(raw_w[0], e, 1), np.roll(w[0], e, 1)
+    offsets = np.concatenate([[0], np.cumsum(lengths)]).astype(np.int32)
+    check(ctx, type_, 0, 9, int(offsets[-1]) + 3, 4096, 1800, act=3 if paired else 0, offsets=offsets, alter=alter)
+
+
 def test_same_call_same_bits(ctx):
     """A call's result does not depend on timing, nor on the calls beside it."""
     rng = np.random.default_rng(5)
