@@ -691,7 +691,10 @@ class MoeContext:
         h = C.c_void_p()
         self._check(self.lib.phx_weight_upload_half(self.h, type_, n_mat, rows, cols, 1 if paired else 0,
                                                     w.ctypes.data if isinstance(w, np.ndarray) else w, C.byref(h)))
+        self._half_types[h.value] = type_
         return h.value
+
+    _half_types: dict[int, int] = {}  # of the handles, for the host forms' rows; a handle's number may come again, with its own type
 
     @staticmethod
     def _halves(type_: int, a, n: int):
@@ -716,6 +719,7 @@ class MoeContext:
         src = None if src is None else _ints(src, np.int32)
         if offsets.shape != (n_mat + 1,) or x.ndim != 2 or x.shape[1] != cols or x.itemsize != 2:
             raise ArgumentError(PHX.ERR_ARG, f"offsets {offsets.shape} and rows {x.shape} {x.dtype} for {n_mat} matrices of {rows} x {cols}")
+        x = self._halves(self._half_types.get(handle), x, x.size)
         n = len(x) if src is None else src.size
         out = rows if act == PHX.QUANT_PLAIN else rows // 2
         y = np.zeros((n, out), np.float32)
@@ -742,6 +746,7 @@ class MoeContext:
         ids, weights = _ints(ids, np.int32), _f32(weights)
         if x.ndim != 2 or x.itemsize != 2 or ids.ndim != 2 or weights.shape != ids.shape or len(ids) != len(x):
             raise ArgumentError(PHX.ERR_ARG, f"rows {x.shape} {x.dtype}, ids {ids.shape}, weights {weights.shape}")
+        x = self._halves(self._half_types.get(gate_up), x, x.size)
         self._fits(gate_up, self.weight_shape(gate_up)[1], x.shape[1])  # down's sizes: phx_experts_half
         return self._on_device([np.ascontiguousarray(x), ids, weights], [(x.shape, np.float32)],
                                lambda *p: self.experts_half_device(gate_up, down, act, x.shape[0], ids.shape[1], *p[:3], PHX.F32,

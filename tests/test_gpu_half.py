@@ -412,6 +412,24 @@ def test_host_forms_refuse_sizes_that_are_not_the_handles(ctx, pkg):
         ctx.weight_free(h)
 
 
+def test_host_forms_refuse_rows_of_another_type(ctx, pkg):
+    for type_, other in ((1, np.uint16), (30, np.float16)):
+        w = np.zeros((1, 16, 8), np.float16 if type_ == 1 else np.uint16)
+        h, d = ctx.weight_upload_half(type_, 1, 16, 8, w, paired=True), ctx.weight_upload_half(type_, 1, 8, 8, w[:, :8])
+        try:
+            for x in (np.zeros((2, 8), other), np.zeros((2, 8), np.int16)):
+                with pytest.raises(pkg.ArgumentError):
+                    ctx.MatMulGrouped(h, 1, np.array([0, 2]), x)
+                with pytest.raises(pkg.ArgumentError):
+                    ctx.ExpertsHalf(h, d, 1, x, np.zeros((2, 1), np.int32), np.ones((2, 1), F32))
+            x = np.zeros((2, 8), w.dtype)
+            assert (ctx.MatMulGrouped(h, 1, np.array([0, 2]), x) == 0).all()
+            assert (ctx.ExpertsHalf(h, d, 1, x, np.zeros((2, 1), np.int32), np.ones((2, 1), F32)) == 0).all()
+        finally:
+            ctx.weight_free(h)
+            ctx.weight_free(d)
+
+
 def test_experts_past_the_caches(ctx):
     """One token's experts, and a decode step's, of matrices of more than 128 MB."""
     for T in (1, 12):
