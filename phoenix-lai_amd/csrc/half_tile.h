@@ -15,8 +15,8 @@ namespace phx {
 // ring by direct loads three to five steps ahead, row-major runs of 128 bytes with the 16-byte chunks XOR-swizzled by half the row's number
 // (16 lanes of a 16-byte read then have 16 distinct bank groups).
 // Measured: one 8192 x 8192 matrix by 8192 places 840 us, 1.31 PF (a library product 757), the matrix cores busy in 76% of the cycles: the
-// last round and the epilogue of 8 us a tile are the rest.  16384 places in 128 uneven groups of 1408 x 2816 250 us at 5.8 TB/s: 1.46 GB read
-// for 1.02 GB, since a group's second tile finds only a third of the weights still in the L2.  Few items are bound by whole rounds:
+// last round and the epilogue of 8 us a tile are the rest.  16384 places in 128 uneven groups of 1408 x 2816 248 us at 5.4 TB/s: 1.33 GB read
+// for 1.02 GB, since a group's second tile finds only a part of the weights still in the L2.  Few items are bound by whole rounds:
 // 16412 places in 32 groups of 2816 x 4096 380 us, 1.0 PF, 918 items on 256 compute units.
 constexpr int TI_WAVE = 32 * (64 * 4 + 16);  // a wave's part of the ring in the epilogue: 32 places' rows of 64 floats
 // slots: as many steps as the ring holds, up to six (MT: the row tiles it is made for, 16 KB each)
