@@ -757,16 +757,33 @@ class MoeContext:
         lora_add_device / lora_free."""
         h = C.c_void_p()
         self._check(self.lib.phx_lora_create(self.h, type_, n_slot, max_rank, rows, cols, C.byref(h)))
+        self._lora_sizes[h.value] = type_, rows, cols
         return h.value
 
+    _lora_sizes: dict[int, tuple[int, int, int]] = {}  # (type, rows, cols) of the handles, for the arrays of lora_set
+
     def lora_set(self, handle: int, slot: int, rank: int, a, b, scale: float = 1.0):
-        """phx_lora_set: A [rank][cols] and B [rows][rank] (numpy arrays of 16-bit values, or addresses of host or device
-        memory) into a slot; rank 0 empties it."""
-        at = [np.ascontiguousarray(m).ctypes.data if isinstance(m, np.ndarray) else m for m in (a, b)]
+        """phx_lora_set: A [rank][cols] and B [rows][rank] (numpy arrays of the handle's type: float16, or uint16 holding bf16
+        bits; or addresses of host or device memory) into a slot; rank 0 empties it (a and b unused)."""
+        if rank == 0:
+            a = b = None
+        if isinstance(a, np.ndarray) or isinstance(b, np.ndarray):
+            if handle not in self._lora_sizes:
+                raise ArgumentError(PHX.ERR_ARG, "lora_set: arrays for a handle that lora_create did not return")
+            type_, rows, cols = self._lora_sizes[handle]
+            a, b = self._adapter(type_, a, (rank, cols)), self._adapter(type_, b, (rows, rank))
+        at = [m.ctypes.data if isinstance(m, np.ndarray) else m for m in (a, b)]
         self._check(self.lib.phx_lora_set(self.h, handle, slot, rank, *at, scale))
+
+    def _adapter(self, type_: int, m, shape):
+        """A matrix of an adapter as _halves takes it, refused where it has another shape; an address stays one."""
+        if isinstance(m, np.ndarray) and m.ndim != 1 and m.shape != shape:
+            raise ArgumentError(PHX.ERR_ARG, f"lora_set: a matrix of {m.shape} for one of {shape}")
+        return self._halves(type_, m, shape[0] * shape[1])
 
     def lora_free(self, handle: int):
         self.lib.phx_lora_free(self.h, handle)
+        self._lora_sizes.pop(handle, None)
 
     def lora_add_device(self, handle: int, T: int, x_ptr: int, ids_ptr: int, y_type: int, ld: int, y_in_ptr: int, y_ptr: int):
         """Enqueue phx_lora_add on device buffers (sync() waits)."""
