@@ -796,17 +796,21 @@ class MoeContext:
                                              qs_ptr, d_ptr))
 
     def AddNormI8(self, x: np.ndarray, branch: np.ndarray, w: np.ndarray, eps: float = 1e-6):
-        """phx_add_norm_i8 on host arrays: x and branch [rows][n] float32 or float16, w [n]; returns (sum of x's type, the
-        normed rows f32, qs int8 [rows][n], d f32 [rows])."""
-        x = np.ascontiguousarray(x) if x.dtype == np.float16 else _f32(x)
+        """phx_add_norm_i8 on host arrays: x and branch [rows][n] float32, float16, or uint16 holding bf16 bits, w [n]; returns
+        (sum of x's type, the normed rows f32, qs int8 [rows][n], d f32 [rows]).  A branch of another float type is rounded
+        to x's; of bf16 bits, both are or neither."""
+        x, branch = np.asarray(x), np.asarray(branch)
+        if (x.dtype == np.uint16) != (branch.dtype == np.uint16):
+            raise ArgumentError(PHX.ERR_ARG, f"rows of {x.dtype}, branch of {branch.dtype}")
+        type_ = {np.dtype(np.uint16): PHX.BF16, np.dtype(np.float16): PHX.F16}.get(x.dtype, PHX.F32)
+        x = _f32(x) if type_ == PHX.F32 else np.ascontiguousarray(x)
         branch, w = np.ascontiguousarray(branch, dtype=x.dtype), _f32(w)
         if x.ndim != 2 or branch.shape != x.shape or w.shape != x.shape[1:]:
             raise ArgumentError(PHX.ERR_ARG, f"rows {x.shape}, branch {branch.shape}, weight {w.shape}")
         rows, n = x.shape
         return self._on_device(
             [x, branch, w], [((rows, n), x.dtype), ((rows, n), np.float32), ((rows, n), np.int8), ((rows,), np.float32)],
-            lambda px, pb, pw, ps, po, pq, pd: self.add_norm_i8_device(PHX.F32 if x.dtype == np.float32 else PHX.F16, px, pb, pw,
-                                                                       rows, n, n, eps, ps, PHX.F32, po, pq, pd))
+            lambda px, pb, pw, ps, po, pq, pd: self.add_norm_i8_device(type_, px, pb, pw, rows, n, n, eps, ps, PHX.F32, po, pq, pd))
 
     def stack_run_device(self, x_ptr: int, T: int):
         """Replay the captured stack on a device-resident x (async; sync() waits)."""
