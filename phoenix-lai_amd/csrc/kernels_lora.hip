@@ -87,7 +87,8 @@ void launch_lora_set(hipStream_t st, const LoraSlots& L, int slot, int rank, con
 
 // ------------------------------------------------------------------------------ A x
 // A value as the sum of TERMS terms of the adapters' type, each the rounding of what the ones before leave: 16 bits of it with two
-// bf16 terms, 22 with two of fp16, more than a float's with four.  An infinity or a NaN is in the first alone.
+// bf16 terms, 22 with two of fp16, more than a float's with four; no finer than 2^-25, fp16's half step near zero.  An infinity
+// or a NaN is in the first alone.
 template <bool BF, int TERMS>
 __device__ __forceinline__ void split(float v, uint16_t (&t)[TERMS])
 {
@@ -102,7 +103,8 @@ __device__ __forceinline__ void split(float v, uint16_t (&t)[TERMS])
 // A workgroup takes 16 rows (x) and RT rank tiles of 16 (z), FEW: for the slot of row y of them alone; its NW waves split the
 // reduction, all of a wave's loads in flight at once for rows of up to NW U steps, and their sums meet in LDS, added in the waves'
 // order.  low [T][rt][TERMS][16 ranks]; fp16's terms are of the value over 2^exps
-// [T][rt], which brings a row's 16 to below 2, so that none leaves the type's range.  One row of 4096, rank 16: 4.9 us, a launch and two
+// [T][rt], which brings the largest of a row's 16 to 2^14 or more and below 2^15: none leaves the type's range, and the half step near
+// zero is 2^-39 of that largest, so that values to 2^-17 of it keep their 22 bits.  One row of 4096, rank 16: 4.9 us, a launch and two
 // dependent trips to memory; 4096 rows, rank 32: 17.4, the rows' 34 MB in 6 and the trips of a workgroup a compute unit behind each other.
 template <int NW, int RT, int TERMS, bool FEW, bool BF>
 __global__ __launch_bounds__(64 * NW) void k_lora_down(LoraSlots L, int T, const uint16_t* __restrict__ x,
@@ -180,7 +182,7 @@ __global__ __launch_bounds__(64 * NW) void k_lora_down(LoraSlots L, int T, const
                 m = m >= 0x7F800000u ? 0u : m;
 #pragma unroll
                 for (int d = 1; d < 16; d *= 2) m = max(m, (unsigned)__shfl_xor((int)m, d));
-                ex = m ? (int)(m >> 23) - 127 : 0;  // |values| < 2^(ex + 1)
+                ex = m ? (int)(m >> 23) - 127 - 14 : 0;  // |values| < 2^(ex + 15)
                 s = __builtin_amdgcn_ldexpf(s, -ex);
             }
             if (rows >> row & 1) {
