@@ -466,9 +466,10 @@ void phx_lora_free(phx_moe_ctx* ctx, phx_lora* lora);
  *   y[t] = y_in[t] + scale * B (A x[t])      with the adapter of slot ids[t]
  *   y[t] = y_in[t]                           where ids[t] is outside [0, n_slot) or the slot is empty
  * A x and its scale in float; B's products take that value in two terms of the adapters' type (16 bits of it with
- * bf16, 22 with fp16), in four where y is float (fp16: none finer than 2^-39 of the largest of 16 ranks); one rounding, to y_type (PHX_F32, PHX_F16, PHX_BF16).  x [T][cols] of the
- * adapters' type; y_in and y of y_type, rows ld values apart (ld >= rows: both may be a section of a wider matrix), y may
- * be y_in.  1 <= T <= PHX_MAX_ROWS_I8, ld <= 2^40; x 16-byte aligned, y_in and y to their values, ids 4-byte. */
+ * bf16, 22 with fp16), in four where y is float (fp16: none finer than 2^-39 of the largest of 16 ranks); one rounding, to
+ * y_type (PHX_F32, PHX_F16, PHX_BF16).  x [T][cols] of the adapters' type; y_in and y of y_type, rows ld values apart
+ * (ld >= rows: both may be a section of a wider matrix, also two sections of one, whose rows do not meet), y may be y_in.
+ * 1 <= T <= PHX_MAX_ROWS_I8, ld <= 2^40; x 16-byte aligned, y_in and y to their values, ids 4-byte. */
 int phx_lora_add(phx_moe_ctx* ctx, const phx_lora* lora, int T, const void* x, const int32_t* ids, int y_type, int64_t ld,
                  const void* y_in, void* y);
 

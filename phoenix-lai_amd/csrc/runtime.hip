@@ -2892,7 +2892,13 @@ int phx_lora_add(phx_moe_ctx* c, const phx_lora* l, int T, const void* x, const 
     if (foreign(c, l->device)) return refuse_foreign(c, "lora_add", "the adapters", l->device);
     const int64_t span = ((T - 1) * ld + L.rows) * eb;
     const CallBuf bx{"x", x, (int64_t)T * L.cols * 2, 16, false}, bi{"ids", ids, T * 4ll, 4, false}, by{"y", y, span, eb, true};
-    int rc = y_in == y ? check_bufs(c, "lora_add", {bx, bi, by}) : check_bufs(c, "lora_add", {bx, bi, by, {"y_in", y_in, span, eb, false}});
+    // two sections of one wider matrix: rows of y between those of y_in, off bytes behind them
+    const uint64_t pitch = (uint64_t)ld * eb, len = (uint64_t)L.rows * eb,
+                   off = ((uintptr_t)y > (uintptr_t)y_in ? (uintptr_t)y - (uintptr_t)y_in : (uintptr_t)y_in - (uintptr_t)y) % pitch;
+    const bool between = off >= len && off <= pitch - len;
+    const CallBuf bn{"y_in", y_in, span, eb, false};
+    int rc = y_in == y || between ? check_bufs(c, "lora_add", {bx, bi, by}) : check_bufs(c, "lora_add", {bx, bi, by, bn});
+    if (!rc && between) rc = check_bufs(c, "lora_add", {bn});
     if (rc) return rc;
     const int chunk = std::min(T, 65536), terms = y_type == PHX_F32 ? 4 : 2;  // the workspace stays bounded
     uint16_t* low;
