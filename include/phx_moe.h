@@ -440,9 +440,10 @@ int phx_matmul_grouped(phx_moe_ctx* ctx, const phx_weight* w, int act, int n, co
                        const int32_t* src, int y_type, void* y);
 
 /* The gated FFN of fp16 or bf16 experts for T rows and a routing (phx_route's, or any ids):
- *   h = act(Wgate[e] x[t]) * (Wup[e] x[t]),  e = ids[t][j], as phx_matmul_grouped forms it, rounded to the weights' type
+ *   h = act(Wgate[e] x[t]) * (Wup[e] x[t]),  e = ids[t][j], as phx_matmul_grouped forms it, in float
  *   out[t] = sum over j, in order, of weights[t][j] * (Wdown[e] h)
- * the products and the sum in float, rounded to out_type at the end.  A place whose id is outside [0, n_expert) is
+ * the products and the sum in float, rounded to out_type at the end.  Wdown's product takes h in two terms of the weights' type (16 bits
+ * of it with bf16, 22 with fp16: there none finer than 2^-25, and past 65504 an infinity).  A place whose id is outside [0, n_expert) is
  * skipped; a row without experts is zero.  An id may come more than once in a row.  gate_up: paired, [n_expert][2 nf][d];
  * down: [n_expert][d][nf], of the same type; x [T][d] of that type, ids and weights [T][k], out [T][d];
  * 1 <= T <= PHX_MAX_ROWS_I8, 1 <= k <= PHX_MAX_USED; x and out 16-byte aligned. */

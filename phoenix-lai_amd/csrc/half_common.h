@@ -47,6 +47,20 @@ __device__ __forceinline__ void store_as(int type, void* p, int64_t i, float v)
     else store_one<PHX_F16>(p, i, v);
 }
 
+// A value as the sum of N terms of a 16-bit type, each the rounding of what the ones before leave: 16 bits of it with two bf16 terms, 22
+// with two of fp16, more than a float's with four; no finer than 2^-25, fp16's half step near zero.  An infinity or a NaN is in
+// the first alone.
+template <bool BF, int N>
+__device__ __forceinline__ void split(float v, uint16_t (&t)[N])
+{
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        t[i] = (uint16_t)(BF ? f2bf_pair(v, 0.0f) : f2h_of(v));
+        const float rest = v - (BF ? bf2f(t[i]) : h2f(t[i]));
+        v = fabsf(rest) < 3.0e38f ? rest : 0.0f;
+    }
+}
+
 // 16 bytes of weights; ONCE: no other workgroup reads them, so they need not stay in the caches
 template <bool ONCE>
 __device__ __forceinline__ w4 load_weights(const uint8_t* p)
@@ -150,11 +164,11 @@ constexpr uint32_t NO_ROW = 0xFFFFFFFFu;
 __device__ __forceinline__ uint32_t out_row(const HalfArgs& g, const Tile& tl, int i)
 {
     if (i >= tl.cnt || x_row(g, tl.start + i) < 0) return NO_ROW;
-    return (uint32_t)(g.dst ? g.dst[tl.start + i] : i) * (uint32_t)g.out_cols * (g.type == PHX_F32 ? 4u : 2u);
+    return (uint32_t)(g.dst ? g.dst[tl.start + i] : i) * (uint32_t)g.out_cols * (g.type == PHX_F32 ? 4u : 2u * g.out_terms);
 }
 __device__ __forceinline__ char* out_base(const HalfArgs& g, const Tile& tl)
 {
-    return (char*)g.out + (g.dst ? 0 : (int64_t)tl.start * g.out_cols * (g.type == PHX_F32 ? 4 : 2));
+    return (char*)g.out + (g.dst ? 0 : (int64_t)tl.start * g.out_cols * (g.type == PHX_F32 ? 4 : 2 * g.out_terms));
 }
 
 }  // namespace phx

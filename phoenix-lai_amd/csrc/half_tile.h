@@ -21,37 +21,60 @@ namespace phx {
 constexpr int TI_WAVE = 32 * (64 * 4 + 16);  // a wave's part of the ring in the epilogue: 32 places' rows of 64 floats
 // slots: as many steps as the ring holds, up to six (MT: the row tiles it is made for, 16 KB each)
 constexpr int ti_ring(int nt, int mt) { return std::min(mt * 4 / nt, 6); }
+// weight loads of group kk of a step, of term t of xt
+constexpr int ti_weights(int xt, int t, int kk) { return xt == 1 || (kk == 0) == (t == 0) ? 2 : 0; }
+// the loads behind the next step's rows where a step of term t waits for them, in its last group
+constexpr int ti_newer(int nt, int ring, int xt, int t)
+{
+    const int dpg = (nt + 3) / 4, t0 = (t + ring) & 1;  // t0: of the step that issued these rows, ring - 2 before
+    int n = std::min(nt, 3 * dpg);
+    for (int kk = 0; kk < 3; kk++) n += ti_weights(xt, t, kk);
+    for (int kk = (nt - 1) / dpg + 1; kk < 4; kk++) n += ti_weights(xt, t0, kk);  // behind its last row
+    for (int j = 1; j <= ring - 3; j++) {
+        n += nt;
+        for (int kk = 0; kk < 4; kk++) n += ti_weights(xt, (t0 + j) & 1, kk);
+    }
+    return n;
+}
 
-template <int NT, int MT, bool PAIRED, bool ONCE, bool BF>
+// TERMS: the rows of x, or a paired product's output, are in two terms.  64 columns of x then are two steps, one a term, which
+// both take the weights' registers, and the second issues the weights' loads.
+template <int NT, int MT, bool PAIRED, bool ONCE, bool BF, bool TERMS>
 __device__ __forceinline__ void half_tile_product(const HalfArgs& g, const Tile& tl, int bx, unsigned char* ring, uint32_t* orow)
 {
-    constexpr int STAGE = NT * 32 * 128, RING = ti_ring(NT, MT);
+    constexpr int STAGE = NT * 32 * 128, RING = ti_ring(NT, MT), XT = TERMS && !PAIRED ? 2 : 1;
     const int tid = threadIdx.x, lane = tid & 63, r32 = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int S = g.kc / 8, row_bytes = g.cols * 2;
+    const int S = g.kc / 8, Q = S * XT, row_bytes = g.cols * 2;  // steps of the weights and of the rows; bytes of a row's term
     // this lane's rows of the direct loads: one per load, the last row again past the tile's end
     const int chunk = ((lane & 7) ^ (lane >> 4)) * 16;  // of the loads whose first row is a multiple of 16; 4 chunks on for 8
-    const __amdgpu_buffer_rsrc_t rsrc = buf_rsrc(g.x + (g.src ? 0 : (int64_t)tl.start * g.cols));
+    const __amdgpu_buffer_rsrc_t rsrc = buf_rsrc(g.x + (g.src ? 0 : (int64_t)tl.start * g.cols * XT));
     uint32_t xr[NT];  // rows that src names lie within 2^32 bytes of x, a tile's own of its first
 #pragma unroll
     for (int i = 0; i < NT; i++) {
         const int at = min(8 * (wave * NT + i) + (lane >> 3), tl.cnt - 1);
-        xr[i] = (uint32_t)(g.src ? max(x_row(g, tl.start + at), 0) : at) * (uint32_t)row_bytes;
+        xr[i] = (uint32_t)(g.src ? max(x_row(g, tl.start + at), 0) : at) * (uint32_t)(row_bytes * XT);
+        if (XT == 2) xr[i] += chunk ^ (64 * ((wave * NT + i) & 1));
     }
     for (int i = tid; i < NT * 32; i += 256) orow[i] = out_row(g, tl, i);
     int slot = 0;  // the ring's slot of a step; the one before it takes the rows of the step RING - 1 on
     auto after = [&](int at) { return at == (RING - 1) * STAGE ? 0 : at + STAGE; };
     auto before = [&](int at) { return at == 0 ? (RING - 1) * STAGE : at - STAGE; };
-    auto column = [&](int s, int i) { return s * 128 + (chunk ^ (64 * ((wave * NT + i) & 1))); };  // the lane's byte of load i's rows
+    auto column = [&](int s, int i) { return s / XT * 128 + (chunk ^ (64 * ((wave * NT + i) & 1))); };  // the lane's byte of load i's rows
     auto dma = [&](int s, int to, auto I) {          // load I of step s's rows
         constexpr int i = decltype(I)::value;
-        const int off = column(min(s, S - 1), i);
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void_t)(ring + to + (wave * NT + i) * 1024), 16,
-                                                 xr[i] + (off < row_bytes ? off : 0), 0, 0, 0);
+        const lds_void_t at = (lds_void_t)(ring + to + (wave * NT + i) * 1024);
+        if constexpr (XT == 2) {  // columns past the row are what stands behind it, for clear() to remove: 128 bytes more than the rows are there
+            const int su = min(s, Q - 1);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, at, 16, xr[i], (su >> 1) * 128 + (su & 1) * row_bytes, 0, 0);
+        } else {
+            const int off = column(min(s, Q - 1), i);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, at, 16, xr[i] + (off < row_bytes ? off : 0), 0, 0, 0);
+        }
     };
     // zeros where a last step's loads, landed, hold columns past the row: against zero weights an infinity is none
     auto clear = [&](int s, int to) {
-        if (s != S - 1 || row_bytes == S * 128) return;  // uniform
+        if (s / XT != S - 1 || row_bytes == S * 128) return;  // uniform
 #pragma unroll
         for (int i = 0; i < NT; i++)
             if (column(s, i) >= row_bytes) *(uint4*)(ring + to + (wave * NT + i) * 1024 + lane * 16) = make_uint4(0u, 0u, 0u, 0u);
@@ -94,13 +117,13 @@ __device__ __forceinline__ void half_tile_product(const HalfArgs& g, const Tile&
     // RING - 1 steps on.  The order is fixed by scheduling barriers:
     // the wait for the rows counts the loads issued after them.
     constexpr int DPG = (NT + 3) / 4;                                     // direct loads of a group
-    constexpr int LAST = (NT - 1) / DPG, AFTER = 2 * (3 - LAST);          // the group of a step's last one, the weights after it
-    constexpr int NEWER = AFTER + (RING - 3) * (8 + NT) + 6 + (NT < 3 * DPG ? NT : 3 * DPG);
+    constexpr int NEWER[2] = {ti_newer(NT, RING, XT, 0), ti_newer(NT, RING, XT, 1)};
     // the loads behind the first step's rows
     constexpr int NEWER_AT_START = (RING - 2) * NT + 14;
-    static_assert(NEWER < 64 && NEWER_AT_START < 64 && RING > 3, "vmcnt's range, and the first step's rows before any weights");
-    auto step = [&](int s, auto P) {
-        constexpr int p = decltype(P)::value;
+    static_assert(NEWER[0] < 64 && NEWER[1] < 64 && NEWER_AT_START < 64 && RING > 3, "vmcnt's range, and the first step's rows before any weights");
+    auto step = [&](int s, auto P, auto TERM) {  // the weights' step and its parity, the rows' term
+        constexpr int p = decltype(P)::value, t = decltype(TERM)::value;
+        const int r = s * XT + t;
         const int next = after(slot), far = before(slot);
         static_for<4>([&](auto KK) {
             constexpr int kk = decltype(KK)::value;
@@ -110,17 +133,18 @@ __device__ __forceinline__ void half_tile_product(const HalfArgs& g, const Tile&
                 acc[j][b] = mma32<BF>(wv[p][b][kk], a[kk & 1][j], acc[j][b]);
                 __builtin_amdgcn_sched_barrier(0);
                 if constexpr (m == 0 && kk == 3) {
-                    __builtin_amdgcn_s_waitcnt(vm_wait(NEWER));
-                    clear(s + 1, next);
+                    __builtin_amdgcn_s_waitcnt(vm_wait(NEWER[t]));
+                    clear(r + 1, next);
                     __builtin_amdgcn_s_barrier();
                 }
                 if constexpr (m < NT) read(kk < 3 ? slot : next, ic<(kk + 1) % 4>{}, ic<(m < NT ? m : 0)>{});
                 static_for<2 + DPG>([&](auto I) {
                     constexpr int i = decltype(I)::value, d = kk * DPG + i - 2;
                     if constexpr (m == NT + i * NT / (2 + DPG)) {
-                        if constexpr (i < 2 && kk == 0) weight(s + 1, i, ic<1 - p>{}, ic<3>{});
+                        if constexpr (i < 2 && ti_weights(XT, t, kk) == 0) {
+                        } else if constexpr (i < 2 && kk == 0) weight(s + 1, i, ic<1 - p>{}, ic<3>{});
                         else if constexpr (i < 2) weight(s + 2, i, ic<p>{}, ic<(kk + 3) % 4>{});
-                        else if constexpr (d < NT) dma(s + RING - 1, far, ic<d>{});
+                        else if constexpr (d < NT) dma(r + RING - 1, far, ic<d>{});
                     }
                 });
             });
@@ -134,13 +158,18 @@ __device__ __forceinline__ void half_tile_product(const HalfArgs& g, const Tile&
     static_for<RING - 3>([&](auto R) {
         static_for<NT>([&](auto I) { dma(decltype(R)::value, decltype(R)::value * STAGE, I); });
     });
+    if constexpr (XT == 2)
+        static_for<3>([&](auto KK) {
+            weight(0, 0, ic<0>{}, KK), weight(0, 1, ic<0>{}, KK);
+            __builtin_amdgcn_sched_barrier(0);
+        });
     static_for<2>([&](auto P) {
-        constexpr int p = decltype(P)::value, r = RING - 3 + p;  // step p - 2, its rows those of step r
+        constexpr int p = decltype(P)::value, r = RING - 3 + p;  // the rows' step p - 2, its loads the rows of step r
         static_for<4>([&](auto KK) {
             constexpr int kk = decltype(KK)::value;
             __builtin_amdgcn_sched_barrier(0);
-            if constexpr (kk > 0) weight(p, 0, ic<p>{}, ic<(kk + 3) % 4>{}), weight(p, 1, ic<p>{}, ic<(kk + 3) % 4>{});
-            else if constexpr (p == 1) weight(0, 0, ic<0>{}, ic<3>{}), weight(0, 1, ic<0>{}, ic<3>{});
+            if constexpr (kk > 0 && (XT == 1 || p == 1)) weight(p, 0, ic<p>{}, ic<(kk + 3) % 4>{}), weight(p, 1, ic<p>{}, ic<(kk + 3) % 4>{});
+            else if constexpr (kk == 0 && p == 2 - XT) weight(0, 0, ic<0>{}, ic<3>{}), weight(0, 1, ic<0>{}, ic<3>{});
             __builtin_amdgcn_sched_barrier(0);
             static_for<DPG>([&](auto D) {
                 constexpr int d = kk * DPG + decltype(D)::value;
@@ -155,10 +184,10 @@ __device__ __forceinline__ void half_tile_product(const HalfArgs& g, const Tile&
     static_for<NT>([&](auto J) { read(slot, ic<0>{}, J); });
     landed(ic<0>{});
     for (int s = 0; s + 1 < S; s += 2) {
-        step(s, ic<0>{});
-        step(s + 1, ic<1>{});
+        static_for<XT>([&](auto T) { step(s, ic<0>{}, T); });
+        static_for<XT>([&](auto T) { step(s + 1, ic<1>{}, T); });
     }
-    if (S & 1) step(S - 1, ic<0>{});
+    if (S & 1) static_for<XT>([&](auto T) { step(S - 1, ic<0>{}, T); });
     __builtin_amdgcn_s_waitcnt(0);  // the direct loads past the last step land before the workgroup's LDS goes
     __syncthreads();
     char* out = out_base(g, tl);
@@ -219,14 +248,49 @@ __device__ __forceinline__ void half_tile_product(const HalfArgs& g, const Tile&
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
         __builtin_amdgcn_sched_barrier(0);
     };
-    if (g.type == PHX_F32) static_for<NT>([&](auto J) { store(ic<4>{}, J); });
+    // the same of a value's two terms, each 32 channels of a place 64 bytes; out_cols is a multiple of 8, as the second product's columns
+    auto store_terms = [&](auto J) {
+        constexpr int j = decltype(J)::value, PITCH = 2 * 2 * 32 + 16;
+#pragma unroll
+        for (int i = 0; i < 16; i += 8) {
+            uint32_t u[2][4];
+#pragma unroll
+            for (int v = 0; v < 8; v += 2) {
+                uint16_t t[2][2];
+#pragma unroll
+                for (int w = 0; w < 2; w++) split<BF>(gated_half(g.act, acc[j][0][i + v + w], acc[j][1][i + v + w]), t[w]);
+#pragma unroll
+                for (int z = 0; z < 2; z++) u[z][v / 2] = t[0][z] | (uint32_t)t[1][z] << 16;
+            }
+#pragma unroll
+            for (int z = 0; z < 2; z++) *(uint4*)(mine + r32 * PITCH + z * 64 + (16 * h + i) * 2) = make_uint4(u[z][0], u[z][1], u[z][2], u[z][3]);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        const int c = lane & 7, col = col0 + (c & 3) * 8;  // eight lanes a place, four a term
+#pragma unroll
+        for (int it = 0; it < 4; it++) {
+            const int tok = it * 8 + (lane >> 3);
+            const uint32_t o = orow[32 * j + tok];
+            const uint4 y = *(const uint4*)(mine + tok * PITCH + c * 16);
+            if (o != NO_ROW && col < g.out_cols) *(uint4*)(out + o + (int64_t)((c >> 2) * g.out_cols + col) * 2) = y;
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    if constexpr (TERMS && PAIRED) static_for<NT>(store_terms);
+    else if constexpr (TERMS) static_for<NT>([&](auto J) { store(ic<4>{}, J); });
+    else if (g.type == PHX_F32) static_for<NT>([&](auto J) { store(ic<4>{}, J); });
     else static_for<NT>([&](auto J) { store(ic<2>{}, J); });
 }
 
 // Workgroup L runs on XCD L % 8.  The items (a tile's block of 256 stored rows) are in the order of groups, blocks, tiles, and
 // each XCD takes an eighth of them as one run: a group's tiles meet a block's weights in one L2 at about one time, and the weights
 // leave memory once.
-template <int MT, bool PAIRED, bool BF>
+template <int MT, bool PAIRED, bool BF, bool TERMS>
 __global__ __launch_bounds__(256, MT > 4 ? 1 : 2) void k_half_tile(HalfArgs g)
 {
     __shared__ __align__(16) unsigned char ring[MT * 16 * 1024];
@@ -243,48 +307,57 @@ __global__ __launch_bounds__(256, MT > 4 ? 1 : 2) void k_half_tile(HalfArgs g)
     tl = {__builtin_amdgcn_readfirstlane(tl.e), __builtin_amdgcn_readfirstlane(tl.start), __builtin_amdgcn_readfirstlane(tl.cnt)};
     bx = __builtin_amdgcn_readfirstlane(bx);
     const int n = (tl.cnt + 31) / 32;
-    if constexpr (MT == 4) {
+    if constexpr (TERMS && !PAIRED) {  // kHalfTerms
+        switch (g.once && alone ? n + 3 : n) {
+        case 1: half_tile_product<1, MT, PAIRED, false, BF, TERMS>(g, tl, bx, ring, orow); break;
+        case 2: half_tile_product<2, MT, PAIRED, false, BF, TERMS>(g, tl, bx, ring, orow); break;
+        case 3: half_tile_product<3, MT, PAIRED, false, BF, TERMS>(g, tl, bx, ring, orow); break;
+        case 4: half_tile_product<1, MT, PAIRED, true, BF, TERMS>(g, tl, bx, ring, orow); break;
+        case 5: half_tile_product<2, MT, PAIRED, true, BF, TERMS>(g, tl, bx, ring, orow); break;
+        default: half_tile_product<3, MT, PAIRED, true, BF, TERMS>(g, tl, bx, ring, orow);
+        }
+    } else if constexpr (MT == 4) {
         // a group's only tile reads its weights alone: past the caches, where the call's are more than they keep to the next (us,
         // through and past them; places in 128 groups of 1408 x 2816: 1624 170, 154; 4000 212, 193; 8000 214, 206; 16384 255, 252;
         // 4000 in 64 of 4096 x 1408 168, 173; past them for every tile, 16384 places: 295)
         switch (g.once && alone ? n + 4 : n) {
-        case 1: half_tile_product<1, MT, PAIRED, false, BF>(g, tl, bx, ring, orow); break;
-        case 2: half_tile_product<2, MT, PAIRED, false, BF>(g, tl, bx, ring, orow); break;
-        case 3: half_tile_product<3, MT, PAIRED, false, BF>(g, tl, bx, ring, orow); break;
-        case 4: half_tile_product<4, MT, PAIRED, false, BF>(g, tl, bx, ring, orow); break;
-        case 5: half_tile_product<1, MT, PAIRED, true, BF>(g, tl, bx, ring, orow); break;
-        case 6: half_tile_product<2, MT, PAIRED, true, BF>(g, tl, bx, ring, orow); break;
-        case 7: half_tile_product<3, MT, PAIRED, true, BF>(g, tl, bx, ring, orow); break;
-        default: half_tile_product<4, MT, PAIRED, true, BF>(g, tl, bx, ring, orow);
+        case 1: half_tile_product<1, MT, PAIRED, false, BF, TERMS>(g, tl, bx, ring, orow); break;
+        case 2: half_tile_product<2, MT, PAIRED, false, BF, TERMS>(g, tl, bx, ring, orow); break;
+        case 3: half_tile_product<3, MT, PAIRED, false, BF, TERMS>(g, tl, bx, ring, orow); break;
+        case 4: half_tile_product<4, MT, PAIRED, false, BF, TERMS>(g, tl, bx, ring, orow); break;
+        case 5: half_tile_product<1, MT, PAIRED, true, BF, TERMS>(g, tl, bx, ring, orow); break;
+        case 6: half_tile_product<2, MT, PAIRED, true, BF, TERMS>(g, tl, bx, ring, orow); break;
+        case 7: half_tile_product<3, MT, PAIRED, true, BF, TERMS>(g, tl, bx, ring, orow); break;
+        default: half_tile_product<4, MT, PAIRED, true, BF, TERMS>(g, tl, bx, ring, orow);
         }
     } else {
         switch (n) {
-        case 1: half_tile_product<1, MT, PAIRED, false, BF>(g, tl, bx, ring, orow); break;
-        case 2: half_tile_product<2, MT, PAIRED, false, BF>(g, tl, bx, ring, orow); break;
-        case 3: half_tile_product<3, MT, PAIRED, false, BF>(g, tl, bx, ring, orow); break;
-        case 4: half_tile_product<4, MT, PAIRED, false, BF>(g, tl, bx, ring, orow); break;
-        case 5: half_tile_product<5, MT, PAIRED, false, BF>(g, tl, bx, ring, orow); break;
-        case 6: half_tile_product<6, MT, PAIRED, false, BF>(g, tl, bx, ring, orow); break;
-        case 7: half_tile_product<7, MT, PAIRED, false, BF>(g, tl, bx, ring, orow); break;
-        default: half_tile_product<8, MT, PAIRED, false, BF>(g, tl, bx, ring, orow);
+        case 1: half_tile_product<1, MT, PAIRED, false, BF, TERMS>(g, tl, bx, ring, orow); break;
+        case 2: half_tile_product<2, MT, PAIRED, false, BF, TERMS>(g, tl, bx, ring, orow); break;
+        case 3: half_tile_product<3, MT, PAIRED, false, BF, TERMS>(g, tl, bx, ring, orow); break;
+        case 4: half_tile_product<4, MT, PAIRED, false, BF, TERMS>(g, tl, bx, ring, orow); break;
+        case 5: half_tile_product<5, MT, PAIRED, false, BF, TERMS>(g, tl, bx, ring, orow); break;
+        case 6: half_tile_product<6, MT, PAIRED, false, BF, TERMS>(g, tl, bx, ring, orow); break;
+        case 7: half_tile_product<7, MT, PAIRED, false, BF, TERMS>(g, tl, bx, ring, orow); break;
+        default: half_tile_product<8, MT, PAIRED, false, BF, TERMS>(g, tl, bx, ring, orow);
         }
     }
 }
 
-template <int MT, bool PAIRED, bool BF>
+template <int MT, bool PAIRED, bool BF, bool TERMS>
 static void half_tiles(hipStream_t st, const HalfMat& m, const HalfArgs& g, int max_tiles)
 {
     const dim3 grid((max_tiles * ((m.rg + 7) / 8) + 7) / 8 * 8);
-    launch(k_half_tile<MT, PAIRED, BF>, grid, dim3(256), 0, st, g);
+    launch(k_half_tile<MT, PAIRED, BF, TERMS>, grid, dim3(256), 0, st, g);
 }
 
-template <bool BF>
+template <bool BF, bool TERMS>
 void launch_half_tiles(hipStream_t st, const HalfMat& m, const HalfArgs& g, int max_tiles)
 {
-    if (g.cap <= kHalfNarrow && m.paired) half_tiles<4, true, BF>(st, m, g, max_tiles);
-    else if (g.cap <= kHalfNarrow) half_tiles<4, false, BF>(st, m, g, max_tiles);
-    else if (m.paired) half_tiles<8, true, BF>(st, m, g, max_tiles);
-    else half_tiles<8, false, BF>(st, m, g, max_tiles);
+    if (g.cap <= kHalfNarrow && m.paired) half_tiles<4, true, BF, TERMS>(st, m, g, max_tiles);
+    else if (TERMS ? !m.paired : g.cap <= kHalfNarrow) half_tiles<4, false, BF, TERMS>(st, m, g, max_tiles);
+    else if (m.paired) half_tiles<8, true, BF, TERMS>(st, m, g, max_tiles);
+    else if constexpr (!TERMS) half_tiles<8, false, BF, TERMS>(st, m, g, max_tiles);
 }
 
 }  // namespace phx

@@ -41,17 +41,18 @@ void launch_half_pack(hipStream_t st, const HalfMat& m, int m0, int n_mat, const
 // (PAIRED: of 16 channels, their gate and up rows) by a tile of up to 16 TT places, both straight from memory to registers:
 // its NW waves split the reduction, so no operand is wanted by two of them, and a matrix of few rows still has loads in
 // flight everywhere.  A wave keeps U steps of 32 columns ahead; the waves' sums meet in LDS, added in the waves' order.
-template <int NW, int RT, int TT, bool PAIRED, bool ONCE, bool BF>
+// XT: the terms of a row of x, both times a step's weights.
+template <int NW, int RT, int TT, int XT, bool PAIRED, bool ONCE, bool BF>
 __device__ __forceinline__ void half_rows_product(const HalfArgs& g, const Tile& tl, float* red, uint32_t* orow)
 {
-    constexpr int NB = PAIRED ? 2 : 1, NR = RT * NB, U = NR + TT <= 3 ? 8 : NR + TT <= 6 ? 4 : 3;
+    constexpr int NB = PAIRED ? 2 : 1, NR = RT * NB, U = NR + TT * XT <= 3 ? 8 : NR + TT * XT <= 6 ? 4 : 3;
     const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, q = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int bx = blockIdx.x, tiles16 = g.rgs * 2 / NB;  // the matrix's row (channel) tiles of 16
     const uint16_t* xr[TT];
 #pragma unroll
     for (int t = 0; t < TT; t++)
-        xr[t] = g.x + (int64_t)max(x_row(g, tl.start + min(16 * t + r16, tl.cnt - 1)), 0) * g.cols;
+        xr[t] = g.x + (int64_t)max(x_row(g, tl.start + min(16 * t + r16, tl.cnt - 1)), 0) * (g.cols * XT);
     const uint8_t* wb[NR];
 #pragma unroll
     for (int r = 0; r < RT; r++)
@@ -63,7 +64,7 @@ __device__ __forceinline__ void half_rows_product(const HalfArgs& g, const Tile&
     const int lo = q * 512 + r16 * 16;
     if (tid < TT * 16) orow[tid] = out_row(g, tl, tid);
     f32x4 acc[TT][NR];
-    w4 w[U][NR], x[U][TT];
+    w4 w[U][NR], x[U][TT][XT];
 #pragma unroll
     for (int t = 0; t < TT; t++)
 #pragma unroll
@@ -74,18 +75,24 @@ __device__ __forceinline__ void half_rows_product(const HalfArgs& g, const Tile&
 #pragma unroll
         for (int r = 0; r < NR; r++) w[u][r] = load_weights<ONCE>(wb[r] + (int64_t)su * 2048 + lo);
 #pragma unroll
-        for (int t = 0; t < TT; t++) x[u][t] = *(const w4*)(xr[t] + k);
+        for (int t = 0; t < TT; t++)
+#pragma unroll
+            for (int z = 0; z < XT; z++) x[u][t][z] = *(const w4*)(xr[t] + z * g.cols + k);
     };
     auto mma = [&](int u, int s) {
         if (32 * s + 32 > g.cols) {  // uniform: the lanes past the row hold its last values; against zero weights an infinity is none
             const bool past = 32 * s + 8 * q >= g.cols;
 #pragma unroll
-            for (int t = 0; t < TT; t++) x[u][t] = past ? w4{0, 0, 0, 0} : x[u][t];
+            for (int t = 0; t < TT; t++)
+#pragma unroll
+                for (int z = 0; z < XT; z++) x[u][t][z] = past ? w4{0, 0, 0, 0} : x[u][t][z];
         }
 #pragma unroll
         for (int t = 0; t < TT; t++)
 #pragma unroll
-            for (int r = 0; r < NR; r++) acc[t][r] = mma16<BF>(x[u][t], w[u][r], acc[t][r]);
+            for (int r = 0; r < NR; r++)
+#pragma unroll
+                for (int z = 0; z < XT; z++) acc[t][r] = mma16<BF>(x[u][t][z], w[u][r], acc[t][r]);
     };
     if (s0 < s1) {  // uniform over the wave
 #pragma unroll
@@ -126,12 +133,16 @@ __device__ __forceinline__ void half_rows_product(const HalfArgs& g, const Tile&
             if (PAIRED) up += red[k * TT * NR * 256 + at + 256];
         }
         if (PAIRED) y = gated_half(g.act, y, up);
-        store_as(g.type, out + orow[tok], col, y);
+        if (PAIRED && g.out_terms == 2) {
+            uint16_t t[2];
+            split<BF>(y, t);
+            for (int z = 0; z < 2; z++) ((uint16_t*)(out + orow[tok]))[z * g.out_cols + col] = t[z];
+        } else store_as(g.type, out + orow[tok], col, y);
     }
 }
 
 // CT: the most place tiles of 16 that a tile may hold (its capacity); a tile takes the product of its own count
-template <int NW, int RT, int CT, bool PAIRED, bool ONCE, bool BF>
+template <int NW, int RT, int CT, int XT, bool PAIRED, bool ONCE, bool BF>
 __global__ __launch_bounds__(64 * NW) void k_half_rows(HalfArgs g)
 {
     __shared__ float red[NW * RT * CT * (PAIRED ? 2 : 1) * 256];
@@ -139,8 +150,8 @@ __global__ __launch_bounds__(64 * NW) void k_half_rows(HalfArgs g)
     Tile tl;
     if (!half_tile(g, blockIdx.y, &tl)) return;  // uniform over the workgroup
     const int n = (tl.cnt + 15) / 16;
-    if (CT == 1 || n == 1) half_rows_product<NW, RT, 1, PAIRED, ONCE, BF>(g, tl, red, orow);
-    else half_rows_product<NW, RT, CT < 2 ? 1 : 2, PAIRED, ONCE, BF>(g, tl, red, orow);
+    if (CT == 1 || n == 1) half_rows_product<NW, RT, 1, XT, PAIRED, ONCE, BF>(g, tl, red, orow);
+    else half_rows_product<NW, RT, CT < 2 ? 1 : 2, XT, PAIRED, ONCE, BF>(g, tl, red, orow);
 }
 
 static void set_matrix(HalfArgs& g, const HalfMat& m)
@@ -158,8 +169,11 @@ template <int NW, int RT, int CT, bool PAIRED, bool ONCE>
 static void half_rows(hipStream_t st, const HalfMat& m, const HalfArgs& g, int max_tiles)
 {
     const dim3 grid(((g.out_cols + 31) / 32 * 32 + 16 * RT - 1) / (16 * RT), max_tiles), blk(64 * NW);  // stored rows in whole groups
-    if (m.type == PHX_BF16) launch(k_half_rows<NW, RT, CT, PAIRED, ONCE, true>, grid, blk, 0, st, g);
-    else launch(k_half_rows<NW, RT, CT, PAIRED, ONCE, false>, grid, blk, 0, st, g);
+    constexpr int XT = PAIRED ? 1 : 2;
+    if (m.type == PHX_BF16 && g.x_terms < XT) launch(k_half_rows<NW, RT, CT, 1, PAIRED, ONCE, true>, grid, blk, 0, st, g);
+    else if (m.type == PHX_BF16) launch(k_half_rows<NW, RT, CT, XT, PAIRED, ONCE, true>, grid, blk, 0, st, g);
+    else if (g.x_terms < XT) launch(k_half_rows<NW, RT, CT, 1, PAIRED, ONCE, false>, grid, blk, 0, st, g);
+    else launch(k_half_rows<NW, RT, CT, XT, PAIRED, ONCE, false>, grid, blk, 0, st, g);
 }
 
 // Four waves and 32 channels or 64 outputs; plain matrices with at most a workgroup a compute unit then, eight waves and 32 outputs (us, four
@@ -182,14 +196,18 @@ void launch_half_product(hipStream_t st, const HalfMat& m, HalfArgs g, int max_t
     else if (g.cap <= 16) rows_by_pair<1, false>(st, m, g, max_tiles);
     else if (g.cap <= kHalfRows && g.once) rows_by_pair<2, true>(st, m, g, max_tiles);
     else if (g.cap <= kHalfRows) rows_by_pair<2, false>(st, m, g, max_tiles);
-    else if (m.type == PHX_BF16) launch_half_tiles<true>(st, m, g, max_tiles);
-    else launch_half_tiles<false>(st, m, g, max_tiles);
+    else if (g.x_terms == 2 || g.out_terms == 2) {
+        if (m.type == PHX_BF16) launch_half_tiles<true, true>(st, m, g, max_tiles);
+        else launch_half_tiles<false, true>(st, m, g, max_tiles);
+    } else if (m.type == PHX_BF16) launch_half_tiles<true, false>(st, m, g, max_tiles);
+    else launch_half_tiles<false, false>(st, m, g, max_tiles);
 }
 
 // ------------------------------------------------------------------------------ experts
 // The down products of few assignments and their weighted sum, for a token (blockIdx.y) and 16 of its outputs: wave w takes
 // the token's places w, w + NW, ..., and the places' values meet in LDS in order.  No lists and no partial outputs go through
-// memory.  One token's eight experts of 2816 x 704 take 7.2 us (a launch 3.4, two dependent trips to memory).
+// memory.  One instruction takes both terms of a place's row, as its even and its odd rows.  One token's eight experts of 2816 x 704 take
+// 8.1 us (a launch 3.4, two dependent trips to memory).
 template <int NW, bool BF>
 __global__ __launch_bounds__(64 * NW) void k_half_down_few(HalfArgs g, int k, const float* __restrict__ weights)
 {
@@ -203,7 +221,8 @@ __global__ __launch_bounds__(64 * NW) void k_half_down_few(HalfArgs g, int k, co
         const int e = g.ids[t * k + j];  // uniform
         if ((unsigned)e >= (unsigned)g.n_mat) continue;
         const uint8_t* wb = g.w + (int64_t)e * g.mat_bytes + (int64_t)(bx >> 1) * g.kc * 512 + (bx & 1) * 256 + q * 512 + r16 * 16;
-        const uint16_t* row = g.x + (t * k + j) * g.cols;
+        // every even row of the first operand is the place's first terms, every odd one its second
+        const uint16_t* row = g.x + ((t * k + j) * 2 + (lane & 1)) * g.cols;
         f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
         for (int s = 0; s < steps; s += U) {
             w4 w[U], x[U];
@@ -215,10 +234,10 @@ __global__ __launch_bounds__(64 * NW) void k_half_down_few(HalfArgs g, int k, co
             for (int u = 0; u < U; u++)
                 if (s + u < steps) {  // uniform
                     if (32 * (s + u) + 8 * q >= g.cols) x[u] = w4{0, 0, 0, 0};
-                    acc = mma16<BF>(x[u], w[u], acc);  // every row of the first operand is the place's
+                    acc = mma16<BF>(x[u], w[u], acc);
                 }
         }
-        if (lane < 16) vals[j][lane] = acc[0];
+        if (lane < 16) vals[j][lane] = acc[0] + acc[1];
     }
     __syncthreads();
     const int slot = bx * 16 + threadIdx.x, col = (slot & ~31) + slot_row(slot & 31);

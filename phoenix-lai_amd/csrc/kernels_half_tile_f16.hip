@@ -1,5 +1,5 @@
 #include "half_tile.h"
 
 namespace phx {
-template void launch_half_tiles<false>(hipStream_t, const HalfMat&, const HalfArgs&, int);
+template void launch_half_tiles<false, false>(hipStream_t, const HalfMat&, const HalfArgs&, int);
 }

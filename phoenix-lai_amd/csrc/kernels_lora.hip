@@ -6,22 +6,9 @@
 // that depends on timing; rows of one request that follow each other, as a prompt's do, cost one pass.
 #include <algorithm>
 
-#include "device_common.h"
-#include "rows_io.h"
+#include "half_common.h"
 
 namespace phx {
-
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t w4 __attribute__((ext_vector_type(4)));
-typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-typedef __bf16 b8 __attribute__((ext_vector_type(8)));
-
-template <bool BF>
-__device__ __forceinline__ f32x4 mma16(w4 a, w4 b, f32x4 c)
-{
-    if constexpr (BF) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
-    else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
-}
 
 // The slots of 16 rows, one after another: mine is lane l's id (of row l % 16, -1 where it has none), left the rows not
 // yet taken.  A slot's rows are taken together, those without one (slot -1) too.
@@ -86,20 +73,6 @@ void launch_lora_set(hipStream_t st, const LoraSlots& L, int slot, int rank, con
 }
 
 // ------------------------------------------------------------------------------ A x
-// A value as the sum of TERMS terms of the adapters' type, each the rounding of what the ones before leave: 16 bits of it with two
-// bf16 terms, 22 with two of fp16, more than a float's with four; no finer than 2^-25, fp16's half step near zero.  An infinity
-// or a NaN is in the first alone.
-template <bool BF, int TERMS>
-__device__ __forceinline__ void split(float v, uint16_t (&t)[TERMS])
-{
-#pragma unroll
-    for (int i = 0; i < TERMS; i++) {
-        t[i] = (uint16_t)(BF ? f2bf_pair(v, 0.0f) : f2h_of(v));
-        const float rest = v - (BF ? bf2f(t[i]) : h2f(t[i]));
-        v = fabsf(rest) < 3.0e38f ? rest : 0.0f;
-    }
-}
-
 // A workgroup takes 16 rows (x) and RT rank tiles of 16 (z), FEW: for the slot of row y of them alone; its NW waves split the
 // reduction, all of a wave's loads in flight at once for rows of up to NW U steps, and their sums meet in LDS, added in the waves'
 // order.  low [T][rt][TERMS][16 ranks]; fp16's terms are of the value over 2^exps

@@ -352,10 +352,13 @@ void launch_half_pack(hipStream_t st, const HalfMat& m, int m0, int n_mat, const
 struct HalfArgs {
     // set by the caller.  Groups: offsets [n_mat + 1] over n places, taken in tiles of cap, or one place each whose group is
     // ids[place].  A place's row of x is src[place] / div (none outside n_x rows), without src the place's own number (with ids
-    // over div); its output row is dst[place], without dst its own number.
+    // over div); its output row is dst[place], without dst its own number.  x_terms, out_terms 2: a row of x (of a plain product) or
+    // of the output (of a paired one, then of the weights' type) is its values' first terms and then their second ones; 128 bytes
+    // more can be read behind such rows of x.
     const uint16_t* x = nullptr;
     const int *src = nullptr, *dst = nullptr, *offsets = nullptr, *ids = nullptr;
     int n = 0, n_x = 0, div = 1, cap = 0, act = 0, type = 0;  // type: the output's
+    int x_terms = 1, out_terms = 1;
     bool once = false;  // weights that nobody reads again soon: all of the row kernel's, the tile kernel's of groups with one tile
     void* out = nullptr;
     // set by launch_half_product from the matrix
@@ -364,10 +367,11 @@ struct HalfArgs {
     int kc, cols, out_cols, rgs, n_mat;
 };
 constexpr int kHalfRows = 32, kHalfNarrow = 128, kHalfTile = 256;  // places a tile: the row kernel's (16 or 32), the tile kernel's two
+constexpr int kHalfTerms = 96;  // the tile kernel's where x's rows are two terms
 void launch_half_product(hipStream_t st, const HalfMat& m, HalfArgs g, int max_tiles);
-template <bool BF>
-void launch_half_tiles(hipStream_t st, const HalfMat& m, const HalfArgs& g, int max_tiles);  // its tile kernel, g's matrix set
-// the down products of T tokens' k places from h [T k][cols], and their weighted sums as out [T][rows]
+template <bool BF, bool TERMS>
+void launch_half_tiles(hipStream_t st, const HalfMat& m, const HalfArgs& g, int max_tiles);  // its tile kernel, g's matrix set; TERMS: two
+// the down products of T tokens' k places from h [T k][2 terms][cols], and their weighted sums as out [T][rows]
 void launch_half_down_few(hipStream_t st, const HalfMat& m, int T, int k, const uint16_t* h, const int* ids, const float* weights,
                           int out_type, void* out);
 

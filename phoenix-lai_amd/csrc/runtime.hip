@@ -2626,11 +2626,15 @@ int half_cap(phx_moe_ctx* c, const HalfMat& m, int n)
 // 192 in 32 of 1408 x 2816 52, 48; 192 in 32 of 1024 x 1024 12.6, 13.9; one group of 16384 x 4096: 12 places 32, 28; 24 49, 50).
 bool half_once(const HalfMat& m, int n) { return m.n_mat * m.mat_bytes() > 128e6 && n <= std::max(8 * m.n_mat, 16); }
 
-// One product over n places.
+// One product over n places.  Rows of two terms in tiles of 96 places on the tile kernel, with two workgroups a compute unit: of 128 the
+// loop's registers spill with the weights held for both terms (us of the whole experts, 96, 128 and 256; 128 experts of 2816 x 704,
+// eight of them for 1024 rows 367, 375, 381; 2048 466, 476, 491; 4096 721, 735, 741; four of 64 of 4096 x 1408 for 2048 616, 633,
+// 642; four of 32 of 2816 x 2048 for 4096 749, 773, 753).
 void half_product(phx_moe_ctx* c, const HalfMat& m, HalfArgs g, int n)
 {
     g.n = n;
     g.cap = half_cap(c, m, n);
+    if (g.x_terms == 2 && g.cap > kHalfRows) g.cap = kHalfTerms;
     g.once = g.cap <= kHalfRows ? half_once(m, n) : m.n_mat * m.mat_bytes() > 128e6;
     launch_half_product(c->stream, m, g, most_tiles(n, m.n_mat, g.cap));
 }
@@ -2747,9 +2751,10 @@ int phx_experts_half(phx_moe_ctx* c, const phx_weight* gu, const phx_weight* dn,
     // 17.7; 64 21.7, 34.7; 32 of them, four a token: T = 8 20.8, 14.9; 24 24.5, 28.0)
     const double each = 6.0 * nf * d, A0 = (double)T * k, again = A0 - E * (1.0 - pow(1.0 - 1.0 / E, A0));
     if (A0 <= 1024 && again * each <= (E * each <= 64e6 ? 144e6 : 48e6)) {
-        if ((rc = i8_ensure(c, I8_H, (int64_t)T * k * nf, &h))) return rc;
+        if ((rc = i8_ensure(c, I8_H, (int64_t)T * k * nf * 2, &h))) return rc;
         g.ids = ids;
         g.div = k;
+        g.out_terms = 2;
         g.n_x = T;
         g.cap = 16;
         g.once = half_once(gu->half, T * k);
@@ -2765,7 +2770,7 @@ int phx_experts_half(phx_moe_ctx* c, const phx_weight* gu, const phx_weight* dn,
     int *perm, *offsets;
     float* y;
     if ((rc = i8_ensure(c, I8_PERM, A, &perm)) || (rc = i8_ensure(c, HALF_OFFSETS, E + 1, &offsets)) ||
-        (rc = i8_ensure(c, I8_H, (int64_t)A * nf, &h)) || (rc = i8_ensure(c, I8_Y, (int64_t)A * d, &y)))
+        (rc = i8_ensure(c, I8_H, (int64_t)A * nf * 2 + 64, &h)) || (rc = i8_ensure(c, I8_Y, (int64_t)A * d, &y)))
         return rc;
     g.offsets = offsets;
     for (int t0 = 0; t0 < T; t0 += chunk) {
@@ -2778,6 +2783,8 @@ int phx_experts_half(phx_moe_ctx* c, const phx_weight* gu, const phx_weight* dn,
         g.src = perm;
         g.div = k;
         g.dst = nullptr;
+        g.x_terms = 1;
+        g.out_terms = 2;
         g.type = gu->type;
         g.out = h;
         half_product(c, gu->half, g, n * k);
@@ -2785,6 +2792,8 @@ int phx_experts_half(phx_moe_ctx* c, const phx_weight* gu, const phx_weight* dn,
         g.src = nullptr;
         g.div = 1;
         g.dst = perm;
+        g.x_terms = 2;
+        g.out_terms = 1;
         g.type = PHX_F32;
         g.out = y;
         half_product(c, dn->half, g, n * k);
