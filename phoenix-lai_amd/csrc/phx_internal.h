@@ -5,6 +5,7 @@
 #include <stdint.h>
 
 #include "phx_moe.h"
+#include "half_rules.h"
 
 #define PHX_Q4_0_DEV 2
 #define PHX_Q8_0_DEV 8
@@ -359,15 +360,13 @@ struct HalfArgs {
     const int *src = nullptr, *dst = nullptr, *offsets = nullptr, *ids = nullptr;
     int n = 0, n_x = 0, div = 1, cap = 0, act = 0, type = 0;  // type: the output's
     int x_terms = 1, out_terms = 1;
-    bool once = false;  // weights that nobody reads again soon: all of the row kernel's, the tile kernel's of groups with one tile
+    bool once = false;  // weights that nobody reads again soon (half_once)
     void* out = nullptr;
     // set by launch_half_product from the matrix
     const uint8_t* w;
     int64_t mat_bytes;
     int kc, cols, out_cols, rgs, n_mat;
 };
-constexpr int kHalfRows = 32, kHalfNarrow = 128, kHalfTile = 256;  // places a tile: the row kernel's (16 or 32), the tile kernel's two
-constexpr int kHalfTerms = 96;  // the tile kernel's where x's rows are two terms
 void launch_half_product(hipStream_t st, const HalfMat& m, HalfArgs g, int max_tiles);
 template <bool BF, bool TERMS>
 void launch_half_tiles(hipStream_t st, const HalfMat& m, const HalfArgs& g, int max_tiles);  // its tile kernel, g's matrix set; TERMS: two

@@ -2602,40 +2602,12 @@ int upload_half(phx_moe_ctx* c, HalfMat& m, const uint16_t* w)
 
 bool half_type(int type) { return type == PHX_F16 || type == PHX_BF16; }
 
-// The tiles of n places in n_mat groups, at most.
-int most_tiles(int n, int n_mat, int cap) { return n / cap + std::min(n, n_mat); }
-
-// The kernel of a product over n places, by its tiles' capacity.
-// Row kernel to 6 places a group, and where its workgroups number under three per compute unit (us, row kernel and tile kernel; 128
-// groups of 1408 x 2816: 4 places 120, 131; 6 153, 153; 7 163, 155; 9.7 181, 161; 64 of 4096 x 1408: 5 102, 110; 6.9 115, 115; 9.4 127,
-// 121; 32 of 1024 x 1024: 12.5 14.1, 15.0; 25 16.4, 17.5; 50 21.3, 19.3; one of 4096 x 4096: 128 places 17.6, 40; 256 29, 41; 512 51,
-// 42; 1024 92, 44).  Its tiles of 16 places to two a group and to 64 in all, else of 32 (one of 4096 x 4096: 64 places 12.7, 16.7; 128
-// 20.5, 17.6; 128 groups, 8.8 places 167, 157).
-// Tiles of 256 places, one workgroup a compute unit, past 192 places a group where they number two per compute unit, else of 128, two
-// workgroups (us, tiles of 128 and 256; 32 groups of 2816 x 4096, 513 places 393, 381; 128 of 1408 x 2816, 128 places 249, 252; one of
-// 4096 x 4096, 2048 places 60, 78; 512 42, 71).
-int half_cap(phx_moe_ctx* c, const HalfMat& m, int n)
-{
-    const int64_t groups = std::min(n, m.n_mat);
-    if (n <= 6 * m.n_mat || (n / 32 + groups / 2) * (m.rg / 2) < 3 * c->ncu) return n <= 64 || n <= 2 * m.n_mat ? 16 : kHalfRows;
-    return n > 192 * m.n_mat && (int64_t)(n / kHalfTile) * (m.rg / 8) >= 2 * c->ncu ? kHalfTile : kHalfNarrow;
-}
-
-// Whether the weights pass the caches by: more than the last cache keeps to the next call, and hardly a group of two tiles (us, through
-// the caches and past them; 96 places in 64 groups of 4096 x 1408 67, 60; 512 in 128 of 1408 x 2816 146, 134; 1120 there 179, 179;
-// 192 in 32 of 1408 x 2816 52, 48; 192 in 32 of 1024 x 1024 12.6, 13.9; one group of 16384 x 4096: 12 places 32, 28; 24 49, 50).
-bool half_once(const HalfMat& m, int n) { return m.n_mat * m.mat_bytes() > 128e6 && n <= std::max(8 * m.n_mat, 16); }
-
-// One product over n places.  Rows of two terms in tiles of 96 places on the tile kernel, with two workgroups a compute unit: of 128 the
-// loop's registers spill with the weights held for both terms (us of the whole experts, 96, 128 and 256; 128 experts of 2816 x 704,
-// eight of them for 1024 rows 367, 375, 381; 2048 466, 476, 491; 4096 721, 735, 741; four of 64 of 4096 x 1408 for 2048 616, 633,
-// 642; four of 32 of 2816 x 2048 for 4096 749, 773, 753).
+// One product over n places.
 void half_product(phx_moe_ctx* c, const HalfMat& m, HalfArgs g, int n)
 {
     g.n = n;
-    g.cap = half_cap(c, m, n);
-    if (g.x_terms == 2 && g.cap > kHalfRows) g.cap = kHalfTerms;
-    g.once = g.cap <= kHalfRows ? half_once(m, n) : m.n_mat * m.mat_bytes() > 128e6;
+    g.cap = half_cap(c->ncu, n, m.n_mat, m.rg, g.x_terms);
+    g.once = half_once(m.n_mat * m.mat_bytes(), m.n_mat, n, g.cap);
     launch_half_product(c->stream, m, g, most_tiles(n, m.n_mat, g.cap));
 }
 }  // namespace
@@ -2757,7 +2729,7 @@ int phx_experts_half(phx_moe_ctx* c, const phx_weight* gu, const phx_weight* dn,
         g.out_terms = 2;
         g.n_x = T;
         g.cap = 16;
-        g.once = half_once(gu->half, T * k);
+        g.once = half_once(E * gu->half.mat_bytes(), E, T * k, g.cap);
         g.type = gu->type;
         g.out = h;
         launch_half_product(st, gu->half, g, T * k);

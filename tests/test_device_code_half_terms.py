@@ -1,6 +1,6 @@
-"""Static checks of the generated gfx950 code (CPU only: hipcc cross-compiles it to assembly) of the float tile kernel where the rows of x,
-or a paired product's output, are in two terms: its explicit LDS reads are waited for before their registers are used, no direct load is in
-a loop of its own, and nothing is spilled."""
+"""Static checks of the generated gfx950 code (CPU only: hipcc cross-compiles it to assembly) of the float tile kernel, for fp16 and where
+the rows of x, or a paired product's output, are in two terms: its explicit LDS reads are waited for before their registers are used, no
+direct load is in a loop of its own, and nothing, or next to nothing, is spilled."""
 import re
 import shutil
 import subprocess
@@ -15,12 +15,18 @@ CSRC = ROOT / "phoenix-lai_amd" / "csrc"
 HIPCC = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
 
 
-def assembly(tmp_path, name):
-    out = tmp_path / "k.s"
-    subprocess.run([HIPCC, "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-Xclang",
-                    "-target-feature", "-Xclang", "-packed-fp32-ops", f"-I{ROOT / 'include'}", "--cuda-device-only", "-S",
-                    str(CSRC / f"{name}.hip"), "-o", str(out)], check=True, capture_output=True, timeout=600)
-    return out.read_text()
+NAMES = ["kernels_half_terms_f16", "kernels_half_terms_bf16", "kernels_half_tile_f16"]
+
+
+@pytest.fixture(scope="module")
+def assembly(tmp_path_factory):
+    """The files' assembly, built side by side."""
+    d = tmp_path_factory.mktemp("asm")
+    run = {n: subprocess.Popen([HIPCC, "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-Xclang",
+                                "-target-feature", "-Xclang", "-packed-fp32-ops", f"-I{ROOT / 'include'}", "--cuda-device-only", "-S",
+                                str(CSRC / f"{n}.hip"), "-o", str(d / f"{n}.s")], stderr=subprocess.DEVNULL) for n in NAMES}
+    assert [p.wait(timeout=600) for p in run.values()] == [0] * len(NAMES)
+    return {n: (d / f"{n}.s").read_text() for n in NAMES}
 
 
 def check(text, kernels, scratch):
@@ -34,10 +40,19 @@ def check(text, kernels, scratch):
     assert loads and not any("s_cbranch_execnz" in line for i in loads for line in lines[i + 1:i + 5])
 
 
-@pytest.mark.skipif(not Path(HIPCC).exists(), reason="hipcc not available")
+pytestmark = pytest.mark.skipif(not Path(HIPCC).exists(), reason="hipcc not available")
+
+
 @pytest.mark.parametrize("type_", ["f16", "bf16"])
-def test_two_terms(tmp_path, type_):
-    text = assembly(tmp_path, f"kernels_half_terms_{type_}")
+def test_two_terms(assembly, type_):
+    text = assembly[f"kernels_half_terms_{type_}"]
     assert "ds_read_b128" in text and f"mfma_f32_32x32x16_{type_}" in text
     check(text, 3, 0)
     assert set(re.findall(r"^\s+\.vgpr_spill_count:\s+(\d+)$", text, re.M)) == {"0"}
+
+
+def test_one_term_of_fp16(assembly):
+    """As the bf16 file: next to nothing spilled, and that outside the loops."""
+    text = assembly["kernels_half_tile_f16"]
+    assert "ds_read_b128" in text and "mfma_f32_32x32x16_f16" in text
+    check(text, 4, 4)
