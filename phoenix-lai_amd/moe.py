@@ -723,10 +723,11 @@ class MoeContext:
         n = len(x) if src is None else src.size
         out = rows if act == PHX.QUANT_PLAIN else rows // 2
         y = np.zeros((n, out), np.float32)
-        bufs = [self.alloc(max(a.nbytes, 16)) for a in (offsets, x, y)] + ([] if src is None else [self.alloc(max(src.nbytes, 16))])
+        bufs = []
         try:
-            for b, a in zip(bufs, (offsets, x, y) if src is None else (offsets, x, y, src)):
-                b.upload(a)
+            for a in (offsets, x, y) if src is None else (offsets, x, y, src):
+                bufs.append(self.alloc(max(a.nbytes, 16)))
+                bufs[-1].upload(a)
             self.matmul_grouped_device(handle, act, n, bufs[0].ptr, bufs[1].ptr, len(x), None if src is None else bufs[3].ptr,
                                        PHX.F32, bufs[2].ptr)
             self.sync()
