@@ -1,10 +1,9 @@
-// What the kernels of products with fp16 and bf16 matrices share (kernels_half.hip, kernels_half_tile.hip).
+// What the kernels of products with fp16 and bf16 matrices share (kernels_half.hip, half_tile.h, kernels_lora.hip).
 #pragma once
 #include "device_common.h"
 #include "rows_io.h"
 
 namespace phx {
-
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -31,8 +30,8 @@ __device__ __forceinline__ f32x16 mma32(w4 a, u32x4 b, f32x16 c)
 }
 
 // act(g) * u, both activations g * sigmoid(z), the exponential and the reciprocal the hardware's (1 ulp each): a few units of
-// 2^-24, and the exponential's argument.  Far below, where the quotient is under every number, the reciprocal is 0; the gate
-// is then held to a number, so that no infinity meets it.
+// 2^-24, and the exponential's argument.  Far below, where the exponential is past every float and the quotient under 2^-120, the
+// reciprocal is 0; the gate is then held to a number, so that no infinity meets it.
 __device__ __forceinline__ float gated_half(int act, float g, float u)
 {
     const float z = act == PHX_QUANT_SILU_MUL ? g : 1.5957691216057308f * (g + 0.044715f * g * g * g);

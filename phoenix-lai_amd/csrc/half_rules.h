@@ -17,7 +17,8 @@ inline int most_tiles(int n, int n_mat, int cap) { return n / cap + std::min(n, 
 // groups of 1408 x 2816: 4 places 120, 131; 6 153, 153; 7 163, 155; 9.7 181, 161; 64 of 4096 x 1408: 5 102, 110; 6.9 115, 115; 9.4 127,
 // 121; 32 of 1024 x 1024: 12.5 14.1, 15.0; 25 16.4, 17.5; 50 21.3, 19.3; one of 4096 x 4096: 128 places 17.6, 40; 256 29, 41; 512 51,
 // 42; 1024 92, 44).  Its tiles of 16 places to two a group and to 64 in all, else of 32 (one of 4096 x 4096: 64 places 12.7, 16.7; 128
-// 20.5, 17.6; 128 groups, 8.8 places 167, 157).
+// 20.5, 17.6; 128 groups, 8.8 places 167, 157).  Matrices of up to 32 rows stay on it whatever the places (one of 32 x 4096: 1000
+// places 15.6, 41; 8000 16.8, 42; 64000 140, 128).
 // Tiles of 256 places, one workgroup a compute unit, past 192 places a group where they number two per compute unit, else of 128, two
 // workgroups (us, tiles of 128 and 256; 32 groups of 2816 x 4096, 513 places 393, 381; 128 of 1408 x 2816, 128 places 249, 252; one of
 // 4096 x 4096, 2048 places 60, 78; 512 42, 71).

@@ -1,6 +1,6 @@
 // The tile kernel of products with fp16 and bf16 matrices in runs of ragged length.  Built apart from the row kernel, since its sums
 // need both halves of the register file, for which the matrix instructions' results have to be left in accumulation registers,
-// and each type by itself, since the widths of a tile are many and long to compile.
+// and each type, and the forms with rows in two terms, by themselves, since the widths of a tile are many and long to compile.
 #pragma once
 #include <algorithm>
 
@@ -38,7 +38,8 @@ constexpr int ti_newer(int nt, int ring, int xt, int t)
 }
 
 // TERMS: the rows of x, or a paired product's output, are in two terms.  64 columns of x then are two steps, one a term, which
-// both take the weights' registers, and the second issues the weights' loads.
+// both take the weights' registers, and the second issues the weights' loads.  16384 rows of two terms by 128 matrices of 2816 x 704
+// to float 175 to 193 us, the matrix cores busy in 38% of the cycles, 610 MB read and 184 written (of one term 150 to 160).
 template <int NT, int MT, bool PAIRED, bool ONCE, bool BF, bool TERMS>
 __device__ __forceinline__ void half_tile_product(const HalfArgs& g, const Tile& tl, int bx, unsigned char* ring, uint32_t* orow)
 {

@@ -24,8 +24,8 @@ __device__ __forceinline__ void store_eight(void* p, int64_t i, const float (&v)
 }
 
 // NT threads per row, eight consecutive values per thread and step, the row held in registers from its load to its integers: one
-// pass over memory, which bounds it (4099 rows of 4096 bf16 values to bf16 and int8: 151 MB in 35 to 50 us, 3.0 to 4.3 TB/s where a
-// copy has 4.7; one row of 2816 floats 3.9 us, a launch).  Values past the row are zeros and not the row's last again: sum may lie over x,
+// pass over memory, which bounds it (4099 rows of 4096 bf16 values to bf16 and int8: 151 MB in 35 us, 4.3 TB/s where a copy has 4.7,
+// and in 27 where they are still in the last cache; one row of 2816 floats 3.9 us, a launch).  Values past the row are zeros and not the row's last again: sum may lie over x,
 // and another wave may have stored there.  The mapping of values to threads, and so every rounding of the sum of squares, is
 // phx_quant_i8's.
 template <int NT, int STEPS, int DT>
