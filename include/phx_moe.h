@@ -443,7 +443,7 @@ int phx_matmul_grouped(phx_moe_ctx* ctx, const phx_weight* w, int act, int n, co
  *   h = act(Wgate[e] x[t]) * (Wup[e] x[t]),  e = ids[t][j], as phx_matmul_grouped forms it, in float
  *   out[t] = sum over j, in order, of weights[t][j] * (Wdown[e] h)
  * the products and the sum in float, rounded to out_type at the end.  Wdown's product takes h in two terms of the weights' type (16 bits
- * of it with bf16, 22 with fp16: there none finer than 2^-25, and past 65504 an infinity).  A place whose id is outside [0, n_expert) is
+ * of it with bf16, 22 with fp16: there none finer than 2^-25, and past 65504 an infinity); against an infinity in Wdown they may be a NaN.  A place whose id is outside [0, n_expert) is
  * skipped; a row without experts is zero.  An id may come more than once in a row.  gate_up: paired, [n_expert][2 nf][d];
  * down: [n_expert][d][nf], of the same type; x [T][d] of that type, ids and weights [T][k], out [T][d];
  * 1 <= T <= PHX_MAX_ROWS_I8, 1 <= k <= PHX_MAX_USED; x and out 16-byte aligned. */
@@ -467,8 +467,8 @@ void phx_lora_free(phx_moe_ctx* ctx, phx_lora* lora);
  *   y[t] = y_in[t] + scale * B (A x[t])      with the adapter of slot ids[t]
  *   y[t] = y_in[t]                           where ids[t] is outside [0, n_slot) or the slot is empty
  * A x and its scale in float; B's products take that value in two terms of the adapters' type (16 bits of it with
- * bf16, 22 with fp16), in four where y is float (fp16: none finer than 2^-39 of the largest of 16 ranks); one rounding, to
- * y_type (PHX_F32, PHX_F16, PHX_BF16).  x [T][cols] of the adapters' type; y_in and y of y_type, rows ld values apart
+ * bf16, 22 with fp16), in four where y is float (fp16: none finer than 2^-39 of the largest of 16 ranks); against an infinity in
+ * B they may be a NaN.  One rounding, to y_type (PHX_F32, PHX_F16, PHX_BF16).  x [T][cols] of the adapters' type; y_in and y of y_type, rows ld values apart
  * (ld >= rows: both may be a section of a wider matrix, also two sections of one, whose rows do not meet), y may be y_in.
  * 1 <= T <= PHX_MAX_ROWS_I8, ld <= 2^40; x 16-byte aligned, y_in and y to their values, ids 4-byte. */
 int phx_lora_add(phx_moe_ctx* ctx, const phx_lora* lora, int T, const void* x, const int32_t* ids, int y_type, int64_t ld,

@@ -117,6 +117,28 @@ def test_infinities_stay_in_their_row(ctx, type_, T, E, d, nf):
     assert not np.isfinite(got[bad]).any()
 
 
+@pytest.mark.parametrize("type_", [1, 30])
+@pytest.mark.parametrize("T,E,d,nf", [(3, 4, 16, 40), (300, 4, 64, 72), (4096, 2, 512, 72)])
+def test_an_infinity_in_down_stays_in_its_output(ctx, type_, T, E, d, nf):
+    """One value of one expert's Wdown: its output is no number in that expert's rows, everything else as it would be."""
+    rng = np.random.default_rng(T + nf)
+    raw, (wg, wd) = expert_weights(rng, E, d, nf, type_)
+    raw[1][1, 5, nf - 1] = np.inf if type_ == 1 else 0x7F80
+    raw_x, x = ref.held(rng.standard_normal((T, d)), type_)
+    ids, weights = (np.arange(T) % E).astype(np.int32)[:, None], np.ones((T, 1), F32)
+    hs = upload(ctx, type_, raw, E, d, nf)
+    try:
+        got = call(ctx, hs, 1, raw_x, ids, weights, 0, d)
+    finally:
+        for h in hs:
+            ctx.weight_free(h)
+    want, bound = experts(x, ids, weights, wg, wd, 1, type_)
+    hit = np.zeros((T, d), bool)
+    hit[ids[:, 0] == 1, 5] = True
+    assert not np.isfinite(got[hit]).any()
+    assert (np.abs(got - want)[~hit] <= ref.rounded(want, bound, 0)[~hit]).all()
+
+
 def test_fp16_past_its_range(ctx):
     """An h past fp16's numbers is an infinity of its sign, without a NaN from its second term."""
     x = np.zeros((2, 8), np.float16)
